@@ -27,6 +27,7 @@ extern "C" {
 #define QE_OUT_BF16 2       /* y is bf16 (round to nearest even), default fp32 */
 #define QE_GLU 4            /* GLU matrix (8 gate + 8 up rows per tile): y = bf16 silu(gate) * up, n / 2 cols */
 #define QE_W8_PER_CHANNEL 8 /* W8 with one scale per output row, s = [N] (group = K) */
+#define QE_F16 16           /* attention: q, k, v and out are fp16 (default bf16) */
 
 int qe_abi_version(void);
 
@@ -63,7 +64,7 @@ void qe_gemm_tune_file(const char* path);
 void qe_gemm_tune_clear(void);
 int qe_gemm_tune_entries(void);
 /* Library-owned workspaces (the prefill GEMMs' split-K partial sums, the fp16-accumulate and W4A8 / W8A8 pre-pass
- * buffers, the part sums of 9..64-row decode) are kept per (device, stream): calls on one stream share a buffer (a
+ * buffers, the part sums of 9..64-row decode and of the attention over the cache) are kept per (device, stream): calls on one stream share a buffer (a
  * call's launches stay together, also with several host threads on the stream), calls on two streams of a device use
  * two, so concurrent streams never overwrite each other's workspace (the reference keeps them thread_local,
  * src/kernels/gemm.cu:3258-3368). A buffer grows on a call outside graph capture. Captured calls use buffers that their
@@ -76,7 +77,7 @@ int qe_gemm_tune_entries(void);
 void qe_gemm_reserve(size_t bytes);
 void qe_gemm_reserve_s(size_t bytes, void* stream);
 /* test hook: how many workspace buffers of a kind (0 split-K, 1 W4A8 / W8A8 pre-pass, 2 fp16-accumulate pre-pass, 3 part
- * sums of 17..64-row decode, 4 slice sums of 9..16-row decode) the library's streams and live graphs hold, over all
+ * sums of 17..64-row decode, 4 slice sums of 9..16-row decode, 5 part sums of qe_attn_tree) the library's streams and live graphs hold, over all
  * devices. No counterpart in the reference. */
 int qe_workspace_count(int kind);
 /* Prefill GEMM with the reference's fp16-accumulate numerics (gemm_h_kernel + x_to_h_kernel,
@@ -336,6 +337,77 @@ void qe_moe_w4_noalloc(const float* logits, const uint16_t* x, const void* recor
  * allocation, no synchronization). */
 void qe_moe_pack_w4(const int32_t* gu_q, const uint16_t* gu_s, const int32_t* dn_q, const uint16_t* dn_s, int E, int H,
                     int I, void* records, void* stream);
+
+/* ---- attention and the paged cache of keys and values. No reference C-ABI exists for them. 16-bit values are bf16, or
+ * fp16 where said; scores, softmax statistics and sums are fp32, probabilities are rounded to the values' type for the
+ * second product (as the matrix cores take them). heads % kv_heads == 0: query head h reads kv head h / (heads / kv_heads).
+ * d = 64, 128 or 256. scale > 0, usually d^-0.5. Pointers 16-byte aligned, strides in elements and multiples of 8, a head's d values contiguous.
+ * lse (NULL: not wanted) [t][heads] fp32: log of the sum of the exponentiated scores.
+ * A row that sees no key has out = 0 and lse = -inf; a key that a row does not see has no effect on it, whatever its bits.
+ * Lengths, tables and indexes live on the device and are not seen by the host: values out of range make a kernel skip
+ * what they name and never touch memory outside the tensors. Every call is one to three launches on `stream`, without
+ * host synchronization, and can be captured. Deterministic: same inputs, same bits. ---- */
+
+/* Causal attention over whole prompts packed without padding: sequence b is rows cu[b] .. cu[b + 1] - 1 (cu [nseq + 1]
+ * int32, ascending), row i of it sees rows 0 .. i. Rows of q, k, v and out have strides of their own, so views into one
+ * fused QKV product do. Rows before cu[0] and from cu[nseq] on are left as they were. flags: QE_F16. */
+void qe_attn_prompt(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
+                    const void* v, int64_t v_row, int64_t v_head, void* out, int64_t out_row, int64_t out_head, float* lse,
+                    const int32_t* cu, int nseq, int t, int heads, int kv_heads, int d, float scale, int flags,
+                    void* stream);
+
+/* A paged cache: token i of sequence slot s lies in row i % page of page table[s][i / page] of every layer's pools. The
+ * caller owns the memory; the description is read during the call only.
+ *   length  committed tokens of a slot; rows appended after them are drafted until qe_kv_accept commits them
+ *   held    pages of a slot (table[s][0 .. held - 1]; the rest -1)
+ *   ref     how many slots hold a page, 0: free
+ * Start: table -1, the others 0. page: a power of two, 16 .. 1024. k and v share the strides. */
+typedef struct qe_kv_cache {
+    void* k;
+    void* v;
+    int64_t layer_stride, page_stride, head_stride, token_stride; /* elements, multiples of 8 */
+    int32_t* table;                                               /* [slots][width] */
+    int32_t* length;                                              /* [slots] */
+    int32_t* held;                                                /* [slots] */
+    int32_t* ref;                                                 /* [pages] */
+    int32_t layers, pages, page, kv_heads, d, slots, width;
+    int32_t f16; /* 0: bf16, 1: fp16 */
+} qe_kv_cache_t;
+
+/* Room for add[i] more tokens in slot seqs[i], i < n <= 1024: free pages with the lowest numbers, entries in order. Where
+ * the slot's last committed token is in a partly filled page that others hold too (after a fork), the slot gets a copy of
+ * it first (all layers), so that an append never writes a shared page. ok[i] 1: done (or nothing to do), 0: nothing
+ * changed: not enough pages for this entry and those before it, more tokens than the table's width, a slot out of range,
+ * or one that an earlier entry names. copies: int32 [n + 1][4], written: [0] = their number, then (from, to, rows). */
+void qe_kv_reserve(const qe_kv_cache_t* cache, const int32_t* seqs, const int32_t* add, int n, int32_t* ok,
+                   int32_t* copies, void* stream);
+/* Slot children[i] gets parents[i]'s committed tokens by sharing their pages (the next reserve copies the partly filled
+ * one). ok[i] 0: nothing done: a slot out of range, a child that holds pages or tokens, is named by an earlier entry or is
+ * one of the call's children as well as a parent. n <= 1024. */
+void qe_kv_fork(const qe_kv_cache_t* cache, const int32_t* parents, const int32_t* children, int n, int32_t* ok,
+                void* stream);
+/* Slot seqs[i] keeps its first min(length, lengths[i]) tokens (lengths NULL: none) and the pages that hold them; the
+ * others are given back, and free once no slot holds them. Later entries of a slot named twice do nothing. n <= 1024. */
+void qe_kv_release(const qe_kv_cache_t* cache, const int32_t* seqs, const int32_t* lengths, int n, void* stream);
+/* New keys and values: row t of sequence b (cu as above; slot seqs[b], distinct) goes to token length + t - cu[b] of the
+ * slot, in `layers` layers from `layer` on. strides: layer, row and head of k, then of v (host memory, elements). Rows
+ * without a held page are not written. length is not changed. */
+void qe_kv_append(const qe_kv_cache_t* cache, int layer, int layers, const void* k, const void* v, const int64_t* strides,
+                  const int32_t* seqs, const int32_t* cu, int nseq, int t, void* stream);
+/* Commits count[i] tokens of slot seqs[i] (distinct). path NULL: the first drafted ones. Else path int32 [n][most], most
+ * <= 64: drafted rows path[i][0 .. count - 1] move to the first places after the committed tokens, in all layers, as if
+ * all were read before any is written. length_out [slots] (NULL: the cache's own) gets length + count, at most what the
+ * held pages take. */
+void qe_kv_accept(const qe_kv_cache_t* cache, const int32_t* seqs, const int32_t* count, const int32_t* path, int most,
+                  int n, int32_t* length_out, void* stream);
+
+/* Attention of drafted tokens over the cache, the drafted rows appended before: row cu[b] + i of q is the drafted token i
+ * of slot seqs[b] and sees the slot's committed tokens and the drafted tokens j with bit j of mask[cu[b] + i] (NULL: j <=
+ * i, a chain). One row a sequence: decode. max_new: the largest number of rows of a sequence, at most 64; rows past it,
+ * and rows before cu[0] or from cu[nseq] on, are left as they were. nseq <= 4096. */
+void qe_attn_tree(const qe_kv_cache_t* cache, int layer, const void* q, int64_t q_row, int64_t q_head, void* out,
+                  int64_t out_row, int64_t out_head, float* lse, const int32_t* seqs, const int32_t* cu, int nseq, int t,
+                  int max_new, const uint64_t* mask, int heads, float scale, void* stream);
 
 /* ---- on-disk weights: .safetensors files (host, memory-mapped) and the quantized-matrix loader ----
  * qe_st_open maps a file and indexes its tensors by name (reference SafeTensors::open, src/safetensors.h:40; a

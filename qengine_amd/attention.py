@@ -1,0 +1,291 @@
+"""Attention over whole prompts and over a paged cache of keys and values, with the cache's own operations (the C-ABI's
+qe_attn_* and qe_kv_* entry points, include/qe_kernels.h).
+
+A serving step of a batch:
+
+    cache = KVCache.empty(layers, pages, page, kv_heads, head_dim, slots, max_tokens)
+    cache.reserve(seqs, counts)                       # pages for the new rows
+    for layer in ...:
+        cache.append(layer, k, v, seqs, cu)           # the new rows' keys and values
+        o = attn_prompt(q, k, v, cu)                  # a prompt's first pass, or
+        o = cache.attend(layer, q, seqs, cu, most)    # one token a sequence, or a drafted chain or tree (mask)
+    cache.accept(seqs, counts)                        # the rows are the sequence's now (path: those of a tree that were kept)
+    cache.fork(parents, children); cache.release(seqs)
+
+Lengths, tables and batches (seqs, cu, counts: int32) stay on the device, so that steps need no host synchronization and
+can be captured into graphs. Shapes, types, devices and strides are checked here (TypeError, ValueError) before the call;
+values on the device are checked by the kernels, which skip what is out of range. Calls run on the current stream of the
+tensors' device.
+"""
+import ctypes
+
+import torch
+
+from .qe import typed
+
+F16 = 16
+MAX_NODES = 64
+MAX_BATCH = 1024
+HEAD_DIMS = (64, 128, 256)
+
+_FN = {}
+
+
+def _fn(name, sig):
+    f = _FN.get(name)
+    if f is None:
+        f = _FN[name] = typed(name, sig)
+    return f
+
+
+def _run(device, name, sig, *args):
+    """the call on the current stream of the tensors' device, which need not be the current one"""
+    if device.type != "cuda":
+        raise ValueError(f"tensors are on a GPU, got {device}")
+    i = device.index
+    if i is None or i == torch._C._cuda_getDevice():
+        _fn(name, sig)(*args, torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+        return
+    with torch.cuda.device(i):
+        _fn(name, sig)(*args, torch._C._cuda_getCurrentRawStream(i))
+
+
+def _rows(name, t, dims, dtype, device):
+    """a [.., d] tensor that the kernels can read: its type, place and strides"""
+    if t.dim() != dims:
+        raise ValueError(f"{name} has {dims} dimensions, got shape {tuple(t.shape)}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} is {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {device}, got {t.device}")
+    if t.numel():
+        if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:-1]):
+            raise ValueError(f"{name}: a row's values lie together and its other strides are multiples of 8, got {t.stride()}")
+        if t.data_ptr() % 16:
+            raise ValueError(f"{name} is 16-byte aligned")
+
+
+def _ints(name, t, shape, device, dtype=torch.int32):
+    if t.dtype != dtype:
+        raise TypeError(f"{name} is {dtype}, got {t.dtype}")
+    if t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} is contiguous of shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {device}, got {t.device}")
+
+
+def _starts(cu, device):
+    if cu.dim() != 1 or cu.shape[0] < 1:
+        raise ValueError(f"cu has one more entry than there are sequences, got shape {tuple(cu.shape)}")
+    _ints("cu", cu, cu.shape, device)
+    return cu.shape[0] - 1
+
+
+def _dtype_of(t):
+    if t.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"values are bfloat16 or float16, got {t.dtype}")
+    return t.dtype
+
+
+def _out_lse(q, out, lse, dtype, device):
+    """(out, lse tensor or None) of a call whose rows are q's"""
+    if out is None:
+        out = torch.empty(q.shape, dtype=dtype, device=device)
+    else:
+        _rows("out", out, 3, dtype, device)
+        if out.shape != q.shape:
+            raise ValueError(f"out has q's shape {tuple(q.shape)}, got {tuple(out.shape)}")
+    return out, torch.empty(q.shape[:2], dtype=torch.float32, device=device) if lse else None
+
+
+def _scale(scale, d):
+    if scale is None:
+        return d ** -0.5
+    if not 0 < scale < float("inf"):
+        raise ValueError(f"scale is positive, got {scale}")
+    return float(scale)
+
+
+def attn_prompt(q, k, v, cu, scale=None, out=None, lse=False):
+    """Causal attention of packed prompts: q [t][heads][d], k and v [t][kv heads][d] (views into one QKV product do),
+    sequence b the rows cu[b] .. cu[b + 1] - 1. -> out like q; with lse=True (out, lse [t][heads] fp32). Rows before cu[0]
+    and from cu[-1] on are left as they were in a given `out` (and have no meaning in a new one)."""
+    device, dtype = q.device, _dtype_of(q)
+    _rows("q", q, 3, dtype, device)
+    _rows("k", k, 3, dtype, device)
+    _rows("v", v, 3, dtype, device)
+    t, heads, d = q.shape
+    kv = k.shape[1]
+    if k.shape != v.shape or k.shape[0] != t or k.shape[2] != d or d not in HEAD_DIMS or kv == 0 or heads % kv or not heads:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: the same rows, d of {HEAD_DIMS}, heads a "
+                         "multiple of the kv heads")
+    n = _starts(cu, device)
+    if n > 4096:
+        raise ValueError(f"at most 4096 sequences, got {n}")
+    scale = _scale(scale, d)
+    out, sums = _out_lse(q, out, lse, dtype, device)
+    if t and n:
+        qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+        _run(device, "qe_attn_prompt", "pllpllpllpllppiiiiifip", q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
+             v.data_ptr(), vs[0], vs[1], out.data_ptr(), os[0], os[1], sums.data_ptr() if lse else None, cu.data_ptr(), n, t,
+             heads, kv, d, scale, F16 if dtype == torch.float16 else 0)
+    return (out, sums) if lse else out
+
+
+class _CacheStruct(ctypes.Structure):
+    """include/qe_kernels.h qe_kv_cache_t"""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("layer_stride", ctypes.c_int64),
+                ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64),
+                ("table", ctypes.c_void_p), ("length", ctypes.c_void_p), ("held", ctypes.c_void_p), ("ref", ctypes.c_void_p)]
+    _fields_ += [(x, ctypes.c_int32) for x in ("layers", "pages", "page", "kv_heads", "d", "slots", "width", "f16")]
+
+
+class KVCache:
+    """Paged keys and values of all layers and the state of its pages, around tensors that the caller may also look at:
+    k, v [layers][pages][kv heads][page][d] (any strides that the kernels can read: a [.., page, kv heads, d] pool goes in
+    as its transposed view), table [slots][width] (-1: none), length [slots], held [slots], ref [pages], int32."""
+
+    def __init__(self, k, v, table, length, held, ref):
+        self.device, self.dtype = device, dtype = k.device, _dtype_of(k)
+        _rows("k", k, 5, dtype, device)
+        _rows("v", v, 5, dtype, device)
+        if k.shape != v.shape or k.stride() != v.stride() or not k.numel():
+            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} have the same shape and strides")
+        layers, pages, kv, page, d = k.shape
+        if d not in HEAD_DIMS or page < 16 or page > 1024 or page & (page - 1) or kv > 1024:
+            raise ValueError(f"pools [layers][pages][kv heads][page][d] with d of {HEAD_DIMS}, at most 1024 kv heads and pages of "
+                             f"16 to 1024 tokens, a power of two: got {tuple(k.shape)}")
+        if table.dim() != 2 or not table.numel() or table.shape[1] * page >= 2 ** 31:
+            raise ValueError(f"table is [slots][pages of a slot], got {tuple(table.shape)}")
+        slots, width = table.shape
+        _ints("table", table, table.shape, device)
+        _ints("length", length, (slots,), device)
+        _ints("held", held, (slots,), device)
+        _ints("ref", ref, (pages,), device)
+        self.k, self.v, self.table, self.length, self.held, self.ref = k, v, table, length, held, ref
+        self.layers, self.pages, self.page, self.kv_heads, self.d, self.slots, self.width = layers, pages, page, kv, d, slots, width
+        s = k.stride()
+        self._c = _CacheStruct(k.data_ptr(), v.data_ptr(), s[0], s[1], s[2], s[3], table.data_ptr(), length.data_ptr(),
+                               held.data_ptr(), ref.data_ptr(), layers, pages, page, kv, d, slots, width,
+                               int(dtype == torch.float16))
+        self._at = ctypes.addressof(self._c)
+
+    @staticmethod
+    def empty(layers, pages, page, kv_heads, d, slots, max_tokens, dtype=torch.bfloat16, device="cuda"):
+        """a cache that holds nothing, for slots of up to max_tokens tokens"""
+        k = torch.empty(layers, pages, kv_heads, page, d, dtype=dtype, device=device)
+        ints = dict(dtype=torch.int32, device=k.device)
+        return KVCache(k, torch.empty_like(k), torch.full((slots, -(-max_tokens // page)), -1, **ints),
+                       torch.zeros(slots, **ints), torch.zeros(slots, **ints), torch.zeros(pages, **ints))
+
+    def _batch(self, name, t, n=None):
+        if t.dim() != 1:
+            raise ValueError(f"{name} has one dimension, got shape {tuple(t.shape)}")
+        n = t.shape[0] if n is None else n
+        _ints(name, t, (n,), self.device)
+        return n
+
+    def _few(self, n):
+        if n > MAX_BATCH:
+            raise ValueError(f"at most {MAX_BATCH} sequences a call, got {n}")
+
+    def reserve(self, seqs, add):
+        """Room for add[i] more tokens in slot seqs[i], entries in order; the last page is copied first where other slots hold
+        it too. -> int32 [n], 1: done, 0: nothing changed (not enough pages, no room in the table, a bad or repeated slot)."""
+        n = self._batch("seqs", seqs)
+        self._batch("add", add, n)
+        self._few(n)
+        got = torch.empty(5 * n + 4, dtype=torch.int32, device=self.device)  # the list of copies, then the answers
+        if n:
+            _run(self.device, "qe_kv_reserve", "pppippp", self._at, seqs.data_ptr(), add.data_ptr(), n,
+                 got.data_ptr() + 16 * (n + 1), got.data_ptr())
+        return got[4 * n + 4:]
+
+    def fork(self, parents, children):
+        """Slot children[i] shares the pages of parents[i]'s committed tokens. -> int32 [n], 1: done, 0: nothing changed (a bad
+        slot, a child that is not empty, is repeated, or is one of the call's parents)."""
+        n = self._batch("parents", parents)
+        self._batch("children", children, n)
+        self._few(n)
+        ok = torch.empty(n, dtype=torch.int32, device=self.device)
+        if n:
+            _run(self.device, "qe_kv_fork", "pppipp", self._at, parents.data_ptr(), children.data_ptr(), n, ok.data_ptr())
+        return ok
+
+    def release(self, seqs, lengths=None):
+        """Slot seqs[i] keeps its first lengths[i] tokens (none without lengths) and gives its other pages back."""
+        n = self._batch("seqs", seqs)
+        if lengths is not None:
+            self._batch("lengths", lengths, n)
+        self._few(n)
+        if n:
+            _run(self.device, "qe_kv_release", "pppip", self._at, seqs.data_ptr(), None if lengths is None else lengths.data_ptr(), n)
+
+    def append(self, layer, k, v, seqs, cu):
+        """New rows k, v [t][kv heads][d] of one layer, or [layers][t][kv heads][d] of all (layer None): rows cu[b] ..
+        cu[b + 1] - 1 go behind the committed tokens of slot seqs[b], into pages reserved before. Slots are distinct."""
+        dims = 4 if layer is None else 3
+        _rows("k", k, dims, self.dtype, self.device)
+        _rows("v", v, dims, self.dtype, self.device)
+        t = k.shape[-3]
+        if k.shape != v.shape or k.shape[-2:] != (self.kv_heads, self.d) or (layer is None and k.shape[0] != self.layers):
+            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} are rows of {self.kv_heads} kv heads of {self.d}"
+                             + (f", of {self.layers} layers" if layer is None else ""))
+        if layer is not None and not 0 <= layer < self.layers:
+            raise ValueError(f"layer {layer} of {self.layers}")
+        n = _starts(cu, self.device)
+        self._batch("seqs", seqs, n)
+        if t and n:
+            ks, vs = k.stride(), v.stride()
+            one = layer is not None
+            strides = (ctypes.c_int64 * 6)(0 if one else ks[0], ks[-3], ks[-2], 0 if one else vs[0], vs[-3], vs[-2])
+            _run(self.device, "qe_kv_append", "piipppppiip", self._at, layer if one else 0, 1 if one else self.layers,
+                 k.data_ptr(), v.data_ptr(), ctypes.addressof(strides), seqs.data_ptr(), cu.data_ptr(), n, t)
+
+    def accept(self, seqs, count, path=None, length=None):
+        """count[i] drafted tokens of slot seqs[i] are committed: the first ones, or those of path int32 [n][at most 64], whose
+        rows move together in all layers. The new lengths go to `length` [slots], or the cache's own. Slots are distinct."""
+        n = self._batch("seqs", seqs)
+        self._batch("count", count, n)
+        most = 0
+        if path is not None:
+            if path.dim() != 2 or path.shape[1] > MAX_NODES:
+                raise ValueError(f"path is [sequences][at most {MAX_NODES}], got {tuple(path.shape)}")
+            most = path.shape[1]
+            _ints("path", path, (n, most), self.device)
+        if length is not None:
+            _ints("length", length, (self.slots,), self.device)
+        if n > 65535:
+            raise ValueError(f"at most 65535 sequences a call, got {n}")
+        if n and (path is None or most):
+            _run(self.device, "qe_kv_accept", "ppppiipp", self._at, seqs.data_ptr(), count.data_ptr(),
+                 None if path is None else path.data_ptr(), most, n, None if length is None else length.data_ptr())
+
+    def attend(self, layer, q, seqs, cu, most, mask=None, scale=None, out=None, lse=False):
+        """Attention of drafted tokens, appended before: row cu[b] + i of q [t][heads][d] is drafted token i of slot seqs[b]; it
+        sees the slot's committed tokens and the drafted tokens whose bit is set in mask[cu[b] + i] (int64 [t]), without a mask
+        those up to itself. most (at most 64): the largest number of rows of a sequence. -> out like q; with lse=True (out,
+        lse [t][heads] fp32). Rows of no sequence, or past `most`, are left as they were in a given `out`."""
+        device, dtype = self.device, self.dtype
+        _rows("q", q, 3, dtype, device)
+        t, heads, d = q.shape
+        if d != self.d or heads == 0 or heads % self.kv_heads:
+            raise ValueError(f"q {tuple(q.shape)}: heads of {self.d}, a multiple of the {self.kv_heads} kv heads")
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer {layer} of {self.layers}")
+        if not 1 <= most <= MAX_NODES:
+            raise ValueError(f"1 to {MAX_NODES} drafted tokens a sequence, got {most}")
+        n = _starts(cu, device)
+        self._batch("seqs", seqs, n)
+        if n > 4096:
+            raise ValueError(f"at most 4096 sequences, got {n}")
+        if mask is not None:
+            _ints("mask", mask, (t,), device, torch.int64)
+        scale = _scale(scale, d)
+        out, sums = _out_lse(q, out, lse, dtype, device)
+        if t and n:
+            qs, os = q.stride(), out.stride()
+            _run(device, "qe_attn_tree", "pipllpllpppiiipifp", self._at, layer, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0],
+                 os[1], sums.data_ptr() if lse else None, seqs.data_ptr(), cu.data_ptr(), n, t, most,
+                 None if mask is None else mask.data_ptr(), heads, scale)
+        return (out, sums) if lse else out

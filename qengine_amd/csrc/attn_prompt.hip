@@ -1,0 +1,290 @@
+// Causal attention over whole prompts, packed without padding, grouped heads.
+//
+//   o[i] = sum_{j <= i} p_ij v[j],  p_ij = softmax_j(scale q[i] . k[j])
+//
+// One pass over the keys with the running maximum and sum of the softmax; a block takes BQ = 32 W rows of one head, a wave
+// 32 of them with its queries, its scores S^T = K Q^T (32 x 32 x 16 MFMA) and its sums O^T = V^T P^T in registers. 64 keys
+// at a time lie in LDS, staged by LDS DMA while the 64 before are worked on. A wave reads K as the A operand in 16-byte
+// pieces and V's transpose by ds_read_b64_tr_b16; both tiles are stored with their 16-byte pieces permuted by row so that
+// these reads meet no bank twice.
+#include "attn_common.hpp"
+#include "kv_cache.hpp"
+#include "mfma_tile.hpp"
+
+#include <algorithm>
+#include <atomic>
+
+namespace qe_prompt {
+using qe_tile::dma16;
+constexpr int kKeys = 64;          // keys of a step
+constexpr int kMaxSeqs = 4096;     // their block counts are kept in LDS
+constexpr float kLazy = 8.f;       // the running maximum follows a row's scores once they pass it by this much (2^8 in the sums)
+
+struct Args {
+    const char *q, *k, *v;
+    char* out;
+    float* lse;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;  // bytes
+    const int32_t* cu;
+    int nseq, t, heads, kv_heads;
+    float scale2;  // log2(e) times the scale: exponentials are powers of two
+};
+
+template <int D>
+__device__ __forceinline__ int k_swz(int row) { return row & (D == 64 ? 7 : 15); }
+template <int D>
+__device__ __forceinline__ int v_swz(int row) { return (row & (D == 64 ? 3 : 7)) << 1; }
+
+template <int DT, int D, int W>
+__global__ __launch_bounds__(64 * W, 2) void prompt_kernel(Args a) {
+    using T = AttnT<DT>;
+    constexpr int BQ = 32 * W, KS = D / 16, DB = D / 32, TILE = kKeys * D * 2, CH = D / 8;
+    extern __shared__ char lds[];  // two stages of K and V tiles; before them the block counts
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, half = lane >> 5;
+
+    // ---- which rows: blocks of all sequences, those with the most keys first
+    const int kvh = blockIdx.x % a.heads % a.kv_heads, grp = blockIdx.x % a.heads / a.kv_heads;
+    const int head = kvh * (a.heads / a.kv_heads) + grp;
+    int slot = blockIdx.x / a.heads, b = 0, qb = 0;
+    auto blocks_of = [&](int i) {
+        const int c0 = min(max(a.cu[i], 0), a.t), c1 = min(a.cu[i + 1], a.t);
+        return c1 > c0 ? (c1 - c0 + BQ - 1) / BQ : 0;
+    };
+    if (a.nseq == 1) {
+        qb = blocks_of(0) - 1 - slot;
+        if (qb < 0) return;
+    } else {
+        int* nb = reinterpret_cast<int*>(lds);
+        for (int i = tid; i < a.nseq; i += 64 * W) nb[i] = blocks_of(i);
+        __syncthreads();
+        // blocks with index >= level, over all sequences
+        auto count = [&](int level) {
+            int n = 0;
+            for (int i = lane; i < a.nseq; i += 64) n += max(0, nb[i] - level);
+#pragma unroll
+            for (int o = 32; o; o /= 2) n += __shfl_xor(n, o);
+            return n;
+        };
+        if (slot >= count(0)) return;
+        int lo = 0, hi = (a.t + BQ - 1) / BQ;  // count(lo) > slot >= count(hi)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (count(mid) > slot) lo = mid;
+            else hi = mid;
+        }
+        qb = lo;
+        int rank = slot - count(lo + 1);  // among the sequences that have a block of this index
+        for (int i0 = 0;; i0 += 64) {
+            const uint64_t has = __ballot(i0 + lane < a.nseq && nb[i0 + lane] > qb);
+            const int n = __popcll(has);
+            if (rank < n) {
+                uint64_t m = has;
+                for (; rank > 0; rank--) m &= m - 1;
+                b = i0 + __ffsll((unsigned long long)m) - 1;
+                break;
+            }
+            rank -= n;
+        }
+        __syncthreads();
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    qb = __builtin_amdgcn_readfirstlane(qb);
+    const int c0 = min(max(a.cu[b], 0), a.t), len = min(a.cu[b + 1], a.t) - c0;
+    const int q0 = qb * BQ, qw = q0 + wave * 32;  // the block's and the wave's first row
+    const int row = qw + col;                     // this lane's query
+
+    u32x4_v q[KS];
+    {
+        const char* p = a.q + (int64_t)(c0 + min(row, len - 1)) * a.q_row + (int64_t)head * a.q_head + half * 16;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) q[ks] = *reinterpret_cast<const u32x4_v*>(p + ks * 32);
+    }
+    const unsigned lds32 = (unsigned)(uintptr_t)lds;
+    const char* kb = a.k + (int64_t)c0 * a.k_row + (int64_t)kvh * a.k_head;
+    const char* vb = a.v + (int64_t)c0 * a.v_row + (int64_t)kvh * a.v_head;
+    // a wave instruction fills 1 KB: 64 / CH rows; lane i lands at piece i, so it loads the piece that belongs there. Keys
+    // past the end re-read the last one (no row sees them).
+    auto stage = [&](int j, int buf) {
+        constexpr int RPI = 64 / CH, N = kKeys / RPI / W;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int r0 = (wave * N + i) * RPI, r = r0 + lane / CH, key = min(j * kKeys + r, len - 1);
+            dma16(kb + (int64_t)key * a.k_row + ((lane % CH) ^ k_swz<D>(r)) * 16, lds32 + buf * 2 * TILE + r0 * D * 2);
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int r0 = (wave * N + i) * RPI, r = r0 + lane / CH, key = min(j * kKeys + r, len - 1);
+            dma16(vb + (int64_t)key * a.v_row + ((lane % CH) ^ v_swz<D>(r)) * 16, lds32 + buf * 2 * TILE + TILE + r0 * D * 2);
+        }
+    };
+    const int steps = (min(len, q0 + BQ) + kKeys - 1) / kKeys;
+    const int mine = qw < len ? (min(len, qw + 32) + kKeys - 1) / kKeys : 0;  // steps with keys that this wave's rows see
+
+    f32x16_v o[DB];
+    float m, l;
+    for (bool careful = false;; careful = true) {
+        m = kNegInf;
+        l = 0.f;
+#pragma unroll
+        for (int d = 0; d < DB; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[d][e] = 0.f;
+        stage(0, 0);
+        for (int j = 0; j < steps; j++) {
+            // step j has landed everywhere, and every wave is done with the stage that step j + 1 goes to
+            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            if (j + 1 < steps) stage(j + 1, (j + 1) & 1);
+            if (j >= mine) continue;
+            const char* kt = lds + (j & 1) * 2 * TILE;
+            const char* vt = kt + TILE;
+            f32x16_v s[2];
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[x][e] = 0.f;
+                const int r = 32 * x + col;
+                const char* kr = kt + r * D * 2;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    const u32x4_v kf = *reinterpret_cast<const u32x4_v*>(kr + ((2 * ks + half) ^ k_swz<D>(r)) * 16);
+                    s[x] = T::mfma32(kf, q[ks], s[x]);
+                }
+            }
+            // a lane's scores: keys j 64 + 32 x + 8 (e / 4) + 4 half + e % 4 of its query
+            const bool masked = j * kKeys + kKeys - 1 > qw;
+            if (masked) {
+                const int first = j * kKeys + 4 * half - row;  // key - row of the lane's first score
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        if (first + 32 * x + 8 * (e / 4) + e % 4 > 0) s[x][e] = kNegInf;
+            }
+            float mx = kNegInf;
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[x][e]);
+            mx *= a.scale2;
+            if (__any(mx > m + kLazy)) {
+                const float top = fmaxf(m, max_over_halves(mx));
+                const float f0 = top == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m - top);
+                m = top;
+                l *= f0;
+#pragma unroll
+                for (int d = 0; d < DB; d++) o[d] *= f0;
+            }
+            const float base = m == kNegInf ? 0.f : m;
+            u32x4_v p[4];
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                    const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], a.scale2, -base));
+                    const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e + 1], a.scale2, -base));
+                    l += w0 + w1;
+                    p[2 * x + e / 8][e % 8 / 2] = T::pack(w0, w1);
+                }
+            // V^T's operand: 32 columns, 16 keys in the order of the scores: 4 half + (0 .. 3) and 8 more
+            const int vr = 4 * half + (lane & 15) / 4, vc = ((lane >> 4) & 1) * 2 + (lane & 3) / 2, sub = (lane & 1) * 8;
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    u32x4_v vf;
+#pragma unroll
+                    for (int z = 0; z < 2; z++) {
+                        const int r = 16 * y + 8 * z + vr;
+                        const char* at = vt + r * D * 2 + ((4 * d + vc) ^ v_swz<D>(r)) * 16 + sub;
+                        const s16x4_v w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_v*)at);
+                        const uint2 w2 = __builtin_bit_cast(uint2, w);
+                        vf[2 * z] = w2.x;
+                        vf[2 * z + 1] = w2.y;
+                    }
+                    if (careful && masked) {
+                        u32x4_v on;  // 1 where the row sees the key
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float s0 = s[y / 2][y % 2 * 8 + 2 * e], s1 = s[y / 2][y % 2 * 8 + 2 * e + 1];
+                            on[e] = (s0 != kNegInf ? T::kOne : 0u) | (s1 != kNegInf ? T::kOne << 16 : 0u);
+                        }
+                        add_kinds32<DT>(o[d], vf, on);
+                        vf = keep<DT, Keep::kFinite>(vf);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    o[d] = T::mfma32(vf, p[y], o[d]);
+                }
+            }
+        }
+        // A value that is not finite in a key that some rows of a step must not see makes those rows' sums NaN (0 times it).
+        // There are none in ordinary data; where sums are not finite the block runs again with such values kept apart.
+        float bad = 0.f;
+#pragma unroll
+        for (int d = 0; d < DB; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) bad = __builtin_fmaf(o[d][e], 0.f, bad);
+        // (also: every wave is done with the stages)
+        if (!__syncthreads_or(row < len && !(bad == 0.f)) || careful) break;
+    }
+
+    l = sum_over_halves(l);
+    if (row >= len) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    char* p = a.out + (int64_t)(c0 + row) * a.o_row + (int64_t)head * a.o_head + half * 8;
+#pragma unroll
+    for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            uint2 w;
+            w.x = T::pack(o[d][e] * inv, o[d][e + 1] * inv);
+            w.y = T::pack(o[d][e + 2] * inv, o[d][e + 3] * inv);
+            *reinterpret_cast<uint2*>(p + d * 64 + e * 4) = w;
+        }
+    if (a.lse && half == 0) a.lse[(int64_t)(c0 + row) * a.heads + head] = l == 0.f ? kNegInf : (m + log2f(l)) * kLn2;
+}
+
+template <int DT, int D, int W>
+void launch(const Args& a, hipStream_t st) {
+    constexpr int BQ = 32 * W;
+    const int64_t blocks = ((int64_t)a.t / BQ + a.nseq) * a.heads;
+    CHECK(blocks < (int64_t)1 << 31, "qe_attn_prompt: %lld blocks", (long long)blocks);
+    const int bytes = std::max(4 * kKeys * D * 2, a.nseq * 4);
+    if (bytes > 64 * 1024) {
+        static std::atomic<uint64_t> done{0};  // per device, one bit
+        int dev = 0;
+        HIP_CHECK(hipGetDevice(&dev));
+        if (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1)) {
+            HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(prompt_kernel<DT, D, W>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+            if (dev < 64) done.fetch_or(1ull << dev);
+        }
+    }
+    prompt_kernel<DT, D, W><<<(int)blocks, 64 * W, bytes, st>>>(a);
+    HIP_CHECK(hipGetLastError());
+}
+
+template <int DT>
+void by_shape(const Args& a, int d, hipStream_t st) {
+    if (d == 64) launch<DT, 64, 4>(a, st);
+    else if (d == 128) launch<DT, 128, 4>(a, st);
+    else launch<DT, 256, 8>(a, st);
+}
+}  // namespace qe_prompt
+
+void attn_prompt(const AttnPromptArgs& x, bool f16, hipStream_t st) {
+    CHECK(x.d == 64 || x.d == 128 || x.d == 256, "qe_attn_prompt: d %d (64, 128 or 256)", x.d);
+    CHECK(x.kv_heads >= 1 && x.heads >= x.kv_heads && x.heads % x.kv_heads == 0 && x.heads <= 65535, "qe_attn_prompt: %d heads over %d",
+          x.heads, x.kv_heads);
+    CHECK(x.nseq >= 0 && x.nseq <= qe_prompt::kMaxSeqs && x.t >= 0, "qe_attn_prompt: nseq %d (at most %d), t %d", x.nseq, qe_prompt::kMaxSeqs, x.t);
+    CHECK(x.scale > 0.f && x.scale < __builtin_huge_valf(), "qe_attn_prompt: scale %g", (double)x.scale);
+    if (x.nseq == 0 || x.t == 0) return;
+    CHECK(x.q && x.k && x.v && x.out && x.cu, "qe_attn_prompt: null pointer");
+    CHECK((((uintptr_t)x.q | (uintptr_t)x.k | (uintptr_t)x.v | (uintptr_t)x.out) & 15) == 0 &&
+              ((x.q_row | x.q_head | x.k_row | x.k_head | x.v_row | x.v_head | x.o_row | x.o_head) & 7) == 0,
+          "qe_attn_prompt: q, k, v and out must be 16-byte aligned with strides of 8 elements");
+    qe_prompt::Args a{(const char*)x.q, (const char*)x.k, (const char*)x.v, (char*)x.out, x.lse,
+                      2 * x.q_row, 2 * x.q_head, 2 * x.k_row, 2 * x.k_head, 2 * x.v_row, 2 * x.v_head, 2 * x.o_row, 2 * x.o_head,
+                      x.cu, x.nseq, x.t, x.heads, x.kv_heads, x.scale * kLog2e};
+    if (f16) qe_prompt::by_shape<kAttnF16>(a, x.d, st);
+    else qe_prompt::by_shape<kAttnBF16>(a, x.d, st);
+}

@@ -1,0 +1,541 @@
+// Attention of drafted tokens (one, a chain or a tree) over the paged cache.
+//
+//   o[i] = sum_j p_ij v[j],  p_ij = softmax over the tokens j that row i sees of scale q[i] . k[j]
+//
+// A sequence's rows of one kv head are its drafted tokens times the query heads of the group: few (1 to some hundred)
+// against thousands of keys, so the call is bound by reading keys and values once from HBM. Every wave takes 32 keys at a
+// time straight into registers (no LDS: nobody else needs them): K as the A operand of S^T = K Q^T as it lies in memory,
+// V's rows 16 bytes a lane, turned into the A operand of O^T = V^T P^T by 16-bit permutes inside the lane (8 keys x 8
+// columns: 32 permutes for 32 keys x 128 columns, hidden behind the loads). The next 32 keys are in flight meanwhile.
+//
+// Work is split over the tokens of all sequences evenly: unit = 128 tokens (32 a wave) of one (sequence, kv head, row
+// block); the units in that order are dealt to as many blocks as the device holds, in ranges of equal length, whatever the
+// sequences' lengths. A (sequence, head, row block) that ends up in several blocks leaves partial sums (fp32, with their
+// running maximum and sum) in a workspace, which a second launch joins in block order.
+#include "attn_common.hpp"
+#include "kv_cache.hpp"
+
+#include <algorithm>
+
+namespace qe_tree {
+constexpr int kThreads = 256, kWaves = 4, kUnit = 128;
+constexpr float kLazy = 8.f;  // the running maximum follows a row's scores once they pass it by this much (2^8 in the sums)
+
+struct Args {
+    const char *q, *k, *v;
+    char* out;
+    float* lse;
+    int64_t q_row, q_head, o_row, o_head, page, head, token;  // bytes
+    const int32_t *table, *length, *seqs, *cu;
+    const uint64_t* mask;
+    int nseq, t, max_new, heads, kv_heads, group, shift, pages, width, slots, rb_max;
+    float scale2;  // log2(e) times the scale: exponentials are powers of two
+    float* part;   // [block][2][rows][D] partial sums, nullptr: every block takes whole (sequence, head, row block)s
+    float2* ml;    // [block][2][rows] maximum and sum
+    int* ends;     // [nseq] end of each sequence's units, then the range length
+};
+
+struct Seq {
+    int first, n, len, total;  // first row, rows, committed tokens, all tokens
+    int slot;
+};
+__device__ __forceinline__ Seq seq_of(const Args& a, int b) {
+    Seq s;
+    const int c0 = a.cu[b], c1 = a.cu[b + 1];
+    s.first = min(max(c0, 0), a.t);
+    s.n = min(min(c1, a.t) - s.first, a.max_new);
+    s.slot = a.seqs[b];
+    const bool ok = s.slot >= 0 && s.slot < a.slots;
+    const int room = a.width << a.shift;
+    s.len = ok ? min(max(a.length[ok ? s.slot : 0], 0), room) : 0;
+    s.total = ok ? min(s.len + max(s.n, 0), room) : 0;
+    return s;
+}
+template <int ROWS>
+__device__ __forceinline__ int row_blocks(const Args& a, int n) {
+    return (n * a.group + ROWS - 1) / ROWS;
+}
+__device__ __forceinline__ int unit_count(int total) { return max(1, (total + kUnit - 1) / kUnit); }
+
+template <int D>
+struct Frag {  // 32 keys of a wave
+    static constexpr int KS = D / 32, VD = D / 32;  // 16-byte pieces of a key row per lane; dwords of a value row per lane
+    u32x4_v k[2][KS];
+    uint32_t v[8][VD];
+    bool ok[2];  // the half's page exists
+};
+
+template <int DT, int D, int NT>
+__global__ __launch_bounds__(kThreads, (NT * D <= 128 ? 2 : 1)) void tree_kernel(Args a) {
+    using T = AttnT<DT>;
+    using F = Frag<D>;
+    constexpr int ROWS = 16 * NT, KS = F::KS, VD = F::VD, DT16 = D / 16;
+    constexpr int PITCH = D + 4;
+    __shared__ float obuf[kWaves][16][PITCH];
+    __shared__ float2 mlbuf[kWaves][16];
+    __shared__ int ends[kMaxTreeBatch];
+    __shared__ int tmp[kWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, grp = lane >> 4;
+
+    int u = 0, u_end = 1, b = 0, range = 0;
+    if (a.part) {
+        int carry = 0;
+        for (int b0 = 0; b0 < a.nseq; b0 += kThreads) {
+            int x = 0;
+            if (b0 + tid < a.nseq) {
+                const Seq s = seq_of(a, b0 + tid);
+                if (s.n > 0) x = unit_count(s.total) * row_blocks<ROWS>(a, s.n) * a.kv_heads;
+            }
+#pragma unroll
+            for (int o = 1; o < 64; o *= 2) {
+                const int y = __shfl_up(x, o);
+                if (lane >= o) x += y;
+            }
+            __syncthreads();
+            if (lane == 63) tmp[wave] = x;
+            __syncthreads();
+            for (int w = 0; w < kWaves; w++) {
+                if (w < wave) x += tmp[w];
+            }
+            if (b0 + tid < a.nseq) ends[b0 + tid] = carry + x;
+            for (int w = 0; w < kWaves; w++) carry += tmp[w];
+        }
+        __syncthreads();
+        range = (carry + gridDim.x - 1) / gridDim.x;
+        if (blockIdx.x == 0) {
+            for (int i = tid; i < a.nseq; i += kThreads) a.ends[i] = ends[i];
+            if (tid == 0) a.ends[a.nseq] = range;
+        }
+        u = blockIdx.x * range;
+        u_end = min(carry, u + range);
+        if (u >= u_end) return;
+        int hi = a.nseq - 1;  // the sequence of the first unit
+        while (b < hi) {
+            const int mid = (b + hi) / 2;
+            if (ends[mid] > u) hi = mid;
+            else b = mid + 1;
+        }
+    } else {
+        b = blockIdx.x / (a.kv_heads * a.rb_max);
+    }
+
+    while (u < u_end) {
+        b = __builtin_amdgcn_readfirstlane(b);
+        const Seq s = seq_of(a, b);
+        if (s.n <= 0) {
+            if (!a.part) return;
+            b++;
+            continue;
+        }
+        const int units = unit_count(s.total), rbs = row_blocks<ROWS>(a, s.n);
+        int h, rb, t0, t1;
+        if (a.part) {
+            const int v = u - (b > 0 ? ends[b - 1] : 0);
+            t0 = v % units;
+            rb = v / units % rbs;
+            h = v / units / rbs;
+            t1 = min(units, t0 + u_end - u);
+        } else {
+            const int v = blockIdx.x % (a.kv_heads * a.rb_max);
+            h = v / a.rb_max;
+            rb = v % a.rb_max;
+            t0 = 0;
+            t1 = units;
+            if (rb >= rbs) return;
+        }
+        h = __builtin_amdgcn_readfirstlane(h);
+        rb = __builtin_amdgcn_readfirstlane(rb);
+        const int rows = s.n * a.group;  // row r: drafted token r / group, query head r % group of the kv head
+
+        // the rows' queries (B operand) and masks
+        u32x4_v q[NT][KS];
+        uint64_t see[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int r = rb * ROWS + nt * 16 + col;
+            const int rc = min(r, rows - 1), i = rc / a.group, g = rc % a.group;
+            const char* p = a.q + (int64_t)(s.first + i) * a.q_row + (int64_t)(h * a.group + g) * a.q_head + grp * 16;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) q[nt][ks] = *reinterpret_cast<const u32x4_v*>(p + ks * 64);
+            see[nt] = a.mask ? a.mask[s.first + i] : ~0ull >> (63 - i);
+        }
+        f32x4_v o[NT][DT16];
+        float m[NT], l[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            m[nt] = kNegInf;
+            l[nt] = 0.f;
+#pragma unroll
+            for (int t = 0; t < DT16; t++) o[nt][t] = f32x4_v{0.f, 0.f, 0.f, 0.f};
+        }
+
+        const int32_t* tab = a.table + (int64_t)s.slot * a.width;
+        const char* kh = a.k + (int64_t)h * a.head + col * a.token + grp * 16;
+        const char* vh = a.v + (int64_t)h * a.head + 4 * grp * a.token + col * (D == 64 ? 8 : 16);
+        const int pmask = (1 << a.shift) - 1;
+        auto page_at = [&](int tok) {  // -1: none
+            const int i = tok >> a.shift;
+            int pg = -1;
+            if (tok < s.total) pg = __builtin_amdgcn_readfirstlane(tab[i]);
+            return pg >= 0 && pg < a.pages ? pg : -1;
+        };
+        auto load = [&](F& f, int tb) {  // the 32 tokens from tb (a multiple of 32); pages are at least 16 tokens
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const int tok = tb + 16 * x, pg = page_at(tok);
+                f.ok[x] = pg >= 0;
+                const int64_t off = (int64_t)max(pg, 0) * a.page + (int64_t)(tok & pmask) * a.token;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) f.k[x][ks] = *reinterpret_cast<const u32x4_v*>(kh + off + ks * 64);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const char* p = vh + off + j * a.token;
+                    if constexpr (D == 64) {
+                        const uint2 w = *reinterpret_cast<const uint2*>(p);
+                        f.v[4 * x + j][0] = w.x;
+                        f.v[4 * x + j][1] = w.y;
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < VD / 4; c++) {
+                            const u32x4_v w = *reinterpret_cast<const u32x4_v*>(p + c * 256);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) f.v[4 * x + j][4 * c + e] = w[e];
+                        }
+                    }
+                }
+            }
+        };
+        // column block t of V^T: lane's column (its 16-byte piece of the rows, value t), 8 keys
+        auto vt = [&](const F& f, int t) {
+            u32x4_v r;
+#pragma unroll
+            for (int p = 0; p < 4; p++)
+                r[p] = __builtin_amdgcn_perm(f.v[2 * p + 1][t / 2], f.v[2 * p][t / 2], t % 2 ? 0x07060302u : 0x05040100u);
+            return r;
+        };
+        auto compute = [&](F& f, int tb) {
+            f32x4_v sc[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    sc[nt][x] = f32x4_v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int ks = 0; ks < KS; ks++) sc[nt][x] = T::mfma16(f.k[x][ks], q[nt][ks], sc[nt][x]);
+                }
+            const bool masked = tb + 32 > s.len || !f.ok[0] || !f.ok[1];
+            bool odd = false;  // a value that is not finite in a tile with a mask
+            if (masked) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int tok = tb + 16 * x + 4 * grp + e, j = tok - s.len;
+                            const bool on = f.ok[x] && (j < 0 || (tok < s.total && (see[nt] >> (j & 63) & 1)));
+                            // times the scale here: a negative one must not turn -inf around
+                            sc[nt][x][e] = on ? sc[nt][x][e] * a.scale2 : kNegInf;
+                        }
+#pragma unroll
+                for (int r = 0; r < 8; r++)
+#pragma unroll
+                    for (int e = 0; e < VD; e++) odd = odd || half_not_finite<DT>(f.v[r][e]);
+                odd = __any(odd);
+            } else {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int x = 0; x < 2; x++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) sc[nt][x][e] *= a.scale2;
+            }
+            u32x4_v p[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float mx = kNegInf;
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mx = fmaxf(mx, sc[nt][x][e]);
+                if (__any(mx > m[nt] + kLazy)) {
+                    const float top = fmaxf(m[nt], max_over_quarters(mx));
+                    const float f0 = top == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m[nt] - top);
+                    m[nt] = top;
+                    l[nt] *= f0;
+#pragma unroll
+                    for (int t = 0; t < DT16; t++) o[nt][t] *= f0;
+                }
+                const float base = m[nt] == kNegInf ? 0.f : m[nt];
+                float w[8];
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        w[4 * x + e] = __builtin_amdgcn_exp2f(sc[nt][x][e] - base);
+                        l[nt] += w[4 * x + e];
+                    }
+#pragma unroll
+                for (int e = 0; e < 4; e++) p[nt][e] = T::pack(w[2 * e], w[2 * e + 1]);
+            }
+            if (odd) {  // out of the ordinary: what is not finite goes to the sums by itself, zeros take its place
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    u32x4_v on;  // 1 where the row sees the key
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        on[e] = (sc[nt][e / 2][e % 2 * 2] != kNegInf ? T::kOne : 0u) | (sc[nt][e / 2][e % 2 * 2 + 1] != kNegInf ? T::kOne << 16 : 0u);
+#pragma unroll
+                    for (int t = 0; t < DT16; t++) {
+                        add_kinds<DT>(o[nt][t], vt(f, t), on);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 8; r++)
+#pragma unroll
+                    for (int e = 0; e < VD; e++) f.v[r][e] = keep_two<DT, Keep::kFinite>(f.v[r][e]);
+            }
+#pragma unroll
+            for (int t = 0; t < DT16; t++) {
+                const u32x4_v v = vt(f, t);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) o[nt][t] = T::mfma16(v, p[nt], o[nt][t]);
+            }
+        };
+
+        // this wave's tokens: 32 of each unit; where the registers allow it the next 32 are on their way meanwhile
+        const int stop = min(t1 * kUnit, s.total);
+        int tb = t0 * kUnit + wave * 32;
+        if (tb < stop) {
+            F f;
+            if constexpr (NT * D <= 256) {
+                load(f, tb);
+                for (; tb < stop; tb += kUnit) {
+                    F next;
+                    load(next, tb + kUnit < stop ? tb + kUnit : tb);
+                    compute(f, tb);
+                    f = next;
+                }
+            } else {
+                for (; tb < stop; tb += kUnit) {
+                    load(f, tb);
+                    compute(f, tb);
+                }
+            }
+        }
+
+        // join the four waves, 16 rows at a time
+        const bool whole = t0 == 0 && t1 == units;
+        const int64_t pslot = ((int64_t)blockIdx.x * 2 + (t0 > 0 ? 0 : 1)) * ROWS;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            l[nt] = sum_over_quarters(l[nt]);
+            __syncthreads();
+            if (lane < 16) mlbuf[wave][col] = make_float2(m[nt], l[nt]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                // lane's columns: piece 4 grp + e of 8 (4 for D = 64) columns, 128 further on for the next pieces
+#pragma unroll
+                for (int t = 0; t < DT16; t += 4) {
+                    const int d = D == 64 ? 4 * (4 * grp + e) : 8 * (4 * grp + e) + t % 8 + t / 8 * 128;
+                    float4 w = make_float4(o[nt][t][e], o[nt][t + 1][e], o[nt][t + 2][e], o[nt][t + 3][e]);
+                    *reinterpret_cast<float4*>(&obuf[wave][col][d]) = w;
+                }
+            }
+            __syncthreads();
+            const int row = tid >> 4, c0 = (tid & 15) * (D / 16), r = rb * ROWS + nt * 16 + row;
+            float top = kNegInf, sum = 0.f, f[kWaves];
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) top = fmaxf(top, mlbuf[w][row].x);
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) {
+                const float2 x = mlbuf[w][row];
+                f[w] = x.x == kNegInf ? 0.f : __builtin_amdgcn_exp2f(x.x - top);
+                if (x.x == __builtin_huge_valf()) f[w] = 1.f;  // the row's sums are NaN already
+                sum += f[w] * x.y;
+            }
+            float y[D / 16];
+#pragma unroll
+            for (int d = 0; d < D / 16; d += 4) {
+                float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kWaves; w++) {
+                    const float4 x = *reinterpret_cast<const float4*>(&obuf[w][row][c0 + d]);
+                    z.x += f[w] * x.x;
+                    z.y += f[w] * x.y;
+                    z.z += f[w] * x.z;
+                    z.w += f[w] * x.w;
+                }
+                y[d] = z.x;
+                y[d + 1] = z.y;
+                y[d + 2] = z.z;
+                y[d + 3] = z.w;
+            }
+            if (r >= rows) continue;
+            if (whole) {
+                const int i = r / a.group, hq = h * a.group + r % a.group;
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                char* p = a.out + (int64_t)(s.first + i) * a.o_row + (int64_t)hq * a.o_head + c0 * 2;
+#pragma unroll
+                for (int d = 0; d < D / 16; d += 4) {
+                    uint2 w;
+                    w.x = T::pack(y[d] * inv, y[d + 1] * inv);
+                    w.y = T::pack(y[d + 2] * inv, y[d + 3] * inv);
+                    *reinterpret_cast<uint2*>(p + d * 2) = w;
+                }
+                if (a.lse && (tid & 15) == 0) a.lse[(int64_t)(s.first + i) * a.heads + hq] = sum == 0.f ? kNegInf : (top + log2f(sum)) * kLn2;
+            } else {
+                float* p = a.part + (pslot + nt * 16 + row) * D + c0;
+#pragma unroll
+                for (int d = 0; d < D / 16; d += 4) *reinterpret_cast<float4*>(p + d) = make_float4(y[d], y[d + 1], y[d + 2], y[d + 3]);
+                if ((tid & 15) == 0) a.ml[pslot + nt * 16 + row] = make_float2(top, sum);
+            }
+        }
+        u += t1 - t0;
+        if (a.part && u >= ends[b]) b++;
+    }
+}
+
+// Joins the parts of one row: block (row, kv head, sequence). Four waves take every fourth part; sums in a fixed order.
+template <int DT, int D, int NT>
+__global__ __launch_bounds__(kThreads) void join_kernel(Args a, int most) {
+    using T = AttnT<DT>;
+    constexpr int ROWS = 16 * NT, E = D / 64;
+    const int r = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int c0 = a.cu[b], first = min(max(c0, 0), a.t), n = min(min(a.cu[b + 1], a.t) - first, a.max_new);
+    if (r >= n * a.group) return;
+    const int u0 = b > 0 ? a.ends[b - 1] : 0, range = a.ends[a.nseq], rbs = row_blocks<ROWS>(a, n), rb = r / ROWS;
+    const int units = (a.ends[b] - u0) / (rbs * a.kv_heads);
+    const int v0 = u0 + (h * rbs + rb) * units, w0 = v0 / range, w1 = (v0 + units - 1) / range, cnt = w1 - w0 + 1;
+    if (cnt == 1) return;
+    extern __shared__ float wgt[];  // [most] weights, then the waves' sums
+    float* acc = wgt + most;
+    __shared__ float red[2][kWaves];
+    auto at = [&](int i) { return ((int64_t)(w0 + i) * 2 + (i > 0 ? 0 : 1)) * ROWS + r % ROWS; };
+    float top = kNegInf;
+    for (int i = tid; i < cnt; i += kThreads) top = fmaxf(top, a.ml[at(i)].x);
+#pragma unroll
+    for (int o = 32; o; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
+    if (lane == 0) red[0][wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) top = fmaxf(top, red[0][w]);
+    float sum = 0.f;
+    for (int i = tid; i < cnt; i += kThreads) {
+        const float2 x = a.ml[at(i)];
+        float f = x.x == kNegInf ? 0.f : __builtin_amdgcn_exp2f(x.x - top);
+        if (x.x == __builtin_huge_valf()) f = 1.f;
+        wgt[i] = f;
+        sum += f * x.y;
+    }
+#pragma unroll
+    for (int o = 32; o; o /= 2) sum += __shfl_xor(sum, o);
+    if (lane == 0) red[1][wave] = sum;
+    __syncthreads();
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) sum += red[1][w];
+    float y[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) y[e] = 0.f;
+#pragma unroll 4
+    for (int i = wave; i < cnt; i += kWaves) {
+        const float f = wgt[i];
+        const float* p = a.part + at(i) * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e++) y[e] += f * p[e];
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) acc[wave * D + lane * E + e] = y[e];
+    __syncthreads();
+    const int i = r / a.group, hq = h * a.group + r % a.group;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (tid < D / 2) {
+        float z0 = 0.f, z1 = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            z0 += acc[w * D + 2 * tid];
+            z1 += acc[w * D + 2 * tid + 1];
+        }
+        *reinterpret_cast<uint32_t*>(a.out + (int64_t)(first + i) * a.o_row + (int64_t)hq * a.o_head + 4 * tid) = T::pack(z0 * inv, z1 * inv);
+    }
+    if (a.lse && tid == 0) a.lse[(int64_t)(first + i) * a.heads + hq] = sum == 0.f ? kNegInf : (top + log2f(sum)) * kLn2;
+}
+
+template <int DT, int D, int NT>
+void launch(Args a, hipStream_t st) {
+    constexpr int ROWS = 16 * NT;
+    a.rb_max = (a.max_new * a.group + ROWS - 1) / ROWS;
+    const int64_t runs = (int64_t)a.nseq * a.kv_heads * a.rb_max;
+    const int64_t most_units = ((int64_t)(a.width << a.shift) + kUnit - 1) / kUnit;
+    CHECK(runs * most_units < (int64_t)1 << 31, "qe_attn_tree: %lld rows x %lld units of tokens", (long long)runs, (long long)most_units);
+    const int grid = (int)std::min<int64_t>(runs * most_units, (NT * D <= 128 ? 2 : 1) * qe_num_cus());
+    const size_t part = (size_t)grid * 2 * ROWS * D * 4, ml = (size_t)grid * 2 * ROWS * 8, ends = ((size_t)a.nseq + 1) * 4;
+    WsHold hold(st);
+    if (char* ws = static_cast<char*>(hold.get(kWsAttn, part + ml + ends))) {
+        a.part = reinterpret_cast<float*>(ws);
+        a.ml = reinterpret_cast<float2*>(ws + part);
+        a.ends = reinterpret_cast<int*>(ws + part + ml);
+        tree_kernel<DT, D, NT><<<grid, kThreads, 0, st>>>(a);
+        HIP_CHECK(hipGetLastError());
+        join_kernel<DT, D, NT><<<dim3(a.max_new * a.group, a.kv_heads, a.nseq), kThreads, (grid + kWaves * D) * 4, st>>>(a, grid);
+    } else {
+        CHECK(runs < (int64_t)1 << 31, "qe_attn_tree: %lld blocks", (long long)runs);
+        tree_kernel<DT, D, NT><<<(int)runs, kThreads, 0, st>>>(a);
+    }
+    HIP_CHECK(hipGetLastError());
+}
+
+template <int DT>
+void by_shape(const Args& a, int d, hipStream_t st) {
+    const int rows = a.max_new * a.group;
+    if (d == 64) rows <= 16 ? launch<DT, 64, 1>(a, st) : rows <= 32 ? launch<DT, 64, 2>(a, st) : launch<DT, 64, 4>(a, st);
+    else if (d == 128) rows <= 16 ? launch<DT, 128, 1>(a, st) : rows <= 32 ? launch<DT, 128, 2>(a, st) : launch<DT, 128, 4>(a, st);
+    else rows <= 16 ? launch<DT, 256, 1>(a, st) : launch<DT, 256, 2>(a, st);
+}
+}  // namespace qe_tree
+
+void attn_tree(const qe_kv_cache_t& c, int layer, const AttnTreeArgs& x, hipStream_t st) {
+    CHECK(layer >= 0 && layer < c.layers, "qe_attn_tree: layer %d of %d", layer, c.layers);
+    CHECK(x.nseq >= 0 && x.nseq <= kMaxTreeBatch, "qe_attn_tree: nseq = %d (at most %d)", x.nseq, kMaxTreeBatch);
+    CHECK(x.t >= 0 && x.max_new >= 1 && x.max_new <= kMaxTreeNodes, "qe_attn_tree: t = %d, max_new = %d (1 .. %d)", x.t, x.max_new, kMaxTreeNodes);
+    CHECK(x.scale > 0.f && x.scale < __builtin_huge_valf(), "qe_attn_tree: scale %g", (double)x.scale);
+    CHECK(x.heads >= c.kv_heads && x.heads % c.kv_heads == 0 && x.heads <= 65535, "qe_attn_tree: %d heads over %d", x.heads, c.kv_heads);
+    if (x.nseq == 0 || x.t == 0) return;
+    CHECK(x.q && x.out && x.seqs && x.cu, "qe_attn_tree: null pointer");
+    CHECK((((uintptr_t)x.q | (uintptr_t)x.out) & 15) == 0 && ((x.q_row | x.q_head | x.o_row | x.o_head) & 7) == 0,
+          "qe_attn_tree: q and out must be 16-byte aligned with strides of 8 elements");
+    qe_tree::Args a{};
+    a.q = (const char*)x.q;
+    a.k = (const char*)c.k + 2 * (int64_t)layer * c.layer_stride;
+    a.v = (const char*)c.v + 2 * (int64_t)layer * c.layer_stride;
+    a.out = (char*)x.out;
+    a.lse = x.lse;
+    a.q_row = 2 * x.q_row;
+    a.q_head = 2 * x.q_head;
+    a.o_row = 2 * x.o_row;
+    a.o_head = 2 * x.o_head;
+    a.page = 2 * c.page_stride;
+    a.head = 2 * c.head_stride;
+    a.token = 2 * c.token_stride;
+    a.table = c.table;
+    a.length = c.length;
+    a.seqs = x.seqs;
+    a.cu = x.cu;
+    a.mask = x.mask;
+    a.nseq = x.nseq;
+    a.t = x.t;
+    a.max_new = x.max_new;
+    a.heads = x.heads;
+    a.kv_heads = c.kv_heads;
+    a.group = x.heads / c.kv_heads;
+    a.shift = log2_of(c.page);
+    a.pages = c.pages;
+    a.width = c.width;
+    a.slots = c.slots;
+    a.scale2 = x.scale * kLog2e;
+    if (c.f16) qe_tree::by_shape<kAttnF16>(a, c.d, st);
+    else qe_tree::by_shape<kAttnBF16>(a, c.d, st);
+}

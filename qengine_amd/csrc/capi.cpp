@@ -4,6 +4,7 @@
 // Build-defined *_ex entry points take an explicit stream, row strides and flags (QeFlags).
 #include "qe_api.hpp"
 #include "gemm_tune.hpp"
+#include "kv_cache.hpp"
 #include "../../include/qe_kernels.h"
 
 #include <algorithm>
@@ -369,6 +370,51 @@ void qe_rows8(const void* q, const void* s, int n, int k, int flags, const uint1
             gemv_w8(w, x + (size_t)r0 * ldx, ldx, y + (size_t)r0 * ldy, ldy, std::min(kMaxGemvRows, m - r0), false,
                     as_stream(st));
     }
+}
+
+// ---------------------------------------------------------------- attention and the paged cache
+void qe_attn_prompt(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
+                    int64_t v_row, int64_t v_head, void* out, int64_t out_row, int64_t out_head, float* lse,
+                    const int32_t* cu, int nseq, int t, int heads, int kv_heads, int d, float scale, int flags, void* st) {
+    attn_prompt({q, k, v, out, lse, q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head, cu, nseq, t, heads, kv_heads,
+                 d, scale},
+                (flags & QE_F16) != 0, as_stream(st));
+}
+
+void qe_kv_reserve(const qe_kv_cache_t* cache, const int32_t* seqs, const int32_t* add, int n, int32_t* ok, int32_t* copies,
+                   void* st) {
+    kv_check(cache, "qe_kv_reserve");
+    kv_reserve(*cache, seqs, add, n, ok, copies, as_stream(st));
+}
+
+void qe_kv_fork(const qe_kv_cache_t* cache, const int32_t* parents, const int32_t* children, int n, int32_t* ok, void* st) {
+    kv_check(cache, "qe_kv_fork");
+    kv_fork(*cache, parents, children, n, ok, as_stream(st));
+}
+
+void qe_kv_release(const qe_kv_cache_t* cache, const int32_t* seqs, const int32_t* lengths, int n, void* st) {
+    kv_check(cache, "qe_kv_release");
+    kv_release(*cache, seqs, lengths, n, as_stream(st));
+}
+
+void qe_kv_append(const qe_kv_cache_t* cache, int layer, int layers, const void* k, const void* v, const int64_t* strides,
+                  const int32_t* seqs, const int32_t* cu, int nseq, int t, void* st) {
+    kv_check(cache, "qe_kv_append");
+    kv_append(*cache, layer, layers, k, v, strides, seqs, cu, nseq, t, as_stream(st));
+}
+
+void qe_kv_accept(const qe_kv_cache_t* cache, const int32_t* seqs, const int32_t* count, const int32_t* path, int most, int n,
+                  int32_t* length_out, void* st) {
+    kv_check(cache, "qe_kv_accept");
+    kv_accept(*cache, seqs, count, path, most, n, length_out, as_stream(st));
+}
+
+void qe_attn_tree(const qe_kv_cache_t* cache, int layer, const void* q, int64_t q_row, int64_t q_head, void* out,
+                  int64_t out_row, int64_t out_head, float* lse, const int32_t* seqs, const int32_t* cu, int nseq, int t,
+                  int max_new, const uint64_t* mask, int heads, float scale, void* st) {
+    kv_check(cache, "qe_attn_tree");
+    attn_tree(*cache, layer, {q, out, lse, q_row, q_head, out_row, out_head, seqs, cu, nseq, t, max_new, mask, heads, scale},
+              as_stream(st));
 }
 
 }  // extern "C"

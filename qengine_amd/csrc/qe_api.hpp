@@ -104,7 +104,7 @@ void qe_config_set(const QeConfig& c);
 void gemv_w8(const W8& w, const uint16_t* x, int ldx, void* y, int ldy, int m, bool out_bf16, hipStream_t st);
 
 // ---- library-owned workspaces, one per (kind, device, stream) (workspace.cpp) ----
-enum WsKind : int { kWsSplit = 0, kWsI8 = 1, kWsH = 2, kWsDec = 3, kWsSkinny = 4, kNumWs = 5 };
+enum WsKind : int { kWsSplit = 0, kWsI8 = 1, kWsH = 2, kWsDec = 3, kWsSkinny = 4, kWsAttn = 5, kNumWs = 6 };
 struct StreamWs;
 // A call's hold on its stream's workspaces: made before the first buffer is asked for and kept until the last launch
 // that uses one, so that no other host thread's launches on the stream come in between.

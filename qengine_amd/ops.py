@@ -471,3 +471,7 @@ class SafeTensorsFile:
         self._lib.qe_load_w4(self.h, names, r0, r1, len(rows), c0, c1, int(glu), ctypes.c_void_p(dq.data_ptr()),
                              ctypes.c_void_p(ds.data_ptr()), _stream())
         return Q8(dq, ds, n, k, glu) if bits == 8 else W4(dq, ds, n, k, glu)
+
+
+# ---------------------------------------------------------------- attention and the paged cache
+from .attention import KVCache, attn_prompt  # noqa: E402,F401
