@@ -61,73 +61,35 @@ __device__ __forceinline__ float sum_over_quarters(float x) {
 }
 
 // ---- values that are not finite in keys that some rows of a tile must not see
-// A masked key has weight 0, but 0 times an infinity or a NaN in the matrix product is NaN. Tiles with a mask therefore
-// look for such values (a vote; there are none in ordinary data), put zeros in their place, and add to each row what the
-// keys that it does see contribute: products of indicators on the matrix cores, which say whether a row sees a +inf, a
-// -inf or a NaN in a column.
+// A masked key has weight 0, but 0 times an infinity or a NaN in the matrix product is NaN. Kernels whose sums come out not
+// finite therefore run again, first over the finite values alone (pass 1: zeros in the others' place), then once for each
+// kind of the others with ones in their place and weight 1 where a row sees a key: where such a sum is positive the row sees
+// a +inf (pass 2), a -inf (3) or a NaN (4) in that column.
+constexpr int kKinds = 4;
 template <int DT>
-__device__ __forceinline__ bool half_not_finite(uint32_t two) {  // either 16-bit value of the pair
-    constexpr uint32_t E = AttnT<DT>::kExpMask;
-    return (two & E) == E || ((two >> 16) & E) == E;
-}
-template <int DT>
-__device__ __forceinline__ bool any_not_finite(u32x4_v v) {
-    return half_not_finite<DT>(v[0]) || half_not_finite<DT>(v[1]) || half_not_finite<DT>(v[2]) || half_not_finite<DT>(v[3]);
-}
-enum class Keep { kFinite, kPosInf, kNegInf, kNan };
-// the finite values with zeros elsewhere, or ones (in the type's own bits) where a value is of the asked kind
-template <int DT, Keep K>
-__device__ __forceinline__ uint32_t keep_half(uint32_t h) {
-    constexpr uint32_t E = AttnT<DT>::kExpMask;
-    if constexpr (K == Keep::kFinite) return (h & E) == E ? 0u : h;
-    bool is = false;
-    if constexpr (K == Keep::kPosInf) is = h == AttnT<DT>::kInf;
-    if constexpr (K == Keep::kNegInf) is = h == (AttnT<DT>::kInf | 0x8000u);
-    if constexpr (K == Keep::kNan) is = (h & 0x7fffu) > AttnT<DT>::kInf;
+__device__ __forceinline__ uint32_t keep_half(uint32_t h, int pass) {
+    constexpr uint32_t E = AttnT<DT>::kExpMask, I = AttnT<DT>::kInf;
+    if (pass == 1) return (h & E) == E ? 0u : h;
+    const bool is = pass == 2 ? h == I : pass == 3 ? h == (I | 0x8000u) : (h & 0x7fffu) > I;
     return is ? AttnT<DT>::kOne : 0u;
 }
-template <int DT, Keep K>
-__device__ __forceinline__ uint32_t keep_two(uint32_t w) {
-    return keep_half<DT, K>(w & 0xffffu) | keep_half<DT, K>(w >> 16) << 16;
-}
-template <int DT, Keep K>
-__device__ __forceinline__ u32x4_v keep(u32x4_v v) {
-    u32x4_v r;
-#pragma unroll
-    for (int i = 0; i < 4; i++) r[i] = keep_two<DT, K>(v[i]);
-    return r;
-}
-// the same for 32 columns x 16 keys
 template <int DT>
-__device__ __forceinline__ void add_kinds32(f32x16_v& o, u32x4_v v, u32x4_v on) {
-    f32x16_v zero;
-#pragma unroll
-    for (int e = 0; e < 16; e++) zero[e] = 0.f;
-    f32x16_v n = AttnT<DT>::mfma32(keep<DT, Keep::kPosInf>(v), on, zero);
-#pragma unroll
-    for (int e = 0; e < 16; e++)
-        if (n[e] > 0.f) o[e] += __builtin_huge_valf();
-    n = AttnT<DT>::mfma32(keep<DT, Keep::kNegInf>(v), on, zero);
-#pragma unroll
-    for (int e = 0; e < 16; e++)
-        if (n[e] > 0.f) o[e] -= __builtin_huge_valf();
-    n = AttnT<DT>::mfma32(keep<DT, Keep::kNan>(v), on, zero);
-#pragma unroll
-    for (int e = 0; e < 16; e++)
-        if (n[e] > 0.f) o[e] = __builtin_nanf("");
+__device__ __forceinline__ uint32_t keep_two(uint32_t w, int pass) {
+    return keep_half<DT>(w & 0xffffu, pass) | keep_half<DT>(w >> 16, pass) << 16;
 }
-// v: 16 columns x 32 keys of V^T (A operand), on: 1 where a row sees a key (B operand); o: the rows' sums of those columns
 template <int DT>
-__device__ __forceinline__ void add_kinds(f32x4_v& o, u32x4_v v, u32x4_v on) {
-    const f32x4_v zero = {0.f, 0.f, 0.f, 0.f};
-    const f32x4_v pos = AttnT<DT>::mfma16(keep<DT, Keep::kPosInf>(v), on, zero);
-    const f32x4_v neg = AttnT<DT>::mfma16(keep<DT, Keep::kNegInf>(v), on, zero);
-    const f32x4_v nan = AttnT<DT>::mfma16(keep<DT, Keep::kNan>(v), on, zero);
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        float y = o[e];
-        if (pos[e] > 0.f) y += __builtin_huge_valf();
-        if (neg[e] > 0.f) y -= __builtin_huge_valf();
-        o[e] = nan[e] > 0.f ? __builtin_nanf("") : y;
+__device__ __forceinline__ void keep_tile(char* tile, int bytes, int pass, int tid, int threads) {
+    for (int i = tid * 4; i < bytes; i += threads * 4) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(tile + i);
+        *w = keep_two<DT>(*w, pass);
     }
+}
+// an output (in the type's bits) where the row sees a value of the pass's kind; the order of the passes makes +inf - inf NaN
+template <int DT>
+__device__ __forceinline__ uint16_t add_kind(uint16_t o, int pass) {
+    constexpr uint32_t I = AttnT<DT>::kInf, N = I | 0x40u;
+    const bool nan = (o & 0x7fffu) > I;
+    if (pass == 2) return nan ? N : I;
+    if (pass == 3) return nan || o == I ? N : (I | 0x8000u);
+    return N;
 }

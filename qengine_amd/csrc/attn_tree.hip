@@ -162,13 +162,7 @@ __global__ __launch_bounds__(kThreads, (NT * D <= 128 ? 2 : 1)) void tree_kernel
         }
         f32x4_v o[NT][DT16];
         float m[NT], l[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            m[nt] = kNegInf;
-            l[nt] = 0.f;
-#pragma unroll
-            for (int t = 0; t < DT16; t++) o[nt][t] = f32x4_v{0.f, 0.f, 0.f, 0.f};
-        }
+        int pass = 0;
 
         const int32_t* tab = a.table + (int64_t)s.slot * a.width;
         const char* kh = a.k + (int64_t)h * a.head + col * a.token + grp * 16;
@@ -225,7 +219,6 @@ __global__ __launch_bounds__(kThreads, (NT * D <= 128 ? 2 : 1)) void tree_kernel
                     for (int ks = 0; ks < KS; ks++) sc[nt][x] = T::mfma16(f.k[x][ks], q[nt][ks], sc[nt][x]);
                 }
             const bool masked = tb + 32 > s.len || !f.ok[0] || !f.ok[1];
-            bool odd = false;  // a value that is not finite in a tile with a mask
             if (masked) {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
@@ -238,11 +231,6 @@ __global__ __launch_bounds__(kThreads, (NT * D <= 128 ? 2 : 1)) void tree_kernel
                             // times the scale here: a negative one must not turn -inf around
                             sc[nt][x][e] = on ? sc[nt][x][e] * a.scale2 : kNegInf;
                         }
-#pragma unroll
-                for (int r = 0; r < 8; r++)
-#pragma unroll
-                    for (int e = 0; e < VD; e++) odd = odd || half_not_finite<DT>(f.v[r][e]);
-                odd = __any(odd);
             } else {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
@@ -261,7 +249,7 @@ __global__ __launch_bounds__(kThreads, (NT * D <= 128 ? 2 : 1)) void tree_kernel
                     for (int e = 0; e < 4; e++) mx = fmaxf(mx, sc[nt][x][e]);
                 if (__any(mx > m[nt] + kLazy)) {
                     const float top = fmaxf(m[nt], max_over_quarters(mx));
-                    const float f0 = top == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m[nt] - top);
+                    const float f0 = top == kNegInf || pass > 1 ? 1.f : __builtin_amdgcn_exp2f(m[nt] - top);
                     m[nt] = top;
                     l[nt] *= f0;
 #pragma unroll
@@ -279,23 +267,18 @@ __global__ __launch_bounds__(kThreads, (NT * D <= 128 ? 2 : 1)) void tree_kernel
 #pragma unroll
                 for (int e = 0; e < 4; e++) p[nt][e] = T::pack(w[2 * e], w[2 * e + 1]);
             }
-            if (odd) {  // out of the ordinary: what is not finite goes to the sums by itself, zeros take its place
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    u32x4_v on;  // 1 where the row sees the key
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        on[e] = (sc[nt][e / 2][e % 2 * 2] != kNegInf ? T::kOne : 0u) | (sc[nt][e / 2][e % 2 * 2 + 1] != kNegInf ? T::kOne << 16 : 0u);
-#pragma unroll
-                    for (int t = 0; t < DT16; t++) {
-                        add_kinds<DT>(o[nt][t], vt(f, t), on);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
+            if (pass) {
 #pragma unroll
                 for (int r = 0; r < 8; r++)
 #pragma unroll
-                    for (int e = 0; e < VD; e++) f.v[r][e] = keep_two<DT, Keep::kFinite>(f.v[r][e]);
+                    for (int e = 0; e < VD; e++) f.v[r][e] = keep_two<DT>(f.v[r][e], pass);
+                if (pass > 1)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            p[nt][e] = (sc[nt][e / 2][e % 2 * 2] != kNegInf ? T::kOne : 0u) |
+                                       (sc[nt][e / 2][e % 2 * 2 + 1] != kNegInf ? T::kOne << 16 : 0u);
             }
 #pragma unroll
             for (int t = 0; t < DT16; t++) {
@@ -307,22 +290,68 @@ __global__ __launch_bounds__(kThreads, (NT * D <= 128 ? 2 : 1)) void tree_kernel
 
         // this wave's tokens: 32 of each unit; where the registers allow it the next 32 are on their way meanwhile
         const int stop = min(t1 * kUnit, s.total);
-        int tb = t0 * kUnit + wave * 32;
-        if (tb < stop) {
-            F f;
-            if constexpr (NT * D <= 256) {
-                load(f, tb);
-                for (; tb < stop; tb += kUnit) {
-                    F next;
-                    load(next, tb + kUnit < stop ? tb + kUnit : tb);
-                    compute(f, tb);
-                    f = next;
-                }
-            } else {
-                for (; tb < stop; tb += kUnit) {
+        uint32_t kinds[3][NT][(DT16 * 4 + 31) / 32];  // bit: the wave's row sees a +inf, -inf, NaN in the column
+        for (;;) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                m[nt] = kNegInf;
+                l[nt] = 0.f;
+#pragma unroll
+                for (int t = 0; t < DT16; t++) o[nt][t] = f32x4_v{0.f, 0.f, 0.f, 0.f};
+            }
+            int tb = t0 * kUnit + wave * 32;
+            if (tb < stop) {
+                F f;
+                if constexpr (NT * D <= 256) {
                     load(f, tb);
-                    compute(f, tb);
+                    for (; tb < stop; tb += kUnit) {
+                        F next;
+                        load(next, tb + kUnit < stop ? tb + kUnit : tb);
+                        compute(f, tb);
+                        f = next;
+                    }
+                } else {
+                    for (; tb < stop; tb += kUnit) {
+                        load(f, tb);
+                        compute(f, tb);
+                    }
                 }
+            }
+            if (pass == 0) {
+                float bad = 0.f;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int t = 0; t < DT16; t++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) bad = __builtin_fmaf(o[nt][t][e], 0.f, bad);
+                if (!__any(!(bad == 0.f))) break;
+                pass = 2;
+            } else if (pass > 1) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int w = 0; w < (DT16 * 4 + 31) / 32; w++) {
+                        uint32_t bits = 0;
+#pragma unroll
+                        for (int i = 32 * w; i < 32 * w + 32 && i < DT16 * 4; i++) bits |= o[nt][i / 4][i % 4] > 0.f ? 1u << (i % 32) : 0u;
+                        if (pass == 2) kinds[0][nt][w] = bits;
+                        else if (pass == 3) kinds[1][nt][w] = bits;
+                        else kinds[2][nt][w] = bits;
+                    }
+                pass = pass == kKinds ? 1 : pass + 1;
+            } else {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int i = 0; i < DT16 * 4; i++) {
+                        float y = o[nt][i / 4][i % 4];
+                        const uint32_t bit = 1u << (i % 32);
+                        if (kinds[0][nt][i / 32] & bit) y += __builtin_huge_valf();
+                        if (kinds[1][nt][i / 32] & bit) y -= __builtin_huge_valf();
+                        o[nt][i / 4][i % 4] = kinds[2][nt][i / 32] & bit ? __builtin_nanf("") : y;
+                    }
+                break;
             }
         }
 
