@@ -28,108 +28,114 @@ MAX_NODES = 64
 MAX_BATCH = 1024
 HEAD_DIMS = (64, 128, 256)
 
+MAX_SEQS = 4096
+_TYPES = (torch.bfloat16, torch.float16)
 _FN = {}
+_current = torch._C._cuda_getDevice
+_stream_of = torch._C._cuda_getCurrentRawStream
 
 
-def _fn(name, sig):
+def _run(at, name, sig, *args):
+    """the call on the current stream of the tensors' device `at`, which need not be the current one"""
+    if at < 0:
+        raise ValueError("tensors are on a GPU")
     f = _FN.get(name)
     if f is None:
         f = _FN[name] = typed(name, sig)
-    return f
-
-
-def _run(device, name, sig, *args):
-    """the call on the current stream of the tensors' device, which need not be the current one"""
-    if device.type != "cuda":
-        raise ValueError(f"tensors are on a GPU, got {device}")
-    i = device.index
-    if i is None or i == torch._C._cuda_getDevice():
-        _fn(name, sig)(*args, torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+    if at == _current():
+        f(*args, _stream_of(at))
         return
-    with torch.cuda.device(i):
-        _fn(name, sig)(*args, torch._C._cuda_getCurrentRawStream(i))
+    with torch.cuda.device(at):
+        f(*args, _stream_of(at))
 
 
-def _rows(name, t, dims, dtype, device):
+# Decode loops call these wrappers for every layer and token, so the checks below read few attributes: devices are compared
+# as numbers (-1: CPU), and each tensor's stride is asked for once.
+def _rows(name, t, dims, dtype, at):
     """a [.., d] tensor that the kernels can read: its type, place and strides"""
-    if t.dim() != dims:
-        raise ValueError(f"{name} has {dims} dimensions, got shape {tuple(t.shape)}")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name} is {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {device}, got {t.device}")
-    if t.numel():
-        if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:-1]):
-            raise ValueError(f"{name}: a row's values lie together and its other strides are multiples of 8, got {t.stride()}")
-        if t.data_ptr() % 16:
-            raise ValueError(f"{name} is 16-byte aligned")
+    s = t.stride()
+    if len(s) != dims:
+        raise ValueError(f"{name} has {dims} dimensions, got shape {tuple(t.shape)}")
+    if t.get_device() != at:
+        raise ValueError(f"{name} is on another device than the other tensors: {t.device}")
+    if s[-1] != 1 or (s[0] | s[1]) & 7 or (dims > 3 and any(x & 7 for x in s[2:-1])):
+        if t.numel():
+            raise ValueError(f"{name}: a row's values lie together and its other strides are multiples of 8, got {s}")
+    if t.data_ptr() & 15:
+        raise ValueError(f"{name} is 16-byte aligned")
 
 
-def _ints(name, t, shape, device, dtype=torch.int32):
-    if t.dtype != dtype:
+def _ints(name, t, shape, at, dtype=torch.int32):
+    if t.dtype is not dtype:
         raise TypeError(f"{name} is {dtype}, got {t.dtype}")
     if t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} is contiguous of shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {device}, got {t.device}")
+    if t.get_device() != at:
+        raise ValueError(f"{name} is on another device than the other tensors: {t.device}")
 
 
-def _starts(cu, device):
-    if cu.dim() != 1 or cu.shape[0] < 1:
-        raise ValueError(f"cu has one more entry than there are sequences, got shape {tuple(cu.shape)}")
-    _ints("cu", cu, cu.shape, device)
-    return cu.shape[0] - 1
+def _starts(cu, at):
+    shape = cu.shape
+    if len(shape) != 1 or shape[0] < 1:
+        raise ValueError(f"cu has one more entry than there are sequences, got shape {tuple(shape)}")
+    _ints("cu", cu, shape, at)
+    return shape[0] - 1
 
 
 def _dtype_of(t):
-    if t.dtype not in (torch.bfloat16, torch.float16):
+    if t.dtype not in _TYPES:
         raise TypeError(f"values are bfloat16 or float16, got {t.dtype}")
     return t.dtype
 
 
-def _out_lse(q, out, lse, dtype, device):
-    """(out, lse tensor or None) of a call whose rows are q's"""
-    if out is None:
-        out = torch.empty(q.shape, dtype=dtype, device=device)
-    else:
-        _rows("out", out, 3, dtype, device)
-        if out.shape != q.shape:
-            raise ValueError(f"out has q's shape {tuple(q.shape)}, got {tuple(out.shape)}")
-    return out, torch.empty(q.shape[:2], dtype=torch.float32, device=device) if lse else None
+def _check_out(out, q, dtype, at):
+    _rows("out", out, 3, dtype, at)
+    if out.shape != q.shape:
+        raise ValueError(f"out has q's shape {tuple(q.shape)}, got {tuple(out.shape)}")
 
 
-def _scale(scale, d):
-    if scale is None:
-        return d ** -0.5
-    if not 0 < scale < float("inf"):
+def _check_scale(scale):
+    if scale is not None and not 0 < scale < float("inf"):
         raise ValueError(f"scale is positive, got {scale}")
-    return float(scale)
 
 
 def attn_prompt(q, k, v, cu, scale=None, out=None, lse=False):
     """Causal attention of packed prompts: q [t][heads][d], k and v [t][kv heads][d] (views into one QKV product do),
     sequence b the rows cu[b] .. cu[b + 1] - 1. -> out like q; with lse=True (out, lse [t][heads] fp32). Rows before cu[0]
     and from cu[-1] on are left as they were in a given `out` (and have no meaning in a new one)."""
-    device, dtype = q.device, _dtype_of(q)
-    _rows("q", q, 3, dtype, device)
-    _rows("k", k, 3, dtype, device)
-    _rows("v", v, 3, dtype, device)
-    t, heads, d = q.shape
-    kv = k.shape[1]
-    if k.shape != v.shape or k.shape[0] != t or k.shape[2] != d or d not in HEAD_DIMS or kv == 0 or heads % kv or not heads:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: the same rows, d of {HEAD_DIMS}, heads a "
-                         "multiple of the kv heads")
-    n = _starts(cu, device)
-    if n > 4096:
-        raise ValueError(f"at most 4096 sequences, got {n}")
-    scale = _scale(scale, d)
-    out, sums = _out_lse(q, out, lse, dtype, device)
+    t, heads, kv, d, n, fresh = _prompt_shapes(q, k, v, cu, scale, out)
+    if fresh:
+        out = torch.empty(t, heads, d, dtype=q.dtype, device=q.device)
+    sums = torch.empty(t, heads, dtype=torch.float32, device=q.device) if lse else None
     if t and n:
         qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
-        _run(device, "qe_attn_prompt", "pllpllpllpllppiiiiifip", q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
+        _run(q.get_device(), "qe_attn_prompt", "pllpllpllpllppiiiiifip", q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
              v.data_ptr(), vs[0], vs[1], out.data_ptr(), os[0], os[1], sums.data_ptr() if lse else None, cu.data_ptr(), n, t,
-             heads, kv, d, scale, F16 if dtype == torch.float16 else 0)
+             heads, kv, d, d ** -0.5 if scale is None else scale, F16 if q.dtype == torch.float16 else 0)
     return (out, sums) if lse else out
+
+
+def _prompt_shapes(q, k, v, cu, scale, out):
+    dtype, at = _dtype_of(q), q.get_device()
+    _rows("q", q, 3, dtype, at)
+    _rows("k", k, 3, dtype, at)
+    _rows("v", v, 3, dtype, at)
+    t, heads, d = q.shape
+    ks, kv = k.shape, k.shape[1]
+    if ks != v.shape or ks[0] != t or ks[2] != d or d not in HEAD_DIMS or kv == 0 or heads % kv or not heads or heads > 65535:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: the same rows, d of {HEAD_DIMS}, heads a "
+                         "multiple of the kv heads")
+    if t > 1 and (k.stride(0) >= 1 << 24 or v.stride(0) >= 1 << 24):
+        raise ValueError(f"rows of k and v are less than 2^24 elements apart, got {k.stride(0)} and {v.stride(0)}")
+    n = _starts(cu, at)
+    if n > MAX_SEQS:
+        raise ValueError(f"at most {MAX_SEQS} sequences, got {n}")
+    _check_scale(scale)
+    if out is not None:
+        _check_out(out, q, dtype, at)
+    return t, heads, kv, d, n, out is None
 
 
 class _CacheStruct(ctypes.Structure):
@@ -146,7 +152,9 @@ class KVCache:
     as its transposed view), table [slots][width] (-1: none), length [slots], held [slots], ref [pages], int32."""
 
     def __init__(self, k, v, table, length, held, ref):
-        self.device, self.dtype = device, dtype = k.device, _dtype_of(k)
+        self.device, self.dtype = k.device, _dtype_of(k)
+        dtype, self._dev = self.dtype, k.get_device()
+        device = self._dev
         _rows("k", k, 5, dtype, device)
         _rows("v", v, 5, dtype, device)
         if k.shape != v.shape or k.stride() != v.stride() or not k.numel():
@@ -169,6 +177,7 @@ class KVCache:
                                held.data_ptr(), ref.data_ptr(), layers, pages, page, kv, d, slots, width,
                                int(dtype == torch.float16))
         self._at = ctypes.addressof(self._c)
+        self._scale = d ** -0.5
 
     @staticmethod
     def empty(layers, pages, page, kv_heads, d, slots, max_tokens, dtype=torch.bfloat16, device="cuda"):
@@ -182,7 +191,7 @@ class KVCache:
         if t.dim() != 1:
             raise ValueError(f"{name} has one dimension, got shape {tuple(t.shape)}")
         n = t.shape[0] if n is None else n
-        _ints(name, t, (n,), self.device)
+        _ints(name, t, (n,), self._dev)
         return n
 
     def _few(self, n):
@@ -197,7 +206,7 @@ class KVCache:
         self._few(n)
         got = torch.empty(5 * n + 4, dtype=torch.int32, device=self.device)  # the list of copies, then the answers
         if n:
-            _run(self.device, "qe_kv_reserve", "pppippp", self._at, seqs.data_ptr(), add.data_ptr(), n,
+            _run(self._dev, "qe_kv_reserve", "pppippp", self._at, seqs.data_ptr(), add.data_ptr(), n,
                  got.data_ptr() + 16 * (n + 1), got.data_ptr())
         return got[4 * n + 4:]
 
@@ -209,7 +218,7 @@ class KVCache:
         self._few(n)
         ok = torch.empty(n, dtype=torch.int32, device=self.device)
         if n:
-            _run(self.device, "qe_kv_fork", "pppipp", self._at, parents.data_ptr(), children.data_ptr(), n, ok.data_ptr())
+            _run(self._dev, "qe_kv_fork", "pppipp", self._at, parents.data_ptr(), children.data_ptr(), n, ok.data_ptr())
         return ok
 
     def release(self, seqs, lengths=None):
@@ -219,27 +228,27 @@ class KVCache:
             self._batch("lengths", lengths, n)
         self._few(n)
         if n:
-            _run(self.device, "qe_kv_release", "pppip", self._at, seqs.data_ptr(), None if lengths is None else lengths.data_ptr(), n)
+            _run(self._dev, "qe_kv_release", "pppip", self._at, seqs.data_ptr(), None if lengths is None else lengths.data_ptr(), n)
 
     def append(self, layer, k, v, seqs, cu):
         """New rows k, v [t][kv heads][d] of one layer, or [layers][t][kv heads][d] of all (layer None): rows cu[b] ..
         cu[b + 1] - 1 go behind the committed tokens of slot seqs[b], into pages reserved before. Slots are distinct."""
         dims = 4 if layer is None else 3
-        _rows("k", k, dims, self.dtype, self.device)
-        _rows("v", v, dims, self.dtype, self.device)
+        _rows("k", k, dims, self.dtype, self._dev)
+        _rows("v", v, dims, self.dtype, self._dev)
         t = k.shape[-3]
         if k.shape != v.shape or k.shape[-2:] != (self.kv_heads, self.d) or (layer is None and k.shape[0] != self.layers):
             raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} are rows of {self.kv_heads} kv heads of {self.d}"
                              + (f", of {self.layers} layers" if layer is None else ""))
         if layer is not None and not 0 <= layer < self.layers:
             raise ValueError(f"layer {layer} of {self.layers}")
-        n = _starts(cu, self.device)
+        n = _starts(cu, self._dev)
         self._batch("seqs", seqs, n)
         if t and n:
             ks, vs = k.stride(), v.stride()
             one = layer is not None
             strides = (ctypes.c_int64 * 6)(0 if one else ks[0], ks[-3], ks[-2], 0 if one else vs[0], vs[-3], vs[-2])
-            _run(self.device, "qe_kv_append", "piipppppiip", self._at, layer if one else 0, 1 if one else self.layers,
+            _run(self._dev, "qe_kv_append", "piipppppiip", self._at, layer if one else 0, 1 if one else self.layers,
                  k.data_ptr(), v.data_ptr(), ctypes.addressof(strides), seqs.data_ptr(), cu.data_ptr(), n, t)
 
     def accept(self, seqs, count, path=None, length=None):
@@ -252,13 +261,13 @@ class KVCache:
             if path.dim() != 2 or path.shape[1] > MAX_NODES:
                 raise ValueError(f"path is [sequences][at most {MAX_NODES}], got {tuple(path.shape)}")
             most = path.shape[1]
-            _ints("path", path, (n, most), self.device)
+            _ints("path", path, (n, most), self._dev)
         if length is not None:
-            _ints("length", length, (self.slots,), self.device)
+            _ints("length", length, (self.slots,), self._dev)
         if n > 65535:
             raise ValueError(f"at most 65535 sequences a call, got {n}")
         if n and (path is None or most):
-            _run(self.device, "qe_kv_accept", "ppppiipp", self._at, seqs.data_ptr(), count.data_ptr(),
+            _run(self._dev, "qe_kv_accept", "ppppiipp", self._at, seqs.data_ptr(), count.data_ptr(),
                  None if path is None else path.data_ptr(), most, n, None if length is None else length.data_ptr())
 
     def attend(self, layer, q, seqs, cu, most, mask=None, scale=None, out=None, lse=False):
@@ -266,26 +275,30 @@ class KVCache:
         sees the slot's committed tokens and the drafted tokens whose bit is set in mask[cu[b] + i] (int64 [t]), without a mask
         those up to itself. most (at most 64): the largest number of rows of a sequence. -> out like q; with lse=True (out,
         lse [t][heads] fp32). Rows of no sequence, or past `most`, are left as they were in a given `out`."""
-        device, dtype = self.device, self.dtype
-        _rows("q", q, 3, dtype, device)
+        at, dtype = self._dev, self.dtype
+        _rows("q", q, 3, dtype, at)
         t, heads, d = q.shape
-        if d != self.d or heads == 0 or heads % self.kv_heads:
+        if d != self.d or heads == 0 or heads % self.kv_heads or heads > 65535:
             raise ValueError(f"q {tuple(q.shape)}: heads of {self.d}, a multiple of the {self.kv_heads} kv heads")
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer {layer} of {self.layers}")
         if not 1 <= most <= MAX_NODES:
             raise ValueError(f"1 to {MAX_NODES} drafted tokens a sequence, got {most}")
-        n = _starts(cu, device)
-        self._batch("seqs", seqs, n)
-        if n > 4096:
-            raise ValueError(f"at most 4096 sequences, got {n}")
+        n = _starts(cu, at)
+        _ints("seqs", seqs, (n,), at)
+        if n > MAX_SEQS:
+            raise ValueError(f"at most {MAX_SEQS} sequences, got {n}")
         if mask is not None:
-            _ints("mask", mask, (t,), device, torch.int64)
-        scale = _scale(scale, d)
-        out, sums = _out_lse(q, out, lse, dtype, device)
+            _ints("mask", mask, (t,), at, torch.int64)
+        _check_scale(scale)
+        if out is None:
+            out = torch.empty(t, heads, d, dtype=dtype, device=self.device)
+        else:
+            _check_out(out, q, dtype, at)
+        sums = torch.empty(t, heads, dtype=torch.float32, device=self.device) if lse else None
         if t and n:
             qs, os = q.stride(), out.stride()
-            _run(device, "qe_attn_tree", "pipllpllpppiiipifp", self._at, layer, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0],
-                 os[1], sums.data_ptr() if lse else None, seqs.data_ptr(), cu.data_ptr(), n, t, most,
-                 None if mask is None else mask.data_ptr(), heads, scale)
+            _run(at, "qe_attn_tree", "pipllpllpppiiipifp", self._at, layer, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1],
+                 sums.data_ptr() if lse else None, seqs.data_ptr(), cu.data_ptr(), n, t, most,
+                 None if mask is None else mask.data_ptr(), heads, self._scale if scale is None else scale)
         return (out, sums) if lse else out

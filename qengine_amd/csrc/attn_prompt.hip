@@ -45,6 +45,14 @@ struct Tile {
     static __device__ __forceinline__ int k_row(int r) { return r / RK * (1024 + PAD) + r % RK * (D * 2); }
 };
 
+__device__ __forceinline__ int wave_sum(int x) {  // the same in every lane
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr 1, 2, 4, 8: sums of rows of 16 in their last lanes
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    return __builtin_amdgcn_readlane(x, 15) + __builtin_amdgcn_readlane(x, 31) + __builtin_amdgcn_readlane(x, 47) + __builtin_amdgcn_readlane(x, 63);
+}
+
 template <int DT, int D, int W>
 __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args a) {
     using T = AttnT<DT>;
@@ -66,38 +74,42 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
         qb = blocks_of(0) - 1 - slot;
         if (qb < 0) return;
     } else {
-        int* nb = reinterpret_cast<int*>(lds);
-        for (int i = tid; i < a.nseq; i += 64 * W) nb[i] = blocks_of(i);
-        __syncthreads();
+        int* more = reinterpret_cast<int*>(lds);  // blocks of the sequences from the 65th on; every wave holds the first 64
+        const int nb = lane < a.nseq ? blocks_of(lane) : 0;
+        if (a.nseq > 64) {
+            for (int i = 64 + tid; i < a.nseq; i += 64 * W) more[i - 64] = blocks_of(i);
+            __syncthreads();
+        }
         // blocks with index >= level, over all sequences
         auto count = [&](int level) {
-            int n = 0;
-            for (int i = lane; i < a.nseq; i += 64) n += max(0, nb[i] - level);
-#pragma unroll
-            for (int o = 32; o; o /= 2) n += __shfl_xor(n, o);
-            return n;
+            int n = max(0, nb - level);
+            for (int i = lane; i < a.nseq - 64; i += 64) n += max(0, more[i] - level);
+            return wave_sum(n);
         };
+        int lo = 0, above = 0;  // the largest level with more than `slot` blocks from it on, and the blocks above it
+        int hi = 1;
         if (slot >= count(0)) return;
-        int lo = 0, hi = (a.t + BQ - 1) / BQ;  // count(lo) > slot >= count(hi)
+        for (int n; (n = count(hi)) > slot; hi *= 2) lo = hi;
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
             if (count(mid) > slot) lo = mid;
             else hi = mid;
         }
+        above = count(lo + 1);
         qb = lo;
-        int rank = slot - count(lo + 1);  // among the sequences that have a block of this index
+        int rank = slot - above;  // among the sequences that have a block of this index
         for (int i0 = 0;; i0 += 64) {
-            const uint64_t has = __ballot(i0 + lane < a.nseq && nb[i0 + lane] > qb);
+            const bool mine = i0 + lane < a.nseq && (i0 == 0 ? nb : more[i0 - 64 + lane]) > qb;
+            const uint64_t has = __ballot(mine);
             const int n = __popcll(has);
             if (rank < n) {
-                uint64_t m = has;
-                for (; rank > 0; rank--) m &= m - 1;
-                b = i0 + __ffsll((unsigned long long)m) - 1;
+                const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
+                b = i0 + __ffsll((unsigned long long)__ballot(mine && before == rank)) - 1;
                 break;
             }
             rank -= n;
         }
-        __syncthreads();
+        if (a.nseq > 64) __syncthreads();
     }
     b = __builtin_amdgcn_readfirstlane(b);
     qb = __builtin_amdgcn_readfirstlane(qb);
@@ -105,22 +117,15 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
     const int q0 = qb * BQ, qw = q0 + wave * 32;  // the block's and the wave's first row
     const int row = qw + col;                     // this lane's query
 
-    u32x4_v q[KS];
-    {
-        const char* p = a.q + (int64_t)(c0 + min(row, len - 1)) * a.q_row + (int64_t)head * a.q_head + half * 16;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) q[ks] = *reinterpret_cast<const u32x4_v*>(p + ks * 32);
-    }
     const unsigned lds32 = (unsigned)(uintptr_t)lds;
     const char* kb = a.k + (int64_t)c0 * a.k_row + (int64_t)kvh * a.k_head;
     const char* vb = a.v + (int64_t)c0 * a.v_row + (int64_t)kvh * a.v_head;
     // a wave instruction fills 1 KB: RK rows; lane i lands at piece i, so it loads the piece that belongs there
     constexpr int N = KEYS / L::RK / W;
     uint32_t k_off[N], v_off[N];  // of a step's first key
-    int key_of[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const int r = key_of[i] = (wave * N + i) * L::RK + lane / L::CH;
+        const int r = (wave * N + i) * L::RK + lane / L::CH;
         k_off[i] = (uint32_t)r * (uint32_t)a.k_row + ((lane % L::CH) ^ L::kx(r)) * 16;
         v_off[i] = (uint32_t)r * (uint32_t)a.v_row + ((lane % L::CH) ^ L::vx(r)) * 16;
     }
@@ -128,18 +133,34 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
         const char* ks = kb + (int64_t)j * KEYS * a.k_row;
         const char* vs = vb + (int64_t)j * KEYS * a.v_row;
         const unsigned at = lds32 + buf * L::STAGE;
-        const int over = (j + 1) * KEYS - len;  // keys past the end re-read the last one (no row sees them)
+        const int over = (j + 1) * KEYS - len;
+        if (over <= 0) {
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const uint32_t back = over > 0 ? max(0, key_of[i] + over - (KEYS - 1)) : 0;
-            dma16_at(ks, k_off[i] - back * (uint32_t)a.k_row, at + (wave * N + i) * (1024 + L::PAD));
+            for (int i = 0; i < N; i++) dma16_at(ks, k_off[i], at + (wave * N + i) * (1024 + L::PAD));
+#pragma unroll
+            for (int i = 0; i < N; i++) dma16_at(vs, v_off[i], at + L::KBYTES + (wave * N + i) * 1024);
+            return;
         }
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const uint32_t back = over > 0 ? max(0, key_of[i] + over - (KEYS - 1)) : 0;
+        for (int i = 0; i < N; i++) {  // keys past the end re-read the last one (no row sees them)
+            const uint32_t back = max(0, (wave * N + i) * L::RK + lane / L::CH + over - (KEYS - 1));
+            dma16_at(ks, k_off[i] - back * (uint32_t)a.k_row, at + (wave * N + i) * (1024 + L::PAD));
             dma16_at(vs, v_off[i] - back * (uint32_t)a.v_row, at + L::KBYTES + (wave * N + i) * 1024);
         }
     };
+    const int steps = (min(len, q0 + BQ) + KEYS - 1) / KEYS;
+    const int mine = qw < len ? (min(len, qw + 32) + KEYS - 1) / KEYS : 0;  // steps with keys that this wave's rows see
+    stage(0, 0);
+    // The queries are waited for here: a use inside the loop would make the compiler wait there for whatever loads are in
+    // flight, which are the next step's.
+    u32x4_v q[KS];
+    {
+        const char* p = a.q + (int64_t)(c0 + min(row, len - 1)) * a.q_row + (int64_t)head * a.q_head + half * 16;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) q[ks] = *reinterpret_cast<const u32x4_v*>(p + ks * 32);
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(q[ks]));
+    }
     // a lane's places in a K tile (row col, piece 2 ks + half for ks = 0 and 1) and in a V tile (row 4 half + (0 .. 3) by lane,
     // columns 32 d + 16 (lane / 16 % 2) + 4 (lane % 4) for d = 0 .. 3)
     int kat[2], vat[4];
@@ -150,9 +171,6 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
 #pragma unroll
         for (int d = 0; d < 4; d++) vat[d] = L::KBYTES + vr * D * 2 + (((4 * d + vc) ^ L::vx(vr)) * 16) + (lane & 1) * 8;
     }
-    const int steps = (min(len, q0 + BQ) + KEYS - 1) / KEYS;
-    const int mine = qw < len ? (min(len, qw + 32) + KEYS - 1) / KEYS : 0;  // steps with keys that this wave's rows see
-
     f32x16_v o[DB];
     float m, l;
     // A value that is not finite in a key that some rows of a step must not see makes those rows' sums NaN (0 times it).
@@ -166,7 +184,7 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
         for (int d = 0; d < DB; d++)
 #pragma unroll
             for (int e = 0; e < 16; e++) o[d][e] = 0.f;
-        stage(0, 0);
+        if (pass) stage(0, 0);
         for (int j = 0; j < steps; j++) {
             // step j has landed everywhere, and every wave is done with the stage that step j + 1 goes to
             asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
