@@ -7,18 +7,15 @@
 // at a time lie in LDS, staged by LDS DMA while the 64 before are worked on. A wave reads K as the A operand in 16-byte
 // pieces and V's transpose by ds_read_b64_tr_b16; both tiles are stored with their 16-byte pieces permuted by row so that
 // these reads meet no bank twice.
-#include "attn_common.hpp"
+#include "attn_wave.hpp"
 #include "kv_cache.hpp"
-#include "mfma_tile.hpp"
 
 #include <algorithm>
 #include <atomic>
 
 namespace qe_prompt {
 using qe_tile::dma16_at;
-constexpr int kKeys = 64;          // keys of a step
 constexpr int kMaxSeqs = 4096;     // their block counts are kept in LDS
-constexpr float kLazy = 8.f;       // the running maximum follows a row's scores once they pass it by this much (2^8 in the sums)
 
 struct Args {
     const char *q, *k, *v;
@@ -28,21 +25,6 @@ struct Args {
     const int32_t* cu;
     int nseq, t, heads, kv_heads;
     float scale2;  // log2(e) times the scale: exponentials are powers of two
-};
-
-// Tiles in LDS. A row is CH = D / 8 pieces of 16 bytes, a DMA instruction fills 1 KB = RK rows.
-// K: a wave reads one piece of 32 rows (ds_read_b128), so 16 neighbouring rows must have it in 16 different places of a
-// 256-byte line: pieces are permuted inside groups of 1, 2 or 4 by row, and each KB starts PAD bytes further on.
-// V: a transposing read (ds_read_b64_tr_b16) takes 64 bytes of 8 rows, 4 rows at a time: the 64-byte windows of a row are
-// permuted by row.
-// Both permutations touch few bits, so a lane's addresses are one to four bases and constants.
-template <int D>
-struct Tile {
-    static constexpr int KEYS = kKeys, CH = D / 8, RK = 64 / CH, PAD = D == 256 ? 32 : 64;
-    static constexpr int KBYTES = KEYS / RK * (1024 + PAD), VBYTES = KEYS * D * 2, STAGE = KBYTES + VBYTES;
-    static __device__ __forceinline__ int kx(int r) { return D == 256 ? r & 1 : D == 128 ? r & 3 : r >> 1 & 3; }
-    static __device__ __forceinline__ int vx(int r) { return (D == 64 ? r >> 1 & 1 : r & 3) << 2; }
-    static __device__ __forceinline__ int k_row(int r) { return r / RK * (1024 + PAD) + r % RK * (D * 2); }
 };
 
 __device__ __forceinline__ int wave_sum(int x) {  // the same in every lane
@@ -55,9 +37,8 @@ __device__ __forceinline__ int wave_sum(int x) {  // the same in every lane
 
 template <int DT, int D, int W>
 __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args a) {
-    using T = AttnT<DT>;
-    constexpr int BQ = 32 * W, KS = D / 16, DB = D / 32, KEYS = kKeys, NX = KEYS / 32;
     using L = Tile<D>;
+    constexpr int BQ = 32 * W, KEYS = kKeys;
     extern __shared__ char lds[];  // two stages of K and V tiles; before them the block counts
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
@@ -120,70 +101,49 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
     const unsigned lds32 = (unsigned)(uintptr_t)lds;
     const char* kb = a.k + (int64_t)c0 * a.k_row + (int64_t)kvh * a.k_head;
     const char* vb = a.v + (int64_t)c0 * a.v_row + (int64_t)kvh * a.v_head;
-    // a wave instruction fills 1 KB: RK rows; lane i lands at piece i, so it loads the piece that belongs there
-    constexpr int N = KEYS / L::RK / W;
-    uint32_t k_off[N], v_off[N];  // of a step's first key
+    // A wave instruction fills 1 KB: RK rows; the wave's n-th starts RK n rows behind its first. Lane i lands at piece i, so
+    // it loads the piece that belongs there: of K the same in all instructions, of V in every second one (d = 256) or all.
+    constexpr int N = KEYS / L::RK / W, NV = D == 256 ? 2 : 1;
+    const int r_wave = wave * N * L::RK, r_lane = lane / L::CH;
+    const uint32_t k_off = (uint32_t)r_lane * (uint32_t)a.k_row + ((lane % L::CH) ^ L::kx(r_lane)) * 16;
+    uint32_t v_off[NV];
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        const int r = (wave * N + i) * L::RK + lane / L::CH;
-        k_off[i] = (uint32_t)r * (uint32_t)a.k_row + ((lane % L::CH) ^ L::kx(r)) * 16;
-        v_off[i] = (uint32_t)r * (uint32_t)a.v_row + ((lane % L::CH) ^ L::vx(r)) * 16;
-    }
+    for (int i = 0; i < NV; i++) v_off[i] = (uint32_t)r_lane * (uint32_t)a.v_row + ((lane % L::CH) ^ L::vx(i * L::RK + r_lane)) * 16;
     auto stage = [&](int j, int buf) {
-        const char* ks = kb + (int64_t)j * KEYS * a.k_row;
-        const char* vs = vb + (int64_t)j * KEYS * a.v_row;
+        const char* ks = kb + (int64_t)(j * KEYS + r_wave) * a.k_row;
+        const char* vs = vb + (int64_t)(j * KEYS + r_wave) * a.v_row;
         const unsigned at = lds32 + buf * L::STAGE;
         const int over = (j + 1) * KEYS - len;
         if (over <= 0) {
 #pragma unroll
-            for (int i = 0; i < N; i++) dma16_at(ks, k_off[i], at + (wave * N + i) * (1024 + L::PAD));
+            for (int i = 0; i < N; i++) dma16_at(ks + i * L::RK * a.k_row, k_off, at + (wave * N + i) * (1024 + L::PAD));
 #pragma unroll
-            for (int i = 0; i < N; i++) dma16_at(vs, v_off[i], at + L::KBYTES + (wave * N + i) * 1024);
+            for (int i = 0; i < N; i++) dma16_at(vs + i * L::RK * a.v_row, v_off[i % NV], at + L::KBYTES + (wave * N + i) * 1024);
             return;
         }
+        // keys past the end re-read the last one (no row sees them)
+        const char* k0 = kb + (int64_t)(j * KEYS) * a.k_row;
+        const char* v0 = vb + (int64_t)(j * KEYS) * a.v_row;
 #pragma unroll
-        for (int i = 0; i < N; i++) {  // keys past the end re-read the last one (no row sees them)
-            const uint32_t back = max(0, (wave * N + i) * L::RK + lane / L::CH + over - (KEYS - 1));
-            dma16_at(ks, k_off[i] - back * (uint32_t)a.k_row, at + (wave * N + i) * (1024 + L::PAD));
-            dma16_at(vs, v_off[i] - back * (uint32_t)a.v_row, at + L::KBYTES + (wave * N + i) * 1024);
+        for (int i = 0; i < N; i++) {
+            const int r = r_wave + i * L::RK + r_lane, key = min(r, KEYS - 1 - over);
+            dma16_at(k0, (uint32_t)key * (uint32_t)a.k_row + ((lane % L::CH) ^ L::kx(r)) * 16, at + (wave * N + i) * (1024 + L::PAD));
+            dma16_at(v0, (uint32_t)key * (uint32_t)a.v_row + ((lane % L::CH) ^ L::vx(r)) * 16, at + L::KBYTES + (wave * N + i) * 1024);
         }
     };
     const int steps = (min(len, q0 + BQ) + KEYS - 1) / KEYS;
     const int mine = qw < len ? (min(len, qw + 32) + KEYS - 1) / KEYS : 0;  // steps with keys that this wave's rows see
     stage(0, 0);
-    // The queries are waited for here: a use inside the loop would make the compiler wait there for whatever loads are in
-    // flight, which are the next step's.
-    u32x4_v q[KS];
-    {
-        const char* p = a.q + (int64_t)(c0 + min(row, len - 1)) * a.q_row + (int64_t)head * a.q_head + half * 16;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) q[ks] = *reinterpret_cast<const u32x4_v*>(p + ks * 32);
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(q[ks]));
-    }
-    // a lane's places in a K tile (row col, piece 2 ks + half for ks = 0 and 1) and in a V tile (row 4 half + (0 .. 3) by lane,
-    // columns 32 d + 16 (lane / 16 % 2) + 4 (lane % 4) for d = 0 .. 3)
-    int kat[2], vat[4];
-#pragma unroll
-    for (int i = 0; i < 2; i++) kat[i] = L::k_row(col) + (((2 * i + half) ^ L::kx(col)) * 16);
-    {
-        const int vr = 4 * half + (lane & 15) / 4, vc = (lane >> 4 & 1) * 2 + (lane & 3) / 2;
-#pragma unroll
-        for (int d = 0; d < 4; d++) vat[d] = L::KBYTES + vr * D * 2 + (((4 * d + vc) ^ L::vx(vr)) * 16) + (lane & 1) * 8;
-    }
-    f32x16_v o[DB];
-    float m, l;
+    Wave32<DT, D> w;
+    w.places(lane);
+    w.load_queries(a.q + (int64_t)(c0 + min(row, len - 1)) * a.q_row + (int64_t)head * a.q_head, half);
+    w.await_queries();
+    char* out = a.out + (int64_t)(c0 + row) * a.o_row + (int64_t)head * a.o_head + half * 8;
     // A value that is not finite in a key that some rows of a step must not see makes those rows' sums NaN (0 times it).
-    // Ordinary data has none; where sums of the first pass are not finite the block runs again, value by value of kKinds:
-    // over the finite values alone, then over ones in the place of each kind of the others, weighted 1 where a row sees the
-    // key, which tells the outputs that are +inf, -inf or NaN.
-    for (int pass = 0;; pass++) {
-        m = kNegInf;
-        l = 0.f;
-#pragma unroll
-        for (int d = 0; d < DB; d++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) o[d][e] = 0.f;
+    // Ordinary data has none; where sums of the first pass are not finite the block runs again over the finite values and
+    // then over each kind of the others (keep_tile).
+    for (int pass = 0; pass <= kKinds; pass++) {
+        w.clear();
         if (pass) stage(0, 0);
         for (int j = 0; j < steps; j++) {
             // step j has landed everywhere, and every wave is done with the stage that step j + 1 goes to
@@ -195,143 +155,21 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
                 __syncthreads();
             }
             if (j >= mine) continue;
-            // operands are read in groups, a group ahead of the products that use it; the sums of one V group follow the
-            // last scores' products, so that its reads are under way during the softmax
-            constexpr int GK = 8, NK = NX * KS / GK, GV = 4, NV = DB * 2 * NX / GV;
-            u32x4_v kf[2][GK], vf[2][GV];
-            auto read_k = [&](int g) {
-#pragma unroll
-                for (int i = 0; i < GK; i++) {
-                    const int x = (g * GK + i) % NX, ks = (g * GK + i) / NX;
-                    constexpr int M = D == 256 ? 1 : 2;  // bases
-                    const int at = kat[ks % M] + ks / M * M * 32 + 32 / L::RK * (1024 + L::PAD) * x;
-                    kf[g % 2][i] = *reinterpret_cast<const u32x4_v*>(tile + at);
-                }
-            };
-            auto read_v = [&](int g) {
-#pragma unroll
-                for (int i = 0; i < GV; i++) {
-                    const int d = (g * GV + i) / (2 * NX), y = (g * GV + i) % (2 * NX);
-#pragma unroll
-                    for (int z = 0; z < 2; z++) {
-                        const int at = vat[d % 4] + d / 4 * 256 + (16 * y + 8 * z) * D * 2;
-                        const s16x4_v w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_v*)(tile + at));
-                        const uint2 w2 = __builtin_bit_cast(uint2, w);
-                        vf[g % 2][i][2 * z] = w2.x;
-                        vf[g % 2][i][2 * z + 1] = w2.y;
-                    }
-                }
-            };
-            f32x16_v s[NX];
-#pragma unroll
-            for (int x = 0; x < NX; x++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) s[x][e] = 0.f;
-            read_k(0);
-#pragma unroll
-            for (int g = 0; g < NK; g++) {
-                if (g + 1 < NK) read_k(g + 1);
-                else read_v(0);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int i = 0; i < GK; i++) s[(g * GK + i) % NX] = T::mfma32(kf[g % 2][i], q[(g * GK + i) / NX], s[(g * GK + i) % NX]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            // a lane's scores: keys j KEYS + 32 x + 8 (e / 4) + 4 half + e % 4 of its query
-            if (j * KEYS + KEYS - 1 > qw) {
-                const int first = j * KEYS + 4 * half - row;  // key - row of the lane's first score
-#pragma unroll
-                for (int x = 0; x < NX; x++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        if (first + 32 * x + 8 * (e / 4) + e % 4 > 0) s[x][e] = kNegInf;
-            }
-            float mx = kNegInf;
-#pragma unroll
-            for (int x = 0; x < NX; x++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[x][e]);
-            mx *= a.scale2;
-            if (__any(mx > m + kLazy)) {
-                const float top = fmaxf(m, max_over_halves(mx));
-                const float f0 = top == kNegInf || pass > 1 ? 1.f : __builtin_amdgcn_exp2f(m - top);
-                m = top;
-                l *= f0;
-#pragma unroll
-                for (int d = 0; d < DB; d++) o[d] *= f0;
-            }
-            const float base = m == kNegInf ? 0.f : m;
-            u32x4_v p[2 * NX];
-#pragma unroll
-            for (int x = 0; x < NX; x++)
-#pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], a.scale2, -base));
-                    const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e + 1], a.scale2, -base));
-                    l += w0 + w1;
-                    p[2 * x + e / 8][e % 8 / 2] = T::pack(w0, w1);
-                }
-            if (pass > 1) {
-#pragma unroll
-                for (int x = 0; x < NX; x++)
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2)
-                        p[2 * x + e / 8][e % 8 / 2] = (s[x][e] != kNegInf ? T::kOne : 0u) | (s[x][e + 1] != kNegInf ? T::kOne << 16 : 0u);
-            }
-            // V^T's operand: 32 columns, 16 keys in the order of the scores: 4 half + (0 .. 3) and 8 more
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int g = 0; g < NV; g++) {
-                if (g + 1 < NV) read_v(g + 1);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int i = 0; i < GV; i++) {
-                    const int d = (g * GV + i) / (2 * NX);
-                    o[d] = T::mfma32(vf[g % 2][i], p[(g * GV + i) % (2 * NX)], o[d]);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-        bool again = false;
-        if (pass == 0) {
-            float bad = 0.f;
-#pragma unroll
-            for (int d = 0; d < DB; d++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) bad = __builtin_fmaf(o[d][e], 0.f, bad);
-            again = row < len && !(bad == 0.f);
+            const int first = j * KEYS + 4 * half - row;  // key - row of the lane's first score
+            w.step(tile, pass, a.scale2, j * KEYS + KEYS - 1 > qw, [&](int x, int e) { return first + 32 * x + 8 * (e / 4) + e % 4 <= 0; });
         }
         // (also: every wave is done with the stages)
-        again = __syncthreads_or(again) || pass > 0;
-        char* p = a.out + (int64_t)(c0 + row) * a.o_row + (int64_t)head * a.o_head + half * 8;
+        const bool again = __syncthreads_or(pass == 0 && row < len && w.bad());
         if (pass > 1) {
-            if (row < len)
-#pragma unroll
-                for (int d = 0; d < DB; d++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        uint16_t* at = reinterpret_cast<uint16_t*>(p + d * 64 + e / 4 * 16 + e % 4 * 2);
-                        if (o[d][e] > 0.f) *at = add_kind<DT>(*at, pass);
-                    }
-            if (pass == kKinds) return;
-            continue;
+            if (row < len) w.store_kind(out, pass);
+        } else if (!again) {
+            const float l = sum_over_halves(w.l);
+            if (row < len) {
+                w.store(out, l == 0.f ? 0.f : 1.f / l);
+                if (a.lse && half == 0) a.lse[(int64_t)(c0 + row) * a.heads + head] = l == 0.f ? kNegInf : (w.m + log2f(l)) * kLn2;
+            }
+            if (pass == 0) return;
         }
-        if (pass == 0 && again) continue;
-        l = sum_over_halves(l);
-        if (row < len) {
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-            for (int d = 0; d < DB; d++)
-#pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    uint2 w;
-                    w.x = T::pack(o[d][e] * inv, o[d][e + 1] * inv);
-                    w.y = T::pack(o[d][e + 2] * inv, o[d][e + 3] * inv);
-                    *reinterpret_cast<uint2*>(p + d * 64 + e * 4) = w;
-                }
-            if (a.lse && half == 0) a.lse[(int64_t)(c0 + row) * a.heads + head] = l == 0.f ? kNegInf : (m + log2f(l)) * kLn2;
-        }
-        if (!again) return;
     }
 }
 

@@ -8,54 +8,12 @@
 // V's rows 16 bytes a lane, turned into the A operand of O^T = V^T P^T by 16-bit permutes inside the lane (8 keys x 8
 // columns: 32 permutes for 32 keys x 128 columns, hidden behind the loads). The next 32 keys are in flight meanwhile.
 //
-// Work is split over the tokens of all sequences evenly: unit = 128 tokens (32 a wave) of one (sequence, kv head, row
-// block); the units in that order are dealt to as many blocks as the device holds, in ranges of equal length, whatever the
-// sequences' lengths. A (sequence, head, row block) that ends up in several blocks leaves partial sums (fp32, with their
-// running maximum and sum) in a workspace, which a second launch joins in block order.
-#include "attn_common.hpp"
-#include "kv_cache.hpp"
-
-#include <algorithm>
+// Work is split over the tokens of all sequences evenly (attn_tree.hpp), in units of 128 tokens, 32 a wave.
+#include "attn_tree.hpp"
 
 namespace qe_tree {
-constexpr int kThreads = 256, kWaves = 4, kUnit = 128;
+constexpr int kWaves = 4, kUnit = 128;
 constexpr float kLazy = 8.f;  // the running maximum follows a row's scores once they pass it by this much (2^8 in the sums)
-
-struct Args {
-    const char *q, *k, *v;
-    char* out;
-    float* lse;
-    int64_t q_row, q_head, o_row, o_head, page, head, token;  // bytes
-    const int32_t *table, *length, *seqs, *cu;
-    const uint64_t* mask;
-    int nseq, t, max_new, heads, kv_heads, group, shift, pages, width, slots, rb_max;
-    float scale2;  // log2(e) times the scale: exponentials are powers of two
-    float* part;   // [block][2][rows][D] partial sums, nullptr: every block takes whole (sequence, head, row block)s
-    float2* ml;    // [block][2][rows] maximum and sum
-    int* ends;     // [nseq] end of each sequence's units, then the range length
-};
-
-struct Seq {
-    int first, n, len, total;  // first row, rows, committed tokens, all tokens
-    int slot;
-};
-__device__ __forceinline__ Seq seq_of(const Args& a, int b) {
-    Seq s;
-    const int c0 = a.cu[b], c1 = a.cu[b + 1];
-    s.first = min(max(c0, 0), a.t);
-    s.n = min(min(c1, a.t) - s.first, a.max_new);
-    s.slot = a.seqs[b];
-    const bool ok = s.slot >= 0 && s.slot < a.slots;
-    const int room = a.width << a.shift;
-    s.len = ok ? min(max(a.length[ok ? s.slot : 0], 0), room) : 0;
-    s.total = ok ? min(s.len + max(s.n, 0), room) : 0;
-    return s;
-}
-template <int ROWS>
-__device__ __forceinline__ int row_blocks(const Args& a, int n) {
-    return (n * a.group + ROWS - 1) / ROWS;
-}
-__device__ __forceinline__ int unit_count(int total) { return max(1, (total + kUnit - 1) / kUnit); }
 
 template <int D>
 struct Frag {  // 32 keys of a wave
@@ -73,53 +31,14 @@ __global__ __launch_bounds__(kThreads, (NT * D <= 128 ? 2 : 1)) void tree_kernel
     constexpr int PITCH = D + 4;
     __shared__ float obuf[kWaves][16][PITCH];
     __shared__ float2 mlbuf[kWaves][16];
-    __shared__ int ends[kMaxTreeBatch];
+    static_assert(sizeof(obuf) >= kMaxTreeBatch * sizeof(int), "the units of all sequences fit the sums' place");
+    int* ends = reinterpret_cast<int*>(obuf);
     __shared__ int tmp[kWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, grp = lane >> 4;
 
-    int u = 0, u_end = 1, b = 0, range = 0;
-    if (a.part) {
-        int carry = 0;
-        for (int b0 = 0; b0 < a.nseq; b0 += kThreads) {
-            int x = 0;
-            if (b0 + tid < a.nseq) {
-                const Seq s = seq_of(a, b0 + tid);
-                if (s.n > 0) x = unit_count(s.total) * row_blocks<ROWS>(a, s.n) * a.kv_heads;
-            }
-#pragma unroll
-            for (int o = 1; o < 64; o *= 2) {
-                const int y = __shfl_up(x, o);
-                if (lane >= o) x += y;
-            }
-            __syncthreads();
-            if (lane == 63) tmp[wave] = x;
-            __syncthreads();
-            for (int w = 0; w < kWaves; w++) {
-                if (w < wave) x += tmp[w];
-            }
-            if (b0 + tid < a.nseq) ends[b0 + tid] = carry + x;
-            for (int w = 0; w < kWaves; w++) carry += tmp[w];
-        }
-        __syncthreads();
-        range = (carry + gridDim.x - 1) / gridDim.x;
-        if (blockIdx.x == 0) {
-            for (int i = tid; i < a.nseq; i += kThreads) a.ends[i] = ends[i];
-            if (tid == 0) a.ends[a.nseq] = range;
-        }
-        u = blockIdx.x * range;
-        u_end = min(carry, u + range);
-        if (u >= u_end) return;
-        int hi = a.nseq - 1;  // the sequence of the first unit
-        while (b < hi) {
-            const int mid = (b + hi) / 2;
-            if (ends[mid] > u) hi = mid;
-            else b = mid + 1;
-        }
-    } else {
-        b = blockIdx.x / (a.kv_heads * a.rb_max);
-    }
-
+    int u, u_end, b, base;
+    if (!my_units<kUnit, ROWS, kThreads>(a, ends, tmp, u, u_end, b, base)) return;
     while (u < u_end) {
         b = __builtin_amdgcn_readfirstlane(b);
         const Seq s = seq_of(a, b);
@@ -128,24 +47,11 @@ __global__ __launch_bounds__(kThreads, (NT * D <= 128 ? 2 : 1)) void tree_kernel
             b++;
             continue;
         }
-        const int units = unit_count(s.total), rbs = row_blocks<ROWS>(a, s.n);
-        int h, rb, t0, t1;
-        if (a.part) {
-            const int v = u - (b > 0 ? ends[b - 1] : 0);
-            t0 = v % units;
-            rb = v / units % rbs;
-            h = v / units / rbs;
-            t1 = min(units, t0 + u_end - u);
-        } else {
-            const int v = blockIdx.x % (a.kv_heads * a.rb_max);
-            h = v / a.rb_max;
-            rb = v % a.rb_max;
-            t0 = 0;
-            t1 = units;
-            if (rb >= rbs) return;
-        }
-        h = __builtin_amdgcn_readfirstlane(h);
-        rb = __builtin_amdgcn_readfirstlane(rb);
+        const int units = unit_count<kUnit>(s.total);
+        const int rbs = row_blocks<ROWS>(a, s.n);
+        Run run;
+        if (!run_of(a, base, u, u_end, units, rbs, run)) return;
+        const int h = run.h, rb = run.rb, t0 = run.t0, t1 = run.t1;
         const int rows = s.n * a.group;  // row r: drafted token r / group, query head r % group of the kv head
 
         // the rows' queries (B operand) and masks
@@ -423,106 +329,26 @@ __global__ __launch_bounds__(kThreads, (NT * D <= 128 ? 2 : 1)) void tree_kernel
             }
         }
         u += t1 - t0;
-        if (a.part && u >= ends[b]) b++;
-    }
-}
-
-// Joins the parts of one row: block (row, kv head, sequence). Four waves take every fourth part; sums in a fixed order.
-template <int DT, int D, int NT>
-__global__ __launch_bounds__(kThreads) void join_kernel(Args a, int most) {
-    using T = AttnT<DT>;
-    constexpr int ROWS = 16 * NT, E = D / 64;
-    const int r = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int c0 = a.cu[b], first = min(max(c0, 0), a.t), n = min(min(a.cu[b + 1], a.t) - first, a.max_new);
-    if (r >= n * a.group) return;
-    const int u0 = b > 0 ? a.ends[b - 1] : 0, range = a.ends[a.nseq], rbs = row_blocks<ROWS>(a, n), rb = r / ROWS;
-    const int units = (a.ends[b] - u0) / (rbs * a.kv_heads);
-    const int v0 = u0 + (h * rbs + rb) * units, w0 = v0 / range, w1 = (v0 + units - 1) / range, cnt = w1 - w0 + 1;
-    if (cnt == 1) return;
-    extern __shared__ float wgt[];  // [most] weights, then the waves' sums
-    float* acc = wgt + most;
-    __shared__ float red[2][kWaves];
-    auto at = [&](int i) { return ((int64_t)(w0 + i) * 2 + (i > 0 ? 0 : 1)) * ROWS + r % ROWS; };
-    float top = kNegInf;
-    for (int i = tid; i < cnt; i += kThreads) top = fmaxf(top, a.ml[at(i)].x);
-#pragma unroll
-    for (int o = 32; o; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
-    if (lane == 0) red[0][wave] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWaves; w++) top = fmaxf(top, red[0][w]);
-    float sum = 0.f;
-    for (int i = tid; i < cnt; i += kThreads) {
-        const float2 x = a.ml[at(i)];
-        float f = x.x == kNegInf ? 0.f : __builtin_amdgcn_exp2f(x.x - top);
-        if (x.x == __builtin_huge_valf()) f = 1.f;
-        wgt[i] = f;
-        sum += f * x.y;
-    }
-#pragma unroll
-    for (int o = 32; o; o /= 2) sum += __shfl_xor(sum, o);
-    if (lane == 0) red[1][wave] = sum;
-    __syncthreads();
-    sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; w++) sum += red[1][w];
-    float y[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) y[e] = 0.f;
-#pragma unroll 4
-    for (int i = wave; i < cnt; i += kWaves) {
-        const float f = wgt[i];
-        const float* p = a.part + at(i) * D + lane * E;
-#pragma unroll
-        for (int e = 0; e < E; e++) y[e] += f * p[e];
-    }
-#pragma unroll
-    for (int e = 0; e < E; e++) acc[wave * D + lane * E + e] = y[e];
-    __syncthreads();
-    const int i = r / a.group, hq = h * a.group + r % a.group;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (tid < D / 2) {
-        float z0 = 0.f, z1 = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            z0 += acc[w * D + 2 * tid];
-            z1 += acc[w * D + 2 * tid + 1];
+        if (u >= base + units * rbs * a.kv_heads) {
+            base += units * rbs * a.kv_heads;
+            b++;
         }
-        *reinterpret_cast<uint32_t*>(a.out + (int64_t)(first + i) * a.o_row + (int64_t)hq * a.o_head + 4 * tid) = T::pack(z0 * inv, z1 * inv);
     }
-    if (a.lse && tid == 0) a.lse[(int64_t)(first + i) * a.heads + hq] = sum == 0.f ? kNegInf : (top + log2f(sum)) * kLn2;
 }
 
 template <int DT, int D, int NT>
-void launch(Args a, hipStream_t st) {
-    constexpr int ROWS = 16 * NT;
-    a.rb_max = (a.max_new * a.group + ROWS - 1) / ROWS;
-    const int64_t runs = (int64_t)a.nseq * a.kv_heads * a.rb_max;
-    const int64_t most_units = ((int64_t)(a.width << a.shift) + kUnit - 1) / kUnit;
-    CHECK(runs * most_units < (int64_t)1 << 31, "qe_attn_tree: %lld rows x %lld units of tokens", (long long)runs, (long long)most_units);
-    const int grid = (int)std::min<int64_t>(runs * most_units, (NT * D <= 128 ? 2 : 1) * qe_num_cus());
-    const size_t part = (size_t)grid * 2 * ROWS * D * 4, ml = (size_t)grid * 2 * ROWS * 8, ends = ((size_t)a.nseq + 1) * 4;
-    WsHold hold(st);
-    if (char* ws = static_cast<char*>(hold.get(kWsAttn, part + ml + ends))) {
-        a.part = reinterpret_cast<float*>(ws);
-        a.ml = reinterpret_cast<float2*>(ws + part);
-        a.ends = reinterpret_cast<int*>(ws + part + ml);
-        tree_kernel<DT, D, NT><<<grid, kThreads, 0, st>>>(a);
-        HIP_CHECK(hipGetLastError());
-        join_kernel<DT, D, NT><<<dim3(a.max_new * a.group, a.kv_heads, a.nseq), kThreads, (grid + kWaves * D) * 4, st>>>(a, grid);
-    } else {
-        CHECK(runs < (int64_t)1 << 31, "qe_attn_tree: %lld blocks", (long long)runs);
-        tree_kernel<DT, D, NT><<<(int)runs, kThreads, 0, st>>>(a);
-    }
-    HIP_CHECK(hipGetLastError());
+void launch(const Args& a, hipStream_t st) {
+    launch_split<DT, D, kUnit, 16 * NT>(a, tree_kernel<DT, D, NT>, kThreads, 0, NT * D <= 128 ? 2 : 1, st);
 }
 
+// Up to 32 rows of a kv head (16 for d = 256): this kernel, above: attn_wide.hip.
 template <int DT>
 void by_shape(const Args& a, int d, hipStream_t st) {
     const int rows = a.max_new * a.group;
-    if (d == 64) rows <= 16 ? launch<DT, 64, 1>(a, st) : rows <= 32 ? launch<DT, 64, 2>(a, st) : launch<DT, 64, 4>(a, st);
-    else if (d == 128) rows <= 16 ? launch<DT, 128, 1>(a, st) : rows <= 32 ? launch<DT, 128, 2>(a, st) : launch<DT, 128, 4>(a, st);
-    else rows <= 16 ? launch<DT, 256, 1>(a, st) : launch<DT, 256, 2>(a, st);
+    if (rows > (d == 256 ? 16 : 32)) attend_wide(a, d, DT == kAttnF16, st);
+    else if (d == 64) rows <= 16 ? launch<DT, 64, 1>(a, st) : launch<DT, 64, 2>(a, st);
+    else if (d == 128) rows <= 16 ? launch<DT, 128, 1>(a, st) : launch<DT, 128, 2>(a, st);
+    else launch<DT, 256, 1>(a, st);
 }
 }  // namespace qe_tree
 
