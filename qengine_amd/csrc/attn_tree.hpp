@@ -130,32 +130,39 @@ __device__ __forceinline__ bool run_of(const Args& a, int base, int u, int u_end
 }
 
 
-// Joins the parts of one row: block (row, kv head, sequence). Four waves take every fourth part; sums in a fixed order.
-template <int DT, int D, int ROWS>
+// Joins the parts of the rows, WPR waves a row, each every WPR-th part; sums in a fixed order. One wave a row where there are
+// rows enough to fill the device: with four, 15360 rows of four parts took 21 us.
+template <int DT, int D, int ROWS, int WPR>
 __global__ __launch_bounds__(kThreads) void join_kernel(Args a, int most) {
     using T = AttnT<DT>;
-    constexpr int E = D / 64, kWaves = kThreads / 64;
-    const int r = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    constexpr int E = D / 64, RPB = kThreads / 64 / WPR;  // columns of a lane, rows of a block
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave % WPR;
+    const int r = blockIdx.x * RPB + wave / WPR, h = blockIdx.y, b = blockIdx.z;
     const int c0 = a.cu[b], first = min(max(c0, 0), a.t), n = min(min(a.cu[b + 1], a.t) - first, a.max_new);
-    if (r >= n * a.group) return;
-    const int u0 = b > 0 ? a.ends[b - 1] : 0, range = a.ends[a.nseq], rbs = row_blocks<ROWS>(a, n), rb = r / ROWS;
-    const int units = (a.ends[b] - u0) / (rbs * a.kv_heads);
-    const int v0 = u0 + (h * rbs + rb) * units, w0 = v0 / range, w1 = (v0 + units - 1) / range, cnt = w1 - w0 + 1;
-    if (cnt == 1) return;
-    extern __shared__ float wgt[];  // [most] weights, then the waves' sums
-    float* acc = wgt + most;
-    __shared__ float red[2][kWaves];
+    int cnt = 0, w0 = 0;
+    if (r < n * a.group) {
+        const int u0 = b > 0 ? a.ends[b - 1] : 0, range = a.ends[a.nseq], rbs = row_blocks<ROWS>(a, n);
+        const int units = (a.ends[b] - u0) / (rbs * a.kv_heads), v0 = u0 + (h * rbs + r / ROWS) * units;
+        w0 = v0 / range;
+        cnt = (v0 + units - 1) / range - w0 + 1;
+    }
+    if (WPR > 1 && cnt < 2) return;  // the whole block: one row
+    extern __shared__ float join_lds[];
+    float* wgt = join_lds + (WPR > 1 ? 0 : wave * most);  // [most] weights of the parts, and the waves' sums
+    float* acc = join_lds + most;
+    __shared__ float red[2][kThreads / 64];
     auto at = [&](int i) { return ((int64_t)(w0 + i) * 2 + (i > 0 ? 0 : 1)) * ROWS + r % ROWS; };
-    float top = kNegInf;
-    for (int i = tid; i < cnt; i += kThreads) top = fmaxf(top, a.ml[at(i)].x);
+    float top = kNegInf, sum = 0.f;
+    for (int i = wr * 64 + lane; i < cnt; i += WPR * 64) top = fmaxf(top, a.ml[at(i)].x);
 #pragma unroll
     for (int o = 32; o; o /= 2) top = fmaxf(top, __shfl_xor(top, o));
-    if (lane == 0) red[0][wave] = top;
-    __syncthreads();
+    if constexpr (WPR > 1) {
+        if (lane == 0) red[0][wave] = top;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) top = fmaxf(top, red[0][w]);
-    float sum = 0.f;
-    for (int i = tid; i < cnt; i += kThreads) {
+        for (int w = 0; w < WPR; w++) top = fmaxf(top, red[0][w]);
+    }
+    for (int i = wr * 64 + lane; i < cnt; i += WPR * 64) {
         const float2 x = a.ml[at(i)];
         float f = x.x == kNegInf ? 0.f : __builtin_amdgcn_exp2f(x.x - top);
         if (x.x == __builtin_huge_valf()) f = 1.f;
@@ -164,36 +171,43 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a, int most) {
     }
 #pragma unroll
     for (int o = 32; o; o /= 2) sum += __shfl_xor(sum, o);
-    if (lane == 0) red[1][wave] = sum;
+    if (WPR > 1 && lane == 0) red[1][wave] = sum;
     __syncthreads();
-    sum = 0.f;
+    if constexpr (WPR > 1) {
+        sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) sum += red[1][w];
+        for (int w = 0; w < WPR; w++) sum += red[1][w];
+    }
     float y[E];
 #pragma unroll
     for (int e = 0; e < E; e++) y[e] = 0.f;
 #pragma unroll 4
-    for (int i = wave; i < cnt; i += kWaves) {
+    for (int i = wr; i < cnt; i += WPR) {
         const float f = wgt[i];
         const float* p = a.part + at(i) * D + lane * E;
 #pragma unroll
         for (int e = 0; e < E; e++) y[e] += f * p[e];
     }
+    if constexpr (WPR > 1) {
 #pragma unroll
-    for (int e = 0; e < E; e++) acc[wave * D + lane * E + e] = y[e];
-    __syncthreads();
+        for (int e = 0; e < E; e++) acc[wave * D + lane * E + e] = y[e];
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            y[e] = 0.f;
+#pragma unroll
+            for (int w = 0; w < WPR; w++) y[e] += acc[w * D + lane * E + e];
+        }
+    }
+    if (cnt < 2) return;
     const int i = r / a.group, hq = h * a.group + r % a.group;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (tid < D / 2) {
-        float z0 = 0.f, z1 = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            z0 += acc[w * D + 2 * tid];
-            z1 += acc[w * D + 2 * tid + 1];
-        }
-        *reinterpret_cast<uint32_t*>(a.out + (int64_t)(first + i) * a.o_row + (int64_t)hq * a.o_head + 4 * tid) = T::pack(z0 * inv, z1 * inv);
-    }
-    if (a.lse && tid == 0) a.lse[(int64_t)(first + i) * a.heads + hq] = sum == 0.f ? kNegInf : (top + log2f(sum)) * kLn2;
+    char* p = a.out + (int64_t)(first + i) * a.o_row + (int64_t)hq * a.o_head + lane * E * 2;
+    if constexpr (E == 1) *reinterpret_cast<uint16_t*>(p) = (uint16_t)T::pack(y[0] * inv, 0.f);
+    else if constexpr (E == 2) *reinterpret_cast<uint32_t*>(p) = T::pack(y[0] * inv, y[1] * inv);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(T::pack(y[0] * inv, y[1] * inv), T::pack(y[2] * inv, y[3] * inv));
+    if (a.lse && lane == 0) a.lse[(int64_t)(first + i) * a.heads + hq] = sum == 0.f ? kNegInf : (top + log2f(sum)) * kLn2;
 }
 
 // kernel and join on the stream, or the kernel alone with a (sequence, head, row block) a block where the device has no
@@ -213,7 +227,11 @@ void launch_split(Args a, Kernel kernel, int threads, size_t lds, int per_cu, hi
         a.ends = reinterpret_cast<int*>(ws + part + ml);
         kernel<<<grid, threads, lds, st>>>(a);
         HIP_CHECK(hipGetLastError());
-        join_kernel<DT, D, ROWS><<<dim3(a.max_new * a.group, a.kv_heads, a.nseq), kThreads, (grid + kThreads / 64 * D) * 4, st>>>(a, grid);
+        const int rows = a.max_new * a.group;
+        if ((int64_t)rows * a.kv_heads * a.nseq >= 8 * qe_num_cus())
+            join_kernel<DT, D, ROWS, 1><<<dim3((rows + 3) / 4, a.kv_heads, a.nseq), kThreads, 4 * grid * 4, st>>>(a, grid);
+        else
+            join_kernel<DT, D, ROWS, 4><<<dim3(rows, a.kv_heads, a.nseq), kThreads, (grid + 4 * D) * 4, st>>>(a, grid);
     } else {
         kernel<<<(int)runs, threads, lds, st>>>(a);
     }
