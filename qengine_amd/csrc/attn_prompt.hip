@@ -35,10 +35,10 @@ __device__ __forceinline__ int wave_sum(int x) {  // the same in every lane
     return __builtin_amdgcn_readlane(x, 15) + __builtin_amdgcn_readlane(x, 31) + __builtin_amdgcn_readlane(x, 47) + __builtin_amdgcn_readlane(x, 63);
 }
 
-template <int DT, int D, int W>
+template <int DT, int D, int KEYS, int W, int STAGES>
 __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args a) {
-    using L = Tile<D>;
-    constexpr int BQ = 32 * W, KEYS = kKeys;
+    using L = Tile<D, KEYS>;
+    constexpr int BQ = 32 * W;
     extern __shared__ char lds[];  // two stages of K and V tiles; before them the block counts
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
@@ -94,7 +94,8 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
     }
     b = __builtin_amdgcn_readfirstlane(b);
     qb = __builtin_amdgcn_readfirstlane(qb);
-    const int c0 = min(max(a.cu[b], 0), a.t), len = min(a.cu[b + 1], a.t) - c0;
+    const int c0 = __builtin_amdgcn_readfirstlane(min(max(a.cu[b], 0), a.t));
+    const int len = __builtin_amdgcn_readfirstlane(min(a.cu[b + 1], a.t)) - c0;
     const int q0 = qb * BQ, qw = q0 + wave * 32;  // the block's and the wave's first row
     const int row = qw + col;                     // this lane's query
 
@@ -109,10 +110,11 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
     uint32_t v_off[NV];
 #pragma unroll
     for (int i = 0; i < NV; i++) v_off[i] = (uint32_t)r_lane * (uint32_t)a.v_row + ((lane % L::CH) ^ L::vx(i * L::RK + r_lane)) * 16;
-    auto stage = [&](int j, int buf) {
+    auto stage = [&](int j) {
+        j = __builtin_amdgcn_readfirstlane(j);
         const char* ks = kb + (int64_t)(j * KEYS + r_wave) * a.k_row;
         const char* vs = vb + (int64_t)(j * KEYS + r_wave) * a.v_row;
-        const unsigned at = lds32 + buf * L::STAGE;
+        const unsigned at = lds32 + j % STAGES * L::STAGE;
         const int over = (j + 1) * KEYS - len;
         if (over <= 0) {
 #pragma unroll
@@ -133,31 +135,41 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
     };
     const int steps = (min(len, q0 + BQ) + KEYS - 1) / KEYS;
     const int mine = qw < len ? (min(len, qw + 32) + KEYS - 1) / KEYS : 0;  // steps with keys that this wave's rows see
-    stage(0, 0);
-    Wave32<DT, D> w;
+    constexpr int AHEAD = STAGES - 1;  // steps that are under way while one is worked on
+    auto first_stages = [&] {
+#pragma unroll 1
+        for (int i = 0; i < min(AHEAD, steps); i++) stage(i);
+    };
+    auto land = [&](int j, int pass) {  // step j is in LDS for every wave, and all are done with the stage that the next step takes
+        if (steps - j >= AHEAD) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * N * (AHEAD - 1)) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        if (j + AHEAD < steps) stage(j + AHEAD);
+        if (pass) {
+            keep_tile<DT>(lds + j % STAGES * L::STAGE + L::KBYTES, L::VBYTES, pass, tid, 64 * W);
+            __syncthreads();
+        }
+    };
+    Wave32<DT, D, KEYS> w;
     w.places(lane);
+    if (W > 4 && wave >= W / 2) __builtin_amdgcn_s_setprio(1);  // one of a SIMD's two waves ahead: its softmax beside the other's products
     w.load_queries(a.q + (int64_t)(c0 + min(row, len - 1)) * a.q_row + (int64_t)head * a.q_head, half);
-    w.await_queries();
     char* out = a.out + (int64_t)(c0 + row) * a.o_row + (int64_t)head * a.o_head + half * 8;
     // A value that is not finite in a key that some rows of a step must not see makes those rows' sums NaN (0 times it).
     // Ordinary data has none; where sums of the first pass are not finite the block runs again over the finite values and
     // then over each kind of the others (keep_tile).
     for (int pass = 0; pass <= kKinds; pass++) {
         w.clear();
-        if (pass) stage(0, 0);
-        for (int j = 0; j < steps; j++) {
-            // step j has landed everywhere, and every wave is done with the stage that step j + 1 goes to
-            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-            if (j + 1 < steps) stage(j + 1, (j + 1) & 1);
-            char* tile = lds + (j & 1) * L::STAGE;
-            if (pass) {
-                keep_tile<DT>(tile + L::KBYTES, L::VBYTES, pass, tid, 64 * W);
-                __syncthreads();
-            }
-            if (j >= mine) continue;
+        first_stages();
+        w.await_queries();
+        auto scores = [&](int j) {
             const int first = j * KEYS + 4 * half - row;  // key - row of the lane's first score
-            w.step(tile, pass, a.scale2, j * KEYS + KEYS - 1 > qw, [&](int x, int e) { return first + 32 * x + 8 * (e / 4) + e % 4 <= 0; });
+            return w.scores(lds + j % STAGES * L::STAGE, j * KEYS + KEYS - 1 > qw, [&](int x, int e) { return first + 32 * x + 8 * (e / 4) + e % 4 <= 0; });
+        };
+        for (int j = 0; j < steps; j++) {
+            land(j, pass);
+            if (j < mine) w.values(lds + j % STAGES * L::STAGE, scores(j), pass, a.scale2);
         }
+        w.settle();
         // (also: every wave is done with the stages)
         const bool again = __syncthreads_or(pass == 0 && row < len && w.bad());
         if (pass > 1) {
@@ -173,30 +185,30 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
     }
 }
 
-template <int DT, int D, int W>
+template <int DT, int D, int KEYS, int W, int STAGES>
 void launch(const Args& a, hipStream_t st) {
-    constexpr int BQ = 32 * W;
+    constexpr int BQ = 32 * W, bytes = STAGES * Tile<D, KEYS>::STAGE;
+    static_assert(bytes >= kMaxSeqs * (int)sizeof(int) && (STAGES & (STAGES - 1)) == 0, "block counts fit; stages by the step's number");
     const int64_t blocks = ((int64_t)a.t / BQ + a.nseq) * a.heads;
     CHECK(blocks < (int64_t)1 << 31, "qe_attn_prompt: %lld blocks", (long long)blocks);
-    const int bytes = std::max(2 * Tile<D>::STAGE, a.nseq * 4);
-    if (bytes > 64 * 1024) {
-        static std::atomic<uint64_t> done{0};  // per device, one bit
-        int dev = 0;
-        HIP_CHECK(hipGetDevice(&dev));
-        if (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1)) {
-            HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(prompt_kernel<DT, D, W>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-            if (dev < 64) done.fetch_or(1ull << dev);
-        }
+    const auto kernel = prompt_kernel<DT, D, KEYS, W, STAGES>;
+    static std::atomic<uint64_t> done{0};  // devices on which the kernel may use so much LDS
+    int dev = 0;
+    HIP_CHECK(hipGetDevice(&dev));
+    if (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1)) {
+        HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        if (dev < 64) done.fetch_or(1ull << dev);
     }
-    prompt_kernel<DT, D, W><<<(int)blocks, 64 * W, bytes, st>>>(a);
+    kernel<<<(int)blocks, 64 * W, bytes, st>>>(a);
     HIP_CHECK(hipGetLastError());
 }
 
 template <int DT>
 void by_shape(const Args& a, int d, hipStream_t st) {
-    if (d == 64) launch<DT, 64, 4>(a, st);
-    else if (d == 128) launch<DT, 128, 4>(a, st);
-    else launch<DT, 256, 4>(a, st);
+    static const int v = getenv("QE_V") ? atoi(getenv("QE_V")) : 0;
+    if (d == 64) v == 1 ? launch<DT, 64, 64, 8, 4>(a, st) : launch<DT, 64, 64, 4, 2>(a, st);
+    else if (d == 128) v == 1 ? launch<DT, 128, 64, 8, 4>(a, st) : launch<DT, 128, 64, 4, 2>(a, st);
+    else v == 1 ? launch<DT, 256, 32, 4, 4>(a, st) : launch<DT, 256, 64, 4, 2>(a, st);
 }
 }  // namespace qe_prompt
 

@@ -133,7 +133,8 @@ __global__ __launch_bounds__(kThreads, (NT * D <= 128 ? 2 : 1)) void tree_kernel
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const int tok = tb + 16 * x + 4 * grp + e, j = tok - s.len;
-                            const bool on = f.ok[x] && (j < 0 || (tok < s.total && (see[nt] >> (j & 63) & 1)));
+                            const uint32_t drafted = (uint32_t)(tok < s.total) & (uint32_t)(see[nt] >> (j & 63));
+                            const bool on = ((uint32_t)f.ok[x] & ((uint32_t)(j < 0) | drafted) & 1) != 0;
                             // times the scale here: a negative one must not turn -inf around
                             sc[nt][x][e] = on ? sc[nt][x][e] * a.scale2 : kNegInf;
                         }

@@ -1,11 +1,10 @@
-// One wave's part of attention with 64 keys a step in LDS (attn_prompt.hip, attn_wide.hip): 32 query rows with their
+// One wave's part of attention with 32 or 64 keys a step in LDS (attn_prompt.hip, attn_wide.hip): 32 query rows with their
 // queries, their scores S^T = K Q^T (32 x 32 x 16 MFMA) and their sums O^T = V^T P^T in registers, the running maximum and
 // sum of the softmax beside them.
 #pragma once
 #include "attn_common.hpp"
 #include "mfma_tile.hpp"
 
-constexpr int kKeys = 64;     // keys of a step
 constexpr float kLazy = 8.f;  // the running maximum follows a row's scores once they pass it by this much (2^8 in the sums)
 
 // Tiles in LDS. A row is CH = D / 8 pieces of 16 bytes, a DMA instruction fills 1 KB = RK rows.
@@ -14,9 +13,9 @@ constexpr float kLazy = 8.f;  // the running maximum follows a row's scores once
 // V: a transposing read (ds_read_b64_tr_b16) takes 64 bytes of 8 rows, 4 rows at a time: the 64-byte windows of a row are
 // permuted by row.
 // Both permutations touch few bits, so a lane's addresses are one to four bases and constants.
-template <int D>
+template <int D, int KEYS>
 struct Tile {
-    static constexpr int KEYS = kKeys, CH = D / 8, RK = 64 / CH, PAD = D == 256 ? 32 : 64;
+    static constexpr int CH = D / 8, RK = 64 / CH, PAD = D == 256 ? 32 : 64;
     static constexpr int KBYTES = KEYS / RK * (1024 + PAD), VBYTES = KEYS * D * 2, STAGE = KBYTES + VBYTES;
     static __device__ __forceinline__ int kx(int r) { return D == 256 ? r & 1 : D == 128 ? r & 3 : r >> 1 & 3; }
     static __device__ __forceinline__ int vx(int r) { return (D == 64 ? r >> 1 & 1 : r & 3) << 2; }
@@ -24,11 +23,14 @@ struct Tile {
 };
 
 
-template <int DT, int D>
+template <int DT, int D, int KEYS>
 struct Wave32 {
     using T = AttnT<DT>;
-    using L = Tile<D>;
-    static constexpr int KS = D / 16, DB = D / 32, NX = kKeys / 32;
+    using L = Tile<D, KEYS>;
+    static constexpr int KS = D / 16, DB = D / 32, NX = KEYS / 32;
+    struct Scores {
+        f32x16_v s[NX];  // keys 32 x + 8 (e / 4) + 4 (lane / 32) + e % 4 of a step
+    };
     u32x4_v q[KS];  // lane: query lane % 32, values 16 ks + 8 (lane / 32) ..
     f32x16_v o[DB]; // lane: query lane % 32, columns 32 db + 8 (e / 4) + 4 (lane / 32) + e % 4
     float m, l;     // maximum (times the scale, base 2) and this half's sum
@@ -62,13 +64,14 @@ struct Wave32 {
 #pragma unroll
             for (int e = 0; e < 16; e++) o[d][e] = 0.f;
     }
-    // seen(x, e): whether the lane's query sees key 32 x + 8 (e / 4) + 4 (lane / 32) + e % 4 of the step (asked if masked)
+    // Scores of a step. seen(x, e): whether the lane's query sees the key of s[x][e] (asked if masked). Operands are read in
+    // groups, a group ahead of the products that use it.
     template <class Seen>
-    __device__ __forceinline__ void step(const char* tile, int pass, float scale2, bool masked, Seen seen) {
-        // operands are read in groups, a group ahead of the products that use it; the sums of one V group follow the
-        // last scores' products, so that its reads are under way during the softmax
-        constexpr int GK = D == 256 ? 4 : 8, NK = NX * KS / GK, GV = 4, NV = DB * 2 * NX / GV;
-        u32x4_v kf[2][GK], vf[2][GV];
+    __device__ __forceinline__ Scores scores(const char* tile, bool masked, Seen seen) const {
+        Scores r;
+        f32x16_v(&s)[NX] = r.s;
+        constexpr int GK = D == 256 ? 4 : 8, NK = NX * KS / GK;
+        u32x4_v kf[2][GK];
         auto read_k = [&](int g) {
 #pragma unroll
             for (int i = 0; i < GK; i++) {
@@ -78,6 +81,33 @@ struct Wave32 {
                 kf[g % 2][i] = *reinterpret_cast<const u32x4_v*>(tile + at);
             }
         };
+#pragma unroll
+        for (int x = 0; x < NX; x++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[x][e] = 0.f;
+        read_k(0);
+#pragma unroll
+        for (int g = 0; g < NK; g++) {
+            if (g + 1 < NK) read_k(g + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < GK; i++) s[(g * GK + i) % NX] = T::mfma32(kf[g % 2][i], q[(g * GK + i) / NX], s[(g * GK + i) % NX]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (masked) {
+#pragma unroll
+            for (int x = 0; x < NX; x++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    s[x][e] = seen(x, e) ? s[x][e] : kNegInf;
+        }
+        return r;
+    }
+    // Softmax of the scores and their products with the step's values, whose first reads are under way during the softmax
+    __device__ __forceinline__ void values(const char* tile, const Scores& r, int pass, float scale2) {
+        const f32x16_v(&s)[NX] = r.s;
+        constexpr int GV = 4, NV = DB * 2 * NX / GV;
+        u32x4_v vf[2][GV];
         auto read_v = [&](int g) {
 #pragma unroll
             for (int i = 0; i < GV; i++) {
@@ -92,28 +122,8 @@ struct Wave32 {
                 }
             }
         };
-        f32x16_v s[NX];
-#pragma unroll
-        for (int x = 0; x < NX; x++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) s[x][e] = 0.f;
-        read_k(0);
-#pragma unroll
-        for (int g = 0; g < NK; g++) {
-            if (g + 1 < NK) read_k(g + 1);
-            else read_v(0);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < GK; i++) s[(g * GK + i) % NX] = T::mfma32(kf[g % 2][i], q[(g * GK + i) / NX], s[(g * GK + i) % NX]);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        if (masked) {
-#pragma unroll
-            for (int x = 0; x < NX; x++)
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    if (!seen(x, e)) s[x][e] = kNegInf;
-        }
+        read_v(0);
+        __builtin_amdgcn_sched_barrier(0);
         float mx = kNegInf;
 #pragma unroll
         for (int x = 0; x < NX; x++)
@@ -159,6 +169,12 @@ struct Wave32 {
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+    }
+    // After the steps: the sums as they are. (Without it the compiler keeps a second copy of them in the order of the stores
+    // that follow and moves all of them at every step.)
+    __device__ __forceinline__ void settle() {
+#pragma unroll
+        for (int d = 0; d < DB; d++) asm volatile("" : "+v"(o[d]));
     }
     // whether a sum is not finite
     __device__ __forceinline__ bool bad() const {

@@ -16,10 +16,10 @@ using qe_tile::dma16_at;
 // page numbers are read by scalar loads: a vector load would make the compiler wait for the DMAs in flight
 typedef const __attribute__((address_space(4))) int32_t* ScalarInts;
 
-template <int DT, int D, int W, int STAGES>
+template <int DT, int D, int KEYS, int W, int STAGES>
 __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void wide_kernel(Args a) {
-    using L = Tile<D>;
-    constexpr int ROWS = 32 * W, N = kKeys / L::RK / W, CHUNK = 16;  // pages are at least 16 tokens
+    using L = Tile<D, KEYS>;
+    constexpr int ROWS = 32 * W, N = KEYS / L::RK / W, CHUNK = 16;  // pages are at least 16 tokens
     extern __shared__ char lds[];
     static_assert(STAGES * L::STAGE >= kMaxTreeBatch * (int)sizeof(int), "the units of all sequences fit the stages' place");
     int* ends = reinterpret_cast<int*>(lds);
@@ -36,14 +36,17 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void wide_kernel(Args a
     uint32_t v_off[NV];
 #pragma unroll
     for (int i = 0; i < NV; i++) v_off[i] = (uint32_t)r_lane * (uint32_t)a.token + ((lane % L::CH) ^ L::vx(i * L::RK + r_lane)) * 16;
-    Wave32<DT, D> w;
+    Wave32<DT, D, KEYS> w;
     w.places(lane);
+    if (W > 4 && wave >= W / 2) __builtin_amdgcn_s_setprio(1);  // one of a SIMD's two waves ahead: its softmax beside the other's products
 
     int u, u_end, b, base;
-    if (!my_units<kKeys, ROWS, 64 * W>(a, ends, tmp, u, u_end, b, base)) return;
+    if (!my_units<KEYS, ROWS, 64 * W>(a, ends, tmp, u, u_end, b, base)) return;
     while (u < u_end) {
         b = __builtin_amdgcn_readfirstlane(b);
         Seq s = seq_of(a, b);
+        s.first = __builtin_amdgcn_readfirstlane(s.first);
+        s.n = __builtin_amdgcn_readfirstlane(s.n);
         s.total = __builtin_amdgcn_readfirstlane(s.total);
         s.len = __builtin_amdgcn_readfirstlane(s.len);
         s.slot = __builtin_amdgcn_readfirstlane(s.slot);
@@ -52,7 +55,7 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void wide_kernel(Args a
             b++;
             continue;
         }
-        const int units = unit_count<kKeys>(s.total);
+        const int units = unit_count<KEYS>(s.total);
         const int rbs = row_blocks<ROWS>(a, s.n);
         Run run;
         if (!run_of(a, base, u, u_end, units, rbs, run)) return;
@@ -64,68 +67,70 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void wide_kernel(Args a
         const char* kh = a.k + (int64_t)run.h * a.head;
         const char* vh = a.v + (int64_t)run.h * a.head;
         const int pmask = (1 << a.shift) - 1;
-        // page of the chunk of 16 tokens from tok, -1: none
-        auto page_at = [&](int tok) {
-            int pg = -1;
-            if (tok < s.total) pg = tab[tok >> a.shift];
-            return pg >= 0 && pg < a.pages ? pg : -1;
-        };
-        // which chunks of step j have a page
-        auto chunks_of = [&](int j) {
-            uint32_t bits = 0;
-#pragma unroll
-            for (int c = 0; c < kKeys / CHUNK; c++) bits |= page_at(j * kKeys + c * CHUNK) >= 0 ? 1u << c : 0u;
-            return bits;
-        };
-        // the wave's rows of step j lie in one chunk of 16 tokens or several
-        constexpr int CW = N * L::RK > CHUNK ? N * L::RK / CHUNK : 1, NC = N / CW;
+        static_assert(N * L::RK <= CHUNK && CHUNK % (N * L::RK) == 0, "a wave's rows of a step are in one page");
+        constexpr int NCH = KEYS / CHUNK;  // chunks of a step
+        uint32_t ring = 0;                 // which chunks of the last 8 steps have a page, NCH bits each
         auto stage = [&](int j) {
-            const unsigned at = lds32 + j % STAGES * L::STAGE;
+            j = __builtin_amdgcn_readfirstlane(j);
+            int pg[NCH];
 #pragma unroll
-            for (int c = 0; c < CW; c++) {
-                const int tok = j * kKeys + r_wave + c * CHUNK, pg = max(page_at(tok & -CHUNK), 0);
-                const int64_t first = (int64_t)pg * a.page + (int64_t)(tok & pmask) * a.token;
+            for (int c = 0; c < NCH; c++) pg[c] = tab[min((j * KEYS + c * CHUNK) >> a.shift, a.width - 1)];
+            uint32_t bits = 0;
+            int mine = 0;
 #pragma unroll
-                for (int i = 0; i < NC; i++) dma16_at(kh + first + i * L::RK * a.token, k_off, at + (wave * N + c * NC + i) * (1024 + L::PAD));
-#pragma unroll
-                for (int i = 0; i < NC; i++) dma16_at(vh + first + i * L::RK * a.token, v_off[i % NV], at + L::KBYTES + (wave * N + c * NC + i) * 1024);
+            for (int c = 0; c < NCH; c++) {
+                const bool ok = j * KEYS + c * CHUNK < s.total && pg[c] >= 0 && pg[c] < a.pages;
+                bits |= ok ? 1u << c : 0u;
+                if (c == r_wave / CHUNK) mine = ok ? pg[c] : 0;
             }
+            ring = (ring & ~(((1u << NCH) - 1) << (j % 8 * NCH))) | bits << (j % 8 * NCH);
+            const unsigned at = lds32 + j % STAGES * L::STAGE;
+            const int64_t first = (int64_t)mine * a.page + (int64_t)((j * KEYS + r_wave) & pmask) * a.token;
+#pragma unroll
+            for (int i = 0; i < N; i++) dma16_at(kh + first + i * L::RK * a.token, k_off, at + (wave * N + i) * (1024 + L::PAD));
+#pragma unroll
+            for (int i = 0; i < N; i++) dma16_at(vh + first + i * L::RK * a.token, v_off[i % NV], at + L::KBYTES + (wave * N + i) * 1024);
         };
         const bool whole = run.t0 == 0 && run.t1 == units;
         const int64_t slot = ((int64_t)blockIdx.x * 2 + (run.t0 > 0 ? 0 : 1)) * ROWS + wave * 32 + col;
         char* out = a.out + (int64_t)(s.first + node) * a.o_row + (int64_t)hq * a.o_head + half * 8;
         float* part = a.part + slot * D + half * 4;
 
+        constexpr int AHEAD = STAGES - 1;  // steps that are under way while one is worked on
         auto first_stages = [&] {
-#pragma unroll
-            for (int i = 0; i < STAGES - 1; i++)
-                if (run.t0 + i < run.t1) stage(run.t0 + i);
+#pragma unroll 1
+            for (int j = run.t0; j < min(run.t0 + AHEAD, run.t1); j++) stage(j);
         };
-        first_stages();
+        auto land = [&](int j, int pass) {  // step j is in LDS for every wave, and all are done with the stage that the next step takes
+            if (run.t1 - j >= AHEAD) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * N * (AHEAD - 1)) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            if (j + AHEAD < run.t1) stage(j + AHEAD);
+            if (pass) {
+                keep_tile<DT>(lds + j % STAGES * L::STAGE + L::KBYTES, L::VBYTES, pass, tid, 64 * W);
+                __syncthreads();
+            }
+        };
+        auto scores = [&](int j) {
+            const uint32_t have = ring >> (j % 8 * NCH) & ((1u << NCH) - 1);
+            const int tok0 = j * KEYS + 4 * half;
+            return w.scores(lds + j % STAGES * L::STAGE, j * KEYS + KEYS > s.len || have != (1u << NCH) - 1, [&](int x, int e) {
+                const int tok = tok0 + 32 * x + 8 * (e / 4) + e % 4, t = tok - s.len;
+                // no && or ||: the compiler made branches of them and lost the assignment behind one
+                const uint32_t drafted = (uint32_t)(tok < s.total) & (uint32_t)(see >> (t & 63));
+                return ((have >> (2 * x + e / 8)) & ((uint32_t)(t < 0) | drafted) & 1) != 0;
+            });
+        };
         w.load_queries(a.q + (int64_t)(s.first + node) * a.q_row + (int64_t)hq * a.q_head, half);
-        w.await_queries();
-        asm volatile("" : "+v"(see));
         for (int pass = 0; pass <= kKinds; pass++) {
             w.clear();
-            if (pass) first_stages();
+            first_stages();
+            w.await_queries();
+            asm volatile("" : "+v"(see));
             for (int j = run.t0; j < run.t1; j++) {
-                const uint32_t have = chunks_of(j);
-                // step j has landed everywhere, and every wave is done with the stage that step j + STAGES - 1 goes to
-                if (run.t1 - j >= STAGES - 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * N * (STAGES - 2)) : "memory");
-                else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-                if (j + STAGES - 1 < run.t1) stage(j + STAGES - 1);
-                char* tile = lds + j % STAGES * L::STAGE;
-                if (pass) {
-                    keep_tile<DT>(tile + L::KBYTES, L::VBYTES, pass, tid, 64 * W);
-                    __syncthreads();
-                }
-                if (!busy) continue;
-                const int tok0 = j * kKeys + 4 * half;
-                w.step(tile, pass, a.scale2, j * kKeys + kKeys > s.len || have != 15u, [&](int x, int e) {
-                    const int tok = tok0 + 32 * x + 8 * (e / 4) + e % 4, t = tok - s.len;
-                    return (have >> (2 * x + e / 8) & 1) && (t < 0 || (tok < s.total && (see >> (t & 63) & 1)));
-                });
+                land(j, pass);
+                if (busy) w.values(lds + j % STAGES * L::STAGE, scores(j), pass, a.scale2);
             }
+            w.settle();
             // (also: every wave is done with the stages)
             const bool again = __syncthreads_or(pass == 0 && busy && r < rows && w.bad());
             if (r < rows && (pass > 0 || !again)) {
@@ -158,26 +163,28 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void wide_kernel(Args a
     }
 }
 
-template <int DT, int D, int W, int STAGES>
+template <int DT, int D, int KEYS, int W, int STAGES>
 void launch_wide(const Args& a, int per_cu, hipStream_t st) {
-    constexpr int bytes = STAGES * Tile<D>::STAGE;
+    constexpr int bytes = STAGES * Tile<D, KEYS>::STAGE;
+    static_assert((STAGES & (STAGES - 1)) == 0 && STAGES <= 8, "stages by the step's number");
+    const auto kernel = wide_kernel<DT, D, KEYS, W, STAGES>;
     static std::atomic<uint64_t> done{0};  // devices on which the kernel may use so much LDS
     int dev = 0;
     HIP_CHECK(hipGetDevice(&dev));
     if (dev >= 64 || !(done.load(std::memory_order_relaxed) >> dev & 1)) {
-        HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(wide_kernel<DT, D, W, STAGES>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
         if (dev < 64) done.fetch_or(1ull << dev);
     }
-    launch_split<DT, D, kKeys, 32 * W>(a, wide_kernel<DT, D, W, STAGES>, 64 * W, bytes, per_cu, st);
+    launch_split<DT, D, KEYS, 32 * W>(a, kernel, 64 * W, bytes, per_cu, st);
 }
 
 template <int DT>
 void wide(const Args& a, int d, hipStream_t st) {
     CHECK(a.token >= 0 && a.token < 1 << 25, "qe_attn_tree: tokens of the cache %lld bytes apart (below 2^25)", (long long)a.token);
     const int rows = a.max_new * a.group;
-    if (d == 64) rows <= 128 ? launch_wide<DT, 64, 4, 4>(a, 2, st) : launch_wide<DT, 64, 8, 4>(a, 1, st);
-    else if (d == 128) rows <= 128 ? launch_wide<DT, 128, 4, 2>(a, 2, st) : launch_wide<DT, 128, 8, 4>(a, 1, st);
-    else launch_wide<DT, 256, 4, 2>(a, 1, st);
+    if (d == 64) rows <= 128 ? launch_wide<DT, 64, 64, 4, 4>(a, 2, st) : launch_wide<DT, 64, 64, 8, 4>(a, 1, st);
+    else if (d == 128) rows <= 64 ? launch_wide<DT, 128, 64, 4, 4>(a, 1, st) : rows <= 128 ? launch_wide<DT, 128, 64, 4, 2>(a, 2, st) : launch_wide<DT, 128, 64, 8, 4>(a, 1, st);
+    else launch_wide<DT, 256, 32, 4, 4>(a, 1, st);
 }
 void attend_wide(const Args& a, int d, bool f16, hipStream_t st) { f16 ? wide<kAttnF16>(a, d, st) : wide<kAttnBF16>(a, d, st); }
 }  // namespace qe_tree
