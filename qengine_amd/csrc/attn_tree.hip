@@ -15,6 +15,9 @@ namespace qe_tree {
 constexpr int kWaves = 4, kUnit = 128;
 constexpr float kLazy = 8.f;  // the running maximum follows a row's scores once they pass it by this much (2^8 in the sums)
 
+// blocks of the kernel on a CU, by its registers
+constexpr int blocks_of(int nt_d) { return nt_d == 64 ? 3 : nt_d == 128 ? 2 : 1; }
+
 template <int D>
 struct Frag {  // 32 keys of a wave
     static constexpr int KS = D / 32, VD = D / 32;  // 16-byte pieces of a key row per lane; dwords of a value row per lane
@@ -24,7 +27,7 @@ struct Frag {  // 32 keys of a wave
 };
 
 template <int DT, int D, int NT>
-__global__ __launch_bounds__(kThreads, (NT * D <= 128 ? 2 : 1)) void tree_kernel(Args a) {
+__global__ __launch_bounds__(kThreads, blocks_of(NT * D)) void tree_kernel(Args a) {
     using T = AttnT<DT>;
     using F = Frag<D>;
     constexpr int ROWS = 16 * NT, KS = F::KS, VD = F::VD, DT16 = D / 16;
@@ -339,16 +342,17 @@ __global__ __launch_bounds__(kThreads, (NT * D <= 128 ? 2 : 1)) void tree_kernel
 
 template <int DT, int D, int NT>
 void launch(const Args& a, hipStream_t st) {
-    launch_split<DT, D, kUnit, 16 * NT>(a, tree_kernel<DT, D, NT>, kThreads, 0, NT * D <= 128 ? 2 : 1, st);
+    launch_split<DT, D, kUnit, 16 * NT>(a, tree_kernel<DT, D, NT>, kThreads, 0, blocks_of(NT * D), st);
 }
 
-// Up to 32 rows of a kv head (16 for d = 256): this kernel, above: attn_wide.hip.
+// Few rows of a kv head: this kernel, more: attn_wide.hip. 16 sequences of about 4600 tokens, 32 rows a head: d = 128 91 us
+// here, 76 us there; d = 64 41.5 and 44.3 us.
 template <int DT>
 void by_shape(const Args& a, int d, hipStream_t st) {
     const int rows = a.max_new * a.group;
-    if (rows > (d == 256 ? 16 : 32)) attend_wide(a, d, DT == kAttnF16, st);
+    if (rows > (d == 64 ? 32 : 16)) attend_wide(a, d, DT == kAttnF16, st);
     else if (d == 64) rows <= 16 ? launch<DT, 64, 1>(a, st) : launch<DT, 64, 2>(a, st);
-    else if (d == 128) rows <= 16 ? launch<DT, 128, 1>(a, st) : launch<DT, 128, 2>(a, st);
+    else if (d == 128) launch<DT, 128, 1>(a, st);
     else launch<DT, 256, 1>(a, st);
 }
 }  // namespace qe_tree

@@ -183,7 +183,7 @@ void wide(const Args& a, int d, hipStream_t st) {
     CHECK(a.token >= 0 && a.token < 1 << 25, "qe_attn_tree: tokens of the cache %lld bytes apart (below 2^25)", (long long)a.token);
     const int rows = a.max_new * a.group;
     if (d == 64) rows <= 128 ? launch_wide<DT, 64, 64, 4, 4>(a, 2, st) : launch_wide<DT, 64, 64, 8, 4>(a, 1, st);
-    else if (d == 128) rows <= 64 ? launch_wide<DT, 128, 64, 4, 4>(a, 1, st) : rows <= 128 ? launch_wide<DT, 128, 64, 4, 2>(a, 2, st) : launch_wide<DT, 128, 64, 8, 4>(a, 1, st);
+    else if (d == 128) rows <= 128 ? launch_wide<DT, 128, 64, 4, 2>(a, 2, st) : launch_wide<DT, 128, 64, 8, 4>(a, 1, st);
     else launch_wide<DT, 256, 32, 4, 4>(a, 1, st);
 }
 void attend_wide(const Args& a, int d, bool f16, hipStream_t st) { f16 ? wide<kAttnF16>(a, d, st) : wide<kAttnBF16>(a, d, st); }
