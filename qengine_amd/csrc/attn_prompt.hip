@@ -47,18 +47,18 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
     const int kvh = blockIdx.x % a.heads % a.kv_heads, grp = blockIdx.x % a.heads / a.kv_heads;
     const int head = kvh * (a.heads / a.kv_heads) + grp;
     int slot = blockIdx.x / a.heads, b = 0, qb = 0;
-    auto blocks_of = [&](int i) {
-        const int c0 = min(max(a.cu[i], 0), a.t), c1 = min(a.cu[i + 1], a.t);
-        return c1 > c0 ? (c1 - c0 + BQ - 1) / BQ : 0;
-    };
+    auto first_of = [&](int i) { return min(max(a.cu[i], 0), a.t); };
+    auto len_of = [&](int i) { return max(0, min(a.cu[i + 1], a.t) - first_of(i)); };
+    // the first 64 sequences are in every wave's lanes
+    const int lane_first = lane < a.nseq ? first_of(lane) : 0, lane_len = lane < a.nseq ? len_of(lane) : 0;
     if (a.nseq == 1) {
-        qb = blocks_of(0) - 1 - slot;
+        qb = (__builtin_amdgcn_readfirstlane(lane_len) + BQ - 1) / BQ - 1 - slot;
         if (qb < 0) return;
     } else {
-        int* more = reinterpret_cast<int*>(lds);  // blocks of the sequences from the 65th on; every wave holds the first 64
-        const int nb = lane < a.nseq ? blocks_of(lane) : 0;
+        int* more = reinterpret_cast<int*>(lds);  // blocks of the sequences from the 65th on
+        const int nb = (lane_len + BQ - 1) / BQ;
         if (a.nseq > 64) {
-            for (int i = 64 + tid; i < a.nseq; i += 64 * W) more[i - 64] = blocks_of(i);
+            for (int i = 64 + tid; i < a.nseq; i += 64 * W) more[i - 64] = (len_of(i) + BQ - 1) / BQ;
             __syncthreads();
         }
         // blocks with index >= level, over all sequences
@@ -94,8 +94,8 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
     }
     b = __builtin_amdgcn_readfirstlane(b);
     qb = __builtin_amdgcn_readfirstlane(qb);
-    const int c0 = __builtin_amdgcn_readfirstlane(min(max(a.cu[b], 0), a.t));
-    const int len = __builtin_amdgcn_readfirstlane(min(a.cu[b + 1], a.t)) - c0;
+    const int c0 = b < 64 ? __builtin_amdgcn_readlane(lane_first, b) : __builtin_amdgcn_readfirstlane(first_of(b));
+    const int len = b < 64 ? __builtin_amdgcn_readlane(lane_len, b) : __builtin_amdgcn_readfirstlane(len_of(b));
     const int q0 = qb * BQ, qw = q0 + wave * 32;  // the block's and the wave's first row
     const int row = qw + col;                     // this lane's query
 
@@ -205,10 +205,10 @@ void launch(const Args& a, hipStream_t st) {
 
 template <int DT>
 void by_shape(const Args& a, int d, hipStream_t st) {
-    static const int v = getenv("QE_V") ? atoi(getenv("QE_V")) : 0;
-    if (d == 64) v == 1 ? launch<DT, 64, 64, 8, 4>(a, st) : launch<DT, 64, 64, 4, 2>(a, st);
-    else if (d == 128) v == 1 ? launch<DT, 128, 64, 8, 4>(a, st) : launch<DT, 128, 64, 4, 2>(a, st);
-    else v == 1 ? launch<DT, 256, 32, 4, 4>(a, st) : launch<DT, 256, 64, 4, 2>(a, st);
+    // 8 waves and 4 stages, steps of 32 keys: see the measurements above
+    if (d == 64) launch<DT, 64, 64, 4, 2>(a, st);
+    else if (d == 128) launch<DT, 128, 64, 4, 2>(a, st);
+    else launch<DT, 256, 64, 4, 2>(a, st);
 }
 }  // namespace qe_prompt
 

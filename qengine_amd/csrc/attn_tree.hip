@@ -36,15 +36,15 @@ __global__ __launch_bounds__(kThreads, blocks_of(NT * D)) void tree_kernel(Args 
     __shared__ float2 mlbuf[kWaves][16];
     static_assert(sizeof(obuf) >= kMaxTreeBatch * sizeof(int), "the units of all sequences fit the sums' place");
     int* ends = reinterpret_cast<int*>(obuf);
-    __shared__ int tmp[kWaves];
+    __shared__ Kept kept;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, grp = lane >> 4;
 
     int u, u_end, b, base;
-    if (!my_units<kUnit, ROWS, kThreads>(a, ends, tmp, u, u_end, b, base)) return;
+    if (!my_units<kUnit, ROWS, kThreads>(a, ends, kept, u, u_end, b, base)) return;
     while (u < u_end) {
         b = __builtin_amdgcn_readfirstlane(b);
-        const Seq s = seq_of(a, b);
+        const Seq s = seq_at(a, kept, b);
         if (s.n <= 0) {
             if (!a.part) return;
             b++;

@@ -44,6 +44,18 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int b) {
     s.total = ok ? min(s.len + max(s.n, 0), room) : 0;
     return s;
 }
+// What a block keeps of the sequences of a call with up to kKept of them, so that it does not read them again (three
+// dependent reads) for every run that it begins.
+constexpr int kKept = 256;
+struct Kept {
+    Seq seq[kKept];
+    int tmp[16];
+};
+__device__ __forceinline__ Seq seq_at(const Args& a, const Kept& kept, int b) {
+    if (!a.part || a.nseq > kKept) return seq_of(a, b);
+    return kept.seq[b];
+}
+
 template <int ROWS>
 __device__ __forceinline__ int row_blocks(const Args& a, int n) {
     return (n * a.group + ROWS - 1) / ROWS;
@@ -54,9 +66,9 @@ __device__ __forceinline__ int unit_count(int total) {
 }
 
 // The block's units [u, u_end), the sequence of the first and that sequence's first unit; false: none. Every thread of the
-// block calls it; ends (nseq ints of LDS) and tmp are free afterwards.
+// block calls it; ends (nseq ints of LDS) is free afterwards.
 template <int UNIT, int ROWS, int THREADS>
-__device__ __forceinline__ bool my_units(const Args& a, int* ends, int* tmp, int& u, int& u_end, int& b, int& base) {
+__device__ __forceinline__ bool my_units(const Args& a, int* ends, Kept& kept, int& u, int& u_end, int& b, int& base) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (!a.part) {  // a (sequence, head, row block) a block
         u = base = 0;
@@ -69,6 +81,7 @@ __device__ __forceinline__ bool my_units(const Args& a, int* ends, int* tmp, int
         int x = 0;
         if (b0 + tid < a.nseq) {
             const Seq s = seq_of(a, b0 + tid);
+            if (b0 + tid < kKept) kept.seq[b0 + tid] = s;
             if (s.n > 0) x = unit_count<UNIT>(s.total) * row_blocks<ROWS>(a, s.n) * a.kv_heads;
         }
 #pragma unroll
@@ -77,12 +90,12 @@ __device__ __forceinline__ bool my_units(const Args& a, int* ends, int* tmp, int
             if (lane >= o) x += y;
         }
         __syncthreads();
-        if (lane == 63) tmp[wave] = x;
+        if (lane == 63) kept.tmp[wave] = x;
         __syncthreads();
         for (int w = 0; w < THREADS / 64; w++)
-            if (w < wave) x += tmp[w];
+            if (w < wave) x += kept.tmp[w];
         if (b0 + tid < a.nseq) ends[b0 + tid] = carry + x;
-        for (int w = 0; w < THREADS / 64; w++) carry += tmp[w];
+        for (int w = 0; w < THREADS / 64; w++) carry += kept.tmp[w];
     }
     __syncthreads();
     const int range = (carry + gridDim.x - 1) / gridDim.x;

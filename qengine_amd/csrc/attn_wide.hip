@@ -23,7 +23,7 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void wide_kernel(Args a
     extern __shared__ char lds[];
     static_assert(STAGES * L::STAGE >= kMaxTreeBatch * (int)sizeof(int), "the units of all sequences fit the stages' place");
     int* ends = reinterpret_cast<int*>(lds);
-    __shared__ int tmp[W];
+    __shared__ Kept kept;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
     const unsigned lds32 = (unsigned)(uintptr_t)lds;
@@ -41,10 +41,10 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void wide_kernel(Args a
     if (W > 4 && wave >= W / 2) __builtin_amdgcn_s_setprio(1);  // one of a SIMD's two waves ahead: its softmax beside the other's products
 
     int u, u_end, b, base;
-    if (!my_units<KEYS, ROWS, 64 * W>(a, ends, tmp, u, u_end, b, base)) return;
+    if (!my_units<KEYS, ROWS, 64 * W>(a, ends, kept, u, u_end, b, base)) return;
     while (u < u_end) {
         b = __builtin_amdgcn_readfirstlane(b);
-        Seq s = seq_of(a, b);
+        Seq s = seq_at(a, kept, b);
         s.first = __builtin_amdgcn_readfirstlane(s.first);
         s.n = __builtin_amdgcn_readfirstlane(s.n);
         s.total = __builtin_amdgcn_readfirstlane(s.total);
