@@ -35,10 +35,12 @@ __device__ __forceinline__ int wave_sum(int x) {  // the same in every lane
     return __builtin_amdgcn_readlane(x, 15) + __builtin_amdgcn_readlane(x, 31) + __builtin_amdgcn_readlane(x, 47) + __builtin_amdgcn_readlane(x, 63);
 }
 
-template <int DT, int D, int KEYS, int W, int STAGES>
-__global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args a) {
+// RW waves take 32 rows each; KG groups of RW waves take every KG-th step, each with two stages of its own, and the first
+// group adds the others' sums at the end (short prompts: the steps of a block follow each other, so its time is theirs).
+template <int DT, int D, int KEYS, int RW, int KG>
+__global__ __launch_bounds__(64 * RW * KG, (D == 256 ? 1 : 2)) void prompt_kernel(Args a) {
     using L = Tile<D, KEYS>;
-    constexpr int BQ = 32 * W;
+    constexpr int W = RW * KG, BQ = 32 * RW;
     extern __shared__ char lds[];  // two stages of K and V tiles; before them the block counts
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
@@ -96,7 +98,8 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
     qb = __builtin_amdgcn_readfirstlane(qb);
     const int c0 = b < 64 ? __builtin_amdgcn_readlane(lane_first, b) : __builtin_amdgcn_readfirstlane(first_of(b));
     const int len = b < 64 ? __builtin_amdgcn_readlane(lane_len, b) : __builtin_amdgcn_readfirstlane(len_of(b));
-    const int q0 = qb * BQ, qw = q0 + wave * 32;  // the block's and the wave's first row
+    const int rw = wave % RW, kg = wave / RW;
+    const int q0 = qb * BQ, qw = q0 + rw * 32;    // the block's and the wave's first row
     const int row = qw + col;                     // this lane's query
 
     const unsigned lds32 = (unsigned)(uintptr_t)lds;
@@ -104,23 +107,24 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
     const char* vb = a.v + (int64_t)c0 * a.v_row + (int64_t)kvh * a.v_head;
     // A wave instruction fills 1 KB: RK rows; the wave's n-th starts RK n rows behind its first. Lane i lands at piece i, so
     // it loads the piece that belongs there: of K the same in all instructions, of V in every second one (d = 256) or all.
-    constexpr int N = KEYS / L::RK / W, NV = D == 256 ? 2 : 1;
-    const int r_wave = wave * N * L::RK, r_lane = lane / L::CH;
+    constexpr int N = KEYS / L::RK / RW, NV = D == 256 ? 2 : 1;
+    const int r_wave = rw * N * L::RK, r_lane = lane / L::CH;
     const uint32_t k_off = (uint32_t)r_lane * (uint32_t)a.k_row + ((lane % L::CH) ^ L::kx(r_lane)) * 16;
     uint32_t v_off[NV];
 #pragma unroll
     for (int i = 0; i < NV; i++) v_off[i] = (uint32_t)r_lane * (uint32_t)a.v_row + ((lane % L::CH) ^ L::vx(i * L::RK + r_lane)) * 16;
+    auto at_of = [&](int j) { return (kg * 2 + j / KG % 2) * L::STAGE; };  // step j is one of the wave's group
     auto stage = [&](int j) {
         j = __builtin_amdgcn_readfirstlane(j);
         const char* ks = kb + (int64_t)(j * KEYS + r_wave) * a.k_row;
         const char* vs = vb + (int64_t)(j * KEYS + r_wave) * a.v_row;
-        const unsigned at = lds32 + j % STAGES * L::STAGE;
+        const unsigned at = lds32 + at_of(j);
         const int over = (j + 1) * KEYS - len;
         if (over <= 0) {
 #pragma unroll
-            for (int i = 0; i < N; i++) dma16_at(ks + i * L::RK * a.k_row, k_off, at + (wave * N + i) * (1024 + L::PAD));
+            for (int i = 0; i < N; i++) dma16_at(ks + i * L::RK * a.k_row, k_off, at + (rw * N + i) * (1024 + L::PAD));
 #pragma unroll
-            for (int i = 0; i < N; i++) dma16_at(vs + i * L::RK * a.v_row, v_off[i % NV], at + L::KBYTES + (wave * N + i) * 1024);
+            for (int i = 0; i < N; i++) dma16_at(vs + i * L::RK * a.v_row, v_off[i % NV], at + L::KBYTES + (rw * N + i) * 1024);
             return;
         }
         // keys past the end re-read the last one (no row sees them)
@@ -129,29 +133,14 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const int r = r_wave + i * L::RK + r_lane, key = min(r, KEYS - 1 - over);
-            dma16_at(k0, (uint32_t)key * (uint32_t)a.k_row + ((lane % L::CH) ^ L::kx(r)) * 16, at + (wave * N + i) * (1024 + L::PAD));
-            dma16_at(v0, (uint32_t)key * (uint32_t)a.v_row + ((lane % L::CH) ^ L::vx(r)) * 16, at + L::KBYTES + (wave * N + i) * 1024);
+            dma16_at(k0, (uint32_t)key * (uint32_t)a.k_row + ((lane % L::CH) ^ L::kx(r)) * 16, at + (rw * N + i) * (1024 + L::PAD));
+            dma16_at(v0, (uint32_t)key * (uint32_t)a.v_row + ((lane % L::CH) ^ L::vx(r)) * 16, at + L::KBYTES + (rw * N + i) * 1024);
         }
     };
     const int steps = (min(len, q0 + BQ) + KEYS - 1) / KEYS;
     const int mine = qw < len ? (min(len, qw + 32) + KEYS - 1) / KEYS : 0;  // steps with keys that this wave's rows see
-    constexpr int AHEAD = STAGES - 1;  // steps that are under way while one is worked on
-    auto first_stages = [&] {
-#pragma unroll 1
-        for (int i = 0; i < min(AHEAD, steps); i++) stage(i);
-    };
-    auto land = [&](int j, int pass) {  // step j is in LDS for every wave, and all are done with the stage that the next step takes
-        if (steps - j >= AHEAD) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(2 * N * (AHEAD - 1)) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        if (j + AHEAD < steps) stage(j + AHEAD);
-        if (pass) {
-            keep_tile<DT>(lds + j % STAGES * L::STAGE + L::KBYTES, L::VBYTES, pass, tid, 64 * W);
-            __syncthreads();
-        }
-    };
     Wave32<DT, D, KEYS> w;
     w.places(lane);
-    if (W > 4 && wave >= W / 2) __builtin_amdgcn_s_setprio(1);  // one of a SIMD's two waves ahead: its softmax beside the other's products
     w.load_queries(a.q + (int64_t)(c0 + min(row, len - 1)) * a.q_row + (int64_t)head * a.q_head, half);
     char* out = a.out + (int64_t)(c0 + row) * a.o_row + (int64_t)head * a.o_head + half * 8;
     // A value that is not finite in a key that some rows of a step must not see makes those rows' sums NaN (0 times it).
@@ -159,24 +148,32 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
     // then over each kind of the others (keep_tile).
     for (int pass = 0; pass <= kKinds; pass++) {
         w.clear();
-        first_stages();
+        if (kg < steps) stage(kg);
         w.await_queries();
-        auto scores = [&](int j) {
+        for (int i = 0; i < steps; i += KG) {
+            const int j = i + kg;
+            // every group's step has landed, and all waves are done with the stages that the next ones take
+            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            if (j + KG < steps) stage(j + KG);
+            char* tile = lds + at_of(j);
+            if (pass) {
+                if (j < steps) keep_tile<DT>(tile + L::KBYTES, L::VBYTES, pass, tid % (64 * RW), 64 * RW);
+                __syncthreads();
+            }
             const int first = j * KEYS + 4 * half - row;  // key - row of the lane's first score
-            return w.scores(lds + j % STAGES * L::STAGE, j * KEYS + KEYS - 1 > qw, [&](int x, int e) { return first + 32 * x + 8 * (e / 4) + e % 4 <= 0; });
-        };
-        for (int j = 0; j < steps; j++) {
-            land(j, pass);
-            if (j < mine) w.values(lds + j % STAGES * L::STAGE, scores(j), pass, a.scale2);
+            if (j < mine)
+                w.values(tile, w.scores(tile, j * KEYS + KEYS - 1 > qw, [&](int x, int e) { return first + 32 * x + 8 * (e / 4) + e % 4 <= 0; }),
+                         pass, a.scale2);
         }
         w.settle();
+        if constexpr (KG > 1) w.add_groups(reinterpret_cast<float*>(lds), rw, kg, RW, KG, lane, pass);
         // (also: every wave is done with the stages)
-        const bool again = __syncthreads_or(pass == 0 && row < len && w.bad());
+        const bool again = __syncthreads_or(pass == 0 && kg == 0 && row < len && w.bad());
         if (pass > 1) {
-            if (row < len) w.store_kind(out, pass);
+            if (kg == 0 && row < len) w.store_kind(out, pass);
         } else if (!again) {
             const float l = sum_over_halves(w.l);
-            if (row < len) {
+            if (kg == 0 && row < len) {
                 w.store(out, l == 0.f ? 0.f : 1.f / l);
                 if (a.lse && half == 0) a.lse[(int64_t)(c0 + row) * a.heads + head] = l == 0.f ? kNegInf : (w.m + log2f(l)) * kLn2;
             }
@@ -185,13 +182,13 @@ __global__ __launch_bounds__(64 * W, (D == 256 ? 1 : 2)) void prompt_kernel(Args
     }
 }
 
-template <int DT, int D, int KEYS, int W, int STAGES>
+template <int DT, int D, int KEYS, int RW, int KG>
 void launch(const Args& a, hipStream_t st) {
-    constexpr int BQ = 32 * W, bytes = STAGES * Tile<D, KEYS>::STAGE;
-    static_assert(bytes >= kMaxSeqs * (int)sizeof(int) && (STAGES & (STAGES - 1)) == 0, "block counts fit; stages by the step's number");
+    constexpr int BQ = 32 * RW, bytes = 2 * KG * Tile<D, KEYS>::STAGE;
+    static_assert(bytes >= kMaxSeqs * (int)sizeof(int) && bytes >= Wave32<DT, D, KEYS>::group_bytes(RW, KG), "block counts and groups' sums fit");
     const int64_t blocks = ((int64_t)a.t / BQ + a.nseq) * a.heads;
     CHECK(blocks < (int64_t)1 << 31, "qe_attn_prompt: %lld blocks", (long long)blocks);
-    const auto kernel = prompt_kernel<DT, D, KEYS, W, STAGES>;
+    const auto kernel = prompt_kernel<DT, D, KEYS, RW, KG>;
     static std::atomic<uint64_t> done{0};  // devices on which the kernel may use so much LDS
     int dev = 0;
     HIP_CHECK(hipGetDevice(&dev));
@@ -199,16 +196,21 @@ void launch(const Args& a, hipStream_t st) {
         HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
         if (dev < 64) done.fetch_or(1ull << dev);
     }
-    kernel<<<(int)blocks, 64 * W, bytes, st>>>(a);
+    kernel<<<(int)blocks, 64 * RW * KG, bytes, st>>>(a);
     HIP_CHECK(hipGetLastError());
 }
 
 template <int DT>
 void by_shape(const Args& a, int d, hipStream_t st) {
-    // 8 waves and 4 stages, steps of 32 keys: see the measurements above
-    if (d == 64) launch<DT, 64, 64, 4, 2>(a, st);
-    else if (d == 128) launch<DT, 128, 64, 4, 2>(a, st);
-    else launch<DT, 256, 64, 4, 2>(a, st);
+    // Blocks of 64 rows in four (two for d = 256) groups that share out the keys, while they fill the CUs once, or twice where
+    // prompts are long: a block's time is its steps, of which the last rows' has most. us, blocks of 128 rows / these: 2000
+    // rows of 8 heads over 1 43.2 / 26.6, 4000 81 / 54, of 40 heads over 8 300 rows 11.6 / 10.8, 500 16.7 / 18.0, 1000 29.4 /
+    // 35.0; d = 256, 16 heads over 2 1000 44.7 / 35.9, 2000 84 / 75, 4000 183 / 251; d = 64 2000 32 / 22, 6000 107 / 125.
+    const int64_t blocks = ((int64_t)a.t / 64 + a.nseq) * a.heads, cus = qe_num_cus();
+    const bool few = blocks <= cus || (blocks <= 2 * cus && a.t >= (int64_t)1000 * a.nseq);
+    if (d == 64) few ? launch<DT, 64, 64, 2, 4>(a, st) : launch<DT, 64, 64, 4, 1>(a, st);
+    else if (d == 128) few ? launch<DT, 128, 32, 2, 4>(a, st) : launch<DT, 128, 64, 4, 1>(a, st);
+    else few ? launch<DT, 256, 32, 2, 2>(a, st) : launch<DT, 256, 64, 4, 1>(a, st);
 }
 }  // namespace qe_prompt
 

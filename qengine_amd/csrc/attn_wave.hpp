@@ -176,6 +176,43 @@ struct Wave32 {
 #pragma unroll
         for (int d = 0; d < DB; d++) asm volatile("" : "+v"(o[d]));
     }
+    // The sums of `groups` waves with the same rows into the first one's, through LDS: every lane's partner holds the same
+    // rows and columns. Every wave of the block calls it.
+    static constexpr int group_bytes(int waves, int groups) { return (groups - 1) * waves * (DB * 16 + 2) * 256; }
+    __device__ __forceinline__ void add_groups(float* lds, int wave, int group, int waves, int groups, int lane, int pass) {
+        __syncthreads();  // all are done with the stages
+        auto at = [&](int g, int i) { return lds + (((g - 1) * waves + wave) * (DB * 16 + 2) + i) * 64 + lane; };
+        if (group > 0) {
+            *at(group, 0) = m;
+            *at(group, 1) = l;
+#pragma unroll
+            for (int d = 0; d < DB; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) *at(group, 2 + d * 16 + e) = o[d][e];
+        }
+        __syncthreads();
+        if (group == 0) {
+            float top = m;
+            for (int g = 1; g < groups; g++) top = fmaxf(top, *at(g, 0));
+            for (int g = 0; g < groups; g++) {
+                const float mg = g ? *at(g, 0) : m;
+                float f = mg == kNegInf ? 0.f : __builtin_amdgcn_exp2f(mg - top);
+                if (mg == __builtin_huge_valf() || pass > 1) f = 1.f;  // (a row with such a maximum is NaN already)
+                if (g == 0) {
+                    l *= f;
+#pragma unroll
+                    for (int d = 0; d < DB; d++) o[d] *= f;
+                } else {
+                    l += f * *at(g, 1);
+#pragma unroll
+                    for (int d = 0; d < DB; d++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[d][e] += f * *at(g, 2 + d * 16 + e);
+                }
+            }
+            m = top;
+        }
+    }
     // whether a sum is not finite
     __device__ __forceinline__ bool bad() const {
         float x = 0.f;
