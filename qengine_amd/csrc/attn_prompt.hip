@@ -38,7 +38,7 @@ __device__ __forceinline__ int wave_sum(int x) {  // the same in every lane
 // RW waves take 32 rows each; KG groups of RW waves take every KG-th step, each with two stages of its own, and the first
 // group adds the others' sums at the end (short prompts: the steps of a block follow each other, so its time is theirs).
 template <int DT, int D, int KEYS, int RW, int KG>
-__global__ __launch_bounds__(64 * RW * KG, (D == 256 ? 1 : 2)) void prompt_kernel(Args a) {
+__global__ __launch_bounds__(64 * RW * KG, (D == 256 ? 1 : KG == 1 && KEYS == 32 ? 3 : 2)) void prompt_kernel(Args a) {
     using L = Tile<D, KEYS>;
     constexpr int W = RW * KG, BQ = 32 * RW;
     extern __shared__ char lds[];  // two stages of K and V tiles; before them the block counts
@@ -208,8 +208,13 @@ void by_shape(const Args& a, int d, hipStream_t st) {
     // 35.0; d = 256, 16 heads over 2 1000 44.7 / 35.9, 2000 84 / 75, 4000 183 / 251; d = 64 2000 32 / 22, 6000 107 / 125.
     const int64_t blocks = ((int64_t)a.t / 64 + a.nseq) * a.heads, cus = qe_num_cus();
     const bool few = blocks <= cus || (blocks <= 2 * cus && a.t >= (int64_t)1000 * a.nseq);
-    if (d == 64) few ? launch<DT, 64, 64, 2, 4>(a, st) : launch<DT, 64, 64, 4, 1>(a, st);
-    else if (d == 128) few ? launch<DT, 128, 32, 2, 4>(a, st) : launch<DT, 128, 64, 4, 1>(a, st);
+    // Else blocks of 128 rows. Steps of 32 keys take registers and LDS for three blocks a CU instead of two: us of 64 / 32
+    // keys, 40 heads over 8: d = 128 20 prompts of 53 to 1451 rows 110 / 100, 64 of 128 67 / 56, one of 8192 629 / 621; d = 64
+    // 20 of 410 55.3 / 51.7, one of 8192 367 / 374.
+    const bool lengthy = a.t >= (int64_t)2000 * a.nseq;
+    const bool loose = ((int64_t)a.t / 128 + a.nseq) * a.heads <= 2 * cus;  // a block's own time counts: 1000 rows 28.5 / 31.0
+    if (d == 64) few ? launch<DT, 64, 64, 2, 4>(a, st) : lengthy ? launch<DT, 64, 64, 4, 1>(a, st) : launch<DT, 64, 32, 4, 1>(a, st);
+    else if (d == 128) few ? launch<DT, 128, 32, 2, 4>(a, st) : loose ? launch<DT, 128, 64, 4, 1>(a, st) : launch<DT, 128, 32, 4, 1>(a, st);
     else few ? launch<DT, 256, 32, 2, 2>(a, st) : launch<DT, 256, 64, 4, 1>(a, st);
 }
 }  // namespace qe_prompt

@@ -70,7 +70,7 @@ struct Wave32 {
     __device__ __forceinline__ Scores scores(const char* tile, bool masked, Seen seen) const {
         Scores r;
         f32x16_v(&s)[NX] = r.s;
-        constexpr int GK = D == 256 ? 4 : 8, NK = NX * KS / GK;
+        constexpr int GK = D == 256 ? 4 : NX == 1 ? 2 : 8, NK = NX * KS / GK;
         u32x4_v kf[2][GK];
         auto read_k = [&](int g) {
 #pragma unroll
@@ -106,7 +106,7 @@ struct Wave32 {
     // Softmax of the scores and their products with the step's values, whose first reads are under way during the softmax
     __device__ __forceinline__ void values(const char* tile, const Scores& r, int pass, float scale2) {
         const f32x16_v(&s)[NX] = r.s;
-        constexpr int GV = 4, NV = DB * 2 * NX / GV;
+        constexpr int GV = NX == 1 ? 2 : 4, NV = DB * 2 * NX / GV;
         u32x4_v vf[2][GV];
         auto read_v = [&](int g) {
 #pragma unroll
