@@ -31,6 +31,7 @@ HEAD_DIMS = (64, 128, 256)
 MAX_SEQS = 4096
 _TYPES = (torch.bfloat16, torch.float16)
 _FN = {}
+_STRIDES = {}
 _current = torch._C._cuda_getDevice
 _stream_of = torch._C._cuda_getCurrentRawStream
 
@@ -80,7 +81,8 @@ def _starts(cu, at):
     shape = cu.shape
     if len(shape) != 1 or shape[0] < 1:
         raise ValueError(f"cu has one more entry than there are sequences, got shape {tuple(shape)}")
-    _ints("cu", cu, shape, at)
+    if cu.dtype is not torch.int32 or not cu.is_contiguous() or cu.get_device() != at:
+        _ints("cu", cu, shape, at)
     return shape[0] - 1
 
 
@@ -188,10 +190,13 @@ class KVCache:
                        torch.zeros(slots, **ints), torch.zeros(slots, **ints), torch.zeros(pages, **ints))
 
     def _batch(self, name, t, n=None):
-        if t.dim() != 1:
-            raise ValueError(f"{name} has one dimension, got shape {tuple(t.shape)}")
-        n = t.shape[0] if n is None else n
-        _ints(name, t, (n,), self._dev)
+        shape = t.shape
+        if len(shape) != 1:
+            raise ValueError(f"{name} has one dimension, got shape {tuple(shape)}")
+        if n is None:
+            n = shape[0]
+        if t.dtype is not torch.int32 or shape[0] != n or not t.is_contiguous() or t.get_device() != self._dev:
+            _ints(name, t, (n,), self._dev)
         return n
 
     def _few(self, n):
@@ -233,23 +238,28 @@ class KVCache:
     def append(self, layer, k, v, seqs, cu):
         """New rows k, v [t][kv heads][d] of one layer, or [layers][t][kv heads][d] of all (layer None): rows cu[b] ..
         cu[b + 1] - 1 go behind the committed tokens of slot seqs[b], into pages reserved before. Slots are distinct."""
-        dims = 4 if layer is None else 3
+        one = layer is not None
+        dims, shape = (3, k.shape) if one else (4, k.shape)
         _rows("k", k, dims, self.dtype, self._dev)
         _rows("v", v, dims, self.dtype, self._dev)
-        t = k.shape[-3]
-        if k.shape != v.shape or k.shape[-2:] != (self.kv_heads, self.d) or (layer is None and k.shape[0] != self.layers):
-            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} are rows of {self.kv_heads} kv heads of {self.d}"
-                             + (f", of {self.layers} layers" if layer is None else ""))
-        if layer is not None and not 0 <= layer < self.layers:
+        if v.shape != shape or shape[-2] != self.kv_heads or shape[-1] != self.d or not (one or shape[0] == self.layers):
+            raise ValueError(f"k {tuple(shape)} and v {tuple(v.shape)} are rows of {self.kv_heads} kv heads of {self.d}"
+                             + ("" if one else f", of {self.layers} layers"))
+        if one and not 0 <= layer < self.layers:
             raise ValueError(f"layer {layer} of {self.layers}")
-        n = _starts(cu, self._dev)
+        n, t = _starts(cu, self._dev), shape[-3]
         self._batch("seqs", seqs, n)
         if t and n:
             ks, vs = k.stride(), v.stride()
-            one = layer is not None
-            strides = (ctypes.c_int64 * 6)(0 if one else ks[0], ks[-3], ks[-2], 0 if one else vs[0], vs[-3], vs[-2])
+            key = (ks[0], ks[-3], ks[-2], vs[0], vs[-3], vs[-2], one)
+            strides = _STRIDES.get(key)  # the C arrays of the strides that have come up
+            if strides is None:
+                if len(_STRIDES) > 255:
+                    _STRIDES.clear()
+                c = (ctypes.c_int64 * 6)(0 if one else ks[0], ks[-3], ks[-2], 0 if one else vs[0], vs[-3], vs[-2])
+                strides = _STRIDES[key] = (ctypes.addressof(c), c)
             _run(self._dev, "qe_kv_append", "piipppppiip", self._at, layer if one else 0, 1 if one else self.layers,
-                 k.data_ptr(), v.data_ptr(), ctypes.addressof(strides), seqs.data_ptr(), cu.data_ptr(), n, t)
+                 k.data_ptr(), v.data_ptr(), strides[0], seqs.data_ptr(), cu.data_ptr(), n, t)
 
     def accept(self, seqs, count, path=None, length=None):
         """count[i] drafted tokens of slot seqs[i] are committed: the first ones, or those of path int32 [n][at most 64], whose
@@ -285,7 +295,7 @@ class KVCache:
         if not 1 <= most <= MAX_NODES:
             raise ValueError(f"1 to {MAX_NODES} drafted tokens a sequence, got {most}")
         n = _starts(cu, at)
-        _ints("seqs", seqs, (n,), at)
+        self._batch("seqs", seqs, n)
         if n > MAX_SEQS:
             raise ValueError(f"at most {MAX_SEQS} sequences, got {n}")
         if mask is not None:
