@@ -349,8 +349,8 @@ void qe_moe_pack_w4(const int32_t* gu_q, const uint16_t* gu_s, const int32_t* dn
  * host synchronization, and can be captured. Deterministic: same inputs, same bits. ---- */
 
 /* Causal attention over whole prompts packed without padding: sequence b is rows cu[b] .. cu[b + 1] - 1 (cu [nseq + 1]
- * int32, ascending), row i of it sees rows 0 .. i. Rows of q, k, v and out have strides of their own, so views into one
- * fused QKV product do. Rows before cu[0] and from cu[nseq] on are left as they were. flags: QE_F16. */
+ * int32, ascending), row i of it sees rows 0 .. i. Rows of q, k, v and out have strides of their own (k_row, v_row below
+ * 2^24), so views into one fused QKV product do; out overlaps none of them. nseq <= 4096. Rows before cu[0] and from cu[nseq] on are left as they were. flags: QE_F16. */
 void qe_attn_prompt(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                     const void* v, int64_t v_row, int64_t v_head, void* out, int64_t out_row, int64_t out_head, float* lse,
                     const int32_t* cu, int nseq, int t, int heads, int kv_heads, int d, float scale, int flags,
@@ -361,7 +361,8 @@ void qe_attn_prompt(const void* q, int64_t q_row, int64_t q_head, const void* k,
  *   length  committed tokens of a slot; rows appended after them are drafted until qe_kv_accept commits them
  *   held    pages of a slot (table[s][0 .. held - 1]; the rest -1)
  *   ref     how many slots hold a page, 0: free
- * Start: table -1, the others 0. page: a power of two, 16 .. 1024. k and v share the strides. */
+ * Start: table -1, the others 0. page: a power of two, 16 .. 1024; width * page at most 2^30. k and v share the strides,
+ * token_stride is below 2^24, pages below 2^29. */
 typedef struct qe_kv_cache {
     void* k;
     void* v;
@@ -408,6 +409,9 @@ void qe_kv_accept(const qe_kv_cache_t* cache, const int32_t* seqs, const int32_t
 void qe_attn_tree(const qe_kv_cache_t* cache, int layer, const void* q, int64_t q_row, int64_t q_head, void* out,
                   int64_t out_row, int64_t out_head, float* lse, const int32_t* seqs, const int32_t* cu, int nseq, int t,
                   int max_new, const uint64_t* mask, int heads, float scale, void* stream);
+/* test hook: 0: later qe_attn_tree calls do not split a sequence's tokens over blocks (what they do by themselves where the
+ * device has no memory for the parts); the same results within fp32 rounding. No counterpart in the reference. */
+void qe_attn_tree_set_split(int on);
 
 /* ---- on-disk weights: .safetensors files (host, memory-mapped) and the quantized-matrix loader ----
  * qe_st_open maps a file and indexes its tensors by name (reference SafeTensors::open, src/safetensors.h:40; a

@@ -162,10 +162,12 @@ class KVCache:
         if k.shape != v.shape or k.stride() != v.stride() or not k.numel():
             raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} have the same shape and strides")
         layers, pages, kv, page, d = k.shape
-        if d not in HEAD_DIMS or page < 16 or page > 1024 or page & (page - 1) or kv > 1024:
+        if k.stride(3) >= 1 << 24:
+            raise ValueError(f"tokens of a page are less than 2^24 elements apart, got {k.stride(3)}")
+        if d not in HEAD_DIMS or pages >= 1 << 29 or page < 16 or page > 1024 or page & (page - 1) or kv > 1024:
             raise ValueError(f"pools [layers][pages][kv heads][page][d] with d of {HEAD_DIMS}, at most 1024 kv heads and pages of "
                              f"16 to 1024 tokens, a power of two: got {tuple(k.shape)}")
-        if table.dim() != 2 or not table.numel() or table.shape[1] * page >= 2 ** 31:
+        if table.dim() != 2 or not table.numel() or table.shape[1] * page > 2 ** 30:
             raise ValueError(f"table is [slots][pages of a slot], got {tuple(table.shape)}")
         slots, width = table.shape
         _ints("table", table, table.shape, device)

@@ -234,7 +234,7 @@ void launch_split(Args a, Kernel kernel, int threads, size_t lds, int per_cu, hi
     const int grid = (int)std::min<int64_t>(runs * most_units, per_cu * qe_num_cus());
     const size_t part = (size_t)grid * 2 * ROWS * D * 4, ml = (size_t)grid * 2 * ROWS * 8, ends = ((size_t)a.nseq + 1) * 4;
     WsHold hold(st);
-    if (char* ws = static_cast<char*>(hold.get(kWsAttn, part + ml + ends))) {
+    if (char* ws = attn_tree_split() ? static_cast<char*>(hold.get(kWsAttn, part + ml + ends)) : nullptr) {
         a.part = reinterpret_cast<float*>(ws);
         a.ml = reinterpret_cast<float2*>(ws + part);
         a.ends = reinterpret_cast<int*>(ws + part + ml);

@@ -178,9 +178,10 @@ void launch_wide(const Args& a, int per_cu, hipStream_t st) {
     launch_split<DT, D, KEYS, 32 * W>(a, kernel, 64 * W, bytes, per_cu, st);
 }
 
+// 128 rows a block: two blocks a CU, a step of 64 keys each on its way (three blocks of 32 keys: 32 sequences of 8 drafted
+// tokens in groups of 5 115 -> 127 us; one block with three steps on their way 129). More rows: one block of 8 waves.
 template <int DT>
 void wide(const Args& a, int d, hipStream_t st) {
-    CHECK(a.token >= 0 && a.token < 1 << 25, "qe_attn_tree: tokens of the cache %lld bytes apart (below 2^25)", (long long)a.token);
     const int rows = a.max_new * a.group;
     if (d == 64) rows <= 128 ? launch_wide<DT, 64, 64, 4, 4>(a, 2, st) : launch_wide<DT, 64, 64, 8, 4>(a, 1, st);
     else if (d == 128) rows <= 128 ? launch_wide<DT, 128, 64, 4, 2>(a, 2, st) : launch_wide<DT, 128, 64, 8, 4>(a, 1, st);

@@ -24,6 +24,7 @@
 namespace {
 std::atomic<int> g_out_bf16{0};
 std::atomic<int> g_sk_maxparts{0};
+std::atomic<bool> g_attn_split{true};
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 inline W4 mk_w4(const void* q, const void* s, int n, int k, bool glu, int sdt) {
     W4 w;
@@ -51,6 +52,8 @@ void gemm_set_out_bf16(bool on) { g_out_bf16.store(on ? 1 : 0); }
 bool gemm_out_bf16() { return g_out_bf16.load() != 0; }
 void gemm_set_sk_maxparts(int n) { g_sk_maxparts.store(n > 0 ? n : 0); }
 int gemm_sk_maxparts() { return g_sk_maxparts.load(); }
+void attn_tree_set_split(bool on) { g_attn_split.store(on); }
+bool attn_tree_split() { return g_attn_split.load(); }
 
 extern "C" {
 
@@ -416,5 +419,7 @@ void qe_attn_tree(const qe_kv_cache_t* cache, int layer, const void* q, int64_t 
     attn_tree(*cache, layer, {q, out, lse, q_row, q_head, out_row, out_head, seqs, cu, nseq, t, max_new, mask, heads, scale},
               as_stream(st));
 }
+
+void qe_attn_tree_set_split(int on) { attn_tree_set_split(on != 0); }
 
 }  // extern "C"

@@ -27,29 +27,31 @@ Slots slots_of(const qe_kv_cache_t& c) {
     return {c.table, c.length, c.held, c.ref, c.slots, c.width, c.pages, log2_of(c.page)};
 }
 
+// sums stop below 2^30, above the number of pages: 1024 entries may ask for more than 2^31
+constexpr int kMost = (1 << 30) - 1;
 __device__ __forceinline__ int wave_incl_scan(int x) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
         const int y = __shfl_up(x, o);
-        if (lane >= o) x += y;
+        if (lane >= o) x = min(x + y, kMost);
     }
     return x;
 }
-// sum over the threads before this one, and over all in *total (every thread calls it)
+// sum over the threads up to this one, and over all in *total (every thread calls it)
 template <int NT>
-__device__ int block_excl_scan(int x, int* tmp, int* total) {
+__device__ int block_incl_scan(int x, int* tmp, int* total) {
     const int incl = wave_incl_scan(x), w = threadIdx.x >> 6;
     __syncthreads();
     if ((threadIdx.x & 63) == 63) tmp[w] = incl;
     __syncthreads();
     int before = 0, all = 0;
     for (int i = 0; i < NT / 64; i++) {
-        if (i < w) before += tmp[i];
-        all += tmp[i];
+        if (i < w) before = min(before + tmp[i], kMost);
+        all = min(all + tmp[i], kMost);
     }
     *total = all;
-    return before + incl - x;
+    return min(before + incl, kMost);
 }
 
 // One block for the whole call: what entry i needs is known from its own slot, where its pages lie in the order of free
@@ -82,8 +84,8 @@ __global__ __launch_bounds__(kOne) void reserve_kernel(Slots s, const int32_t* _
         }
     }
     int total, n_free;
-    const int first = block_excl_scan<kOne>(need, tmp, &total);
-    end_of[i] = first + need;
+    const int end = block_incl_scan<kOne>(need, tmp, &total);
+    end_of[i] = end;
     cow_of[i] = old >= 0;
     fresh_of[i] = -1;
     // the free pages of this thread's range; whole 16 bytes of ref where the pool has them
@@ -99,14 +101,14 @@ __global__ __launch_bounds__(kOne) void reserve_kernel(Slots s, const int32_t* _
             }
         for (; p < p1; p++) mine += s.ref[p] == 0;
     }
-    int rank = block_excl_scan<kOne>(mine, tmp, &n_free);
-    const bool ok = valid && (need == 0 || first + need <= n_free);
+    int rank = block_incl_scan<kOne>(mine, tmp, &n_free) - mine;
+    const bool ok = valid && (need == 0 || end <= n_free);
     // entries are served up to the first that does not fit: the sums only grow
     int given = __syncthreads_or(!ok && need > 0) ? 0 : total;
     if (given == 0 && total > 0) {
         if (i == 0) tmp[0] = 0;
         __syncthreads();
-        if (ok && need > 0) atomicMax(&tmp[0], first + need);
+        if (ok && need > 0) atomicMax(&tmp[0], end);
         __syncthreads();
         given = tmp[0];
         __syncthreads();
@@ -130,7 +132,7 @@ __global__ __launch_bounds__(kOne) void reserve_kernel(Slots s, const int32_t* _
     __syncthreads();
     const bool copied = ok && old >= 0;
     int n_copies;
-    const int c = block_excl_scan<kOne>(copied, tmp, &n_copies);
+    const int c = block_incl_scan<kOne>(copied, tmp, &n_copies) - copied;
     if (copied) {
         s.table[(int64_t)slot * s.width + (len >> s.shift)] = fresh_of[i];
         atomicSub(&s.ref[old], 1);
@@ -322,7 +324,9 @@ void kv_check(const qe_kv_cache_t* c, const char* who) {
     CHECK(c->page >= 16 && c->page <= 1024 && (c->page & (c->page - 1)) == 0, "%s: page %d (a power of two, 16 .. 1024)", who, c->page);
     CHECK(c->layer_stride % 8 == 0 && c->page_stride % 8 == 0 && c->head_stride % 8 == 0 && c->token_stride % 8 == 0,
           "%s: cache strides must be multiples of 8", who);
-    CHECK((int64_t)c->width * c->page < (int64_t)1 << 31, "%s: width %d pages of %d pass 2^31 tokens", who, c->width, c->page);
+    CHECK((int64_t)c->width * c->page <= (int64_t)1 << 30, "%s: width %d pages of %d pass 2^30 tokens", who, c->width, c->page);
+    CHECK(c->pages < 1 << 29, "%s: %d pages (below 2^29)", who, c->pages);
+    CHECK(c->token_stride >= 0 && c->token_stride < 1 << 24, "%s: tokens %lld elements apart (below 2^24)", who, (long long)c->token_stride);
     CHECK(c->f16 == 0 || c->f16 == 1, "%s: f16 %d", who, c->f16);
 }
 

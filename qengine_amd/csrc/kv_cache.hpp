@@ -48,3 +48,6 @@ struct AttnTreeArgs {
     float scale;
 };
 void attn_tree(const qe_kv_cache_t& c, int layer, const AttnTreeArgs& a, hipStream_t st);
+// off: as where the device has no memory for the parts of rows (a test hook)
+void attn_tree_set_split(bool on);
+bool attn_tree_split();

@@ -136,7 +136,9 @@ f = lambda name, sig, *a: typed(name, sig)(*a)
     ("f('qe_kv_release', 'pppip', 0, 0, 0, 1, 0)", "qe_kv_release: no cache"),
     ("c._c.page = 24; f('qe_kv_release', 'pppip', p, 0, 0, 1, 0)", "page 24"),
     ("c._c.d = 80; f('qe_kv_release', 'pppip', p, 0, 0, 1, 0)", "d 80"),
-    ("c._c.width = 1 << 27; f('qe_kv_release', 'pppip', p, 0, 0, 1, 0)", "pass 2^31 tokens"),
+    ("c._c.width = 1 << 27; f('qe_kv_release', 'pppip', p, 0, 0, 1, 0)", "pass 2^30 tokens"),
+    ("c._c.pages = 1 << 30; f('qe_kv_release', 'pppip', p, 0, 0, 1, 0)", "1073741824 pages"),
+    ("c._c.token_stride = 1 << 24; f('qe_kv_release', 'pppip', p, 0, 0, 1, 0)", "16777216 elements apart"),
     ("c._c.token_stride = 4; f('qe_kv_release', 'pppip', p, 0, 0, 1, 0)", "strides must be multiples of 8"),
     ("f('qe_kv_append', 'piipppppiip', p, 1, 2, 0, 0, 0, 0, 0, 1, 1, 0)", "qe_kv_append: layers 1 .. 3 of 2"),
     ("f('qe_kv_accept', 'ppppiipp', p, 16, 16, 16, 65, 1, 0, 0)", "paths of 65"),

@@ -60,6 +60,21 @@ def test_long(dev, d, dtype):
     compare(q, k, v, cu, *ops.attn_prompt(q, k, v, cu, lse=True))
 
 
+# shapes of every tile choice: blocks of 128 rows in steps of 32 and 64 keys, blocks of 64 rows in groups
+@pytest.mark.parametrize("lens,heads,kv,d,dtype", [
+    ([1700, 1, 255, 64], 40, 8, 128, BF), ([700], 40, 8, 128, F16), ([2000], 8, 1, 128, BF), ([333, 129], 40, 8, 128, BF),
+    ([3000], 32, 4, 64, BF), ([500, 31, 33, 257], 64, 8, 64, F16), ([2000], 16, 2, 64, BF),
+    ([2100, 40], 32, 2, 256, BF), ([1000], 16, 2, 256, F16), ([2000], 16, 2, 256, BF)])
+def test_tile_choices(dev, lens, heads, kv, d, dtype):
+    q, k, v, cu = inputs(dev, lens, heads, kv, d, dtype, seed=sum(lens))
+    group = heads // kv
+    out, lse = ops.attn_prompt(q, k, v, cu, lse=True)
+    for h in (0, heads // 2, heads - 1):
+        m = h // group
+        compare(q[:, h:h + 1], k[:, m:m + 1], v[:, m:m + 1], cu, out[:, h:h + 1], lse[:, h:h + 1])
+    assert torch.equal(out, ops.attn_prompt(q, k, v, cu))
+
+
 @pytest.mark.parametrize("nseq", [63, 64, 65, 300])
 def test_many_sequences(dev, nseq):
     lens = [(i * 37) % 90 if i % 7 else 0 for i in range(nseq)]
@@ -95,18 +110,19 @@ def test_strides_of_out_and_heads(dev):
     assert torch.equal(buf[:, :, :64], want) and (buf[:, :, 64:] == 3).all()
 
 
+@pytest.mark.parametrize("heads", [2, 160])
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
-def test_later_keys_that_are_not_finite(dev, bad, d):
+def test_later_keys_that_are_not_finite(dev, bad, d, heads):
     """a row is not touched by what later keys and values hold; the rows that see them get what the formula says"""
-    q, k, v, cu = inputs(dev, [150, 200], 2, 1, d, BF, seed=8)
+    q, k, v, cu = inputs(dev, [150, 200], heads, 1, d, BF, seed=8)
     v[100, 0, 3] = bad          # rows 100.. of the first sequence see it
     k[150 + 130, 0, 5] = float("nan")
     out = ops.attn_prompt(q, k, v, cu)
     clean = v.clone()
     clean[100, 0, 3] = 0
     seen = torch.ones(100, 100, dtype=torch.bool, device=dev).tril()
-    for h in range(2):
+    for h in (0, heads - 1):
         ref.check(out[:100, h], None, *ref.rows(q[:100, h], k[:100, 0], v[:100, 0], seen, d ** -0.5))
         seen2 = torch.ones(130, 130, dtype=torch.bool, device=dev).tril()
         ref.check(out[150:280, h], None, *ref.rows(q[150:280, h], k[150:280, 0], v[150:280, 0], seen2, d ** -0.5))

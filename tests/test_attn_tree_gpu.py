@@ -170,23 +170,24 @@ def test_offsets_past_32_bits(dev):
 
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
-def test_drafts_that_are_not_finite(dev, bad, d):
+@pytest.mark.parametrize("new,context", [(20, 45), (7, 45), (7, 5000), (20, 5000), (64, 900)])
+def test_drafts_that_are_not_finite(dev, bad, d, new, context):
     """a drafted value that some rows see: theirs is what the formula says, the others' as if it were not there"""
-    c, q, seqs, cu, mask, words = setup(dev, [45], [20], 2, 1, d, 16, BF, seed=7, tree="tree")
+    c, q, seqs, cu, mask, words = setup(dev, [context], [new], 2, 1, d, 16, BF, seed=7, tree="tree")
     s, col = seqs.item(), 3
     state = ref.Pages(c)
-    pg, off = state.place(s, 45 + 2)
+    pg, off = state.place(s, context + 2)
     c.v[0, pg, 0, off, col] = bad
-    out = attend(c, q, seqs, cu, 20, mask)
-    k, v = state.tokens(0, s, 65)
-    sees = [i for i in range(20) if words[i] >> 2 & 1]
-    others = [i for i in range(20) if i not in sees]
+    out = attend(c, q, seqs, cu, new, mask)
+    k, v = state.tokens(0, s, context + new)
+    sees = [i for i in range(new) if words[i] >> 2 & 1]
+    others = [i for i in range(new) if i not in sees]
     assert sees and others
-    seen = torch.ones(20, 65, dtype=torch.bool)
-    for i in range(20):
-        seen[i, 45:] = torch.tensor([bool(words[i] >> j & 1) for j in range(20)])
+    seen = torch.ones(new, context + new, dtype=torch.bool)
+    for i in range(new):
+        seen[i, context:] = torch.tensor([bool(words[i] >> j & 1) for j in range(new)])
     clean = v.clone()
-    clean[47, 0, col] = 0
+    clean[context + 2, 0, col] = 0
     rest = [i for i in range(d) if i != col]
     for h in range(2):
         o, _, ob, _ = ref.rows(q[:, h], k[:, 0], clean[:, 0], seen.to(dev), d ** -0.5)
@@ -241,10 +242,27 @@ def test_rows_outside_sequences_stay(dev):
     assert (short[2] == 7).all() and torch.isfinite(short).all() and not (short[1] == 7).all()
 
 
-def test_without_workspace_the_rows_are_the_same_within_bounds(dev):
-    """every block takes whole rows then; the bound holds for both orders of the sums"""
-    c, q, seqs, cu, mask, words = setup(dev, [3000, 5, 700], [3, 1, 8], 10, 2, 128, 32, BF, seed=13, tree="tree")
-    compare(c, q, seqs, cu, words, *attend(c, q, seqs, cu, 8, mask, lse=True))
+@pytest.mark.parametrize("heads,d", [(4, 128), (10, 128), (10, 64), (64, 256), (64, 128)])
+def test_without_parts(dev, heads, d):
+    """a block takes whole rows where there is no memory for parts"""
+    c, q, seqs, cu, mask, words = setup(dev, [3000, 5, 700, 0], [3, 1, 8, 0], heads, 2, d, 32, BF, seed=13, tree="tree", stale=float("nan"))
+    call("qe_attn_tree_set_split", 0)
+    try:
+        compare(c, q, seqs, cu, words, *attend(c, q, seqs, cu, 8, mask, lse=True))
+    finally:
+        call("qe_attn_tree_set_split", 1)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [5, 16, 17, 32, 33, 128, 129, 256, 257])
+def test_row_counts(dev, rows, d, dtype):
+    """the rows of a kv head around the sizes at which the kernel changes, over ragged contexts"""
+    n = min(rows, 16)
+    heads = -(-rows // n)
+    c, q, seqs, cu, mask, words = setup(dev, [200, 0, 1000, 65], [n, 1, n - 1, n], heads, 1, d, 16, dtype, seed=rows, tree="random",
+                                        stale=float("nan"))
+    compare(c, q, seqs, cu, words, *attend(c, q, seqs, cu, n, mask, lse=True))
 
 
 def test_same_bits_streams_and_graphs(dev):

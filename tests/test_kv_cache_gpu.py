@@ -68,6 +68,15 @@ def test_reserve_finds_free_pages_anywhere(dev, pages):
     assert taken == free[:len(taken)] and c.ref.sum().item() == pages - len(free) + len(taken)
 
 
+def test_reserve_of_more_than_an_int(dev):
+    """1024 entries whose wishes sum past 2^31 pages: those that fit are served, the others refused"""
+    c = ops.KVCache.empty(1, 50, 16, 1, 64, 1100, 16, device=dev)
+    c = ops.KVCache(c.k, c.v, torch.full((1100, 1 << 22), -1, dtype=torch.int32, device=dev), c.length, c.held, c.ref)
+    add = [16 * 10, 16 * 40] + [16 << 22] * 1022
+    got = c.reserve(ints(range(1024), dev), ints(add, dev)).tolist()
+    assert got == [1, 1] + [0] * 1022 and c.ref.sum().item() == 50 and c.held[:3].tolist() == [10, 40, 0]
+
+
 def test_reserve_of_many(dev):
     """1024 entries: pages for each, copies for half of them"""
     c, p, _ = make(dev, layers=1, pages=3000, kv=1, slots=1200, tokens=64)
