@@ -1,4 +1,4 @@
-/* qe_kernels.h - C-ABI of libqe_kernels.so, the MI355X (gfx950) weight-only quantized matmul path.
+/* qe_kernels.h - C-ABI of libqe_kernels.so, the MI355X (gfx950) weight-only quantized matmul path, and attention beside it.
  *
  * Every pointer argument is a DEVICE pointer unless stated; `stream` is a hipStream_t (NULL = default
  * stream). 16-bit floats cross the ABI as raw uint16_t bit patterns. A violated shape precondition prints

@@ -2,11 +2,12 @@
 //
 //   o[i] = sum_j p_ij v[j],  p_ij = softmax over the tokens j that row i sees of scale q[i] . k[j]
 //
-// A sequence's rows of one kv head are its drafted tokens times the query heads of the group: few (1 to some hundred)
-// against thousands of keys, so the call is bound by reading keys and values once from HBM. Every wave takes 32 keys at a
+// A sequence's rows of one kv head are its drafted tokens times the query heads of the group: here few (1 to 32) against
+// thousands of keys, so the call is bound by reading keys and values once from HBM. Every wave takes 32 keys at a
 // time straight into registers (no LDS: nobody else needs them): K as the A operand of S^T = K Q^T as it lies in memory,
 // V's rows 16 bytes a lane, turned into the A operand of O^T = V^T P^T by 16-bit permutes inside the lane (8 keys x 8
-// columns: 32 permutes for 32 keys x 128 columns, hidden behind the loads). The next 32 keys are in flight meanwhile.
+// columns: 32 permutes for 32 keys x 128 columns, hidden behind the loads). The next 32 keys are in flight meanwhile:
+// 128 KB a CU at d = 128. 64 sequences of up to 8000 tokens, 8 kv heads (1.3 GB): 237 us, 5.5 TB/s.
 //
 // Work is split over the tokens of all sequences evenly (attn_tree.hpp), in units of 128 tokens, 32 a wave.
 #include "attn_tree.hpp"
