@@ -341,7 +341,7 @@ void qe_moe_pack_w4(const int32_t* gu_q, const uint16_t* gu_s, const int32_t* dn
 /* ---- attention and the paged cache of keys and values. No reference C-ABI exists for them. 16-bit values are bf16, or
  * fp16 where said; scores, softmax statistics and sums are fp32, probabilities are rounded to the values' type for the
  * second product (as the matrix cores take them). heads % kv_heads == 0: query head h reads kv head h / (heads / kv_heads).
- * d = 64, 128 or 256. scale > 0, usually d^-0.5. Pointers 16-byte aligned, strides in elements and multiples of 8, a head's d values contiguous.
+ * d = 64, 128 or 256. scale 2^-126 .. 2^126, usually d^-0.5. Pointers 16-byte aligned, strides in elements and multiples of 8, a head's d values contiguous.
  * lse (NULL: not wanted) [t][heads] fp32: log of the sum of the exponentiated scores.
  * A row that sees no key has out = 0 and lse = -inf; a key that a row does not see has no effect on it, whatever its bits.
  * Lengths, tables and indexes live on the device and are not seen by the host: values out of range make a kernel skip
@@ -392,12 +392,13 @@ void qe_kv_fork(const qe_kv_cache_t* cache, const int32_t* parents, const int32_
 void qe_kv_release(const qe_kv_cache_t* cache, const int32_t* seqs, const int32_t* lengths, int n, void* stream);
 /* New keys and values: row t of sequence b (cu as above; slot seqs[b], distinct) goes to token length + t - cu[b] of the
  * slot, in `layers` layers from `layer` on. strides: layer, row and head of k, then of v (host memory, elements). Rows
- * without a held page are not written. length is not changed. */
+ * without a held page, or whose page other slots hold too (no reserve since a fork or a cut), are not written. length is
+ * not changed. */
 void qe_kv_append(const qe_kv_cache_t* cache, int layer, int layers, const void* k, const void* v, const int64_t* strides,
                   const int32_t* seqs, const int32_t* cu, int nseq, int t, void* stream);
 /* Commits count[i] tokens of slot seqs[i] (distinct). path NULL: the first drafted ones. Else path int32 [n][most], most
  * <= 64: drafted rows path[i][0 .. count - 1] move to the first places after the committed tokens, in all layers, as if
- * all were read before any is written. length_out [slots] (NULL: the cache's own) gets length + count, at most what the
+ * all were read before any is written (none moves into a page that other slots hold too). length_out [slots] (NULL: the cache's own) gets length + count, at most what the
  * held pages take. */
 void qe_kv_accept(const qe_kv_cache_t* cache, const int32_t* seqs, const int32_t* count, const int32_t* path, int most,
                   int n, int32_t* length_out, void* stream);
@@ -405,7 +406,8 @@ void qe_kv_accept(const qe_kv_cache_t* cache, const int32_t* seqs, const int32_t
 /* Attention of drafted tokens over the cache, the drafted rows appended before: row cu[b] + i of q is the drafted token i
  * of slot seqs[b] and sees the slot's committed tokens and the drafted tokens j with bit j of mask[cu[b] + i] (NULL: j <=
  * i, a chain). One row a sequence: decode. max_new: the largest number of rows of a sequence, at most 64; rows past it,
- * and rows before cu[0] or from cu[nseq] on, are left as they were. nseq <= 4096. */
+ * and rows before cu[0] or from cu[nseq] on, are left as they were. nseq <= 4096, and nseq * kv_heads * ceil(max_new *
+ * (heads / kv_heads) / 128) * ceil(width * page / 32) <= 2^30. */
 void qe_attn_tree(const qe_kv_cache_t* cache, int layer, const void* q, int64_t q_row, int64_t q_head, void* out,
                   int64_t out_row, int64_t out_head, float* lse, const int32_t* seqs, const int32_t* cu, int nseq, int t,
                   int max_new, const uint64_t* mask, int heads, float scale, void* stream);

@@ -99,8 +99,8 @@ def _check_out(out, q, dtype, at):
 
 
 def _check_scale(scale):
-    if scale is not None and not 0 < scale < float("inf"):
-        raise ValueError(f"scale is positive, got {scale}")
+    if scale is not None and not 2.0 ** -126 <= scale <= 2.0 ** 126:
+        raise ValueError(f"scale is positive and in the range of fp32, got {scale}")
 
 
 def attn_prompt(q, k, v, cu, scale=None, out=None, lse=False):
@@ -182,13 +182,15 @@ class KVCache:
                                int(dtype == torch.float16))
         self._at = ctypes.addressof(self._c)
         self._scale = d ** -0.5
+        self._units = -(-width * page // 32)  # what attend counts tokens in, at the least
 
     @staticmethod
     def empty(layers, pages, page, kv_heads, d, slots, max_tokens, dtype=torch.bfloat16, device="cuda"):
         """a cache that holds nothing, for slots of up to max_tokens tokens"""
-        k = torch.empty(layers, pages, kv_heads, page, d, dtype=dtype, device=device)
+        # zeros: a NaN behind a page's rows would not change results, but make the kernels look again at what they read
+        k = torch.zeros(layers, pages, kv_heads, page, d, dtype=dtype, device=device)
         ints = dict(dtype=torch.int32, device=k.device)
-        return KVCache(k, torch.empty_like(k), torch.full((slots, -(-max_tokens // page)), -1, **ints),
+        return KVCache(k, torch.zeros_like(k), torch.full((slots, -(-max_tokens // page)), -1, **ints),
                        torch.zeros(slots, **ints), torch.zeros(slots, **ints), torch.zeros(pages, **ints))
 
     def _batch(self, name, t, n=None):
@@ -239,7 +241,8 @@ class KVCache:
 
     def append(self, layer, k, v, seqs, cu):
         """New rows k, v [t][kv heads][d] of one layer, or [layers][t][kv heads][d] of all (layer None): rows cu[b] ..
-        cu[b + 1] - 1 go behind the committed tokens of slot seqs[b], into pages reserved before. Slots are distinct."""
+        cu[b + 1] - 1 go behind the committed tokens of slot seqs[b], into pages reserved before (after a fork or a cut
+        again: rows are not written into a page that other slots hold too). Slots are distinct."""
         one = layer is not None
         dims, shape = (3, k.shape) if one else (4, k.shape)
         _rows("k", k, dims, self.dtype, self._dev)
@@ -278,9 +281,9 @@ class KVCache:
             _ints("length", length, (self.slots,), self._dev)
         if n > 65535:
             raise ValueError(f"at most 65535 sequences a call, got {n}")
-        if n and (path is None or most):
+        if n:  # (a path of no columns has no address, but is one)
             _run(self._dev, "qe_kv_accept", "ppppiipp", self._at, seqs.data_ptr(), count.data_ptr(),
-                 None if path is None else path.data_ptr(), most, n, None if length is None else length.data_ptr())
+                 None if path is None else path.data_ptr() or seqs.data_ptr(), most, n, None if length is None else length.data_ptr())
 
     def attend(self, layer, q, seqs, cu, most, mask=None, scale=None, out=None, lse=False):
         """Attention of drafted tokens, appended before: row cu[b] + i of q [t][heads][d] is drafted token i of slot seqs[b]; it
@@ -302,6 +305,8 @@ class KVCache:
             raise ValueError(f"at most {MAX_SEQS} sequences, got {n}")
         if mask is not None:
             _ints("mask", mask, (t,), at, torch.int64)
+        if n * self.kv_heads * -(-most * (heads // self.kv_heads) // 128) * self._units > 1 << 30:
+            raise ValueError(f"{n} sequences of {most} rows over tables of {self.width} pages: more than 2^30 units of work")
         _check_scale(scale)
         if out is None:
             out = torch.empty(t, heads, d, dtype=dtype, device=self.device)

@@ -245,7 +245,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(Pool p, Slots s, Appen
     const int64_t pos = (int64_t)s.length[slot] + t - cu[b], idx = pos >> s.shift;
     if (pos < 0 || idx >= s.held[slot] || idx >= s.width) return;
     const int pg = s.table[(int64_t)slot * s.width + idx];
-    if (pg < 0 || pg >= p.pages) return;
+    if (pg < 0 || pg >= p.pages || s.ref[pg] > 1) return;  // never into a page that other slots hold too
     const int chunks = p.d / 8, each = p.heads * chunks;
     const int64_t to = (int64_t)(a.layer0 + blockIdx.y) * p.layer + (int64_t)pg * p.page + (pos & ((1 << s.shift) - 1)) * p.token;
     const char* ks = a.k + blockIdx.y * a.kl + t * a.kr;
@@ -279,7 +279,7 @@ __global__ __launch_bounds__(kThreads) void accept_rows_kernel(Pool p, Slots s, 
         const int64_t a = (int64_t)len + j, b = (int64_t)len + lane;
         if (j >= 0 && j != lane && (a >> s.shift) < held && (b >> s.shift) < held) {
             const int pa = s.table[(int64_t)slot * s.width + (a >> s.shift)], pb = s.table[(int64_t)slot * s.width + (b >> s.shift)];
-            if (pa >= 0 && pa < p.pages && pb >= 0 && pb < p.pages) {
+            if (pa >= 0 && pa < p.pages && pb >= 0 && pb < p.pages && s.ref[pb] <= 1) {
                 from = pa * p.page + (a & ((1 << s.shift) - 1)) * p.token;
                 to = pb * p.page + (b & ((1 << s.shift) - 1)) * p.token;
             }

@@ -129,6 +129,29 @@ def test_a_cut_slot_does_not_write_its_siblings_page(dev):
     assert p.table[0][1] != p.table[1][1] and p.table[0][0] == p.table[1][0]
 
 
+def test_without_reserve_a_shared_page_stays(dev):
+    """rows appended or moved after a fork without a reserve are not written into the page that the parent holds too"""
+    c, p, g = make(dev)
+    fill(c, p, [20], dev)
+    c.fork(ints([0], dev), ints([1], dev)), p.fork([0], [1])
+    k, v = (torch.randn(3, 2, 64, device=dev, generator=g).to(BF) for _ in range(2))
+    c.append(0, k, v, ints([1], dev), ints([0, 3], dev))
+    c.append(None, torch.stack([k, v]), torch.stack([v, k]), ints([0], dev), ints([0, 3], dev))
+    c.accept(ints([1], dev), ints([3], dev), ints([[2, 0, 1]], dev)), p.accept([1], [3])
+    p.same()
+
+
+def test_a_path_of_no_columns(dev):
+    """commits nothing; the lengths are written all the same"""
+    c, p, _ = make(dev)
+    fill(c, p, [20, 7], dev)
+    after = torch.full_like(c.length, -5)
+    c.accept(ints([1, 0], dev), ints([4, 0], dev), torch.empty(2, 0, dtype=torch.int32, device=dev), length=after)
+    assert after.tolist() == [20, 7] + [-5] * 6
+    c.accept(ints([1, 0], dev), ints([4, 0], dev), torch.empty(2, 0, dtype=torch.int32, device=dev))
+    p.same()
+
+
 @pytest.mark.parametrize("d,kv,page", [(64, 1, 16), (64, 3, 32), (128, 8, 16), (256, 2, 64), (128, 5, 1024)])
 def test_append(dev, d, kv, page):
     c, p, g = make(dev, layers=3, pages=24, page=page, kv=kv, d=d, tokens=6 * page, dtype=F16)
