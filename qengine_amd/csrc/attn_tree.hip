@@ -362,8 +362,12 @@ void attn_tree(const qe_kv_cache_t& c, int layer, const AttnTreeArgs& x, hipStre
     CHECK(layer >= 0 && layer < c.layers, "qe_attn_tree: layer %d of %d", layer, c.layers);
     CHECK(x.nseq >= 0 && x.nseq <= kMaxTreeBatch, "qe_attn_tree: nseq = %d (at most %d)", x.nseq, kMaxTreeBatch);
     CHECK(x.t >= 0 && x.max_new >= 1 && x.max_new <= kMaxTreeNodes, "qe_attn_tree: t = %d, max_new = %d (1 .. %d)", x.t, x.max_new, kMaxTreeNodes);
-    CHECK(x.scale > 0.f && x.scale < __builtin_huge_valf(), "qe_attn_tree: scale %g", (double)x.scale);
+    CHECK(x.scale >= 0x1p-126f && x.scale <= 0x1p126f, "qe_attn_tree: scale %g", (double)x.scale);
     CHECK(x.heads >= c.kv_heads && x.heads % c.kv_heads == 0 && x.heads <= 65535, "qe_attn_tree: %d heads over %d", x.heads, c.kv_heads);
+    // units of tokens are counted in 32 bits; no kernel has smaller ones than 128 rows (or all) and 32 tokens
+    const int64_t rbs = ((int64_t)x.max_new * (x.heads / c.kv_heads) + 127) / 128, units = ((int64_t)c.width * c.page + 31) / 32;
+    CHECK((int64_t)x.nseq * c.kv_heads * rbs <= ((int64_t)1 << 30) / units, "qe_attn_tree: %d sequences x %d heads x %lld blocks of rows x %lld of tokens pass 2^30",
+          x.nseq, c.kv_heads, (long long)rbs, (long long)units);
     if (x.nseq == 0 || x.t == 0) return;
     CHECK(x.q && x.out && x.seqs && x.cu, "qe_attn_tree: null pointer");
     CHECK((((uintptr_t)x.q | (uintptr_t)x.out) & 15) == 0 && ((x.q_row | x.q_head | x.o_row | x.o_head) & 7) == 0,

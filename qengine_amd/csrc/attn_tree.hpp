@@ -230,7 +230,6 @@ void launch_split(Args a, Kernel kernel, int threads, size_t lds, int per_cu, hi
     a.rb_max = (a.max_new * a.group + ROWS - 1) / ROWS;
     const int64_t runs = (int64_t)a.nseq * a.kv_heads * a.rb_max;
     const int64_t most_units = ((int64_t)(a.width << a.shift) + UNIT - 1) / UNIT;
-    CHECK(runs * most_units < (int64_t)1 << 31, "qe_attn_tree: %lld rows x %lld units of tokens", (long long)runs, (long long)most_units);
     const int grid = (int)std::min<int64_t>(runs * most_units, per_cu * qe_num_cus());
     const size_t part = (size_t)grid * 2 * ROWS * D * 4, ml = (size_t)grid * 2 * ROWS * 8, ends = ((size_t)a.nseq + 1) * 4;
     WsHold hold(st);

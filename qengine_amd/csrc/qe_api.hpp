@@ -116,7 +116,7 @@ class WsHold {
     WsHold& operator=(const WsHold&) = delete;
     // the buffer of (kind, current device, stream), at least `bytes`, grown on a call outside graph capture. During
     // capture: a buffer that the graph holds; nullptr for kWsSplit, kWsI8 and kWsH where the stream's own has not that
-    // size. nullptr too where the device has no memory for a kWsSplit, kWsDec or kWsSkinny buffer. kWsDec buffers
+    // size. nullptr too where the device has no memory for a kWsSplit, kWsDec, kWsSkinny or kWsAttn buffer. kWsDec buffers
     // (the one-pass decode's tail counters and sums) are zero-filled when allocated; the kernel leaves its counters zero.
     // retry: ask the device also shortly after it had no memory.
     void* get(int kind, size_t bytes, bool retry = false);

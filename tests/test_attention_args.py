@@ -154,3 +154,22 @@ def test_entry_points_abort_with_check_message(code, msg):
     r = subprocess.run([sys.executable, "-c", HEAD + code], capture_output=True, text=True, timeout=120)
     assert r.returncode != 0
     assert "check failed" in r.stderr and msg in r.stderr, r.stderr
+
+
+@pytest.mark.parametrize("scale", [1e-46, 1e-39, 1e38, 1e39, float("inf")])
+def test_scales_that_fp32_does_not_hold(scale):
+    """too small or too large for the kernels' fp32 (the C-ABI would abort on what they become there)"""
+    with pytest.raises(ValueError, match="scale"):
+        ops.attn_prompt(z(4, 4, 64), z(4, 2, 64), z(4, 2, 64), i32(0, 4), scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        cache().attend(0, z(1, 4, 64), i32(0), i32(0, 1), 1, scale=scale)
+
+
+def test_more_units_of_work_than_are_counted():
+    c = cache(slots=1, max_tokens=1 << 30, page=1024)  # 2^25 units of 32 tokens, of 2 heads
+    with pytest.raises(ValueError, match="not on|on a GPU"):
+        c.attend(0, z(16, 4, 64), z(16, dtype=I32), z(17, dtype=I32), 64)
+    with pytest.raises(ValueError, match="units of work"):
+        c.attend(0, z(17, 4, 64), z(17, dtype=I32), z(18, dtype=I32), 64)
+    with pytest.raises(ValueError, match="units of work"):
+        c.attend(0, z(9, 6, 64), z(9, dtype=I32), z(10, dtype=I32), 64)  # 192 rows a head: two blocks
