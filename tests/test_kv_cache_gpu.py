@@ -77,6 +77,36 @@ def test_reserve_of_more_than_an_int(dev):
     assert got == [1, 1] + [0] * 1022 and c.ref.sum().item() == 50 and c.held[:3].tolist() == [10, 40, 0]
 
 
+@pytest.mark.parametrize("pages,each,first", [(20000, 9, 0), (150000, 20, 0), (5003, 4, 1)])
+def test_reserve_of_many_pages(dev, pages, each, first):
+    """thousands of pages in one call, scattered over the pool, for 1024 entries of which some name a slot again; the counts
+    also where they do not start at 16 bytes"""
+    c = ops.KVCache.empty(1, pages, 16, 1, 64, 1200, 16 * 40, device=dev)
+    counts = torch.ones(pages + first, dtype=torch.int32, device=dev)[first:]
+    c = ops.KVCache(c.k, c.v, c.table, c.length, c.held, counts)
+    rng = random.Random(pages)
+    free = sorted(rng.sample(range(pages), min(pages * 4 // 5, 1010 * each + 7)))
+    counts[torch.tensor(free, device=dev)] = 0
+    seqs = rng.sample(range(1200), 1024)
+    for i in (1, 2, 3, 4, 5, 64, 127, 500, 1023):  # repeated from one to many places before
+        seqs[i] = seqs[rng.randrange(i)]
+    got = c.reserve(ints(seqs, dev), ints([16 * each] * 1024, dev)).tolist()
+    want, used, table = [], 0, {}
+    for i, s in enumerate(seqs):
+        ok = s not in seqs[:i]
+        if ok:
+            used += each
+            ok = used <= len(free)
+            if ok:
+                table[s] = free[used - each:used]
+        want.append(int(ok))
+    assert got == want
+    held, rows = c.held.tolist(), c.table.tolist()
+    assert all(rows[s] == table.get(s, []) + [-1] * (40 - len(table.get(s, []))) and held[s] == len(table.get(s, [])) for s in range(1200))
+    taken = sum(len(x) for x in table.values())
+    assert counts.sum().item() == pages - len(free) + taken and counts.max().item() == 1
+
+
 def test_reserve_of_many(dev):
     """1024 entries: pages for each, copies for half of them"""
     c, p, _ = make(dev, layers=1, pages=3000, kv=1, slots=1200, tokens=64)
