@@ -9,6 +9,7 @@
 // (dependent reads of the starts, then queries and keys: about 4 us).
 #include "attn_wave.hpp"
 #include "kv_cache.hpp"
+#include "seq_rows.hpp"
 
 #include <algorithm>
 #include <atomic>
@@ -49,10 +50,11 @@ __global__ __launch_bounds__(64 * RW * KG, (D == 256 ? 1 : KG == 1 && KEYS == 32
     const int kvh = blockIdx.x % a.heads % a.kv_heads, grp = blockIdx.x % a.heads / a.kv_heads;
     const int head = kvh * (a.heads / a.kv_heads) + grp;
     int slot = blockIdx.x / a.heads, b = 0, qb = 0;
-    auto first_of = [&](int i) { return min(max(a.cu[i], 0), a.t); };
-    auto len_of = [&](int i) { return max(0, min(a.cu[i + 1], a.t) - first_of(i)); };
+    auto rows_at = [&](int i) { return rows_of(a.cu[i], a.cu[i + 1], a.t); };
     // the first 64 sequences are in every wave's lanes
-    const int lane_first = lane < a.nseq ? first_of(lane) : 0, lane_len = lane < a.nseq ? len_of(lane) : 0;
+    RowRange of_lane{0, 0};
+    if (lane < a.nseq) of_lane = rows_at(lane);
+    const int lane_first = of_lane.first, lane_len = of_lane.n;
     if (a.nseq == 1) {
         qb = (__builtin_amdgcn_readfirstlane(lane_len) + BQ - 1) / BQ - 1 - slot;
         if (qb < 0) return;
@@ -60,7 +62,7 @@ __global__ __launch_bounds__(64 * RW * KG, (D == 256 ? 1 : KG == 1 && KEYS == 32
         int* more = reinterpret_cast<int*>(lds);  // blocks of the sequences from the 65th on
         const int nb = (lane_len + BQ - 1) / BQ;
         if (a.nseq > 64) {
-            for (int i = 64 + tid; i < a.nseq; i += 64 * W) more[i - 64] = (len_of(i) + BQ - 1) / BQ;
+            for (int i = 64 + tid; i < a.nseq; i += 64 * W) more[i - 64] = (rows_at(i).n + BQ - 1) / BQ;
             __syncthreads();
         }
         // blocks with index >= level, over all sequences
@@ -96,8 +98,8 @@ __global__ __launch_bounds__(64 * RW * KG, (D == 256 ? 1 : KG == 1 && KEYS == 32
     }
     b = __builtin_amdgcn_readfirstlane(b);
     qb = __builtin_amdgcn_readfirstlane(qb);
-    const int c0 = b < 64 ? __builtin_amdgcn_readlane(lane_first, b) : __builtin_amdgcn_readfirstlane(first_of(b));
-    const int len = b < 64 ? __builtin_amdgcn_readlane(lane_len, b) : __builtin_amdgcn_readfirstlane(len_of(b));
+    const int c0 = b < 64 ? __builtin_amdgcn_readlane(lane_first, b) : __builtin_amdgcn_readfirstlane(rows_at(b).first);
+    const int len = b < 64 ? __builtin_amdgcn_readlane(lane_len, b) : __builtin_amdgcn_readfirstlane(rows_at(b).n);
     const int rw = wave % RW, kg = wave / RW;
     const int q0 = qb * BQ, qw = q0 + rw * 32;    // the block's and the wave's first row
     const int row = qw + col;                     // this lane's query

@@ -8,6 +8,7 @@
 #pragma once
 #include "attn_common.hpp"
 #include "kv_cache.hpp"
+#include "seq_rows.hpp"
 
 #include <algorithm>
 
@@ -34,14 +35,14 @@ struct Seq {
 };
 __device__ __forceinline__ Seq seq_of(const Args& a, int b) {
     Seq s;
-    const int c0 = a.cu[b], c1 = a.cu[b + 1];
-    s.first = min(max(c0, 0), a.t);
-    s.n = min(min(c1, a.t) - s.first, a.max_new);
+    const RowRange r = rows_of(a.cu[b], a.cu[b + 1], a.t);
+    s.first = r.first;
+    s.n = min(r.n, a.max_new);
     s.slot = a.seqs[b];
     const bool ok = s.slot >= 0 && s.slot < a.slots;
     const int room = a.width << a.shift;
     s.len = ok ? min(max(a.length[ok ? s.slot : 0], 0), room) : 0;
-    s.total = ok ? min(s.len + max(s.n, 0), room) : 0;
+    s.total = ok ? min(s.len + s.n, room) : 0;
     return s;
 }
 // What a block keeps of the sequences of a call with up to kKept of them, so that it does not read them again (three
@@ -151,7 +152,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a, int most) {
     constexpr int E = D / 64, RPB = kThreads / 64 / WPR;  // columns of a lane, rows of a block
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave % WPR;
     const int r = blockIdx.x * RPB + wave / WPR, h = blockIdx.y, b = blockIdx.z;
-    const int c0 = a.cu[b], first = min(max(c0, 0), a.t), n = min(min(a.cu[b + 1], a.t) - first, a.max_new);
+    const RowRange seq = rows_of(a.cu[b], a.cu[b + 1], a.t);
+    const int first = seq.first, n = min(seq.n, a.max_new);
     int cnt = 0, w0 = 0;
     if (r < n * a.group) {
         const int u0 = b > 0 ? a.ends[b - 1] : 0, range = a.ends[a.nseq], rbs = row_blocks<ROWS>(a, n);
