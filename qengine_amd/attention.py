@@ -26,9 +26,9 @@ from .qe import typed
 F16 = 16
 MAX_NODES = 64
 MAX_BATCH = 1024
-HEAD_DIMS = (64, 128, 256)
-
 MAX_SEQS = 4096
+MAX_ROWS = 1 << 30
+HEAD_DIMS = (64, 128, 256)
 _TYPES = (torch.bfloat16, torch.float16)
 _FN = {}
 _STRIDES = {}
@@ -126,9 +126,10 @@ def _prompt_shapes(q, k, v, cu, scale, out):
     _rows("v", v, 3, dtype, at)
     t, heads, d = q.shape
     ks, kv = k.shape, k.shape[1]
-    if ks != v.shape or ks[0] != t or ks[2] != d or d not in HEAD_DIMS or kv == 0 or heads % kv or not heads or heads > 65535:
-        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: the same rows, d of {HEAD_DIMS}, heads a "
-                         "multiple of the kv heads")
+    if ks != v.shape or ks[0] != t or ks[2] != d or d not in HEAD_DIMS or kv == 0 or heads % kv or not heads or heads > 65535 \
+            or t > MAX_ROWS:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: the same rows (at most {MAX_ROWS}), d of "
+                         f"{HEAD_DIMS}, heads a multiple of the kv heads")
     if t > 1 and (k.stride(0) >= 1 << 24 or v.stride(0) >= 1 << 24):
         raise ValueError(f"rows of k and v are less than 2^24 elements apart, got {k.stride(0)} and {v.stride(0)}")
     n = _starts(cu, at)
@@ -247,8 +248,9 @@ class KVCache:
         dims, shape = (3, k.shape) if one else (4, k.shape)
         _rows("k", k, dims, self.dtype, self._dev)
         _rows("v", v, dims, self.dtype, self._dev)
-        if v.shape != shape or shape[-2] != self.kv_heads or shape[-1] != self.d or not (one or shape[0] == self.layers):
-            raise ValueError(f"k {tuple(shape)} and v {tuple(v.shape)} are rows of {self.kv_heads} kv heads of {self.d}"
+        if v.shape != shape or shape[-2] != self.kv_heads or shape[-1] != self.d or shape[-3] > MAX_ROWS \
+                or not (one or shape[0] == self.layers):
+            raise ValueError(f"k {tuple(shape)} and v {tuple(v.shape)} are at most {MAX_ROWS} rows of {self.kv_heads} kv heads of {self.d}"
                              + ("" if one else f", of {self.layers} layers"))
         if one and not 0 <= layer < self.layers:
             raise ValueError(f"layer {layer} of {self.layers}")
@@ -293,8 +295,8 @@ class KVCache:
         at, dtype = self._dev, self.dtype
         _rows("q", q, 3, dtype, at)
         t, heads, d = q.shape
-        if d != self.d or heads == 0 or heads % self.kv_heads or heads > 65535:
-            raise ValueError(f"q {tuple(q.shape)}: heads of {self.d}, a multiple of the {self.kv_heads} kv heads")
+        if d != self.d or heads == 0 or heads % self.kv_heads or heads > 65535 or t > MAX_ROWS:
+            raise ValueError(f"q {tuple(q.shape)}: at most {MAX_ROWS} rows of heads of {self.d}, a multiple of the {self.kv_heads} kv heads")
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer {layer} of {self.layers}")
         if not 1 <= most <= MAX_NODES:

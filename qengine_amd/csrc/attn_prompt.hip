@@ -225,7 +225,8 @@ void attn_prompt(const AttnPromptArgs& x, bool f16, hipStream_t st) {
     CHECK(x.d == 64 || x.d == 128 || x.d == 256, "qe_attn_prompt: d %d (64, 128 or 256)", x.d);
     CHECK(x.kv_heads >= 1 && x.heads >= x.kv_heads && x.heads % x.kv_heads == 0 && x.heads <= 65535, "qe_attn_prompt: %d heads over %d",
           x.heads, x.kv_heads);
-    CHECK(x.nseq >= 0 && x.nseq <= qe_prompt::kMaxSeqs && x.t >= 0, "qe_attn_prompt: nseq %d (at most %d), t %d", x.nseq, qe_prompt::kMaxSeqs, x.t);
+    CHECK(x.nseq >= 0 && x.nseq <= qe_prompt::kMaxSeqs && x.t >= 0 && x.t <= kMaxRows, "qe_attn_prompt: nseq %d (at most %d), t %d (at most 2^30)",
+          x.nseq, qe_prompt::kMaxSeqs, x.t);
     CHECK(x.scale >= 0x1p-126f && x.scale <= 0x1p126f, "qe_attn_prompt: scale %g", (double)x.scale);
     if (x.nseq == 0 || x.t == 0) return;
     CHECK(x.q && x.k && x.v && x.out && x.cu, "qe_attn_prompt: null pointer");

@@ -361,7 +361,7 @@ void by_shape(const Args& a, int d, hipStream_t st) {
 void attn_tree(const qe_kv_cache_t& c, int layer, const AttnTreeArgs& x, hipStream_t st) {
     CHECK(layer >= 0 && layer < c.layers, "qe_attn_tree: layer %d of %d", layer, c.layers);
     CHECK(x.nseq >= 0 && x.nseq <= kMaxTreeBatch, "qe_attn_tree: nseq = %d (at most %d)", x.nseq, kMaxTreeBatch);
-    CHECK(x.t >= 0 && x.max_new >= 1 && x.max_new <= kMaxTreeNodes, "qe_attn_tree: t = %d, max_new = %d (1 .. %d)", x.t, x.max_new, kMaxTreeNodes);
+    CHECK(x.t >= 0 && x.t <= kMaxRows && x.max_new >= 1 && x.max_new <= kMaxTreeNodes, "qe_attn_tree: t = %d, max_new = %d (1 .. %d)", x.t, x.max_new, kMaxTreeNodes);
     CHECK(x.scale >= 0x1p-126f && x.scale <= 0x1p126f, "qe_attn_tree: scale %g", (double)x.scale);
     CHECK(x.heads >= c.kv_heads && x.heads % c.kv_heads == 0 && x.heads <= 65535, "qe_attn_tree: %d heads over %d", x.heads, c.kv_heads);
     // units of tokens are counted in 32 bits; no kernel has smaller ones than 128 rows (or all) and 32 tokens

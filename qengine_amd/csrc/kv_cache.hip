@@ -406,7 +406,7 @@ void kv_release(const qe_kv_cache_t& c, const int32_t* seqs, const int32_t* leng
 void kv_append(const qe_kv_cache_t& c, int layer, int layers, const void* k, const void* v, const int64_t* strides,
                const int32_t* seqs, const int32_t* cu, int nseq, int t, hipStream_t st) {
     CHECK(layer >= 0 && layers >= 1 && layer <= c.layers - layers, "qe_kv_append: layers %d .. %d of %d", layer, layer + layers, c.layers);
-    CHECK(nseq >= 0 && t >= 0 && layers <= 65535, "qe_kv_append: nseq %d t %d layers %d", nseq, t, layers);
+    CHECK(nseq >= 0 && t >= 0 && t <= kMaxRows && layers <= 65535, "qe_kv_append: nseq %d t %d layers %d", nseq, t, layers);
     if (nseq == 0 || t == 0) return;
     CHECK(k && v && strides && seqs && cu, "qe_kv_append: null pointer");
     CHECK((((uintptr_t)k | (uintptr_t)v) & 15) == 0, "qe_kv_append: k and v must be 16-byte aligned");

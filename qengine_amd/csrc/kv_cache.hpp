@@ -4,6 +4,7 @@
 #include "qe_api.hpp"
 
 constexpr int kMaxCacheBatch = 1024;  // sequences of one reserve, fork or release call (one block looks at all of them)
+constexpr int kMaxRows = 1 << 30;     // rows of one append or attention call: row numbers and their tiles' ends fit 32 bits
 constexpr int kMaxTreeNodes = 64;     // drafted tokens of a sequence: the bits of a mask word
 constexpr int kMaxTreeBatch = 4096;   // sequences of one attention call (their tile counts are summed in LDS)
 

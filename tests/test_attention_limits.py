@@ -1,0 +1,60 @@
+"""Sizes at the limits of the attention and cache entry points, refused by exceptions before the C-ABI would abort or cut them to
+32 bits (CPU only)."""
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from qengine_amd import ops
+from test_abi import LIB
+from test_attention_args import HEAD
+
+BF, I32 = torch.bfloat16, torch.int32
+
+
+def rows(n, heads, d=64):
+    """n rows that take the memory of one"""
+    return torch.zeros(1, heads, d, dtype=BF).expand(n, heads, d)
+
+
+def i32(*v):
+    return torch.tensor(v, dtype=I32)
+
+
+def cache(layers=2):
+    return ops.KVCache.empty(layers, 2, 16, 1, 64, 3, 32, device="cpu")
+
+
+@pytest.mark.parametrize("n", [2 ** 30 + 1, 2 ** 31, 2 ** 32 + 4])
+def test_more_rows_than_are_counted(n):
+    with pytest.raises(ValueError, match="rows"):
+        ops.attn_prompt(rows(n, 4), rows(n, 2), rows(n, 2), i32(0, 4))
+    with pytest.raises(ValueError, match="rows"):
+        cache().attend(0, rows(n, 1), i32(0), i32(0, 4), 4)
+    with pytest.raises(ValueError, match="rows"):
+        cache().append(0, rows(n, 1), rows(n, 1), i32(0), i32(0, 4))
+    with pytest.raises(ValueError, match="rows"):
+        cache().append(None, rows(n, 1)[None].expand(2, n, 1, 64), rows(n, 1)[None].expand(2, n, 1, 64), i32(0), i32(0, 4))
+
+
+def test_the_most_rows_reach_the_gpu_check():
+    n = 2 ** 30
+    with pytest.raises(ValueError, match="on a GPU"):
+        cache().append(0, rows(n, 1), rows(n, 1), i32(0), i32(0, 4))
+
+
+ROWS = 2 ** 30 + 1
+
+
+@pytest.mark.parametrize("code,msg", [
+    (f"f('qe_kv_append', 'piipppppiip', p, 0, 1, 16, 16, 16, 16, 16, 1, {ROWS}, 0)", f"t {ROWS}"),
+    (f"f('qe_attn_tree', 'pipllpllpppiiipifp', p, 0, 16, 8, 8, 16, 8, 8, 0, 16, 16, 1, {ROWS}, 1, 0, 4, 0.1, 0)", f"t = {ROWS}"),
+    (f"f('qe_attn_prompt', 'pllpllpllpllppiiiiifip', *[16, 8, 8] * 4, 0, 16, 1, {ROWS}, 4, 2, 64, 0.1, 0, 0)", f"t {ROWS}"),
+])
+def test_entry_points_abort_with_check_message(code, msg):
+    assert os.path.exists(LIB)
+    r = subprocess.run([sys.executable, "-c", HEAD + code], capture_output=True, text=True, timeout=120)
+    assert r.returncode != 0
+    assert "check failed" in r.stderr and msg in r.stderr, r.stderr
