@@ -65,24 +65,15 @@ __global__ __launch_bounds__(64 * RW * KG, (D == 256 ? 1 : KG == 1 && KEYS == 32
             for (int i = 64 + tid; i < a.nseq; i += 64 * W) more[i - 64] = (rows_at(i).n + BQ - 1) / BQ;
             __syncthreads();
         }
-        // blocks with index >= level, over all sequences
-        auto count = [&](int level) {
-            int n = max(0, nb - level);
-            for (int i = lane; i < a.nseq - 64; i += 64) n += max(0, more[i] - level);
+        BlockPlace place;
+        const bool there = place_of(slot, [&](int level) {
+            int n = add_blocks(0, nb, level);
+            for (int i = lane; i < a.nseq - 64; i += 64) n = add_blocks(n, more[i], level);
             return wave_sum(n);
-        };
-        int lo = 0, above = 0;  // the largest level with more than `slot` blocks from it on, and the blocks above it
-        int hi = 1;
-        if (slot >= count(0)) return;
-        for (int n; (n = count(hi)) > slot; hi *= 2) lo = hi;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (count(mid) > slot) lo = mid;
-            else hi = mid;
-        }
-        above = count(lo + 1);
-        qb = lo;
-        int rank = slot - above;  // among the sequences that have a block of this index
+        }, place);
+        if (!there) return;
+        qb = place.level;
+        int rank = place.rank;
         for (int i0 = 0;; i0 += 64) {
             const bool mine = i0 + lane < a.nseq && (i0 == 0 ? nb : more[i0 - 64 + lane]) > qb;
             const uint64_t has = __ballot(mine);
