@@ -113,8 +113,9 @@ def attn_prompt(q, k, v, cu, scale=None, out=None, lse=False):
     sums = torch.empty(t, heads, dtype=torch.float32, device=q.device) if lse else None
     if t and n:
         qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
-        _run(q.get_device(), "qe_attn_prompt", "pllpllpllpllppiiiiifip", q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
-             v.data_ptr(), vs[0], vs[1], out.data_ptr(), os[0], os[1], sums.data_ptr() if lse else None, cu.data_ptr(), n, t,
+        kr, vr = (ks[0], vs[0]) if t > 1 else (0, 0)  # one row: its row stride may be anything
+        _run(q.get_device(), "qe_attn_prompt", "pllpllpllpllppiiiiifip", q.data_ptr(), qs[0], qs[1], k.data_ptr(), kr, ks[1],
+             v.data_ptr(), vr, vs[1], out.data_ptr(), os[0], os[1], sums.data_ptr() if lse else None, cu.data_ptr(), n, t,
              heads, kv, d, d ** -0.5 if scale is None else scale, F16 if q.dtype == torch.float16 else 0)
     return (out, sums) if lse else out
 

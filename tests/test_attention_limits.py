@@ -58,3 +58,15 @@ def test_entry_points_abort_with_check_message(code, msg):
     r = subprocess.run([sys.executable, "-c", HEAD + code], capture_output=True, text=True, timeout=120)
     assert r.returncode != 0
     assert "check failed" in r.stderr and msg in r.stderr, r.stderr
+
+
+def test_the_row_stride_of_one_row_is_not_passed_on(monkeypatch):
+    """one row of a very wide buffer: its row stride is past what the C-ABI takes, and never used"""
+    from qengine_amd import attention
+    calls = []
+    monkeypatch.setattr(attention, "_run", lambda at, name, sig, *a: calls.append((name, a)))
+    wide = torch.empty_strided((1, 2, 64), (1 << 25, 64, 1), dtype=BF)
+    q = torch.zeros(1, 4, 64, dtype=BF)
+    ops.attn_prompt(q, wide, wide, i32(0, 1))
+    (name, a), = calls
+    assert name == "qe_attn_prompt" and a[4] < 1 << 24 and a[7] < 1 << 24
