@@ -166,9 +166,9 @@ class KVCache:
         layers, pages, kv, page, d = k.shape
         if k.stride(3) >= 1 << 24:
             raise ValueError(f"tokens of a page are less than 2^24 elements apart, got {k.stride(3)}")
-        if d not in HEAD_DIMS or pages >= 1 << 29 or page < 16 or page > 1024 or page & (page - 1) or kv > 1024:
-            raise ValueError(f"pools [layers][pages][kv heads][page][d] with d of {HEAD_DIMS}, at most 1024 kv heads and pages of "
-                             f"16 to 1024 tokens, a power of two: got {tuple(k.shape)}")
+        if d not in HEAD_DIMS or pages >= 1 << 29 or page < 16 or page > 1024 or page & (page - 1) or kv > 1024 or layers > 65535:
+            raise ValueError(f"pools [layers][pages][kv heads][page][d] with d of {HEAD_DIMS}, at most 65535 layers, 1024 kv heads and "
+                             f"pages of 16 to 1024 tokens, a power of two: got {tuple(k.shape)}")
         if table.dim() != 2 or not table.numel() or table.shape[1] * page > 2 ** 30:
             raise ValueError(f"table is [slots][pages of a slot], got {tuple(table.shape)}")
         slots, width = table.shape

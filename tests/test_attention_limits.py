@@ -70,3 +70,12 @@ def test_the_row_stride_of_one_row_is_not_passed_on(monkeypatch):
     ops.attn_prompt(q, wide, wide, i32(0, 1))
     (name, a), = calls
     assert name == "qe_attn_prompt" and a[4] < 1 << 24 and a[7] < 1 << 24
+
+
+def test_more_layers_than_a_launch_takes():
+    """append and accept would abort on them"""
+    pool = torch.zeros(1, 2, 1, 16, 64, dtype=BF).expand(65536, 2, 1, 16, 64)
+    ints = [torch.zeros(*x, dtype=I32) for x in ((3, 2), (3,), (3,), (2,))]
+    ops.KVCache(pool[:65535], pool[:65535], *ints)
+    with pytest.raises(ValueError, match="layers"):
+        ops.KVCache(pool, pool, *ints)
