@@ -15,6 +15,18 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -__builtin_huge_valf();
 
+constexpr float kLazy = 8.f;  // the running maximum follows a row's scores once they pass it by this much (2^8 in the sums)
+constexpr float kFar = 1048576.f;  // maxima beyond which an exponent is not one FMA (below)
+
+// A product that the compiler does not join with a subtraction behind it. The largest score's exponent is score * scale - maximum
+// with the maximum that product rounded: an FMA gives the rounding error in its place, up to half a step of the maximum. It is
+// the same factor in a row's sums and cancels while weights stay in range: up to a maximum of 2^20 it is below 2^-4. From 2^28
+// on fp16 weights, from 2^31 on fp32 ones, left their type.
+__device__ __forceinline__ float mul_rounded(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
+
 enum AttnType : int { kAttnBF16 = 0, kAttnF16 = 1 };
 
 template <int DT>

@@ -14,7 +14,6 @@
 
 namespace qe_tree {
 constexpr int kWaves = 4, kUnit = 128;
-constexpr float kLazy = 8.f;  // the running maximum follows a row's scores once they pass it by this much (2^8 in the sums)
 
 // blocks of the kernel on a CU, by its registers
 constexpr int blocks_of(int nt_d) { return nt_d == 64 ? 3 : nt_d == 128 ? 2 : 1; }
@@ -139,8 +138,7 @@ __global__ __launch_bounds__(kThreads, blocks_of(NT * D)) void tree_kernel(Args 
                             const int tok = tb + 16 * x + 4 * grp + e, j = tok - s.len;
                             const uint32_t drafted = (uint32_t)(tok < s.total) & (uint32_t)(see[nt] >> (j & 63));
                             const bool on = ((uint32_t)f.ok[x] & ((uint32_t)(j < 0) | drafted) & 1) != 0;
-                            // times the scale here: a negative one must not turn -inf around
-                            sc[nt][x][e] = on ? sc[nt][x][e] * a.scale2 : kNegInf;
+                            sc[nt][x][e] = on ? mul_rounded(sc[nt][x][e], a.scale2) : kNegInf;
                         }
             } else {
 #pragma unroll
@@ -148,7 +146,7 @@ __global__ __launch_bounds__(kThreads, blocks_of(NT * D)) void tree_kernel(Args 
 #pragma unroll
                     for (int x = 0; x < 2; x++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) sc[nt][x][e] *= a.scale2;
+                        for (int e = 0; e < 4; e++) sc[nt][x][e] = mul_rounded(sc[nt][x][e], a.scale2);
             }
             u32x4_v p[NT];
 #pragma unroll
@@ -158,7 +156,7 @@ __global__ __launch_bounds__(kThreads, blocks_of(NT * D)) void tree_kernel(Args 
                 for (int x = 0; x < 2; x++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) mx = fmaxf(mx, sc[nt][x][e]);
-                if (__any(mx > m[nt] + kLazy)) {
+                if (__any(mx - m[nt] > kLazy)) {  // (m + kLazy would round up to the next number where that is 2 kLazy away)
                     const float top = fmaxf(m[nt], max_over_quarters(mx));
                     const float f0 = top == kNegInf || pass > 1 ? 1.f : __builtin_amdgcn_exp2f(m[nt] - top);
                     m[nt] = top;

@@ -5,8 +5,6 @@
 #include "attn_common.hpp"
 #include "mfma_tile.hpp"
 
-constexpr float kLazy = 8.f;  // the running maximum follows a row's scores once they pass it by this much (2^8 in the sums)
-
 // Tiles in LDS. A row is CH = D / 8 pieces of 16 bytes, a DMA instruction fills 1 KB = RK rows.
 // K: a wave reads one piece of 32 rows (ds_read_b128), so 16 neighbouring rows must have it in 16 different places of a
 // 256-byte line: pieces are permuted inside groups of 1, 2 or 4 by row, and each KB starts PAD bytes further on.
@@ -34,6 +32,7 @@ struct Wave32 {
     u32x4_v q[KS];  // lane: query lane % 32, values 16 ks + 8 (lane / 32) ..
     f32x16_v o[DB]; // lane: query lane % 32, columns 32 db + 8 (e / 4) + 4 (lane / 32) + e % 4
     float m, l;     // maximum (times the scale, base 2) and this half's sum
+    float lazy;     // kLazy, or -inf once a row of the wave has its maximum beyond kFar
     // the lane's places in a K tile (row lane % 32, piece 2 ks + lane / 32 for ks = 0 and 1) and in a V tile (row 4 (lane /
     // 32) + (0 .. 3) by lane, columns 32 d + 16 (lane / 16 % 2) + 4 (lane % 4) for d = 0 .. 3)
     int kat[2], vat[4];
@@ -59,6 +58,7 @@ struct Wave32 {
     __device__ __forceinline__ void clear() {
         m = kNegInf;
         l = 0.f;
+        lazy = kLazy;
 #pragma unroll
         for (int d = 0; d < DB; d++)
 #pragma unroll
@@ -104,8 +104,8 @@ struct Wave32 {
         return r;
     }
     // Softmax of the scores and their products with the step's values, whose first reads are under way during the softmax
-    __device__ __forceinline__ void values(const char* tile, const Scores& r, int pass, float scale2) {
-        const f32x16_v(&s)[NX] = r.s;
+    __device__ __forceinline__ void values(const char* tile, Scores r, int pass, float scale2) {
+        f32x16_v(&s)[NX] = r.s;
         constexpr int GV = NX == 1 ? 2 : 4, NV = DB * 2 * NX / GV;
         u32x4_v vf[2][GV];
         auto read_v = [&](int g) {
@@ -129,23 +129,34 @@ struct Wave32 {
         for (int x = 0; x < NX; x++)
 #pragma unroll
             for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[x][e]);
-        mx *= scale2;
-        if (__any(mx > m + kLazy)) {
+        mx = mul_rounded(mx, scale2);
+        float less = m == kNegInf ? 0.f : m;
+        if (__any(mx - m > lazy)) {  // (m + kLazy would round up to the next number where that is 2 kLazy away)
             const float top = fmaxf(m, max_over_halves(mx));
             const float f0 = top == kNegInf || pass > 1 ? 1.f : __builtin_amdgcn_exp2f(m - top);
             m = top;
             l *= f0;
 #pragma unroll
             for (int d = 0; d < DB; d++) o[d] *= f0;
+            less = m == kNegInf ? 0.f : m;
+            if (pass <= 1 && __any(fabsf(less) > kFar)) {  // this step's exponents, and from now on every step's
+                lazy = kNegInf;
+#pragma unroll
+                for (int x = 0; x < NX; x++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) s[x][e] = mul_rounded(s[x][e], scale2) - less;
+                scale2 = 1.f;
+                less = 0.f;
+                asm volatile("" : "+s"(scale2), "+v"(less));  // no copy of the products below for these constants
+            }
         }
-        const float base = m == kNegInf ? 0.f : m;
         u32x4_v p[2 * NX];
 #pragma unroll
         for (int x = 0; x < NX; x++)
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-                const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], scale2, -base));
-                const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e + 1], scale2, -base));
+                const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e], scale2, -less));
+                const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e + 1], scale2, -less));
                 l += w0 + w1;
                 p[2 * x + e / 8][e % 8 / 2] = T::pack(w0, w1);
             }
