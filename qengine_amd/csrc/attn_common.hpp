@@ -41,6 +41,7 @@ struct AttnT<kAttnBF16> {
     }
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
     static constexpr uint32_t kExpMask = 0x7f80u, kInf = 0x7f80u, kOne = 0x3f80u;
+    static constexpr float kRoom = 40.f;
 };
 template <>
 struct AttnT<kAttnF16> {
@@ -52,6 +53,7 @@ struct AttnT<kAttnF16> {
     }
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_f16x2(lo, hi); }
     static constexpr uint32_t kExpMask = 0x7c00u, kInf = 0x7c00u, kOne = 0x3c00u;
+    static constexpr float kRoom = 0.f;
 };
 
 // x of the lane 32 (16) places away, combined: every lane gets op over the pair
@@ -74,10 +76,16 @@ __device__ __forceinline__ float sum_over_quarters(float x) {
 
 // ---- values that are not finite in keys that some rows of a tile must not see
 // A masked key has weight 0, but 0 times an infinity or a NaN in the matrix product is NaN. Kernels whose sums come out not
-// finite therefore run again, first over the finite values alone (pass 1: zeros in the others' place), then once for each
-// kind of the others with ones in their place and weight 1 where a row sees a key: where such a sum is positive the row sees
-// a +inf (pass 2), a -inf (3) or a NaN (4) in that column.
+// finite, or so large that they soon would, therefore run again, first over the finite values alone (pass 1: zeros in the
+// others' place), then once for each kind of the others with ones in their place and weight 1 where a row sees a key: where
+// such a sum is positive the row sees a +inf (pass 2), a -inf (3) or a NaN (4) in that column.
+// Sums of bf16 values can pass fp32 although the result, their mean, does not (weights reach 2^8, and there are many): pass 1
+// holds the maximum kRoom higher than the scores, so that weights are 2^-40 of what they were. bf16 probabilities lose nothing
+// by it; columns with values below 2^-86 do, beside others above 2^100, and maxima beyond 2^29 have no digits for it. fp16
+// values are too small to get there.
 constexpr int kKinds = 4;
+// NaN where a sum is not finite or past 2^108 (parts that are below it stay finite when they are added), else x
+__device__ __forceinline__ float if_bad(float sum, float x) { return __builtin_fmaf(sum * 0x1p20f, 0.f, x); }
 template <int DT>
 __device__ __forceinline__ uint32_t keep_half(uint32_t h, int pass) {
     constexpr uint32_t E = AttnT<DT>::kExpMask, I = AttnT<DT>::kInf;

@@ -156,6 +156,7 @@ __global__ __launch_bounds__(kThreads, blocks_of(NT * D)) void tree_kernel(Args 
                 for (int x = 0; x < 2; x++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) mx = fmaxf(mx, sc[nt][x][e]);
+                if (pass == 1) mx += T::kRoom;
                 if (__any(mx - m[nt] > kLazy)) {  // (m + kLazy would round up to the next number where that is 2 kLazy away)
                     const float top = fmaxf(m[nt], max_over_quarters(mx));
                     const float f0 = top == kNegInf || pass > 1 ? 1.f : __builtin_amdgcn_exp2f(m[nt] - top);
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(kThreads, blocks_of(NT * D)) void tree_kernel(Args 
 #pragma unroll
                     for (int t = 0; t < DT16; t++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) bad = __builtin_fmaf(o[nt][t][e], 0.f, bad);
+                        for (int e = 0; e < 4; e++) bad = if_bad(o[nt][t][e], bad);
                 if (!__any(!(bad == 0.f))) break;
                 pass = 2;
             } else if (pass > 1) {

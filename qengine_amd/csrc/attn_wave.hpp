@@ -129,7 +129,7 @@ struct Wave32 {
         for (int x = 0; x < NX; x++)
 #pragma unroll
             for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[x][e]);
-        mx = mul_rounded(mx, scale2);
+        mx = __builtin_fmaf(mx, scale2, pass == 1 ? T::kRoom : 0.f);
         float less = m == kNegInf ? 0.f : m;
         if (__any(mx - m > lazy)) {  // (m + kLazy would round up to the next number where that is 2 kLazy away)
             const float top = fmaxf(m, max_over_halves(mx));
@@ -224,13 +224,13 @@ struct Wave32 {
             m = top;
         }
     }
-    // whether a sum is not finite
+    // whether a sum is not finite, or about not to be
     __device__ __forceinline__ bool bad() const {
         float x = 0.f;
 #pragma unroll
         for (int d = 0; d < DB; d++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) x = __builtin_fmaf(o[d][e], 0.f, x);
+            for (int e = 0; e < 16; e++) x = if_bad(o[d][e], x);
         return !(x == 0.f);
     }
     // out: column 4 (lane / 32) of the lane's row; l: the whole row's sum
