@@ -86,6 +86,10 @@ __device__ __forceinline__ float sum_over_quarters(float x) {
 constexpr int kKinds = 4;
 // NaN where a sum is not finite or past 2^108 (parts that are below it stay finite when they are added), else x
 __device__ __forceinline__ float if_bad(float sum, float x) { return __builtin_fmaf(sum * 0x1p20f, 0.f, x); }
+// A part's sums join the others times the power of two that its maximum is below theirs. Sums that are not finite must not meet
+// a 0 there (a row that is not split gets an infinity of a key under any weight that is not masked), so that of a part with
+// keys stays above it.
+__device__ __forceinline__ float above_zero(float f) { return fmaxf(f, 0x1p-149f); }
 template <int DT>
 __device__ __forceinline__ uint32_t keep_half(uint32_t h, int pass) {
     constexpr uint32_t E = AttnT<DT>::kExpMask, I = AttnT<DT>::kInf;

@@ -294,6 +294,7 @@ __global__ __launch_bounds__(kThreads, blocks_of(NT * D)) void tree_kernel(Args 
                 f[w] = x.x == kNegInf ? 0.f : __builtin_amdgcn_exp2f(x.x - top);
                 if (x.x == __builtin_huge_valf()) f[w] = 1.f;  // the row's sums are NaN already
                 sum += f[w] * x.y;
+                if (x.x != kNegInf) f[w] = above_zero(f[w]);
             }
             float y[D / 16];
 #pragma unroll

@@ -181,7 +181,7 @@ __global__ __launch_bounds__(kThreads) void join_kernel(Args a, int most) {
         const float2 x = a.ml[at(i)];
         float f = x.x == kNegInf ? 0.f : __builtin_amdgcn_exp2f(x.x - top);
         if (x.x == __builtin_huge_valf()) f = 1.f;
-        wgt[i] = f;
+        wgt[i] = x.x == kNegInf ? 0.f : above_zero(f);
         sum += f * x.y;
     }
 #pragma unroll

@@ -72,6 +72,51 @@ def test_some_parts_alone_pass_fp32(dev):
     compare_tree(c, q, seqs, cu, None, *attend(c, q, seqs, cu, 2, lse=True))
 
 
+# where the key with the large score and the infinity under a weight that underflows lie: in two waves of a block, two steps,
+# two parts
+PLACES = [(100, 5, 40), (100, 40, 5), (700, 3, 690), (9000, 8990, 5), (9000, 5, 8990), (9000, 4000, 4040)]
+
+
+@pytest.mark.parametrize("parts", [1, 0])
+@pytest.mark.parametrize("context,top,far_key", PLACES)
+@pytest.mark.parametrize("d,rows", ROWS)
+def test_infinities_under_small_weights(dev, d, rows, context, top, far_key, parts):
+    """a row that sees an infinity gets it, wherever the key is and whatever its weight; other columns are what the formula says"""
+    n = min(rows, 16)
+    heads = -(-rows // n)
+    c, q, seqs, cu, _, _ = setup(dev, [context], [n], heads, 1, d, 16, BF, seed=rows)
+    s = seqs.item()
+    table = c.table[s].tolist()
+    q.mul_(0.125)
+    q[..., 0] = 16
+    c.k.mul_(0.125)
+    c.k[..., 0] = 0
+    put = lambda x, i, col, y: x[0, table[i // 16], 0, i % 16].__setitem__(col, y)
+    put(c.k, top, 0, 16.0)
+    put(c.k, far_key, 0, -16.0)  # exponents 256 + 256 apart
+    for col, y in ((1, INF), (2, -INF), (3, NAN)):
+        put(c.v, far_key, col, y)
+    put(c.v, far_key, 4, INF), put(c.v, top, 4, -INF)
+    put(c.v, far_key, 5, -INF), put(c.v, top, 5, 3.0)
+    call("qe_attn_tree_set_split", parts)
+    try:
+        out, lse = attend(c, q, seqs, cu, n, scale=far.LN2, lse=True)
+    finally:
+        call("qe_attn_tree_set_split", 1)
+    for col, y in ((1, INF), (2, -INF), (5, -INF)):
+        assert (out[..., col].float() == y).all(), col
+    assert torch.isnan(out[..., 3]).all() and torch.isnan(out[..., 4]).all()
+    at = torch.arange(context + n, device=dev)
+    pg = torch.tensor(table, device=dev)[at // 16]
+    k, v = c.k[0, pg, 0, at % 16], c.v[0, pg, 0, at % 16].clone()
+    v[:, 1:6] = 0
+    seen = torch.ones(n, context + n, dtype=torch.bool, device=dev).tril(context)
+    rest = [0] + list(range(6, d))
+    for h in range(heads):
+        o, l, ob, lb = ref.rows(q[:, h], k, v, seen, far.LN2)
+        ref.check(out[:, h][:, rest], lse[:, h], o[:, rest], l, ob[:, rest], lb)
+
+
 @pytest.mark.parametrize("lens,heads,kv,d", PROMPTS, ids=str)
 def test_prompt_infinities_and_their_lse(dev, lens, heads, kv, d):
     q, k, v, cu = inputs(dev, lens, heads, kv, d, BF, seed=d)
