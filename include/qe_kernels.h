@@ -348,7 +348,9 @@ void qe_moe_pack_w4(const int32_t* gu_q, const uint16_t* gu_s, const int32_t* dn
  * A row that sees no key has out = 0 and lse = -inf; a key that a row does not see has no effect on it, whatever its bits.
  * Lengths, tables and indexes live on the device and are not seen by the host: values out of range make a kernel skip
  * what they name and never touch memory outside the tensors. Every call is one to three launches on `stream`, without
- * host synchronization, and can be captured. Deterministic: same inputs, same bits. ---- */
+ * host synchronization, and can be captured; but the first qe_attn_tree of a stream, and the first whose head size or rows
+ * take a kernel with a larger workspace than those before (9 or 68 MB at d = 128, whatever the batch), allocates it and
+ * waits for the stream. Deterministic: same inputs, same bits. ---- */
 
 /* Causal attention over whole prompts packed without padding: sequence b is rows cu[b] .. cu[b + 1] - 1 (cu [nseq + 1]
  * int32, ascending), row i of it sees rows 0 .. i. Rows of q, k, v and out have strides of their own (k_row, v_row below

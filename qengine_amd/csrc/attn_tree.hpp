@@ -233,7 +233,10 @@ void launch_split(Args a, Kernel kernel, int threads, size_t lds, int per_cu, hi
     const int64_t runs = (int64_t)a.nseq * a.kv_heads * a.rb_max;
     const int64_t most_units = ((int64_t)(a.width << a.shift) + UNIT - 1) / UNIT;
     const int grid = (int)std::min<int64_t>(runs * most_units, per_cu * qe_num_cus());
-    const size_t part = (size_t)grid * 2 * ROWS * D * 4, ml = (size_t)grid * 2 * ROWS * 8, ends = ((size_t)a.nseq + 1) * 4;
+    // the same for every call of a kernel, whatever its batch and grid: a stream's buffer is allocated by its first call and
+    // kept, not replaced (a hipMalloc and a wait for the stream) by each batch that is larger than those before
+    const size_t blocks = (size_t)per_cu * qe_num_cus();
+    const size_t part = blocks * 2 * ROWS * D * 4, ml = blocks * 2 * ROWS * 8, ends = ((size_t)kMaxTreeBatch + 1) * 4;
     WsHold hold(st);
     if (char* ws = attn_tree_split() ? static_cast<char*>(hold.get(kWsAttn, part + ml + ends)) : nullptr) {
         a.part = reinterpret_cast<float*>(ws);
