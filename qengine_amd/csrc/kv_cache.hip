@@ -269,14 +269,14 @@ __global__ __launch_bounds__(kThreads) void release_kernel(Slots s, const int32_
 struct AppendArgs {
     const char *k, *v;
     int64_t kl, kr, kh, vl, vr, vh;  // bytes
-    int layer0, nseq, t;
+    int layer0, nseq, first, t;  // rows first .. t - 1
 };
 // A wave per row and layer: its lanes find the row's sequence with one vote per 64 sequences, then move the row's keys and
 // values, 16 bytes a lane. 2048 rows, 32 layers, 8 heads of 128: 537 MB in 101-105 us.
 __global__ __launch_bounds__(kThreads) void append_kernel(Pool p, Slots s, AppendArgs a, const int32_t* __restrict__ seqs,
                                                           const int32_t* __restrict__ cu) {
     const int lane = threadIdx.x & 63;
-    const int t = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+    const int t = a.first + blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
     if (t >= a.t) return;
     int b = 0;
     for (int j = 0; j < a.nseq; j += 64) b += __popcll(__ballot(j + lane < a.nseq && cu[j + lane + 1] <= t));
@@ -412,9 +412,14 @@ void kv_append(const qe_kv_cache_t& c, int layer, int layers, const void* k, con
     CHECK((((uintptr_t)k | (uintptr_t)v) & 15) == 0, "qe_kv_append: k and v must be 16-byte aligned");
     for (int i = 0; i < 6; i++) CHECK(strides[i] % 8 == 0, "qe_kv_append: stride %lld (a multiple of 8)", (long long)strides[i]);
     AppendArgs a{(const char*)k, (const char*)v, 2 * strides[0], 2 * strides[1], 2 * strides[2], 2 * strides[3], 2 * strides[4],
-                 2 * strides[5], layer, nseq, t};
-    append_kernel<<<dim3((t - 1) / (kThreads / 64) + 1, layers), kThreads, 0, st>>>(pool_of(c), slots_of(c), a, seqs, cu);
-    HIP_CHECK(hipGetLastError());
+                 2 * strides[5], layer, nseq, 0, 0};
+    constexpr int kLaunch = 1 << 25;  // rows of a launch: a grid has fewer than 2^32 threads in x, 64 a row
+    for (int first = 0; first < t; first += kLaunch) {
+        a.first = first;
+        a.t = std::min(t, first + kLaunch);
+        append_kernel<<<dim3((a.t - first - 1) / (kThreads / 64) + 1, layers), kThreads, 0, st>>>(pool_of(c), slots_of(c), a, seqs, cu);
+        HIP_CHECK(hipGetLastError());
+    }
 }
 
 void kv_accept(const qe_kv_cache_t& c, const int32_t* seqs, const int32_t* count, const int32_t* path, int most, int n,
