@@ -96,6 +96,11 @@ def _check_out(out, q, dtype, at):
     _rows("out", out, 3, dtype, at)
     if out.shape != q.shape:
         raise ValueError(f"out has q's shape {tuple(q.shape)}, got {tuple(out.shape)}")
+    s, (t, heads, d) = out.stride(), q.shape
+    if s[0] < heads * s[1] or s[1] < d:  # not row after row of heads side by side
+        (near, n), (far, m) = sorted(((s[0], t), (s[1], heads)))
+        if n > 1 and near < d or m > 1 and far < (near * (n - 1) if n > 1 else 0) + d:
+            raise ValueError(f"out's rows overlap: shape {tuple(q.shape)}, strides {s}")
 
 
 def _check_scale(scale):

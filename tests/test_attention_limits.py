@@ -79,3 +79,26 @@ def test_more_layers_than_a_launch_takes():
     ops.KVCache(pool[:65535], pool[:65535], *ints)
     with pytest.raises(ValueError, match="layers"):
         ops.KVCache(pool, pool, *ints)
+
+
+@pytest.mark.parametrize("shape,strides", [((4, 4, 64), (0, 64, 1)), ((4, 4, 64), (256, 0, 1)), ((4, 4, 64), (64, 64, 1)), ((4, 4, 64), (128, 64, 1)),
+                                           ((4, 4, 64), (256, 32, 1)), ((4, 4, 64), (64, 192, 1)), ((4, 1, 64), (32, 64, 1))])
+def test_an_output_whose_rows_overlap(shape, strides):
+    """expanded or overlapping outputs: which row's value stays would be a race"""
+    out = torch.zeros(4096, dtype=BF).as_strided(shape, strides)
+    heads = shape[1]
+    with pytest.raises(ValueError, match="overlap"):
+        ops.attn_prompt(rows(4, heads), rows(4, 1), rows(4, 1), i32(0, 4), out=out)
+    with pytest.raises(ValueError, match="overlap"):
+        cache().attend(0, rows(4, heads), i32(0), i32(0, 4), 4, out=out)
+
+
+@pytest.mark.parametrize("shape,strides", [((4, 4, 64), (256, 64, 1)), ((4, 4, 64), (64, 256, 1)), ((4, 4, 64), (1024, 128, 1)), ((1, 4, 64), (0, 64, 1)),
+                                           ((4, 1, 64), (64, 0, 1)), ((4, 4, 64), (64, 264, 1))])
+def test_outputs_whose_rows_lie_apart(shape, strides):
+    out = torch.zeros(4096, dtype=BF).as_strided(shape, strides)
+    heads, n = shape[1], shape[0]
+    with pytest.raises(ValueError, match="on a GPU"):
+        ops.attn_prompt(rows(n, heads), rows(n, 1), rows(n, 1), i32(0, n), out=out)
+    with pytest.raises(ValueError, match="on a GPU"):
+        cache().attend(0, rows(n, heads), i32(0), i32(0, n), 4, out=out)
