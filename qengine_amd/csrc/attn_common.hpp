@@ -8,7 +8,6 @@
 #include "qe_common.hpp"
 
 typedef short s16x4_v __attribute__((ext_vector_type(4)));
-typedef short s16x8_v __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4_v __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;

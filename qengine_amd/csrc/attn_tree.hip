@@ -30,6 +30,7 @@ template <int DT, int D, int NT>
 __global__ __launch_bounds__(kThreads, blocks_of(NT * D)) void tree_kernel(Args a) {
     using T = AttnT<DT>;
     using F = Frag<D>;
+    static_assert(NT * D <= 256, "registers for the next keys and values beside these");
     constexpr int ROWS = 16 * NT, KS = F::KS, VD = F::VD, DT16 = D / 16;
     constexpr int PITCH = D + 4;
     __shared__ float obuf[kWaves][16][PITCH];
@@ -198,7 +199,7 @@ __global__ __launch_bounds__(kThreads, blocks_of(NT * D)) void tree_kernel(Args 
             }
         };
 
-        // this wave's tokens: 32 of each unit; where the registers allow it the next 32 are on their way meanwhile
+        // this wave's tokens: 32 of each unit; the next 32 are on their way meanwhile
         const int stop = min(t1 * kUnit, s.total);
         uint32_t kinds[3][NT][(DT16 * 4 + 31) / 32];  // bit: the wave's row sees a +inf, -inf, NaN in the column
         for (;;) {
@@ -212,19 +213,12 @@ __global__ __launch_bounds__(kThreads, blocks_of(NT * D)) void tree_kernel(Args 
             int tb = t0 * kUnit + wave * 32;
             if (tb < stop) {
                 F f;
-                if constexpr (NT * D <= 256) {
-                    load(f, tb);
-                    for (; tb < stop; tb += kUnit) {
-                        F next;
-                        load(next, tb + kUnit < stop ? tb + kUnit : tb);
-                        compute(f, tb);
-                        f = next;
-                    }
-                } else {
-                    for (; tb < stop; tb += kUnit) {
-                        load(f, tb);
-                        compute(f, tb);
-                    }
+                load(f, tb);
+                for (; tb < stop; tb += kUnit) {
+                    F next;
+                    load(next, tb + kUnit < stop ? tb + kUnit : tb);
+                    compute(f, tb);
+                    f = next;
                 }
             }
             if (pass == 0) {
