@@ -64,8 +64,8 @@ void qe_gemm_tune_file(const char* path);
 void qe_gemm_tune_clear(void);
 int qe_gemm_tune_entries(void);
 /* Library-owned workspaces (the prefill GEMMs' split-K partial sums, the fp16-accumulate and W4A8 / W8A8 pre-pass
- * buffers, the part sums of 9..64-row decode and of the attention over the cache) are kept per (device, stream): calls on one stream share a buffer (a
- * call's launches stay together, also with several host threads on the stream), calls on two streams of a device use
+ * buffers, the part sums of 9..64-row decode and of the attention over the cache) are kept per (device, stream): calls on
+ * one stream share a buffer (a call's launches stay together, also with several host threads on the stream), calls on two streams of a device use
  * two, so concurrent streams never overwrite each other's workspace (the reference keeps them thread_local,
  * src/kernels/gemm.cu:3258-3368). A buffer grows on a call outside graph capture. Captured calls use buffers that their
  * graph holds (a HIP user object), so graphs may replay on any streams, beside each other and eager calls; destroying
@@ -354,7 +354,8 @@ void qe_moe_pack_w4(const int32_t* gu_q, const uint16_t* gu_s, const int32_t* dn
 
 /* Causal attention over whole prompts packed without padding: sequence b is rows cu[b] .. cu[b + 1] - 1 (cu [nseq + 1]
  * int32, ascending), row i of it sees rows 0 .. i. Rows of q, k, v and out have strides of their own (k_row, v_row below
- * 2^24), so views into one fused QKV product do; out overlaps none of them. nseq <= 4096. Rows before cu[0] and from cu[nseq] on are left as they were. flags: QE_F16. */
+ * 2^24), so views into one fused QKV product do; out overlaps none of them. nseq <= 4096. Rows before cu[0] and from cu[nseq]
+ * on are left as they were. flags: QE_F16. */
 void qe_attn_prompt(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head,
                     const void* v, int64_t v_row, int64_t v_head, void* out, int64_t out_row, int64_t out_head, float* lse,
                     const int32_t* cu, int nseq, int t, int heads, int kv_heads, int d, float scale, int flags,
@@ -387,8 +388,8 @@ typedef struct qe_kv_cache {
 void qe_kv_reserve(const qe_kv_cache_t* cache, const int32_t* seqs, const int32_t* add, int n, int32_t* ok,
                    int32_t* copies, void* stream);
 /* Slot children[i] gets parents[i]'s committed tokens by sharing their pages (the next reserve copies the partly filled
- * one). ok[i] 0: nothing done: a slot out of range, a child that holds pages or tokens, is named by an earlier entry or is
- * one of the call's children as well as a parent. n <= 1024. */
+ * one). ok[i] 0: nothing done: a slot out of range, a child that holds pages or tokens or is named as a child by an earlier
+ * entry, or a parent that is one of the call's children. n <= 1024. */
 void qe_kv_fork(const qe_kv_cache_t* cache, const int32_t* parents, const int32_t* children, int n, int32_t* ok,
                 void* stream);
 /* Slot seqs[i] keeps its first min(length, lengths[i]) tokens (lengths NULL: none) and the pages that hold them; the
@@ -396,14 +397,14 @@ void qe_kv_fork(const qe_kv_cache_t* cache, const int32_t* parents, const int32_
 void qe_kv_release(const qe_kv_cache_t* cache, const int32_t* seqs, const int32_t* lengths, int n, void* stream);
 /* New keys and values: row t of sequence b (cu as above; slot seqs[b], distinct) goes to token length + t - cu[b] of the
  * slot, in `layers` layers from `layer` on. strides: layer, row and head of k, then of v (host memory, elements). Rows
- * without a held page, or whose page other slots hold too (no reserve since a fork or a cut), are not written. length is
- * not changed. */
+ * without a held page, or whose page other slots hold too (no reserve since a fork or a cut), are not written; the answers
+ * of qe_kv_reserve say for which slots there is room. length is not changed. */
 void qe_kv_append(const qe_kv_cache_t* cache, int layer, int layers, const void* k, const void* v, const int64_t* strides,
                   const int32_t* seqs, const int32_t* cu, int nseq, int t, void* stream);
 /* Commits count[i] tokens of slot seqs[i] (distinct). path NULL: the first drafted ones. Else path int32 [n][most], most
  * <= 64: drafted rows path[i][0 .. count - 1] move to the first places after the committed tokens, in all layers, as if
- * all were read before any is written (none moves into a page that other slots hold too). length_out [slots] (NULL: the cache's own) gets length + count, at most what the
- * held pages take. */
+ * all were read before any is written (none moves into a page that other slots hold too: commit before a fork). length_out
+ * [slots] (NULL: the cache's own) gets length + count, at most what the held pages take, whatever was written there. */
 void qe_kv_accept(const qe_kv_cache_t* cache, const int32_t* seqs, const int32_t* count, const int32_t* path, int most,
                   int n, int32_t* length_out, void* stream);
 

@@ -111,7 +111,8 @@ def _check_scale(scale):
 def attn_prompt(q, k, v, cu, scale=None, out=None, lse=False):
     """Causal attention of packed prompts: q [t][heads][d], k and v [t][kv heads][d] (views into one QKV product do),
     sequence b the rows cu[b] .. cu[b + 1] - 1. -> out like q; with lse=True (out, lse [t][heads] fp32). Rows before cu[0]
-    and from cu[-1] on are left as they were in a given `out` (and have no meaning in a new one)."""
+    and from cu[-1] on are left as they were in a given `out` (and have no meaning in a new one), which is memory of its own,
+    not part of q, k or v."""
     t, heads, kv, d, n, fresh = _prompt_shapes(q, k, v, cu, scale, out)
     if fresh:
         out = torch.empty(t, heads, d, dtype=q.dtype, device=q.device)
@@ -228,7 +229,8 @@ class KVCache:
 
     def fork(self, parents, children):
         """Slot children[i] shares the pages of parents[i]'s committed tokens. -> int32 [n], 1: done, 0: nothing changed (a bad
-        slot, a child that is not empty, is repeated, or is one of the call's parents)."""
+        slot, a child that is not empty or is repeated, or a parent that is one of the call's children). Drafted tokens that the
+        parent has not committed stay its own: commit them before a fork, since rows do not move in a page that is shared."""
         n = self._batch("parents", parents)
         self._batch("children", children, n)
         self._few(n)
@@ -249,7 +251,8 @@ class KVCache:
     def append(self, layer, k, v, seqs, cu):
         """New rows k, v [t][kv heads][d] of one layer, or [layers][t][kv heads][d] of all (layer None): rows cu[b] ..
         cu[b + 1] - 1 go behind the committed tokens of slot seqs[b], into pages reserved before (after a fork or a cut
-        again: rows are not written into a page that other slots hold too). Slots are distinct."""
+        again: rows are not written into a page that other slots hold too). Slots are distinct. Rows without room are left
+        out and nothing says so here: reserve's answer does."""
         one = layer is not None
         dims, shape = (3, k.shape) if one else (4, k.shape)
         _rows("k", k, dims, self.dtype, self._dev)
@@ -276,7 +279,9 @@ class KVCache:
 
     def accept(self, seqs, count, path=None, length=None):
         """count[i] drafted tokens of slot seqs[i] are committed: the first ones, or those of path int32 [n][at most 64], whose
-        rows move together in all layers. The new lengths go to `length` [slots], or the cache's own. Slots are distinct."""
+        rows move together in all layers. The new lengths go to `length` [slots], or the cache's own. Slots are distinct. What
+        counts is `count`, up to the slot's pages: also rows are committed that append left out, or that could not move, since
+        their page is shared. So only slots whose reserve answered 1 are appended to and committed."""
         n = self._batch("seqs", seqs)
         self._batch("count", count, n)
         most = 0

@@ -20,7 +20,6 @@ struct Tile {
     static __device__ __forceinline__ int k_row(int r) { return r / RK * (1024 + PAD) + r % RK * (D * 2); }
 };
 
-
 template <int DT, int D, int KEYS>
 struct Wave32 {
     using T = AttnT<DT>;
@@ -150,6 +149,7 @@ struct Wave32 {
                 asm volatile("" : "+s"(scale2), "+v"(less));  // no copy of the products below for these constants
             }
         }
+        // rounded to the values' type, since the matrix cores take nothing wider at that rate; their sum is not
         u32x4_v p[2 * NX];
 #pragma unroll
         for (int x = 0; x < NX; x++)

@@ -49,9 +49,8 @@ def _conv(a):
 
 
 def typed(name, sig, restype=None):
-    """A library function with its argument types fixed (sig: 'p' pointer, 'i' int, 'l' int64, 'z' size_t,
-    'f' float, one letter each), for the
-    wrappers that decode loops call: ctypes then takes plain ints and addresses. `call` builds a ctypes object per
+    """A library function with its argument types fixed (sig: 'p' pointer, 'i' int, 'l' int64, 'z' size_t, 'f' float, one
+    letter each), for the wrappers that decode loops call: ctypes then takes plain ints and addresses. `call` builds a ctypes object per
     argument; one row of an 8192 x 2048 INT8 matrix (4.8 us on the GPU) took 9.7 us a call through it, 4.9 us so."""
     f = lib()[name]  # a function object of its own (an attribute would be shared with `call`)
     f.argtypes = [{"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_int64, "z": ctypes.c_size_t, "f": ctypes.c_float}[c] for c in sig]
