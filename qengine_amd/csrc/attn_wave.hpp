@@ -125,9 +125,11 @@ struct Wave32 {
         __builtin_amdgcn_sched_barrier(0);
         float mx = kNegInf;
 #pragma unroll
-        for (int x = 0; x < NX; x++)
+        for (int x = 0; x < NX; x++) {
+            if constexpr (D == 256) asm("" : "+v"(s[x]));  // not in accumulators, from where each use below would read them
 #pragma unroll
             for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[x][e]);
+        }
         mx = __builtin_fmaf(mx, scale2, pass == 1 ? T::kRoom : 0.f);
         float less = m == kNegInf ? 0.f : m;
         if (__any(mx - m > lazy)) {  // (m + kLazy would round up to the next number where that is 2 kLazy away)
