@@ -4,9 +4,10 @@
 //
 // One pass over the keys with the running maximum and sum of the softmax; a block takes BQ = 32 RW rows of one head, a wave
 // 32 of them (attn_wave.hpp). KEYS keys at a time lie in LDS, staged by DMA while the step before is worked on. 16384 rows of
-// 16 heads over 2: d = 128 967 us (1137 TFLOP/s, bounded by MFMA and softmax of three waves a SIMD), d = 64 567 us, d = 256
-// 2.46-2.55 ms (one wave a SIMD: MFMA, LDS reads and softmax add up). Short prompts are bounded by the start of a block
-// (dependent reads of the starts, then queries and keys: about 4 us).
+// 16 heads over 2, inputs rotating over three sets, by card: d = 128 1014-1064 us (1035-1085 TFLOP/s; MFMA busy 65 %, beside the
+// softmax of three waves a SIMD; 12 bytes a lane are spilled), d = 64 587-613 us, d = 256 2.57-2.60 ms (one wave a SIMD: MFMA,
+// LDS reads and softmax add up). Short prompts are bounded by the start of a block (dependent reads of the starts, then queries
+// and keys: about 4 us).
 #include "attn_wave.hpp"
 #include "kv_cache.hpp"
 #include "seq_rows.hpp"
@@ -196,16 +197,18 @@ void launch(const Args& a, hipStream_t st) {
 template <int DT>
 void by_shape(const Args& a, int d, hipStream_t st) {
     // Blocks of 64 rows in four (two for d = 256) groups that share out the keys, while they fill the CUs once, or twice where
-    // prompts are long: a block's time is its steps, of which the last rows' has most. us, blocks of 128 rows / these: 2000
-    // rows of 8 heads over 1 43.2 / 26.6, 4000 81 / 54, of 40 heads over 8 300 rows 11.6 / 10.8, 500 16.7 / 18.0, 1000 29.4 /
-    // 35.0; d = 256, 16 heads over 2 1000 44.7 / 35.9, 2000 84 / 75, 4000 183 / 251; d = 64 2000 32 / 22, 6000 107 / 125.
+    // prompts are long: a block's time is its steps, of which the last rows' has most. us, blocks of 128 rows (steps of 64
+    // keys) / these, inputs rotating over three sets: d = 128, 8 heads over 1: 1000 rows 25.4 / 16.6, 2000 44.3 / 26.0, 4000
+    // 82 / 54, 40 heads over 8: 300 rows 11.6 / 10.5, 500 16.7 / 18.1, 1000 29.0 / 35.4; d = 256, 16 heads over 2: 1000 48.6 /
+    // 38.7, 2000 86 / 78, 4000 181 / 255; d = 64, 8 heads over 1: 2000 31.4 / 16.2 (6000 rows, past the rule, 86 / 68).
     const int64_t blocks = ((int64_t)a.t / 64 + a.nseq) * a.heads, cus = qe_num_cus();
     const bool few = blocks <= cus || (blocks <= 2 * cus && a.t >= (int64_t)1000 * a.nseq);
     // Else blocks of 128 rows. Steps of 32 keys take registers and LDS for three blocks a CU instead of two: us of 64 / 32
-    // keys, 40 heads over 8: d = 128 20 prompts of 53 to 1451 rows 110 / 100, 64 of 128 67 / 56, one of 8192 629 / 621; d = 64
-    // 20 of 410 55.3 / 51.7, one of 8192 367 / 374.
+    // keys, 40 heads over 8, the same way: d = 128 20 prompts of 8191 rows together, uniformly mixed, 105 / 98, 64 of 128 73 /
+    // 64, 4 of 2048 199 / 191, one of 8192 644 / 630; d = 64 the 20 59.5 / 56.4, 4 of 2048 114.9 / 113.2, one of 8192 365 / 373
+    // (one of 1000, which the rule gives steps of 32, 19.7 / 23.1).
     const bool lengthy = a.t >= (int64_t)2000 * a.nseq;
-    const bool loose = ((int64_t)a.t / 128 + a.nseq) * a.heads <= 2 * cus;  // a block's own time counts: 1000 rows 28.5 / 31.0
+    const bool loose = ((int64_t)a.t / 128 + a.nseq) * a.heads <= 2 * cus;  // a block's own time counts: 1000 rows 29.0 / 31.4
     if (d == 64) few ? launch<DT, 64, 64, 2, 4>(a, st) : lengthy ? launch<DT, 64, 64, 4, 1>(a, st) : launch<DT, 64, 32, 4, 1>(a, st);
     else if (d == 128) few ? launch<DT, 128, 32, 2, 4>(a, st) : loose ? launch<DT, 128, 64, 4, 1>(a, st) : launch<DT, 128, 32, 4, 1>(a, st);
     else few ? launch<DT, 256, 32, 2, 2>(a, st) : launch<DT, 256, 64, 4, 1>(a, st);

@@ -7,7 +7,7 @@
 // time straight into registers (no LDS: nobody else needs them): K as the A operand of S^T = K Q^T as it lies in memory,
 // V's rows 16 bytes a lane, turned into the A operand of O^T = V^T P^T by 16-bit permutes inside the lane (8 keys x 8
 // columns: 32 permutes for 32 keys x 128 columns, hidden behind the loads). The next 32 keys are in flight meanwhile:
-// 128 KB a CU at d = 128. 64 sequences of up to 8000 tokens, 8 kv heads (1.3 GB): 237 us, 5.5 TB/s.
+// 128 KB a CU at d = 128. 64 sequences of up to 8000 tokens, 8 kv heads (1.24 GB): 227 us, 5.5 TB/s.
 //
 // Work is split over the tokens of all sequences evenly (attn_tree.hpp), in units of 128 tokens, 32 a wave.
 #include "attn_tree.hpp"
@@ -340,8 +340,9 @@ void launch(const Args& a, hipStream_t st) {
     launch_split<DT, D, kUnit, 16 * NT>(a, tree_kernel<DT, D, NT>, kThreads, 0, blocks_of(NT * D), st);
 }
 
-// Few rows of a kv head: this kernel, more: attn_wide.hip. 16 sequences of about 4600 tokens, 32 rows a head: d = 128 91 us
-// here, 76 us there; d = 64 41.5 and 44.3 us.
+// Few rows of a kv head: this kernel, more: attn_wide.hip. us here / there, 16 sequences of 4600 tokens over 8 kv heads, inputs
+// rotating over three sets: d = 64 16 rows a head 39.0 / 44.8, 32 rows 43.8 / 45.6; d = 128 16 rows 67.5 / 63.6, 32 rows 72 / 66.
+// 5 rows, d = 128: one sequence of 2100 tokens 11.9 / 12.7, 64 of up to 8000 227 / 224.
 template <int DT>
 void by_shape(const Args& a, int d, hipStream_t st) {
     const int rows = a.max_new * a.group;

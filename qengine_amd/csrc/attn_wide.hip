@@ -4,8 +4,9 @@
 // The waves of a block take 32 rows each (attn_wave.hpp) and share 64 keys a step in LDS, so keys and values are read from
 // HBM once for 32 W rows. Steps are staged by LDS DMA from the pages, STAGES - 1 of them ahead: one block of 8 waves a CU
 // keeps three steps (100 KB at d = 128) on their way, blocks of 4 waves one step each. Work is split over the tokens of all
-// sequences evenly (attn_tree.hpp), in units of one step. 12 trees of 32 tokens, 160 rows a kv head (161 MB): 67 us; 32
-// sequences of 40 rows (486 MB): 115 us, 4.2 TB/s; 2 of 40 rows, d = 256 (453 MB): 104 us, 4.35 TB/s.
+// sequences evenly (attn_tree.hpp), in units of one step. With the join: 12 trees of up to 32 tokens over up to 6000, 160 rows a
+// kv head (206 MB) 77 us; 32 sequences of up to 8000 tokens, 40 rows (718 MB) 155 us, 4.6 TB/s; 2 of 131072 tokens, 40 rows,
+// d = 256 (472 MB) 109 us, 4.3 TB/s.
 #include "attn_tree.hpp"
 #include "attn_wave.hpp"
 
