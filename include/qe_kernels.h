@@ -342,15 +342,15 @@ void qe_moe_pack_w4(const int32_t* gu_q, const uint16_t* gu_s, const int32_t* dn
  * fp16 where said; scores, softmax statistics and sums are fp32, probabilities are rounded to the values' type for the
  * second product (as the matrix cores take them). heads % kv_heads == 0: query head h reads kv head h / (heads / kv_heads).
  * At most 2^30 rows a call. d = 64, 128 or 256. scale 2^-126 .. 2^126, usually d^-0.5; a score q . k, and that times the scale
- * times log2(e), are fp32 numbers (past 2^128 they are infinite, and a row whose largest one is has NaN). Pointers 16-byte
+ * times log2(e), are fp32 numbers (past 2^128 infinite; a row whose largest score is +inf has NaN). Pointers 16-byte
  * aligned, strides in elements and multiples of 8, a head's d values contiguous.
  * lse (NULL: not wanted) [t][heads] fp32: log of the sum of the exponentiated scores.
  * A row that sees no key has out = 0 and lse = -inf; a key that a row does not see has no effect on it, whatever its bits.
  * Lengths, tables and indexes live on the device and are not seen by the host: values out of range make a kernel skip
  * what they name and never touch memory outside the tensors. Every call is one to three launches on `stream`, without
  * host synchronization, and can be captured; but the first qe_attn_tree of a stream, and the first whose head size or rows
- * take a kernel with a larger workspace than those before (9 or 68 MB at d = 128, whatever the batch), allocates it and
- * waits for the stream. Deterministic: same inputs, same bits. ---- */
+ * take a kernel with a larger workspace than those before (9 or 68 MB at d = 128, whatever the batch), allocates it, the
+ * latter after a wait for the stream. Deterministic: same inputs, same bits. ---- */
 
 /* Causal attention over whole prompts packed without padding: sequence b is rows cu[b] .. cu[b + 1] - 1 (cu [nseq + 1]
  * int32, ascending), row i of it sees rows 0 .. i. Rows of q, k, v and out have strides of their own (k_row, v_row below
