@@ -89,13 +89,13 @@ def draw(rng):
                 return c
         elif kind == "linear":
             c = {"kind": kind, "rows": _log(rng, 1, 8192), "n": _log(rng, 256, 34816, step), "k": _log(rng, 256, 17408, 16 * rng.choice([1, 8])),
-                 "out": rng.choice(["bf16", "bf16", "f16", "f32"])}
+                 "out": rng.choice(["bf16", "bf16", "f16"])}
             if work(c)["flops"] <= MOST_FLOPS:
                 return c
         elif kind == "experts":
             c = {"kind": kind, "experts": rng.choice([8, 32, 60, 128, 256, 512]), "topk": rng.randint(1, 10), "tokens": _log(rng, 1, 4096),
                  "n": _log(rng, 256, 4096, step), "k": _log(rng, 256, 4096, 16 * rng.choice([1, 8])), "gather": rng.random() < 0.5,
-                 "out": rng.choice(["bf16", "bf16", "f16", "f32"])}
+                 "out": rng.choice(["bf16", "bf16", "f16"])}
             if c["topk"] <= c["experts"] and work(c)["flops"] <= MOST_EXPERT_FLOPS and c["experts"] * c["n"] * c["k"] <= MOST_WEIGHTS:
                 return c
         else:
