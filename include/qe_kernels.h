@@ -27,7 +27,8 @@ extern "C" {
 #define QE_OUT_BF16 2       /* y is bf16 (round to nearest even), default fp32 */
 #define QE_GLU 4            /* GLU matrix (8 gate + 8 up rows per tile): y = bf16 silu(gate) * up, n / 2 cols */
 #define QE_W8_PER_CHANNEL 8 /* W8 with one scale per output row, s = [N] (group = K) */
-#define QE_F16 16           /* attention: q, k, v and out are fp16 (default bf16) */
+#define QE_F16 16           /* attention, 8-bit layers: 16-bit values are fp16 (default bf16) */
+#define QE_W_F32 32         /* rms_norm: the weights are fp32 (default: the values' 16-bit type) */
 
 int qe_abi_version(void);
 
@@ -419,6 +420,55 @@ void qe_attn_tree(const qe_kv_cache_t* cache, int layer, const void* q, int64_t 
 /* test hook: 0: later qe_attn_tree calls do not split a sequence's tokens over blocks (what they do by themselves where the
  * device has no memory for the parts); the same results within fp32 rounding. No counterpart in the reference. */
 void qe_attn_tree_set_split(int on);
+
+/* ---- layers in 8-bit floating point: from the residual stream (norm), through products with 8-bit weights and activations,
+ * dense or grouped by expert, and back (combine). No reference C-ABI exists for them. 8-bit values are e4m3 (OCP: largest 448,
+ * no infinities). Weights [n][k] have one fp32 scale for each block of 128 x 128, s [ceil(n / 128)][ceil(k / 128)];
+ * activations one for each group of 128 columns of a row, anywhere in memory (strides s_row, s_group in elements; group-major is what
+ * the products read best). The last block or group may be shorter. Strides are in elements and below 2^31 for rows; a row's values
+ * lie together; outputs overlap neither inputs nor each other, except where said. 16-bit and fp32 values need the alignment of
+ * their type; 16-byte aligned rows of a multiple of 8 run faster. At most 2^24 rows a call, n and k at most 2^20. Every
+ * call is one or two launches on `stream`, without host synchronization, and can be captured. Deterministic. ---- */
+
+/* h = x + res, rounded to their type and written to res_out (which may be res, or x), or h = x (res and res_out NULL);
+ * y = h / sqrt(mean(h^2) + eps) * w in fp32, rounded to y (NULL: not wanted) and / or quantized to q with scales s (q NULL: not
+ * wanted) as qe_act_f8 does. x, res, y: bf16, or fp16 (QE_F16); w [d] the same or fp32 (QE_W_F32). y may be x where res_out is
+ * not. d <= 65536, eps 2^-100 .. 2^100. Finite rows have finite results up to the type's largest values. */
+void qe_rms_norm(const void* x, int64_t ldx, const void* res, int64_t ldr, void* res_out, int64_t ldro, const void* w, float eps,
+                 void* y, int64_t ldy, void* q, int64_t ldq, float* s, int64_t s_row, int64_t s_group, int t, int d, int flags,
+                 void* stream);
+
+/* v = x, or (glu) silu(gate) * up of rows [d gate values][d up values], in fp32; each group of 128 columns: a = max(max |v|,
+ * 448 * 2^-100), scale a / 448, q = e4m3(v * (448 / a)) to nearest even. A NaN stays one in its place; an infinity makes its
+ * group's scale infinite and itself a NaN. x bf16 or (QE_F16) fp16. t * ceil(d / 2048) <= 2^23. */
+void qe_act_f8(const void* x, int64_t ldx, int glu, void* q, int64_t ldq, float* s, int64_t s_row, int64_t s_group, int t, int d,
+               int flags, void* stream);
+
+/* row-major e4m3 matrices [experts][n][k] (row stride ldq, matrix stride mat, multiples of 16; k % 16 == 0; 16-byte aligned) ->
+ * the products' layout: dq, experts * qe_f8_bytes(n, k) bytes, 16-byte aligned. experts <= 1024. */
+void qe_tile_f8(const void* q, int64_t ldq, int64_t mat, int n, int k, int experts, void* dq, void* stream);
+size_t qe_f8_bytes(int n, int k);
+
+/* y[t][n] = x[t][k] . W^T, bf16 or (QE_F16) fp16: sums of a block of 128 k by the matrix cores, then over the blocks in fp32 with
+ * the product of the two scales, an fp32 number. (The matrix cores add products of 8 consecutive k to 13 bits below the largest
+ * exponent among them, 1e-5 of a usual result, and the rest as fp32.) x: 16-byte aligned rows, ldx a multiple of 16. */
+void qe_matmul_f8(const void* q, const float* s, int n, int k, const void* x, int64_t ldx, const float* xs, int64_t xs_row,
+                  int64_t xs_group, int t, void* y, int64_t ldy, int flags, void* stream);
+
+/* The same for each segment of rows with its own matrix: rows off[e] .. off[e + 1] - 1 of y (off int32 [experts + 1], ascending,
+ * on the device) are W_e times rows of x: those of the same number, or rows[i] for row i (NULL: none; a number outside
+ * 0 .. t - 1 gives a row of zeros). Rows of y before off[0] and from off[experts] on are left as they were; no row past r is
+ * written whatever off holds. qe_moe_segment's off and slot_tok are such. */
+void qe_matmul_f8_grouped(const void* q, const float* s, int n, int k, int experts, const void* x, int64_t ldx, const float* xs,
+                          int64_t xs_row, int64_t xs_group, int t, const int32_t* off, const int32_t* rows, int r, void* y,
+                          int64_t ldy, int flags, void* stream);
+
+/* out[i] = add[i] + sum over j of w[i][j] * y[inv[i * topk + j]], in the order of j in fp32, rounded once: the rows of a
+ * grouped product back into tokens (inv and w as qe_moe_segment and qe_moe_route give them; add NULL: none). An index outside
+ * 0 .. rows - 1 adds nothing. y: fp32, bf16 (yflags QE_OUT_BF16) or fp16 (QE_F16); out and add: y's type or fp32 (flags). out may
+ * be add. topk <= 1024, t * ceil(d / 2048) <= 2^23. */
+void qe_moe_combine(const void* y, int64_t ldy, int rows, const int32_t* inv, const float* w, const void* add, int64_t ldadd, void* out,
+                    int64_t ldout, int t, int topk, int d, int yflags, int flags, void* stream);
 
 /* ---- on-disk weights: .safetensors files (host, memory-mapped) and the quantized-matrix loader ----
  * qe_st_open maps a file and indexes its tensors by name (reference SafeTensors::open, src/safetensors.h:40; a

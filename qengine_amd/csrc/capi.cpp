@@ -3,6 +3,7 @@
 // pointers, default stream, bf16 scales, fp32 outputs, fatal abort on a violated precondition.
 // Build-defined *_ex entry points take an explicit stream, row strides and flags (QeFlags).
 #include "qe_api.hpp"
+#include "f8.hpp"
 #include "gemm_tune.hpp"
 #include "kv_cache.hpp"
 #include "../../include/qe_kernels.h"
@@ -421,5 +422,57 @@ void qe_attn_tree(const qe_kv_cache_t* cache, int layer, const void* q, int64_t 
 }
 
 void qe_attn_tree_set_split(int on) { attn_tree_set_split(on != 0); }
+
+// ---------------------------------------------------------------- layers in 8-bit floating point
+namespace {
+inline int f8_type(int flags, int others, const char* what) {  // of 16-bit values
+    CHECK((flags & ~(QE_F16 | others)) == 0, "%s: flags %d", what, flags);
+    return flags & QE_F16 ? kF8F16 : kF8BF16;
+}
+inline int f8_any(int flags, const char* what) {  // fp32 unless said
+    CHECK((flags & ~(QE_F16 | QE_OUT_BF16)) == 0 && flags != (QE_F16 | QE_OUT_BF16), "%s: flags %d", what, flags);
+    return flags & QE_F16 ? kF8F16 : flags & QE_OUT_BF16 ? kF8BF16 : kF8F32;
+}
+}  // namespace
+
+void qe_rms_norm(const void* x, int64_t ldx, const void* res, int64_t ldr, void* res_out, int64_t ldro, const void* w, float eps,
+                 void* y, int64_t ldy, void* q, int64_t ldq, float* s, int64_t s_row, int64_t s_group, int t, int d, int flags,
+                 void* st) {
+    const int type = f8_type(flags, QE_W_F32, "qe_rms_norm");
+    f8_norm({x, res, w, res_out, y, q, s, ldx, ldr, ldro, ldy, ldq, s_row, s_group, t, d, type, flags & QE_W_F32 ? kF8F32 : type, eps},
+            as_stream(st));
+}
+
+void qe_act_f8(const void* x, int64_t ldx, int glu, void* q, int64_t ldq, float* s, int64_t s_row, int64_t s_group, int t, int d,
+               int flags, void* st) {
+    f8_act({x, q, s, ldx, ldq, s_row, s_group, t, d, f8_type(flags, 0, "qe_act_f8"), glu != 0}, as_stream(st));
+}
+
+void qe_tile_f8(const void* q, int64_t ldq, int64_t mat, int n, int k, int experts, void* dq, void* st) {
+    f8_tile(q, ldq, mat, n, k, experts, dq, as_stream(st));
+}
+
+size_t qe_f8_bytes(int n, int k) { return (size_t)((n + 15) / 16) * ((k + 127) / 128) * 2048; }
+
+void qe_matmul_f8(const void* q, const float* s, int n, int k, const void* x, int64_t ldx, const float* xs, int64_t xs_row,
+                  int64_t xs_group, int t, void* y, int64_t ldy, int flags, void* st) {
+    f8_matmul({q, s, x, xs, nullptr, nullptr, y, ldx, xs_row, xs_group, ldy, n, k, t, t, 1, f8_type(flags, 0, "qe_matmul_f8")}, as_stream(st));
+}
+
+void qe_matmul_f8_grouped(const void* q, const float* s, int n, int k, int experts, const void* x, int64_t ldx, const float* xs,
+                          int64_t xs_row, int64_t xs_group, int t, const int32_t* off, const int32_t* rows, int r, void* y,
+                          int64_t ldy, int flags, void* st) {
+    CHECK(off != nullptr, "qe_matmul_f8_grouped: off is missing");
+    CHECK(rows || r <= t, "qe_matmul_f8_grouped: %d rows of y, %d of x", r, t);
+    f8_matmul({q, s, x, xs, off, rows, y, ldx, xs_row, xs_group, ldy, n, k, t, r, experts, f8_type(flags, 0, "qe_matmul_f8_grouped")},
+              as_stream(st));
+}
+
+void qe_moe_combine(const void* y, int64_t ldy, int rows, const int32_t* inv, const float* w, const void* add, int64_t ldadd, void* out,
+                    int64_t ldout, int t, int topk, int d, int yflags, int flags, void* st) {
+    const int type = f8_any(yflags, "qe_moe_combine"), otype = f8_any(flags, "qe_moe_combine");
+    CHECK(otype == type || otype == kF8F32, "qe_moe_combine: the output has y's type or fp32");
+    f8_combine({y, add, inv, w, out, ldy, ldadd, ldout, t, topk, rows, d, type, otype}, as_stream(st));
+}
 
 }  // extern "C"

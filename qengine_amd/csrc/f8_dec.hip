@@ -1,0 +1,103 @@
+// 8-bit products of few rows (f8.hpp): up to 16 MT rows of one matrix, or of an expert's segment, in one pass over the weights.
+// Bound by the weights' bytes. A block holds NT tiles of 16 weight rows; its NW waves share out the 128-k blocks, read their
+// weights straight from memory into the matrix core's operands (nothing is shared, so no LDS), and add their sums in the
+// order of the waves at the end.
+#include "f8.hpp"
+
+namespace {
+template <int MT, int NT, int NW, int OUT, bool GROUPED>
+__global__ void __launch_bounds__(NW * 64) dec_kernel(F8Mat a, int ntiles, bool vec) {
+    __shared__ f32x4_v part[NW * NT * MT * 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, g = lane >> 4, kb = (a.k + 127) >> 7, n16 = (a.n + 15) >> 4;
+    const int wt = blockIdx.x % ntiles, job = blockIdx.x / ntiles;
+    int e = 0, row0 = job * 16 * MT, rows = min(16 * MT, a.r - row0);
+    if constexpr (GROUPED) {
+        if (!f8_job<NW * 64>(a.off, a.experts, a.r, 16 * MT, job, reinterpret_cast<int*>(part), e, row0, rows)) return;
+        __syncthreads();
+    }
+    const int n0 = wt * NT;  // first tile of 16 weight rows
+    const uint8_t* wp[NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+        wp[i] = static_cast<const uint8_t*>(a.q) + (((size_t)e * n16 + min(n0 + i, n16 - 1)) * kb) * 2048 + lane * 16;
+    const float* sw = a.s + ((size_t)e * ((a.n + 127) >> 7) + (n0 >> 3)) * kb;
+    const uint8_t* xp[MT];
+    const float* sx[MT];
+    bool has[MT];
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+        int64_t row = row0 + min(16 * m + r, rows - 1);
+        has[m] = true;
+        if (GROUPED && a.rows) {
+            row = a.rows[row];
+            has[m] = (uint64_t)row < (uint64_t)a.t;
+            if (!has[m]) row = 0;
+        }
+        xp[m] = static_cast<const uint8_t*>(a.x) + row * a.ldx + g * 16;
+        sx[m] = a.xs + row * a.xs_row;
+    }
+    f32x4_v acc[NT][MT] = {};
+    for (int b = wave; b < kb; b += NW) {
+        const int at = b * 128 + g * 16;  // of chunks g and 4 + g
+        i32x8_f8 w[NT], x[MT];
+        float s[MT];
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+            w[i] = f8_join(*reinterpret_cast<const i32x4_f8*>(wp[i] + (size_t)b * 2048), *reinterpret_cast<const i32x4_f8*>(wp[i] + (size_t)b * 2048 + 1024));
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+            i32x4_f8 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+            s[m] = 0.f;
+            if (has[m]) {
+                if (at < a.k) lo = *reinterpret_cast<const i32x4_f8*>(xp[m] + b * 128);
+                if (at + 64 < a.k) hi = *reinterpret_cast<const i32x4_f8*>(xp[m] + b * 128 + 64);
+                s[m] = sx[m][b * a.xs_group] * sw[b];
+            }
+            x[m] = f8_join(lo, hi);
+        }
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                const f32x4_v p = f8_mfma(w[i], x[m]);
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[i][m][j] = fmaf(p[j], s[m], acc[i][m][j]);
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int m = 0; m < MT; m++) part[((wave * NT + i) * MT + m) * 64 + lane] = acc[i][m];
+    __syncthreads();
+    for (int j = tid; j < NT * MT * 64; j += NW * 64) {
+        f32x4_v v = part[j];
+#pragma unroll
+        for (int w = 1; w < NW; w++) {
+            const f32x4_v p = part[w * NT * MT * 64 + j];
+#pragma unroll
+            for (int c = 0; c < 4; c++) v[c] += p[c];
+        }
+        const int l = j & 63, m = (j >> 6) % MT, i = (j >> 6) / MT, row = 16 * m + (l & 15), col = (n0 + i) * 16 + 4 * (l >> 4);
+        if (row < rows && col < a.n) f8_store4<OUT>(static_cast<uint16_t*>(a.y) + (int64_t)(row0 + row) * a.ldy, col, a.n, v, vec);
+    }
+}
+
+template <int MT, int NT, int NW, bool GROUPED>
+void dec_t(const F8Mat& a, hipStream_t st) {
+    const int ntiles = ((a.n + 15) / 16 + NT - 1) / NT;
+    const int64_t jobs = GROUPED ? f8_most_jobs(a.r, a.experts, 16 * MT) : (a.r + 16 * MT - 1) / (16 * MT);
+    CHECK(jobs * ntiles <= kF8MaxBlocks, "matmul_f8: %lld row blocks by %d column blocks are too many for a call", (long long)jobs, ntiles);
+    const dim3 grid((unsigned)(jobs * ntiles)), block(NW * 64);
+    const bool vec = f8_vec_ok(a.y, a.ldy);
+    if (a.out == kF8BF16) dec_kernel<MT, NT, NW, kF8BF16, GROUPED><<<grid, block, 0, st>>>(a, ntiles, vec);
+    else dec_kernel<MT, NT, NW, kF8F16, GROUPED><<<grid, block, 0, st>>>(a, ntiles, vec);
+    HIP_CHECK(hipGetLastError());
+}
+}  // namespace
+
+void f8_dec(const F8Mat& a, hipStream_t st) {
+    if (a.off) dec_t<1, 2, 8, true>(a, st);
+    else if (a.r <= 16) dec_t<1, 1, 8, false>(a, st);
+    else dec_t<2, 2, 8, false>(a, st);
+}

@@ -1,0 +1,288 @@
+"""Layers in 8-bit floating point (the C-ABI's qe_rms_norm, *_f8* and qe_moe_combine entry points, include/qe_kernels.h).
+
+8-bit values are torch.float8_e4m3fn; weights have a scale for each block of 128 x 128, activations one for each row's 128
+columns. An MLP block and an expert layer, from the residual stream `h` and back:
+
+    w1, w2 = tile_f8(q1, s1), tile_f8(q2, s2)              # once; gate and up rows in one matrix
+    q, s = rms_norm(x, norm, eps, res=h, f8=True)          # h += x, then the norm of it in 8 bits
+    a, t = silu_mul_f8(matmul_f8(w1, q, s))
+    x = matmul_f8(w2, a, t)
+
+    seg = moe_segment(*moe_route(logits, topk), experts, chunk)
+    g = matmul_f8_grouped(w1, q, s, seg["off"], rows=seg["slot_tok"])   # w1, w2: tile_f8 of [experts][n][k]
+    y = matmul_f8_grouped(w2, *silu_mul_f8(g), seg["off"])
+    x = moe_combine(y, seg["inv"], weights)
+
+Shapes, types, devices and strides are checked here (TypeError, ValueError) before the call; indexes on the device are checked
+by the kernels. Calls run on the current stream of the tensors' device, need no host synchronization and can be captured.
+Nothing here has a backward pass.
+"""
+from dataclasses import dataclass
+
+import torch
+
+from .attention import _run
+
+E4M3 = torch.float8_e4m3fn
+OUT_BF16, F16, W_F32 = 2, 16, 32
+MAX_EXPERTS = 1024
+MAX_COLS = 65536
+MAX_DIM = 1 << 20
+MAX_ROWS = 1 << 24
+MAX_PARTS = 1 << 23
+MAX_STRIDE = 1 << 31
+_OUT = {torch.float32: 0, torch.bfloat16: OUT_BF16, torch.float16: F16}
+_IN = {torch.bfloat16: 0, torch.float16: F16}
+
+
+def _matrix(name, t, at, align=1):
+    """[rows][columns] whose rows the kernels can read: strides and place; -> row stride"""
+    if t.dim() != 2:
+        raise ValueError(f"{name} has two dimensions, got shape {tuple(t.shape)}")
+    if t.get_device() != at:
+        raise ValueError(f"{name} is on another device than the other tensors: {t.device}")
+    rows, cols = t.shape
+    row, col = t.stride()
+    if cols > 1 and col != 1:
+        raise ValueError(f"{name}: a row's values lie together, got strides {t.stride()}")
+    if rows < 2:
+        return -(-cols // 16) * 16  # one row: its stride may be anything
+    if row < 0 or row >= MAX_STRIDE or row % align:
+        raise ValueError(f"{name}: rows are {align if align > 1 else 'up to 2^31'} elements apart or a multiple, got {row}")
+    return row
+
+
+def _written(name, t, shape, dtype, at):
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} is {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(shape)}, got {tuple(t.shape)}")
+    row = _matrix(name, t, at)
+    if t.shape[0] > 1 and row < t.shape[1]:
+        raise ValueError(f"{name}'s rows overlap: strides {t.stride()}")
+    return row
+
+
+def _ints(name, t, shape, at):
+    if t.dtype is not torch.int32:
+        raise TypeError(f"{name} is int32, got {t.dtype}")
+    if t.shape != shape or not t.is_contiguous() or t.get_device() != at:
+        raise ValueError(f"{name} is contiguous of shape {tuple(shape)} on {at}, got {tuple(t.shape)} on {t.device}")
+
+
+def _in_type(name, t):
+    f = _IN.get(t.dtype)
+    if f is None:
+        raise TypeError(f"{name} is bfloat16 or float16, got {t.dtype}")
+    return f
+
+
+def _rows_fit(t, d, what):
+    if t > MAX_ROWS or d > MAX_DIM or t * -(-d // 2048) > MAX_PARTS:
+        raise ValueError(f"{what}: {t} rows of {d} are too many for a call")
+
+
+def _quantized(t, d, device):
+    """room for [t][d] in 8 bits, rows that the products can read, and its scales, group after group"""
+    q = torch.empty(t, -(-d // 16) * 16, dtype=E4M3, device=device)
+    s = torch.empty(-(-d // 128), t, dtype=torch.float32, device=device)
+    return q if d % 16 == 0 else q[:, :d], s.t()
+
+
+@dataclass
+class F8:
+    """Weights in 8 bits (tile_f8): q uint8 in the products' layout, s fp32 [experts][blocks of n][blocks of k]."""
+    q: torch.Tensor
+    s: torch.Tensor
+    n: int
+    k: int
+    experts: int = 1
+
+
+def tile_f8(q, s):
+    """e4m3 [n][k] with scales [ceil(n / 128)][ceil(k / 128)] fp32, or [experts][n][k] with [experts][..][..] -> F8. k is a
+    multiple of 16."""
+    if q.dtype is not E4M3 or s.dtype is not torch.float32:
+        raise TypeError(f"weights are {E4M3} with float32 scales, got {q.dtype} and {s.dtype}")
+    if q.dim() not in (2, 3):
+        raise ValueError(f"weights are [n][k] or [experts][n][k], got shape {tuple(q.shape)}")
+    lead, (n, k) = q.shape[:-2], q.shape[-2:]
+    experts = lead[0] if lead else 1
+    if not 0 < experts <= MAX_EXPERTS or not 0 < n <= MAX_DIM or not 0 < k <= MAX_DIM or k % 16:
+        raise ValueError(f"at most {MAX_EXPERTS} matrices, n and k at most {MAX_DIM}, k a multiple of 16, got {tuple(q.shape)}")
+    if s.shape != (*lead, -(-n // 128), -(-k // 128)):
+        raise ValueError(f"scales have shape {(*lead, -(-n // 128), -(-k // 128))}, got {tuple(s.shape)}")
+    at = q.get_device()
+    if s.get_device() != at:
+        raise ValueError(f"scales are on another device than the weights: {s.device}")
+    q = q.view(-1, n, k) if q.is_contiguous() else q if lead else q[None]
+    if (k > 1 and q.stride(2) != 1) or q.stride(0) % 16 and experts > 1 or q.stride(1) % 16 and n > 1 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    dq = torch.empty(experts * -(-n // 16) * -(-k // 128) * 2048, dtype=torch.uint8, device=q.device)
+    _run(at, "qe_tile_f8", "plliiipp", q.data_ptr(), q.stride(1) if n > 1 else k, q.stride(0) if experts > 1 else 0, n, k, experts,
+         dq.data_ptr())
+    return F8(dq, s.contiguous().clone(), n, k, experts)
+
+
+def rms_norm(x, w, eps=1e-6, res=None, res_out=None, out=None, f8=False):
+    """Root-mean-square norm of rows x [t][d] (bfloat16 or float16) with weights w [d] (their type or float32). res [t][d]: the
+    residual stream; x + res, rounded to their type, goes to res_out (default: res itself) and is what the norm takes.
+    -> [t][d] of x's type (out, if given); f8=True: (q, s), e4m3 with scales, and the 16-bit values go to `out` if given."""
+    flags, at = _in_type("x", x), x.get_device()
+    ldx = _matrix("x", x, at)
+    t, d = x.shape
+    if t > MAX_ROWS or not 0 < d <= MAX_COLS:
+        raise ValueError(f"at most {MAX_ROWS} rows of 1 to {MAX_COLS}, got {tuple(x.shape)}")
+    if not 2.0 ** -100 <= eps <= 2.0 ** 100:
+        raise ValueError(f"eps is between 2^-100 and 2^100, got {eps}")
+    if w.dtype is torch.float32:
+        flags |= W_F32
+    elif w.dtype is not x.dtype:
+        raise TypeError(f"w has x's type or float32, got {w.dtype}")
+    if w.shape != (d,) or not w.is_contiguous() or w.get_device() != at:
+        raise ValueError(f"w is contiguous of shape {(d,)} on x's device, got {tuple(w.shape)} on {w.device}")
+    ldr = ldro = 0
+    if res is not None:
+        if res_out is None:
+            res_out = res
+        ldro = _written("res_out", res_out, x.shape, x.dtype, at)
+        if res.dtype is not x.dtype:
+            raise TypeError(f"res is {x.dtype}, got {res.dtype}")
+        if res.shape != x.shape:
+            raise ValueError(f"res has x's shape {tuple(x.shape)}, got {tuple(res.shape)}")
+        ldr = _matrix("res", res, at)
+    elif res_out is not None:
+        raise ValueError("res_out without res")
+    y, ldy, q, s = out, 0, None, None
+    if out is not None:
+        ldy = _written("out", out, x.shape, x.dtype, at)
+    elif not f8:
+        y = torch.empty(t, d, dtype=x.dtype, device=x.device)
+        ldy = d
+    if f8:
+        q, s = _quantized(t, d, x.device)
+    if t:
+        _run(at, "qe_rms_norm", "plplplpfplplplliiip", x.data_ptr(), ldx, None if res is None else res.data_ptr(), ldr,
+             None if res is None else res_out.data_ptr(), ldro, w.data_ptr(), eps, None if y is None else y.data_ptr(), ldy,
+             q.data_ptr() if f8 else None, q.stride(0) if f8 else 0, s.data_ptr() if f8 else None, 1, t, t, d, flags)
+    return (q, s) if f8 else y
+
+
+def _act(x, glu):
+    flags, at = _in_type("x", x), x.get_device()
+    ldx = _matrix("x", x, at)
+    t, d = x.shape
+    if glu:
+        if d % 2:
+            raise ValueError(f"rows hold as many gate as up values, got {d}")
+        d //= 2
+    _rows_fit(t, d, "x")
+    if d == 0:
+        raise ValueError("rows without columns")
+    q, s = _quantized(t, d, x.device)
+    if t:
+        _run(at, "qe_act_f8", "pliplplliiip", x.data_ptr(), ldx, int(glu), q.data_ptr(), q.stride(0), s.data_ptr(), 1, t, t, d, flags)
+    return q, s
+
+
+def quant_f8(x):
+    """rows x [t][d] (bfloat16 or float16) in 8 bits -> (q e4m3 [t][d], s fp32 [t][ceil(d / 128)])"""
+    return _act(x, False)
+
+
+def silu_mul_f8(x):
+    """silu(gate) * up of rows x [t][2 d] = [gate][up] (bfloat16 or float16), in 8 bits -> (q [t][d], s [t][ceil(d / 128)])"""
+    return _act(x, True)
+
+
+def _operands(w, q, s, experts):
+    if not isinstance(w, F8):
+        raise TypeError(f"weights are an F8, got {type(w).__name__}")
+    if q.dtype is not E4M3 or s.dtype is not torch.float32:
+        raise TypeError(f"activations are {E4M3} with float32 scales, got {q.dtype} and {s.dtype}")
+    at = w.q.get_device()
+    if experts != (w.s.dim() == 3):
+        raise ValueError("one matrix for matmul_f8, [experts] of them for matmul_f8_grouped")
+    ldx = _matrix("q", q, at, 16)
+    t = q.shape[0]
+    if q.shape[1] != w.k or t > MAX_ROWS:
+        raise ValueError(f"q is at most {MAX_ROWS} rows of {w.k}, got {tuple(q.shape)}")
+    if q.data_ptr() % 16:
+        raise ValueError("q is 16-byte aligned")
+    if s.shape != (t, -(-w.k // 128)) or s.get_device() != at or not all(0 <= x < MAX_STRIDE for x in s.stride()):
+        raise ValueError(f"scales have shape {(t, -(-w.k // 128))} on the weights' device, got {tuple(s.shape)} on {s.device}")
+    return at, ldx, t
+
+
+def _product(w, r, dtype, y, at):
+    dtype = dtype if y is None else y.dtype
+    flags = _IN.get(dtype)
+    if flags is None:
+        raise TypeError(f"products are bfloat16 or float16, got {dtype}")
+    if r > MAX_ROWS or -(-r // 16) * -(-w.n // 16) > 1 << 28:
+        raise ValueError(f"{r} rows of {w.n} are too many for a call")
+    if y is None:
+        y = torch.empty(r, w.n, dtype=dtype, device=w.q.device)
+        return y, w.n, flags
+    return y, _written("y", y, (r, w.n), y.dtype, at), flags
+
+
+def matmul_f8(w: F8, q, s, dtype=torch.bfloat16, y=None):
+    """y [t][n] = rows (q e4m3 [t][k], s fp32 [t][ceil(k / 128)]) times the matrix w; into y, or a new tensor of
+    type dtype (bfloat16 or float16)"""
+    at, ldx, t = _operands(w, q, s, False)
+    y, ldy, flags = _product(w, t, dtype, y, at)
+    if t:
+        _run(at, "qe_matmul_f8", "ppiiplplliplip", w.q.data_ptr(), w.s.data_ptr(), w.n, w.k, q.data_ptr(), ldx, s.data_ptr(), s.stride(0),
+             s.stride(1), t, y.data_ptr(), ldy, flags)
+    return y
+
+
+def matmul_f8_grouped(w: F8, q, s, off, rows=None, dtype=torch.bfloat16, y=None):
+    """Rows off[e] .. off[e + 1] - 1 of y (off int32 [experts + 1], ascending) = matrix e of w times the same rows of (q, s), or
+    rows[i] of them for row i (rows int32; a number outside q gives a row of zeros). Rows of y in no segment are left as
+    they were in a given y (and have no meaning in a new one). y has as many rows as `rows`, or as q."""
+    at, ldx, t = _operands(w, q, s, True)
+    _ints("off", off, (w.experts + 1,), at)
+    r = t
+    if rows is not None:
+        _ints("rows", rows, (rows.numel(),), at)
+        r = rows.numel()
+    y, ldy, flags = _product(w, r, dtype, y, at)
+    if r:
+        _run(at, "qe_matmul_f8_grouped", "ppiiiplpllippiplip", w.q.data_ptr(), w.s.data_ptr(), w.n, w.k, w.experts, q.data_ptr(), ldx,
+             s.data_ptr(), s.stride(0), s.stride(1), t, off.data_ptr(), None if rows is None else rows.data_ptr(), r, y.data_ptr(), ldy, flags)
+    return y
+
+
+def moe_combine(y, inv, w, add=None, out=None):
+    """out [t][d] = add + sum over j of w[i][j] * y[inv[i * topk + j]]: the rows y [slots][d] of a grouped product back into
+    tokens, inv int32 [t * topk] and w fp32 [t][topk] as moe_segment and moe_route give them (an index outside y adds nothing).
+    y: bfloat16, float16 or float32; out (default: new, of add's or y's type; it may be add itself) and add have y's type or
+    float32."""
+    yflags, at = _OUT.get(y.dtype), y.get_device()
+    if yflags is None:
+        raise TypeError(f"y is bfloat16, float16 or float32, got {y.dtype}")
+    ldy = _matrix("y", y, at)
+    if w.dtype is not torch.float32:
+        raise TypeError(f"w is float32, got {w.dtype}")
+    if w.dim() != 2 or not w.is_contiguous() or w.get_device() != at:
+        raise ValueError(f"w is contiguous [t][topk] on y's device, got {tuple(w.shape)} on {w.device}")
+    (t, topk), (slots, d) = w.shape, y.shape
+    _ints("inv", inv, (t * topk,), at)
+    _rows_fit(t, d, "y")
+    if slots >= 1 << 31 or topk > 1024 or d == 0:
+        raise ValueError(f"at most 2^31 rows and 1024 of them a token, got {tuple(y.shape)} and {tuple(w.shape)}")
+    dtype = out.dtype if out is not None else add.dtype if add is not None else y.dtype
+    if dtype not in (y.dtype, torch.float32):
+        raise TypeError(f"out and add have y's type or float32, got {dtype}")
+    ldadd = 0 if add is None else _written("add", add, (t, d), dtype, at)
+    if out is None:
+        out = torch.empty(t, d, dtype=dtype, device=y.device)
+        ldout = d
+    else:
+        ldout = _written("out", out, (t, d), dtype, at)
+    if t:
+        _run(at, "qe_moe_combine", "plippplpliiiiip", y.data_ptr(), ldy, slots, inv.data_ptr(), w.data_ptr(),
+             None if add is None else add.data_ptr(), ldadd, out.data_ptr(), ldout, t, topk, d, yflags, _OUT[dtype])
+    return out

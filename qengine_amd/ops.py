@@ -475,3 +475,6 @@ class SafeTensorsFile:
 
 # ---------------------------------------------------------------- attention and the paged cache
 from .attention import KVCache, attn_prompt  # noqa: E402,F401
+
+# ---------------------------------------------------------------- layers in 8-bit floating point
+from .fp8 import F8, matmul_f8, matmul_f8_grouped, moe_combine, quant_f8, rms_norm, silu_mul_f8, tile_f8  # noqa: E402,F401
