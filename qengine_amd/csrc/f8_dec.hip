@@ -24,22 +24,19 @@ __global__ void __launch_bounds__(NW * 64) dec_kernel(F8Mat a, int ntiles, bool 
     const float* sw = a.s + ((size_t)e * ((a.n + 127) >> 7) + (n0 >> 3)) * kb;
     const uint8_t* xp[MT];
     const float* sx[MT];
-    bool has[MT];
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         int64_t row = row0 + min(16 * m + r, rows - 1);
-        has[m] = true;
         if (GROUPED && a.rows) {
             row = a.rows[row];
-            has[m] = (uint64_t)row < (uint64_t)a.t;
-            if (!has[m]) row = 0;
+            if ((uint64_t)row >= (uint64_t)a.t) row = 0;  // an index outside x: zeros in y
         }
-        xp[m] = static_cast<const uint8_t*>(a.x) + row * a.ldx + g * 16;
+        xp[m] = static_cast<const uint8_t*>(a.x) + row * a.ldx;
         sx[m] = a.xs + row * a.xs_row;
     }
     f32x4_v acc[NT][MT] = {};
     for (int b = wave; b < kb; b += NW) {
-        const int at = b * 128 + g * 16;  // of chunks g and 4 + g
+        const int at = b * 128 + g * 16;  // of chunks g and 4 + g; behind k the block's first, which meets zeros
         i32x8_f8 w[NT], x[MT];
         float s[MT];
 #pragma unroll
@@ -47,14 +44,9 @@ __global__ void __launch_bounds__(NW * 64) dec_kernel(F8Mat a, int ntiles, bool 
             w[i] = f8_join(*reinterpret_cast<const i32x4_f8*>(wp[i] + (size_t)b * 2048), *reinterpret_cast<const i32x4_f8*>(wp[i] + (size_t)b * 2048 + 1024));
 #pragma unroll
         for (int m = 0; m < MT; m++) {
-            i32x4_f8 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-            s[m] = 0.f;
-            if (has[m]) {
-                if (at < a.k) lo = *reinterpret_cast<const i32x4_f8*>(xp[m] + b * 128);
-                if (at + 64 < a.k) hi = *reinterpret_cast<const i32x4_f8*>(xp[m] + b * 128 + 64);
-                s[m] = sx[m][b * a.xs_group] * sw[b];
-            }
-            x[m] = f8_join(lo, hi);
+            x[m] = f8_join(*reinterpret_cast<const i32x4_f8*>(xp[m] + (at < a.k ? at : b * 128)),
+                           *reinterpret_cast<const i32x4_f8*>(xp[m] + (at + 64 < a.k ? at + 64 : b * 128)));
+            s[m] = sx[m][b * a.xs_group] * sw[b];
         }
 #pragma unroll
         for (int i = 0; i < NT; i++)
@@ -79,7 +71,9 @@ __global__ void __launch_bounds__(NW * 64) dec_kernel(F8Mat a, int ntiles, bool 
             for (int c = 0; c < 4; c++) v[c] += p[c];
         }
         const int l = j & 63, m = (j >> 6) % MT, i = (j >> 6) / MT, row = 16 * m + (l & 15), col = (n0 + i) * 16 + 4 * (l >> 4);
-        if (row < rows && col < a.n) f8_store4<OUT>(static_cast<uint16_t*>(a.y) + (int64_t)(row0 + row) * a.ldy, col, a.n, v, vec);
+        if (row >= rows || col >= a.n) continue;
+        if (GROUPED && a.rows && (unsigned)a.rows[row0 + row] >= (unsigned)a.t) v = f32x4_v{0.f, 0.f, 0.f, 0.f};
+        f8_store4<OUT>(static_cast<uint16_t*>(a.y) + (int64_t)(row0 + row) * a.ldy, col, a.n, v, vec);
     }
 }
 

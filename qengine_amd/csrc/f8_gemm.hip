@@ -1,23 +1,29 @@
-// 8-bit products of many rows (f8.hpp): tiles of BT rows x BW weight rows, steps of 128 k through LDS.
+// 8-bit products of many rows (f8.hpp): tiles of BT rows x BW weight rows in steps of 128 k.
 //
-// LDS holds two stages of activations ([BT][128 bytes], 16-byte chunk c of row r at c ^ (r % 8)), weights (as they lie in
-// memory) and the rows' scales of the step, filled by LDS DMA a step ahead. Each MFMA of depth 128 starts from zero and its
-// four sums are added at sx sw in fp32.
+// A wave holds TT x WT tiles of 16 x 16 sums. Activations go through LDS (three stages of [BT][128 bytes], chunk c of row r at c ^ (r %
+// 8), and the rows' scales), filled by LDS DMA two steps ahead; weights are read a step ahead from memory into registers, where
+// they lie as the matrix core takes them. So LDS carries a third of what it would with both operands (256 x 256, 8 waves: 128 KB
+// of reads and 32 KB of fills a step, 1280 of the 2048 cycles that the step's MFMAs take at 128 bytes a cycle), and a step's one
+// barrier comes when the next operands are in registers. Each MFMA of depth 128 starts from zero; its four sums are added at
+// sx sw in fp32 behind the next ones.
 #include "mfma_tile.hpp"
 #include "f8.hpp"
+#include <type_traits>
 
 namespace {
 using qe_tile::dma16;
+using qe_tile::dma16_at;
 using qe_tile::dma4;
 
-__device__ const uint4 kZeros[4] = {};  // what stands behind a row's last column
+typedef const __attribute__((address_space(4))) float* scalar_f32;  // read by scalar loads
 
 template <int BT, int BW, int WVT, int WVW, int OUT, bool GROUPED>
-__global__ void __launch_bounds__(WVT * WVW * 64) gemm_kernel(F8Mat a, int ntt, int ntw, bool vec) {
+__global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int ntt, int ntw, bool vec) {
     constexpr int NW = WVT * WVW, NTH = NW * 64, TT = BT / WVT / 16, WT = BW / WVW / 16;
-    constexpr int kX = BT * 128, kW = BW * 128, kStage = kX + kW + BT * 4;
-    constexpr int XD = BT / 8 / NW, WD = BW / 8 / NW;  // DMAs of a wave and step
-    static_assert(XD * 8 * NW == BT && WD * 8 * NW == BW && BT / 64 <= NW, "whole DMAs");
+    constexpr int kX = BT * 128, kStage = kX + BT * 4;
+    constexpr int XD = BT / 8 / NW;  // DMAs of a wave and step
+    static_assert(XD * 8 * NW == BT && BT / 64 <= NW && TT % 2 == 0, "whole DMAs");
+    static_assert(128 % (WT * 16) == 0, "a wave's weight rows lie in one block of 128");
     extern __shared__ __align__(16) char lds[];
     const unsigned lds32 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)lds);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -41,78 +47,123 @@ __global__ void __launch_bounds__(WVT * WVW * 64) gemm_kernel(F8Mat a, int ntt, 
         row0 = tt * BT;
         rows = min(BT, a.r - row0);
     }
-    auto x_row = [&](int i) -> int64_t {  // row i of the tile (the last one again behind it), -1: an index outside x
+    // row i of the tile (the last one again behind it) in x; an index outside x: row 0, and zeros in y
+    auto x_row = [&](int i) -> int64_t {
         const int64_t row = row0 + min(i, rows - 1);
         if (!GROUPED || !a.rows) return row;
         const int at = a.rows[row];
-        return (unsigned)at < (unsigned)a.t ? at : -1;
+        return (unsigned)at < (unsigned)a.t ? at : 0;
     };
-    const char *xp[XD], *wp[WD];
-    bool has[XD];
-    const int chunk = (lane & 7) ^ (lane >> 3);
+    // chunks behind k take the block's first: a row's own finite values times the weights' zeros there
+    const int chunk = (lane & 7) ^ (lane >> 3), last = chunk * 16 < a.k - (kb - 1) * 128 ? chunk * 16 : 0;
+    // one matrix: offsets from the tile's first row (rows are less than 2^24 bytes apart); grouped: addresses
+    const char* x0 = static_cast<const char*>(a.x) + (GROUPED ? 0 : (int64_t)row0 * a.ldx);
+    const char* xp[XD];
+    uint32_t xi[XD];
 #pragma unroll
     for (int i = 0; i < XD; i++) {
-        const int64_t row = x_row((wave * XD + i) * 8 + (lane >> 3));
-        has[i] = row >= 0;
-        xp[i] = static_cast<const char*>(a.x) + (has[i] ? row : 0) * a.ldx + chunk * 16;
+        const int row = (wave * XD + i) * 8 + (lane >> 3);
+        if constexpr (GROUPED) xp[i] = x0 + x_row(row) * a.ldx;
+        else xi[i] = (uint32_t)min(row, rows - 1) * (uint32_t)a.ldx;
     }
-#pragma unroll
-    for (int i = 0; i < WD; i++) {
-        const int d = wave * WD + i, t16 = min(tw * (BW / 16) + (d >> 1), n16 - 1);
-        wp[i] = static_cast<const char*>(a.q) + ((size_t)e * n16 + t16) * kb * 2048 + (d & 1) * 1024 + lane * 16;
-    }
-    const int64_t srow = wave < BT / 64 ? x_row(wave * 64 + lane) : 0;
-    const float* sp = a.xs + (srow < 0 ? 0 : srow) * a.xs_row;
+    const float* sp = wave < BT / 64 ? a.xs + x_row(wave * 64 + lane) * a.xs_row : nullptr;
     auto dma_step = [&](int b, int stage) {
         const unsigned to = lds32 + stage * kStage;
-        const bool last = b * 128 + 128 > a.k;
+        const int at = b == kb - 1 ? last : chunk * 16;
 #pragma unroll
         for (int i = 0; i < XD; i++) {
-            const char* p = xp[i] + (size_t)b * 128;
-            if (!has[i] || (last && b * 128 + chunk * 16 >= a.k)) p = reinterpret_cast<const char*>(kZeros);
-            dma16(p, to + (wave * XD + i) * 1024);
+            if constexpr (GROUPED) dma16(xp[i] + b * 128 + at, to + (wave * XD + i) * 1024);
+            else dma16_at(x0 + b * 128, xi[i] + at, to + (wave * XD + i) * 1024);
         }
-#pragma unroll
-        for (int i = 0; i < WD; i++) dma16(wp[i] + (size_t)b * 2048, to + kX + (wave * WD + i) * 1024);
-        if (wave < BT / 64) dma4(srow < 0 ? reinterpret_cast<const float*>(kZeros) : sp + b * a.xs_group, to + kX + kW + wave * 256);
+        if (wave < BT / 64) dma4(sp + b * a.xs_group, to + kX + wave * 256);
     };
-    const int nb = min((tw * BW + ww * WT * 16) >> 7, (a.n - 1) >> 7);
-    const float* sw = a.s + ((size_t)e * ((a.n + 127) >> 7) + nb) * kb;
-    static_assert(128 % (WT * 16) == 0, "a wave's weight rows lie in one block of 128");
+    const int t16 = tw * (BW / 16) + ww * WT;  // the wave's first 16 weight rows
+    const char* const w0 = static_cast<const char*>(a.q) + (size_t)e * n16 * kb * 2048;
+    const scalar_f32 sw = (scalar_f32)(a.s + ((size_t)e * ((a.n + 127) >> 7) + min(t16 >> 3, (a.n - 1) >> 7)) * kb);
 
-    f32x4_v acc[WT][TT] = {};
-    const int xo = (wt * TT * 16 + r) * 128 + ((g ^ (r & 7)) << 4), wo = ww * WT * 2048 + lane * 16;
-    dma_step(0, 0);
-    for (int b = 0; b < kb; b++) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (b + 1 < kb) dma_step(b + 1, (b + 1) & 1);
-        const char* x = lds + (b & 1) * kStage;
-        const char* w = x + kX;
-        const float* sx = reinterpret_cast<const float*>(w + kW);
-        const float swb = sw[b];
-        i32x8_f8 wf[WT];
+    // The sums of product number p = t WT + i wait in a ring while the next three products are under way
+    constexpr int RING = 4, LAG = RING - 1, NP = TT * WT;
+    static_assert(NP % RING == 0 && TT > 2 && (TT - 2) * WT >= LAG, "a step begins at the ring's begin; scales outlast their sums");
+    f32x4_v acc[WT][TT] = {}, part[RING] = {};
+    i32x8_f8 w[2][WT];
+    i32x8_f8 x[2];
+    float sc[TT] = {};  // scales of the step's rows; the last two's of the step before until their turn
+    const int xo = (wt * TT * 16 + r) * 128 + ((g ^ (r & 7)) << 4), so = kX + (wt * TT * 16 + r) * 4;
+    auto load_w = [&](int b, int to) {
 #pragma unroll
-        for (int i = 0; i < WT; i++)
-            wf[i] = f8_join(*reinterpret_cast<const i32x4_f8*>(w + wo + i * 2048), *reinterpret_cast<const i32x4_f8*>(w + wo + i * 2048 + 1024));
+        for (int i = 0; i < WT; i++) {
+            const char* p = w0 + ((size_t)min(t16 + i, n16 - 1) * kb + b) * 2048;
+            w[to][i] = f8_join(*reinterpret_cast<const i32x4_f8*>(p + lane * 16), *reinterpret_cast<const i32x4_f8*>(p + 1024 + lane * 16));
+        }
+    };
+    auto load_x = [&](int stage, int t) {
+        const char* p = lds + stage * kStage;
+        x[t & 1] = f8_join(*reinterpret_cast<const i32x4_f8*>(p + xo + t * 2048), *reinterpret_cast<const i32x4_f8*>(p + (xo ^ 64) + t * 2048));
+        return *reinterpret_cast<const float*>(p + so + t * 64);
+    };
+    // every load and DMA of this wave is there (the compiler learns it by the operands), and the other waves'
+    auto arrive = [&](int to) {
+#pragma unroll
+        for (int i = 0; i < WT; i++) asm volatile("" : "+v"(w[to][i]));
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    auto flush = [&](int p) {
+        const int i = p % WT, t = p / WT;
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[i][t][j] = fmaf(part[p % RING][j], sc[t], acc[i][t][j]);
+        asm volatile("" : "+v"(acc[i][t]));  // here, not behind the step's branches, where the compiler sinks it
+    };
+    dma_step(0, 0);
+    if (kb > 1) dma_step(1, 1);
+    load_w(0, 0);
+    arrive(0);
+    int stage = 0;
+    float s0 = load_x(0, 0);
+    // step b with weights w[cur]: stage b + 1 is filled and stage b - 1 free
+    auto step = [&](int b, auto c) {
+        constexpr int cur = decltype(c)::value;
+        const int next = stage == 2 ? 0 : stage + 1, after = next == 2 ? 0 : next + 1;
+        const float swb = sw[b];
+        load_w(b + 1 < kb ? b + 1 : b, cur ^ 1);
+        if (b + 2 < kb) dma_step(b + 2, after);
+        __builtin_amdgcn_sched_barrier(0);
+        float s = s0;
 #pragma unroll
         for (int t = 0; t < TT; t++) {
-            const i32x8_f8 xf = f8_join(*reinterpret_cast<const i32x4_f8*>(x + xo + t * 2048), *reinterpret_cast<const i32x4_f8*>(x + (xo ^ 64) + t * 2048));
-            const float s = sx[wt * TT * 16 + t * 16 + r] * swb;
+            sc[t] = s * swb;
+            const float sn = t + 1 < TT ? load_x(stage, t + 1) : load_x(next, 0);
 #pragma unroll
             for (int i = 0; i < WT; i++) {
-                const f32x4_v p = f8_mfma(wf[i], xf);
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][t][j] = fmaf(p[j], s, acc[i][t][j]);
+                const int p = t * WT + i;
+                part[p % RING] = f8_mfma(w[cur][i], x[t & 1]);
+                flush((p + NP - LAG) % NP);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            s = sn;
         }
+        s0 = s;
+        stage = next;
+        arrive(cur ^ 1);
+    };
+    int b = 0;
+    for (; b + 2 <= kb; b += 2) {
+        step(b, std::integral_constant<int, 0>{});
+        step(b + 1, std::integral_constant<int, 1>{});
     }
+    if (b < kb) step(b, std::integral_constant<int, 0>{});
+#pragma unroll
+    for (int p = NP - LAG; p < NP; p++) flush(p);
 #pragma unroll
     for (int t = 0; t < TT; t++) {
         const int row = wt * TT * 16 + t * 16 + r;
         if (row >= rows) continue;
+        if (GROUPED && a.rows && (unsigned)a.rows[row0 + row] >= (unsigned)a.t) {
+#pragma unroll
+            for (int i = 0; i < WT; i++) acc[i][t] = f32x4_v{0.f, 0.f, 0.f, 0.f};
+        }
 #pragma unroll
         for (int i = 0; i < WT; i++) {
-            const int col = tw * BW + (ww * WT + i) * 16 + 4 * g;
+            const int col = (t16 + i) * 16 + 4 * g;
             if (col < a.n) f8_store4<OUT>(static_cast<uint16_t*>(a.y) + (int64_t)(row0 + row) * a.ldy, col, a.n, acc[i][t], vec);
         }
     }
@@ -120,7 +171,7 @@ __global__ void __launch_bounds__(WVT * WVW * 64) gemm_kernel(F8Mat a, int ntt, 
 
 template <int BT, int BW, int WVT, int WVW, bool GROUPED>
 void gemm_t(const F8Mat& a, hipStream_t st) {
-    constexpr int kLds = 2 * (BT * 128 + BW * 128 + BT * 4);
+    constexpr int kLds = 3 * (BT * 128 + BT * 4);
     const int64_t ntt = GROUPED ? f8_most_jobs(a.r, a.experts, BT) : (a.r + BT - 1) / BT, ntw = (a.n + BW - 1) / BW;
     CHECK(ntt * ntw <= kF8MaxBlocks, "matmul_f8: %lld row tiles by %lld column tiles are too many for a call", (long long)ntt, (long long)ntw);
     const dim3 grid((unsigned)((ntt * ntw + 7) / 8 * 8)), block(WVT * WVW * 64);
@@ -144,7 +195,14 @@ void f8_matmul(const F8Mat& a, hipStream_t st) {
     CHECK(a.experts > 0 && a.experts <= kF8MaxExperts && (a.off || (a.experts == 1 && !a.rows)), "matmul_f8: %d matrices", a.experts);
     CHECK(a.q && a.s && a.y && (a.t == 0 || (a.x && a.xs)), "matmul_f8: a tensor is missing");
     CHECK(((uintptr_t)a.q & 15) == 0 && ((uintptr_t)a.x & 15) == 0 && a.ldx % 16 == 0, "matmul_f8: x and its rows are 16-byte aligned");
+    F8Mat m = a;
+    if (a.t == 0) {  // every index is outside x: rows that are read and not used
+        m.x = a.q;
+        m.xs = a.s;
+        m.ldx = m.xs_row = 0;
+        m.xs_group = 1;
+    }
     const bool few = a.off ? a.r <= (int64_t)a.experts * 8 : a.r <= 32;
-    if (few) f8_dec(a, st);
-    else f8_gemm(a, st);
+    if (few) f8_dec(m, st);
+    else f8_gemm(m, st);
 }
