@@ -1,11 +1,11 @@
 // 8-bit products of many rows (f8.hpp): tiles of BT rows x BW weight rows in steps of 128 k.
 //
-// A wave holds TT x WT tiles of 16 x 16 sums. Activations go through LDS (three stages of [BT][128 bytes], chunk c of row r at c ^ (r %
-// 8), and the rows' scales), filled by LDS DMA two steps ahead; weights are read a step ahead from memory into registers, where
-// they lie as the matrix core takes them. So LDS carries a third of what it would with both operands (256 x 256, 8 waves: 128 KB
-// of reads and 32 KB of fills a step, 1280 of the 2048 cycles that the step's MFMAs take at 128 bytes a cycle), and a step's one
-// barrier comes when the next operands are in registers. Each MFMA of depth 128 starts from zero; its four sums are added at
-// sx sw in fp32 behind the next ones.
+// A wave holds TT x WT tiles of 16 x 16 sums. Both operands go through LDS, filled by LDS DMA. What a step begins with is there a
+// step early, so that no wave waits for LDS behind the barrier: weights are read into registers a step ahead, and the first 16 rows
+// of each wave and the rows' scales have rings of three. A step's DMAs are spread over its first half: issued at once they kept the
+// waves at the address unit (64 bytes a cycle: 1000 to 1500 cycles of a step), and the step's products waited behind them (256 x
+// 256 tiles: 4490 cycles a step with 2048 of products). Each MFMA of depth 128 starts from zero; its four sums are added
+// at sx sw in fp32 behind the next ones.
 #include "mfma_tile.hpp"
 #include "f8.hpp"
 #include <type_traits>
@@ -17,12 +17,20 @@ using qe_tile::dma4;
 
 typedef const __attribute__((address_space(4))) float* scalar_f32;  // read by scalar loads
 
+// the same address in scalar registers, where a DMA takes its base from
+__device__ __forceinline__ const char* scalar(const char* p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    return reinterpret_cast<const char*>((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 |
+                                         (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v));
+}
+
 template <int BT, int BW, int WVT, int WVW, int OUT, bool GROUPED>
 __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int ntt, int ntw, bool vec) {
     constexpr int NW = WVT * WVW, NTH = NW * 64, TT = BT / WVT / 16, WT = BW / WVW / 16;
-    constexpr int kX = BT * 128, kStage = kX + BT * 4;
-    constexpr int XD = BT / 8 / NW;  // DMAs of a wave and step
-    static_assert(XD * 8 * NW == BT && BT / 64 <= NW && TT % 2 == 0, "whole DMAs");
+    constexpr int kX = BT * 128, kW = BW * 128, kFirst = WVT * 2048, kS = BT * 4;  // bytes of a stage
+    constexpr int oW = 2 * kX, oFirst = oW + 2 * kW, oS = oFirst + 3 * kFirst;
+    constexpr int XD = BT / 8 / NW, WD = BW / 8 / NW;  // DMAs of a wave and step
+    static_assert(XD * 8 * NW == BT && WD * 8 * NW == BW && BT / 64 <= NW && TT % 2 == 0, "whole DMAs");
     static_assert(128 % (WT * 16) == 0, "a wave's weight rows lie in one block of 128");
     extern __shared__ __align__(16) char lds[];
     const unsigned lds32 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)lds);
@@ -67,83 +75,106 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int nt
         else xi[i] = (uint32_t)min(row, rows - 1) * (uint32_t)a.ldx;
     }
     const float* sp = wave < BT / 64 ? a.xs + x_row(wave * 64 + lane) * a.xs_row : nullptr;
-    auto dma_step = [&](int b, int stage) {
-        const unsigned to = lds32 + stage * kStage;
-        const int at = b == kb - 1 ? last : chunk * 16;
-#pragma unroll
-        for (int i = 0; i < XD; i++) {
-            if constexpr (GROUPED) dma16(xp[i] + b * 128 + at, to + (wave * XD + i) * 1024);
-            else dma16_at(x0 + b * 128, xi[i] + at, to + (wave * XD + i) * 1024);
-        }
-        if (wave < BT / 64) dma4(sp + b * a.xs_group, to + kX + wave * 256);
-    };
     const int t16 = tw * (BW / 16) + ww * WT;  // the wave's first 16 weight rows
     const char* const w0 = static_cast<const char*>(a.q) + (size_t)e * n16 * kb * 2048;
     const scalar_f32 sw = (scalar_f32)(a.s + ((size_t)e * ((a.n + 127) >> 7) + min(t16 >> 3, (a.n - 1) >> 7)) * kb);
+    // DMAs of this wave, past the last block that block again (nobody reads it): 8 rows of x, block b, to LDS byte `to`
+    auto dma_x = [&](int i, int b, unsigned to) {
+        const int at = b >= kb - 1 ? last : chunk * 16;
+        b = min(b, kb - 1);
+        if constexpr (GROUPED) dma16(xp[i] + b * 128 + at, to);
+        else dma16_at(scalar(x0 + b * 128), xi[i] + at, to);
+    };
+    auto dma_w = [&](int i, int b, unsigned to) {
+        const int d = wave * WD + i;
+        dma16_at(scalar(w0 + ((size_t)min(tw * (BW / 16) + (d >> 1), n16 - 1) * kb + min(b, kb - 1)) * 2048 + (d & 1) * 1024), lane * 16, to + d * 1024);
+    };
+    auto dma_s = [&](int b, unsigned to) {
+        if (wave < BT / 64) dma4(sp + min(b, kb - 1) * a.xs_group, to + wave * 256);
+    };
+    // the same for DMA number i of a wave's rows: their first 16 go to the ring for block `early`, the others to a stage
+    auto dma_rows = [&](int i, int b, unsigned to, int early, unsigned ring) {
+        const int d = wave * XD + i, f = d % (2 * TT);
+        dma_x(i, f < 2 ? early : b, f < 2 ? ring + (d / (2 * TT) * 2 + f) * 1024 : to + d * 1024);
+    };
 
     // The sums of product number p = t WT + i wait in a ring while the next three products are under way
-    constexpr int RING = 4, LAG = RING - 1, NP = TT * WT;
+    constexpr int RING = 4, LAG = RING - 1, NP = TT * WT, EV = 2 * (WD + XD) < NP ? 2 : 1;
     static_assert(NP % RING == 0 && TT > 2 && (TT - 2) * WT >= LAG, "a step begins at the ring's begin; scales outlast their sums");
+    static_assert(WD + XD < NP && NP / 2 + WT <= NP, "a step's DMAs and reads find a product");
     f32x4_v acc[WT][TT] = {}, part[RING] = {};
     i32x8_f8 w[2][WT];
     i32x8_f8 x[2];
     float sc[TT] = {};  // scales of the step's rows; the last two's of the step before until their turn
-    const int xo = (wt * TT * 16 + r) * 128 + ((g ^ (r & 7)) << 4), so = kX + (wt * TT * 16 + r) * 4;
-    auto load_w = [&](int b, int to) {
-#pragma unroll
-        for (int i = 0; i < WT; i++) {
-            const char* p = w0 + ((size_t)min(t16 + i, n16 - 1) * kb + b) * 2048;
-            w[to][i] = f8_join(*reinterpret_cast<const i32x4_f8*>(p + lane * 16), *reinterpret_cast<const i32x4_f8*>(p + 1024 + lane * 16));
-        }
+    const int xo = r * 128 + ((g ^ (r & 7)) << 4), so = (wt * TT * 16 + r) * 4;
+    auto load_w = [&](int to, int i, const char* p) {
+        p += (ww * WT + i) * 2048 + lane * 16;
+        w[to][i] = f8_join(*reinterpret_cast<const i32x4_f8*>(p), *reinterpret_cast<const i32x4_f8*>(p + 1024));
     };
-    auto load_x = [&](int stage, int t) {
-        const char* p = lds + stage * kStage;
-        x[t & 1] = f8_join(*reinterpret_cast<const i32x4_f8*>(p + xo + t * 2048), *reinterpret_cast<const i32x4_f8*>(p + (xo ^ 64) + t * 2048));
-        return *reinterpret_cast<const float*>(p + so + t * 64);
+    auto load_x = [&](int to, const char* p) {  // p: 16 rows
+        x[to] = f8_join(*reinterpret_cast<const i32x4_f8*>(p + xo), *reinterpret_cast<const i32x4_f8*>(p + (xo ^ 64)));
     };
-    // every load and DMA of this wave is there (the compiler learns it by the operands), and the other waves'
-    auto arrive = [&](int to) {
-#pragma unroll
-        for (int i = 0; i < WT; i++) asm volatile("" : "+v"(w[to][i]));
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    };
+    auto load_s = [&](const char* p, int t) { return *reinterpret_cast<const float*>(p + so + t * 64); };
+    auto arrive = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
     auto flush = [&](int p) {
         const int i = p % WT, t = p / WT;
 #pragma unroll
         for (int j = 0; j < 4; j++) acc[i][t][j] = fmaf(part[p % RING][j], sc[t], acc[i][t][j]);
         asm volatile("" : "+v"(acc[i][t]));  // here, not behind the step's branches, where the compiler sinks it
     };
-    dma_step(0, 0);
-    if (kb > 1) dma_step(1, 1);
-    load_w(0, 0);
-    arrive(0);
-    int stage = 0;
-    float s0 = load_x(0, 0);
-    // step b with weights w[cur]: stage b + 1 is filled and stage b - 1 free
+#pragma unroll
+    for (int i = 0; i < XD; i++) {
+        dma_rows(i, 0, lds32, 0, lds32 + oFirst);
+        dma_rows(i, 0, lds32, 1, lds32 + oFirst + kFirst);
+    }
+#pragma unroll
+    for (int i = 0; i < WD; i++) {
+        dma_w(i, 0, lds32 + oW);
+        dma_w(i, 1, lds32 + oW + kW);
+    }
+    dma_s(0, lds32 + oS);
+    dma_s(1, lds32 + oS + kS);
+    arrive();
+    int ring = 0;
+#pragma unroll
+    for (int i = 0; i < WT; i++) load_w(0, i, lds + oW);
+    load_x(0, lds + oFirst + wt * 2048);
+    float s0 = load_s(lds + oS, 0);
+    arrive();  // the first weights are read: their stage is free
+    // Step b, c = b % 2: products of weights w[c] and rows in stage c and in the ring; reads weights b + 1 from stage 1 - c; fetches
+    // rows b + 1 to stage 1 - c, weights b + 2 to stage c, first rows and scales b + 2 to the ring
     auto step = [&](int b, auto c) {
         constexpr int cur = decltype(c)::value;
-        const int next = stage == 2 ? 0 : stage + 1, after = next == 2 ? 0 : next + 1;
+        const int next = ring == 2 ? 0 : ring + 1, after = next == 2 ? 0 : next + 1;
         const float swb = sw[b];
-        load_w(b + 1 < kb ? b + 1 : b, cur ^ 1);
-        if (b + 2 < kb) dma_step(b + 2, after);
-        __builtin_amdgcn_sched_barrier(0);
         float s = s0;
 #pragma unroll
         for (int t = 0; t < TT; t++) {
             sc[t] = s * swb;
-            const float sn = t + 1 < TT ? load_x(stage, t + 1) : load_x(next, 0);
+            if (t + 1 < TT) {
+                load_x((t + 1) & 1, lds + cur * kX + (wt * TT + t + 1) * 2048);
+                s = load_s(lds + oS + ring * kS, t + 1);
+            } else {
+                load_x(0, lds + oFirst + next * kFirst + wt * 2048);
+                s0 = load_s(lds + oS + next * kS, 0);
+            }
 #pragma unroll
             for (int i = 0; i < WT; i++) {
                 const int p = t * WT + i;
                 part[p % RING] = f8_mfma(w[cur][i], x[t & 1]);
                 flush((p + NP - LAG) % NP);
+                const int j = p / EV;  // a DMA behind every product, or every second
+                if (p % EV == 0) {
+                    if (j < WD) dma_w(j, b + 2, lds32 + oW + cur * kW);
+                    else if (j < WD + XD) dma_rows(j - WD, b + 1, lds32 + (cur ^ 1) * kX, b + 2, lds32 + oFirst + after * kFirst);
+                    else if (j == WD + XD) dma_s(b + 2, lds32 + oS + after * kS);
+                }
+                if (p >= NP / 2 && p - NP / 2 < WT) load_w(cur ^ 1, p - NP / 2, lds + oW + (cur ^ 1) * kW);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            s = sn;
         }
-        s0 = s;
-        stage = next;
-        arrive(cur ^ 1);
+        ring = next;
+        arrive();
     };
     int b = 0;
     for (; b + 2 <= kb; b += 2) {
@@ -171,7 +202,7 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int nt
 
 template <int BT, int BW, int WVT, int WVW, bool GROUPED>
 void gemm_t(const F8Mat& a, hipStream_t st) {
-    constexpr int kLds = 3 * (BT * 128 + BT * 4);
+    constexpr int kLds = 2 * 128 * (BT + BW) + 3 * (WVT * 2048 + BT * 4);
     const int64_t ntt = GROUPED ? f8_most_jobs(a.r, a.experts, BT) : (a.r + BT - 1) / BT, ntw = (a.n + BW - 1) / BW;
     CHECK(ntt * ntw <= kF8MaxBlocks, "matmul_f8: %lld row tiles by %lld column tiles are too many for a call", (long long)ntt, (long long)ntw);
     const dim3 grid((unsigned)((ntt * ntw + 7) / 8 * 8)), block(WVT * WVW * 64);
