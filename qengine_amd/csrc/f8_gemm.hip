@@ -15,8 +15,6 @@ using qe_tile::dma16;
 using qe_tile::dma16_at;
 using qe_tile::dma4;
 
-typedef const __attribute__((address_space(4))) float* scalar_f32;  // read by scalar loads
-
 // the same address in scalar registers, where a DMA takes its base from
 __device__ __forceinline__ const char* scalar(const char* p) {
     const uint64_t v = reinterpret_cast<uint64_t>(p);
@@ -27,10 +25,10 @@ __device__ __forceinline__ const char* scalar(const char* p) {
 template <int BT, int BW, int WVT, int WVW, int OUT, bool GROUPED>
 __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int ntt, int ntw, bool vec) {
     constexpr int NW = WVT * WVW, NTH = NW * 64, TT = BT / WVT / 16, WT = BW / WVW / 16;
-    constexpr int kX = BT * 128, kW = BW * 128, kFirst = WVT * 2048, kS = BT * 4;  // bytes of a stage
+    constexpr int kX = BT * 128, kW = BW * 128, kFirst = WVT * 2048, kS = BT * 4 + 256;  // bytes of a stage
     constexpr int oW = 2 * kX, oFirst = oW + 2 * kW, oS = oFirst + 3 * kFirst;
     constexpr int XD = BT / 8 / NW, WD = BW / 8 / NW;  // DMAs of a wave and step
-    static_assert(XD * 8 * NW == BT && WD * 8 * NW == BW && BT / 64 <= NW && TT % 2 == 0, "whole DMAs");
+    static_assert(XD * 8 * NW == BT && WD * 8 * NW == BW && BT / 64 < NW && TT % 2 == 0 && BW % 128 == 0, "whole DMAs");
     static_assert(128 % (WT * 16) == 0, "a wave's weight rows lie in one block of 128");
     extern __shared__ __align__(16) char lds[];
     const unsigned lds32 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)lds);
@@ -74,10 +72,15 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int nt
         if constexpr (GROUPED) xp[i] = x0 + x_row(row) * a.ldx;
         else xi[i] = (uint32_t)min(row, rows - 1) * (uint32_t)a.ldx;
     }
-    const float* sp = wave < BT / 64 ? a.xs + x_row(wave * 64 + lane) * a.xs_row : nullptr;
+    // scales of the rows, 64 a wave, and of the tile's blocks of 128 weight rows, by the wave after them
+    const float* sp = a.xs + (wave < BT / 64 ? x_row(wave * 64 + lane) * a.xs_row : 0);
+    int64_t sp_next = a.xs_group;
+    if (wave == BT / 64) {
+        sp = a.s + ((size_t)e * ((a.n + 127) >> 7) + min(tw * (BW / 128) + (lane & (BW / 128 - 1)), (a.n - 1) >> 7)) * kb;
+        sp_next = 1;
+    }
     const int t16 = tw * (BW / 16) + ww * WT;  // the wave's first 16 weight rows
     const char* const w0 = static_cast<const char*>(a.q) + (size_t)e * n16 * kb * 2048;
-    const scalar_f32 sw = (scalar_f32)(a.s + ((size_t)e * ((a.n + 127) >> 7) + min(t16 >> 3, (a.n - 1) >> 7)) * kb);
     // DMAs of this wave, past the last block that block again (nobody reads it): 8 rows of x, block b, to LDS byte `to`
     auto dma_x = [&](int i, int b, unsigned to) {
         const int at = b >= kb - 1 ? last : chunk * 16;
@@ -90,7 +93,7 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int nt
         dma16_at(scalar(w0 + ((size_t)min(tw * (BW / 16) + (d >> 1), n16 - 1) * kb + min(b, kb - 1)) * 2048 + (d & 1) * 1024), lane * 16, to + d * 1024);
     };
     auto dma_s = [&](int b, unsigned to) {
-        if (wave < BT / 64) dma4(sp + min(b, kb - 1) * a.xs_group, to + wave * 256);
+        if (wave <= BT / 64) dma4(sp + min(b, kb - 1) * sp_next, to + wave * 256);
     };
     // the same for DMA number i of a wave's rows: their first 16 go to the ring for block `early`, the others to a stage
     auto dma_rows = [&](int i, int b, unsigned to, int early, unsigned ring) {
@@ -115,6 +118,7 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int nt
         x[to] = f8_join(*reinterpret_cast<const i32x4_f8*>(p + xo), *reinterpret_cast<const i32x4_f8*>(p + (xo ^ 64)));
     };
     auto load_s = [&](const char* p, int t) { return *reinterpret_cast<const float*>(p + so + t * 64); };
+    auto load_sw = [&](const char* p) { return *reinterpret_cast<const float*>(p + BT * 4 + (ww * WT >> 3) * 4); };
     auto arrive = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
     auto flush = [&](int p) {
         const int i = p % WT, t = p / WT;
@@ -139,14 +143,14 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int nt
 #pragma unroll
     for (int i = 0; i < WT; i++) load_w(0, i, lds + oW);
     load_x(0, lds + oFirst + wt * 2048);
-    float s0 = load_s(lds + oS, 0);
+    float s0 = load_s(lds + oS, 0), sw0 = load_sw(lds + oS);
     arrive();  // the first weights are read: their stage is free
     // Step b, c = b % 2: products of weights w[c] and rows in stage c and in the ring; reads weights b + 1 from stage 1 - c; fetches
     // rows b + 1 to stage 1 - c, weights b + 2 to stage c, first rows and scales b + 2 to the ring
     auto step = [&](int b, auto c) {
         constexpr int cur = decltype(c)::value;
         const int next = ring == 2 ? 0 : ring + 1, after = next == 2 ? 0 : next + 1;
-        const float swb = sw[b];
+        const float swb = sw0;
         float s = s0;
 #pragma unroll
         for (int t = 0; t < TT; t++) {
@@ -157,6 +161,7 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int nt
             } else {
                 load_x(0, lds + oFirst + next * kFirst + wt * 2048);
                 s0 = load_s(lds + oS + next * kS, 0);
+                sw0 = load_sw(lds + oS + next * kS);
             }
 #pragma unroll
             for (int i = 0; i < WT; i++) {
@@ -184,29 +189,48 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int nt
     if (b < kb) step(b, std::integral_constant<int, 0>{});
 #pragma unroll
     for (int p = NP - LAG; p < NP; p++) flush(p);
+    // Rows of y through LDS, which the last barrier freed: a wave's 16 x 16 sums as they lie (8 bytes of 16 rows a store: 7 us for a tile
+    // of 256 x 256), read back as 16-byte pieces of whole rows, chunk c of row i at c ^ (i % C).
+    constexpr int C = WT * 2;  // 16-byte chunks of a wave's row
+    char* const out = lds + wave * TT * 16 * C * 16;
+    static_assert(NW * TT * 16 * C * 16 <= 2 * (kX + kW), "every wave's rows fit the stages");
 #pragma unroll
-    for (int t = 0; t < TT; t++) {
-        const int row = wt * TT * 16 + t * 16 + r;
-        if (row >= rows) continue;
-        if (GROUPED && a.rows && (unsigned)a.rows[row0 + row] >= (unsigned)a.t) {
-#pragma unroll
-            for (int i = 0; i < WT; i++) acc[i][t] = f32x4_v{0.f, 0.f, 0.f, 0.f};
-        }
+    for (int t = 0; t < TT; t++)
 #pragma unroll
         for (int i = 0; i < WT; i++) {
-            const int col = (t16 + i) * 16 + 4 * g;
-            if (col < a.n) f8_store4<OUT>(static_cast<uint16_t*>(a.y) + (int64_t)(row0 + row) * a.ldy, col, a.n, acc[i][t], vec);
+            const f32x4_v v = acc[i][t];
+            *reinterpret_cast<uint2*>(out + ((t * 16 + r) * C + ((2 * i + (g >> 1)) ^ (r & (C - 1)))) * 16 + (g & 1) * 8) =
+                OUT == kF8BF16 ? uint2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])} : uint2{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
+        }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int first = wt * TT * 16;  // row of the tile
+    uint16_t* const y = static_cast<uint16_t*>(a.y) + (int64_t)(row0 + first) * a.ldy + t16 * 16;
+    const int cols = a.n - t16 * 16;
+#pragma unroll 4
+    for (int j = 0; j < TT * C / 4; j++) {
+        const int at = j * 64 + lane, i = at / C, c = at % C;
+        uint4 v = *reinterpret_cast<const uint4*>(out + (i * C + (c ^ (i & (C - 1)))) * 16);
+        if (first + i >= rows || c * 8 >= cols) continue;
+        if (GROUPED && a.rows && (unsigned)a.rows[row0 + first + i] >= (unsigned)a.t) v = uint4{0, 0, 0, 0};
+        uint16_t* const to = y + i * a.ldy + c * 8;
+        if (vec && c * 8 + 8 <= cols) {
+            *reinterpret_cast<uint4*>(to) = v;
+        } else {
+            const uint32_t part4[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (c * 8 + k < cols) to[k] = (uint16_t)(part4[k >> 1] >> (16 * (k & 1)));
         }
     }
 }
 
 template <int BT, int BW, int WVT, int WVW, bool GROUPED>
 void gemm_t(const F8Mat& a, hipStream_t st) {
-    constexpr int kLds = 2 * 128 * (BT + BW) + 3 * (WVT * 2048 + BT * 4);
+    constexpr int kLds = 2 * 128 * (BT + BW) + 3 * (WVT * 2048 + BT * 4 + 256);
     const int64_t ntt = GROUPED ? f8_most_jobs(a.r, a.experts, BT) : (a.r + BT - 1) / BT, ntw = (a.n + BW - 1) / BW;
     CHECK(ntt * ntw <= kF8MaxBlocks, "matmul_f8: %lld row tiles by %lld column tiles are too many for a call", (long long)ntt, (long long)ntw);
     const dim3 grid((unsigned)((ntt * ntw + 7) / 8 * 8)), block(WVT * WVW * 64);
-    const bool vec = f8_vec_ok(a.y, a.ldy);
+    const bool vec = a.ldy % 8 == 0 && ((uintptr_t)a.y & 15) == 0;
     if (a.out == kF8BF16) gemm_kernel<BT, BW, WVT, WVW, kF8BF16, GROUPED><<<grid, block, kLds, st>>>(a, (int)ntt, (int)ntw, vec);
     else gemm_kernel<BT, BW, WVT, WVW, kF8F16, GROUPED><<<grid, block, kLds, st>>>(a, (int)ntt, (int)ntw, vec);
     HIP_CHECK(hipGetLastError());
