@@ -102,17 +102,18 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int nt
     };
 
     // The sums of product number p = t WT + i wait in a ring while the next three products are under way
-    constexpr int RING = 4, LAG = RING - 1, NP = TT * WT, EV = 2 * (WD + XD) < NP ? 2 : 1;
+    constexpr int RING = 4, LAG = RING - 1, NP = TT * WT, EV = 2 * (WD + XD) < NP ? 2 : 1, RW = NP / (2 * WT);
     static_assert(NP % RING == 0 && TT > 2 && (TT - 2) * WT >= LAG, "a step begins at the ring's begin; scales outlast their sums");
-    static_assert(WD + XD < NP && NP / 2 + WT <= NP, "a step's DMAs and reads find a product");
+    static_assert(WD + XD < NP && RW * 2 * WT == NP, "a step's DMAs and reads find a product");
     f32x4_v acc[WT][TT] = {}, part[RING] = {};
     i32x8_f8 w[2][WT];
     i32x8_f8 x[2];
     float sc[TT] = {};  // scales of the step's rows; the last two's of the step before until their turn
     const int xo = r * 128 + ((g ^ (r & 7)) << 4), so = (wt * TT * 16 + r) * 4;
-    auto load_w = [&](int to, int i, const char* p) {
-        p += (ww * WT + i) * 2048 + lane * 16;
-        w[to][i] = f8_join(*reinterpret_cast<const i32x4_f8*>(p), *reinterpret_cast<const i32x4_f8*>(p + 1024));
+    auto load_w = [&](int to, int i, int h, const char* p) {  // half h of tile i
+        const i32x4_f8 v = *reinterpret_cast<const i32x4_f8*>(p + (ww * WT + i) * 2048 + h * 1024 + lane * 16);
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[to][i][h * 4 + j] = v[j];
     };
     auto load_x = [&](int to, const char* p) {  // p: 16 rows
         x[to] = f8_join(*reinterpret_cast<const i32x4_f8*>(p + xo), *reinterpret_cast<const i32x4_f8*>(p + (xo ^ 64)));
@@ -141,7 +142,7 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int nt
     arrive();
     int ring = 0;
 #pragma unroll
-    for (int i = 0; i < WT; i++) load_w(0, i, lds + oW);
+    for (int i = 0; i < 2 * WT; i++) load_w(0, i / 2, i % 2, lds + oW);
     load_x(0, lds + oFirst + wt * 2048);
     float s0 = load_s(lds + oS, 0), sw0 = load_sw(lds + oS);
     arrive();  // the first weights are read: their stage is free
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int nt
                     else if (j < WD + XD) dma_rows(j - WD, b + 1, lds32 + (cur ^ 1) * kX, b + 2, lds32 + oFirst + after * kFirst);
                     else if (j == WD + XD) dma_s(b + 2, lds32 + oS + after * kS);
                 }
-                if (p >= NP / 2 && p - NP / 2 < WT) load_w(cur ^ 1, p - NP / 2, lds + oW + (cur ^ 1) * kW);
+                if (p % RW == RW / 2) load_w(cur ^ 1, p / RW / 2, p / RW % 2, lds + oW + (cur ^ 1) * kW);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
