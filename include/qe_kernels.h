@@ -78,7 +78,8 @@ int qe_gemm_tune_entries(void);
 void qe_gemm_reserve(size_t bytes);
 void qe_gemm_reserve_s(size_t bytes, void* stream);
 /* test hook: how many workspace buffers of a kind (0 split-K, 1 W4A8 / W8A8 pre-pass, 2 fp16-accumulate pre-pass, 3 part
- * sums of 17..64-row decode, 4 slice sums of 9..16-row decode, 5 part sums of qe_attn_tree) the library's streams and live graphs hold, over all
+ * sums of 17..64-row decode, 4 slice sums of 9..16-row decode, 5 part sums of qe_attn_tree, 6 part sums of
+ * qe_matmul_f8) the library's streams and live graphs hold, over all
  * devices. No counterpart in the reference. */
 int qe_workspace_count(int kind);
 /* Prefill GEMM with the reference's fp16-accumulate numerics (gemm_h_kernel + x_to_h_kernel,

@@ -14,7 +14,7 @@
 // chunks g and 4 + g: two loads of 1 KB a wave, every byte of which is used. Which k the matrix core takes for which byte does
 // not matter as long as both operands have the same; activations are read by the same chunks.
 #pragma once
-#include "qe_common.hpp"
+#include "qe_api.hpp"
 
 enum F8Type : int { kF8F32 = 0, kF8BF16 = 1, kF8F16 = 2 };  // types of outputs, and of the row operators' inputs
 

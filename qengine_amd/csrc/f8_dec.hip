@@ -5,7 +5,7 @@
 #include "f8.hpp"
 
 namespace {
-template <int MT, int NT, int NW, int OUT, bool GROUPED>
+template <int MT, int NT, int NW, int D, int OUT, bool GROUPED>
 __global__ void __launch_bounds__(NW * 64) dec_kernel(F8Mat a, int ntiles, bool vec) {
     __shared__ f32x4_v part[NW * NT * MT * 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -34,28 +34,40 @@ __global__ void __launch_bounds__(NW * 64) dec_kernel(F8Mat a, int ntiles, bool 
         xp[m] = static_cast<const uint8_t*>(a.x) + row * a.ldx;
         sx[m] = a.xs + row * a.xs_row;
     }
+    // D blocks of 128 k on their way; past the last one the last again, with a scale of zero
     f32x4_v acc[NT][MT] = {};
-    for (int b = wave; b < kb; b += NW) {
-        const int at = b * 128 + g * 16;  // of chunks g and 4 + g; behind k the block's first, which meets zeros
-        i32x8_f8 w[NT], x[MT];
-        float s[MT];
+    i32x8_f8 w[D][NT], x[D][MT];
+    float s[D][MT], swb[D];
+    auto load = [&](int d, int b) {
+        swb[d] = b < kb ? sw[b] : 0.f;
+        b = min(b, kb - 1);
+        const int at = b * 128 + g * 16, lo = at < a.k ? at : b * 128, hi = at + 64 < a.k ? at + 64 : b * 128;  // behind k the block's first
 #pragma unroll
         for (int i = 0; i < NT; i++)
-            w[i] = f8_join(*reinterpret_cast<const i32x4_f8*>(wp[i] + (size_t)b * 2048), *reinterpret_cast<const i32x4_f8*>(wp[i] + (size_t)b * 2048 + 1024));
+            w[d][i] = f8_join(*reinterpret_cast<const i32x4_f8*>(wp[i] + (size_t)b * 2048), *reinterpret_cast<const i32x4_f8*>(wp[i] + (size_t)b * 2048 + 1024));
 #pragma unroll
         for (int m = 0; m < MT; m++) {
-            x[m] = f8_join(*reinterpret_cast<const i32x4_f8*>(xp[m] + (at < a.k ? at : b * 128)),
-                           *reinterpret_cast<const i32x4_f8*>(xp[m] + (at + 64 < a.k ? at + 64 : b * 128)));
-            s[m] = sx[m][b * a.xs_group] * sw[b];
+            x[d][m] = f8_join(*reinterpret_cast<const i32x4_f8*>(xp[m] + lo), *reinterpret_cast<const i32x4_f8*>(xp[m] + hi));
+            s[d][m] = sx[m][b * a.xs_group];
         }
+    };
 #pragma unroll
-        for (int i = 0; i < NT; i++)
+    for (int d = 0; d < D - 1; d++) load(d, wave + d * NW);
+    for (int b0 = wave; b0 < kb; b0 += D * NW) {
+#pragma unroll
+        for (int d = 0; d < D; d++) {
+            load((d + D - 1) % D, b0 + (d + D - 1) * NW);
 #pragma unroll
             for (int m = 0; m < MT; m++) {
-                const f32x4_v p = f8_mfma(w[i], x[m]);
+                const float f = s[d][m] * swb[d];
 #pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][m][j] = fmaf(p[j], s[m], acc[i][m][j]);
+                for (int i = 0; i < NT; i++) {
+                    const f32x4_v p = f8_mfma(w[d][i], x[d][m]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) acc[i][m][j] = fmaf(p[j], f, acc[i][m][j]);
+                }
             }
+        }
     }
 #pragma unroll
     for (int i = 0; i < NT; i++)
@@ -77,21 +89,21 @@ __global__ void __launch_bounds__(NW * 64) dec_kernel(F8Mat a, int ntiles, bool 
     }
 }
 
-template <int MT, int NT, int NW, bool GROUPED>
+template <int MT, int NT, int NW, int D, bool GROUPED>
 void dec_t(const F8Mat& a, hipStream_t st) {
     const int ntiles = ((a.n + 15) / 16 + NT - 1) / NT;
     const int64_t jobs = GROUPED ? f8_most_jobs(a.r, a.experts, 16 * MT) : (a.r + 16 * MT - 1) / (16 * MT);
     CHECK(jobs * ntiles <= kF8MaxBlocks, "matmul_f8: %lld row blocks by %d column blocks are too many for a call", (long long)jobs, ntiles);
     const dim3 grid((unsigned)(jobs * ntiles)), block(NW * 64);
     const bool vec = f8_vec_ok(a.y, a.ldy);
-    if (a.out == kF8BF16) dec_kernel<MT, NT, NW, kF8BF16, GROUPED><<<grid, block, 0, st>>>(a, ntiles, vec);
-    else dec_kernel<MT, NT, NW, kF8F16, GROUPED><<<grid, block, 0, st>>>(a, ntiles, vec);
+    if (a.out == kF8BF16) dec_kernel<MT, NT, NW, D, kF8BF16, GROUPED><<<grid, block, 0, st>>>(a, ntiles, vec);
+    else dec_kernel<MT, NT, NW, D, kF8F16, GROUPED><<<grid, block, 0, st>>>(a, ntiles, vec);
     HIP_CHECK(hipGetLastError());
 }
 }  // namespace
 
 void f8_dec(const F8Mat& a, hipStream_t st) {
-    if (a.off) dec_t<1, 2, 8, true>(a, st);
-    else if (a.r <= 16) dec_t<1, 1, 8, false>(a, st);
-    else dec_t<2, 2, 8, false>(a, st);
+    if (a.off) dec_t<1, 2, 8, 2, true>(a, st);
+    else if (a.r <= 16) dec_t<1, 1, 8, 2, false>(a, st);
+    else dec_t<2, 2, 8, 2, false>(a, st);
 }

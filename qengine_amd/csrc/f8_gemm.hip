@@ -6,24 +6,12 @@
 // waves at the address unit (64 bytes a cycle: 1000 to 1500 cycles of a step), and the step's products waited behind them (256 x
 // 256 tiles: 4490 cycles a step with 2048 of products). Each MFMA of depth 128 starts from zero; its four sums are added
 // at sx sw in fp32 behind the next ones.
-#include "mfma_tile.hpp"
-#include "f8.hpp"
+#include "f8_tile.hpp"
 #include <type_traits>
 
 namespace {
-using qe_tile::dma16;
-using qe_tile::dma16_at;
-using qe_tile::dma4;
-
-// the same address in scalar registers, where a DMA takes its base from
-__device__ __forceinline__ const char* scalar(const char* p) {
-    const uint64_t v = reinterpret_cast<uint64_t>(p);
-    return reinterpret_cast<const char*>((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 |
-                                         (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v));
-}
-
 template <int BT, int BW, int WVT, int WVW, int OUT, bool GROUPED>
-__global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int ntt, int ntw, bool vec) {
+__global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Split sp, int ntt, int ntw, bool vec) {
     constexpr int NW = WVT * WVW, NTH = NW * 64, TT = BT / WVT / 16, WT = BW / WVW / 16;
     constexpr int kX = BT * 128, kW = BW * 128, kFirst = WVT * 2048, kS = BT * 4 + 256;  // bytes of a stage
     constexpr int oW = 2 * kX, oFirst = oW + 2 * kW, oS = oFirst + 3 * kFirst;
@@ -34,25 +22,23 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int nt
     const unsigned lds32 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)lds);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wt = wave / WVW, ww = wave % WVW, r = lane & 15, g = lane >> 4;
-    const int kb = (a.k + 127) >> 7, n16 = (a.n + 15) >> 4;
+    const int blocks = (a.k + 127) >> 7, n16 = (a.n + 15) >> 4;  // of 128 k
 
-    // block b runs on XCD b % 8; an XCD takes a run of tiles, in groups of 8 row tiles, so that those on it at a time
-    // share their rows and weights in its L2
-    const int ntiles = ntt * ntw, per = (ntiles + 7) >> 3, tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per || tile >= ntiles) return;
-    int tt, tw, e = 0, row0, rows;
+    int item, tt, tw, e = 0, row0, rows, z = 0;
+    if (!xcd_item(ntt * ntw * sp.parts, item)) return;
+    const int tile = GROUPED ? item : item % (ntt * ntw);
     if constexpr (GROUPED) {
         tt = tile / ntw;
         tw = tile % ntw;
         if (!f8_job<NTH>(a.off, a.experts, a.r, BT, tt, reinterpret_cast<int*>(lds), e, row0, rows)) return;
         __syncthreads();
     } else {
-        const int full = tile / (8 * ntw), left = min(8, ntt - full * 8), in = tile - full * 8 * ntw;
-        tt = full * 8 + in % left;
-        tw = in / left;
+        z = item / (ntt * ntw);
+        tile_place(tile, ntt, ntw, tt, tw);
         row0 = tt * BT;
         rows = min(BT, a.r - row0);
     }
+    const int from = GROUPED ? 0 : (int)((int64_t)blocks * z / sp.parts), kb = GROUPED ? blocks : (int)((int64_t)blocks * (z + 1) / sp.parts) - from;  // this range
     // row i of the tile (the last one again behind it) in x; an index outside x: row 0, and zeros in y
     auto x_row = [&](int i) -> int64_t {
         const int64_t row = row0 + min(i, rows - 1);
@@ -61,39 +47,41 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int nt
         return (unsigned)at < (unsigned)a.t ? at : 0;
     };
     // chunks behind k take the block's first: a row's own finite values times the weights' zeros there
-    const int chunk = (lane & 7) ^ (lane >> 3), last = chunk * 16 < a.k - (kb - 1) * 128 ? chunk * 16 : 0;
+    const int chunk = (lane & 7) ^ (lane >> 3), back = chunk * 16 < a.k - (blocks - 1) * 128 ? 0 : -chunk * 16;
     // one matrix: offsets from the tile's first row (rows are less than 2^24 bytes apart); grouped: addresses
-    const char* x0 = static_cast<const char*>(a.x) + (GROUPED ? 0 : (int64_t)row0 * a.ldx);
+    const char* x0 = static_cast<const char*>(a.x) + (GROUPED ? 0 : (int64_t)row0 * a.ldx) + (int64_t)from * 128;
     const char* xp[XD];
     uint32_t xi[XD];
 #pragma unroll
     for (int i = 0; i < XD; i++) {
         const int row = (wave * XD + i) * 8 + (lane >> 3);
-        if constexpr (GROUPED) xp[i] = x0 + x_row(row) * a.ldx;
-        else xi[i] = (uint32_t)min(row, rows - 1) * (uint32_t)a.ldx;
+        if constexpr (GROUPED) xp[i] = x0 + x_row(row) * a.ldx + chunk * 16;
+        else xi[i] = (uint32_t)min(row, rows - 1) * (uint32_t)a.ldx + chunk * 16;
     }
     // scales of the rows, 64 a wave, and of the tile's blocks of 128 weight rows, by the wave after them
-    const float* sp = a.xs + (wave < BT / 64 ? x_row(wave * 64 + lane) * a.xs_row : 0);
-    int64_t sp_next = a.xs_group;
+    const float* sc_at = a.xs + (wave < BT / 64 ? x_row(wave * 64 + lane) * a.xs_row : 0);
+    int64_t sc_next = a.xs_group;
     if (wave == BT / 64) {
-        sp = a.s + ((size_t)e * ((a.n + 127) >> 7) + min(tw * (BW / 128) + (lane & (BW / 128 - 1)), (a.n - 1) >> 7)) * kb;
-        sp_next = 1;
+        sc_at = a.s + ((size_t)e * ((a.n + 127) >> 7) + min(tw * (BW / 128) + (lane & (BW / 128 - 1)), (a.n - 1) >> 7)) * blocks;
+        sc_next = 1;
     }
     const int t16 = tw * (BW / 16) + ww * WT;  // the wave's first 16 weight rows
-    const char* const w0 = static_cast<const char*>(a.q) + (size_t)e * n16 * kb * 2048;
+    const char* const w0 = static_cast<const char*>(a.q) + ((size_t)e * n16 * blocks + from) * 2048;
     // DMAs of this wave, past the last block that block again (nobody reads it): 8 rows of x, block b, to LDS byte `to`
+    const int tail = blocks - 1 - from;  // the matrix's last block
     auto dma_x = [&](int i, int b, unsigned to) {
-        const int at = b >= kb - 1 ? last : chunk * 16;
         b = min(b, kb - 1);
+        const int at = b == tail ? back : 0;
         if constexpr (GROUPED) dma16(xp[i] + b * 128 + at, to);
         else dma16_at(scalar(x0 + b * 128), xi[i] + at, to);
     };
     auto dma_w = [&](int i, int b, unsigned to) {
         const int d = wave * WD + i;
-        dma16_at(scalar(w0 + ((size_t)min(tw * (BW / 16) + (d >> 1), n16 - 1) * kb + min(b, kb - 1)) * 2048 + (d & 1) * 1024), lane * 16, to + d * 1024);
+        dma16_at(scalar(w0 + ((size_t)min(tw * (BW / 16) + (d >> 1), n16 - 1) * blocks + min(b, kb - 1)) * 2048 + (d & 1) * 1024), lane * 16, to + d * 1024);
     };
+    sc_at += from * sc_next;
     auto dma_s = [&](int b, unsigned to) {
-        if (wave <= BT / 64) dma4(sp + min(b, kb - 1) * sp_next, to + wave * 256);
+        if (wave <= BT / 64) dma4(sc_at + min(b, kb - 1) * sc_next, to + wave * 256);
     };
     // the same for DMA number i of a wave's rows: their first 16 go to the ring for block `early`, the others to a stage
     auto dma_rows = [&](int i, int b, unsigned to, int early, unsigned ring) {
@@ -102,7 +90,7 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int nt
     };
 
     // The sums of product number p = t WT + i wait in a ring while the next three products are under way
-    constexpr int RING = 4, LAG = RING - 1, NP = TT * WT, EV = 2 * (WD + XD) < NP ? 2 : 1, RW = NP / (2 * WT);
+    constexpr int RING = 2, LAG = RING - 1, NP = TT * WT, EV = 2 * (WD + XD) < NP ? 2 : 1, RW = NP / (2 * WT);
     static_assert(NP % RING == 0 && TT > 2 && (TT - 2) * WT >= LAG, "a step begins at the ring's begin; scales outlast their sums");
     static_assert(WD + XD < NP && RW * 2 * WT == NP, "a step's DMAs and reads find a product");
     f32x4_v acc[WT][TT] = {}, part[RING] = {};
@@ -190,59 +178,65 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, int nt
     if (b < kb) step(b, std::integral_constant<int, 0>{});
 #pragma unroll
     for (int p = NP - LAG; p < NP; p++) flush(p);
-    // Rows of y through LDS, which the last barrier freed: a wave's 16 x 16 sums as they lie (8 bytes of 16 rows a store: 7 us for a tile
-    // of 256 x 256), read back as 16-byte pieces of whole rows, chunk c of row i at c ^ (i % C).
-    constexpr int C = WT * 2;  // 16-byte chunks of a wave's row
-    char* const out = lds + wave * TT * 16 * C * 16;
-    static_assert(NW * TT * 16 * C * 16 <= 2 * (kX + kW), "every wave's rows fit the stages");
-#pragma unroll
-    for (int t = 0; t < TT; t++)
-#pragma unroll
-        for (int i = 0; i < WT; i++) {
-            const f32x4_v v = acc[i][t];
-            *reinterpret_cast<uint2*>(out + ((t * 16 + r) * C + ((2 * i + (g >> 1)) ^ (r & (C - 1)))) * 16 + (g & 1) * 8) =
-                OUT == kF8BF16 ? uint2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])} : uint2{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
-        }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const int first = wt * TT * 16;  // row of the tile
-    uint16_t* const y = static_cast<uint16_t*>(a.y) + (int64_t)(row0 + first) * a.ldy + t16 * 16;
-    const int cols = a.n - t16 * 16;
-#pragma unroll 4
-    for (int j = 0; j < TT * C / 4; j++) {
-        const int at = j * 64 + lane, i = at / C, c = at % C;
-        uint4 v = *reinterpret_cast<const uint4*>(out + (i * C + (c ^ (i & (C - 1)))) * 16);
-        if (first + i >= rows || c * 8 >= cols) continue;
-        if (GROUPED && a.rows && (unsigned)a.rows[row0 + first + i] >= (unsigned)a.t) v = uint4{0, 0, 0, 0};
-        uint16_t* const to = y + i * a.ldy + c * 8;
-        if (vec && c * 8 + 8 <= cols) {
-            *reinterpret_cast<uint4*>(to) = v;
-        } else {
-            const uint32_t part4[4] = {v.x, v.y, v.z, v.w};
+    if (!GROUPED && sp.parts > 1) {
+        f32x4_v* const to = sp.sums + (((size_t)tile * sp.parts + z) * NW + wave) * NP * 64 + lane;
 #pragma unroll
-            for (int k = 0; k < 8; k++)
-                if (c * 8 + k < cols) to[k] = (uint16_t)(part4[k >> 1] >> (16 * (k & 1)));
-        }
+        for (int p = 0; p < NP; p++) to[p * 64] = acc[p % WT][p / WT];
+        return;
     }
+    // through the stages' LDS, which the last barrier freed
+    static_assert(NW * TT * 16 * WT * 32 <= 2 * (kX + kW), "every wave's rows fit the stages");
+    if (first < rows && t16 * 16 < a.n)
+        store_wave<TT, WT, OUT>(acc, lds + wave * TT * 16 * WT * 32, lane, static_cast<uint16_t*>(a.y) + (int64_t)(row0 + first) * a.ldy + t16 * 16,
+                                a.ldy, rows - first, a.n - t16 * 16, vec,
+                                [&](int i) { return GROUPED && a.rows && (unsigned)a.rows[row0 + first + i] >= (unsigned)a.t; });
 }
 
 template <int BT, int BW, int WVT, int WVW, bool GROUPED>
-void gemm_t(const F8Mat& a, hipStream_t st) {
+void gemm_t(const F8Mat& a, int parts, hipStream_t st) {
     constexpr int kLds = 2 * 128 * (BT + BW) + 3 * (WVT * 2048 + BT * 4 + 256);
     const int64_t ntt = GROUPED ? f8_most_jobs(a.r, a.experts, BT) : (a.r + BT - 1) / BT, ntw = (a.n + BW - 1) / BW;
     CHECK(ntt * ntw <= kF8MaxBlocks, "matmul_f8: %lld row tiles by %lld column tiles are too many for a call", (long long)ntt, (long long)ntw);
-    const dim3 grid((unsigned)((ntt * ntw + 7) / 8 * 8)), block(WVT * WVW * 64);
     const bool vec = a.ldy % 8 == 0 && ((uintptr_t)a.y & 15) == 0;
-    if (a.out == kF8BF16) gemm_kernel<BT, BW, WVT, WVW, kF8BF16, GROUPED><<<grid, block, kLds, st>>>(a, (int)ntt, (int)ntw, vec);
-    else gemm_kernel<BT, BW, WVT, WVW, kF8F16, GROUPED><<<grid, block, kLds, st>>>(a, (int)ntt, (int)ntw, vec);
+    auto run = [&](const F8Split& sp) {
+        const dim3 grid(xcd_blocks(ntt * ntw * sp.parts)), block(WVT * WVW * 64);
+        if (a.out == kF8BF16) gemm_kernel<BT, BW, WVT, WVW, kF8BF16, GROUPED><<<grid, block, kLds, st>>>(a, sp, (int)ntt, (int)ntw, vec);
+        else gemm_kernel<BT, BW, WVT, WVW, kF8F16, GROUPED><<<grid, block, kLds, st>>>(a, sp, (int)ntt, (int)ntw, vec);
+        HIP_CHECK(hipGetLastError());
+    };
+    if (GROUPED || parts < 2) return run({});
+    WsHold hold(st);
+    const F8Split sp = f8_split(hold, ntt * ntw, parts, BT, BW);
+    run(sp);
+    if (sp.parts < 2) return;
+    constexpr int QT = BT / WVT / 16 < 4 ? 1 : 2;
+    const dim3 grid((unsigned)(ntt * ntw * WVT * WVW * (BT / WVT / 16 / QT)));
+    if (a.out == kF8BF16) sum_kernel<BT, BW, WVT, WVW, QT, kF8BF16><<<grid, dim3(64), 0, st>>>(a, sp, (int)ntt, (int)ntw, vec);
+    else sum_kernel<BT, BW, WVT, WVW, QT, kF8F16><<<grid, dim3(64), 0, st>>>(a, sp, (int)ntt, (int)ntw, vec);
     HIP_CHECK(hipGetLastError());
+}
+
+// K ranges of tiles that do not fill the CUs: rounds of steps of 1.6 us, 6 us to start and end a tile, and the sums written and
+// read again
+int parts_of(const F8Mat& a, int bt, int bw) {
+    const int64_t tiles = (int64_t)((a.r + bt - 1) / bt) * ((a.n + bw - 1) / bw);
+    const int blocks = (a.k + 127) / 128, cus = qe_num_cus();
+    int best = 1;
+    double best_us = 1e30;
+    for (int p = 1; p <= 16 && p <= blocks && (p == 1 || tiles * p <= cus); p++) {
+        const double us = (double)((tiles * p + cus - 1) / cus) * (((blocks + p - 1) / p) * 1.6 + 6) + (p > 1 ? 4 + tiles * p * bt * bw * 8 / 4.0e6 : 0);
+        if (us < best_us) best_us = us, best = p;
+    }
+    return best;
 }
 }  // namespace
 
 void f8_gemm(const F8Mat& a, hipStream_t st) {
-    if (a.off) gemm_t<64, 128, 1, 4, true>(a, st);
-    else if (a.r <= 64) gemm_t<64, 128, 1, 4, false>(a, st);
-    else if (a.r <= 1024) gemm_t<128, 128, 2, 2, false>(a, st);
-    else gemm_t<256, 256, 2, 4, false>(a, st);
+    if (a.off) gemm_t<64, 128, 1, 4, true>(a, 1, st);
+    else if (a.r <= 64) gemm_t<64, 128, 1, 4, false>(a, 1, st);
+    else if (a.r <= 128) gemm_t<128, 128, 2, 2, false>(a, 1, st);
+    else gemm_t<256, 256, 2, 4, false>(a, parts_of(a, 256, 256), st);
 }
 
 void f8_matmul(const F8Mat& a, hipStream_t st) {

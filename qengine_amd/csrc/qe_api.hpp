@@ -104,7 +104,7 @@ void qe_config_set(const QeConfig& c);
 void gemv_w8(const W8& w, const uint16_t* x, int ldx, void* y, int ldy, int m, bool out_bf16, hipStream_t st);
 
 // ---- library-owned workspaces, one per (kind, device, stream) (workspace.cpp) ----
-enum WsKind : int { kWsSplit = 0, kWsI8 = 1, kWsH = 2, kWsDec = 3, kWsSkinny = 4, kWsAttn = 5, kNumWs = 6 };
+enum WsKind : int { kWsSplit = 0, kWsI8 = 1, kWsH = 2, kWsDec = 3, kWsSkinny = 4, kWsAttn = 5, kWsF8 = 6, kNumWs = 7 };
 struct StreamWs;
 // A call's hold on its stream's workspaces: made before the first buffer is asked for and kept until the last launch
 // that uses one, so that no other host thread's launches on the stream come in between.
@@ -116,7 +116,7 @@ class WsHold {
     WsHold& operator=(const WsHold&) = delete;
     // the buffer of (kind, current device, stream), at least `bytes`, grown on a call outside graph capture. During
     // capture: a buffer that the graph holds; nullptr for kWsSplit, kWsI8 and kWsH where the stream's own has not that
-    // size. nullptr too where the device has no memory for a kWsSplit, kWsDec, kWsSkinny or kWsAttn buffer. kWsDec buffers
+    // size. nullptr too where the device has no memory for a kWsSplit, kWsDec, kWsSkinny, kWsAttn or kWsF8 buffer. kWsDec buffers
     // (the one-pass decode's tail counters and sums) are zero-filled when allocated; the kernel leaves its counters zero.
     // retry: ask the device also shortly after it had no memory.
     void* get(int kind, size_t bytes, bool retry = false);

@@ -1,6 +1,6 @@
 // Library-owned workspaces of the prefill GEMMs (split-K partial sums, the W4A8 / W8A8 and fp16-accumulate
-// pre-pass buffers), of the one-pass decode's tail (counters and part sums), of the skinny kernel's slice sums and of the
-// attention over the cache (part sums), one buffer per (kind, device, stream).
+// pre-pass buffers), of the one-pass decode's tail (counters and part sums), of the skinny kernel's slice sums, of the
+// attention over the cache and of the 8-bit products (part sums), one buffer per (kind, device, stream).
 //
 // The reference keeps these buffers thread_local (src/kernels/gemm.cu:3258-3368), so two host threads never share
 // one. Here the key is the stream a call is enqueued on: calls on one stream run in order, so they can share a
@@ -16,7 +16,7 @@
 // which return to a pool, for later captures, when the last of these is destroyed. So the pool is as large as the graphs
 // that lived at one time needed. The pre-passes and the GEMM's split keep the rule that a capture needs its stream
 // sized first (an eager call or ws_reserve there): get returns nullptr else, and the caller runs without the buffer (the
-// split) or aborts with a message (the pre-passes). The decode and attention kernels' buffers need no preparation. They and the split
+// split) or aborts with a message (the pre-passes). The decode, attention and 8-bit kernels' buffers need no preparation. They and the split
 // also run without a buffer when the device has no memory left for it; a failed hipMalloc takes longer than the call,
 // so the next kRetry calls do not try again.
 #include <map>
