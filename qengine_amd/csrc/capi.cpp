@@ -459,6 +459,12 @@ void qe_matmul_f8(const void* q, const float* s, int n, int k, const void* x, in
     f8_matmul({q, s, x, xs, nullptr, nullptr, y, ldx, xs_row, xs_group, ldy, n, k, t, t, 1, f8_type(flags, 0, "qe_matmul_f8")}, as_stream(st));
 }
 
+void qe_matmul_f8_choice(const void* q, const float* s, int n, int k, const void* x, int64_t ldx, const float* xs, int64_t xs_row,
+                         int64_t xs_group, int t, void* y, int64_t ldy, int flags, int bt, int bw, int parts, void* st) {
+    f8_matmul_choice({q, s, x, xs, nullptr, nullptr, y, ldx, xs_row, xs_group, ldy, n, k, t, t, 1, f8_type(flags, 0, "qe_matmul_f8_choice")}, bt,
+                     bw, parts, as_stream(st));
+}
+
 void qe_matmul_f8_grouped(const void* q, const float* s, int n, int k, int experts, const void* x, int64_t ldx, const float* xs,
                           int64_t xs_row, int64_t xs_group, int t, const int32_t* off, const int32_t* rows, int r, void* y,
                           int64_t ldy, int flags, void* st) {

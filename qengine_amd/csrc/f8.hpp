@@ -56,6 +56,7 @@ constexpr int kF8MaxExperts = 1024;
 constexpr int kF8MaxCols = 65536;       // of a norm's row
 constexpr int kF8MaxDim = 1 << 20;      // n and k
 constexpr int kF8MaxRows = 1 << 24;     // of a call
+constexpr int kF8MaxRowBytes = 1 << 24;  // from a row of x to the next
 constexpr int64_t kF8MaxBlocks = 1 << 22;  // blocks of 512 threads: a launch takes less than 2^32 threads
 
 void f8_norm(const F8Norm& a, hipStream_t st);
@@ -63,8 +64,10 @@ void f8_act(const F8Act& a, hipStream_t st);
 void f8_combine(const F8Combine& a, hipStream_t st);
 void f8_tile(const void* src, int64_t ld, int64_t mat, int n, int k, int experts, void* dst, hipStream_t st);
 void f8_matmul(const F8Mat& a, hipStream_t st);
-void f8_dec(const F8Mat& a, hipStream_t st);   // few rows (of a segment)
-void f8_gemm(const F8Mat& a, hipStream_t st);  // many
+void f8_matmul_choice(const F8Mat& a, int bt, int bw, int parts, hipStream_t st);  // bt 16: f8_dec, 256: f8_gemm
+void f8_dec(const F8Mat& a, hipStream_t st);  // up to 16 rows, or segments of few
+void f8_ring(const F8Mat& a, int bt, int bw, int parts, hipStream_t st);  // blocks of bt rows x bw weight rows, K in ranges
+void f8_gemm(const F8Mat& a, int parts, hipStream_t st);                  // tiles of 256 x 256
 
 #ifdef __HIPCC__
 typedef int i32x4_f8 __attribute__((ext_vector_type(4)));
@@ -90,12 +93,13 @@ __device__ __forceinline__ void f8_store4(uint16_t* row, int c, int n, f32x4_v v
 }
 inline bool f8_vec_ok(const void* y, int64_t ldy) { return ldy % 4 == 0 && ((uintptr_t)y & 7) == 0; }
 
-// Segments of experts in blocks of BT rows: block number `job` -> expert, first row, rows of it. Every thread of the block
-// calls it; sh: NTH / 64 + 3 ints of LDS, free again after the next barrier. Entries of `off` are taken as
+// Segments of experts in blocks of bt rows, shared out evenly in `ways` runs: number `idx` of run `way` -> expert, first row, rows of
+// it, or false: there are not so many (a launch has blocks for the most there can be). Every thread of the block
+// calls it; sh: NTH / 64 + 4 ints of LDS, free again after the next barrier. Entries of `off` are taken as
 // rows in [0, r], segments that do not ascend as empty, so no answer names a row outside.
 template <int NTH>
-__device__ __forceinline__ bool f8_job(const int32_t* __restrict__ off, int experts, int r, int bt, int job, int* sh, int& e,
-                                       int& row0, int& rows) {
+__device__ __forceinline__ bool f8_job(const int32_t* __restrict__ off, int experts, int r, int bt, int way, int ways, int idx, int* sh,
+                                       int& e, int& row0, int& rows) {
     constexpr int NWV = NTH / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int per = (experts + NTH - 1) / NTH, first = tid * per;
@@ -115,8 +119,12 @@ __device__ __forceinline__ bool f8_job(const int32_t* __restrict__ off, int expe
     if (lane == 63) sh[wave] = sum;
     if (tid == 0) sh[NWV] = -1;
     __syncthreads();
-    int before = sum - mine;
-    for (int w = 0; w < wave; w++) before += sh[w];
+    int before = sum - mine, total = 0;
+    for (int w = 0; w < NWV; w++) {
+        if (w < wave) before += sh[w];
+        total += sh[w];
+    }
+    const int share = (total + ways - 1) / ways, job = idx < share ? way * share + idx : total;
     if (job >= before && job < before + mine) {
         int j = job - before;
         prev = at(first);
@@ -137,5 +145,5 @@ __device__ __forceinline__ bool f8_job(const int32_t* __restrict__ off, int expe
     rows = __builtin_amdgcn_readfirstlane(sh[NWV + 2]);
     return e >= 0;
 }
-inline int64_t f8_most_jobs(int64_t r, int64_t experts, int bt) { return r / bt + (r < experts ? r : experts); }
 #endif
+inline int64_t f8_most_jobs(int64_t r, int64_t experts, int bt) { return r / bt + (r < experts ? r : experts); }

@@ -13,7 +13,7 @@ __global__ void __launch_bounds__(NW * 64) dec_kernel(F8Mat a, int ntiles, bool 
     const int wt = blockIdx.x % ntiles, job = blockIdx.x / ntiles;
     int e = 0, row0 = job * 16 * MT, rows = min(16 * MT, a.r - row0);
     if constexpr (GROUPED) {
-        if (!f8_job<NW * 64>(a.off, a.experts, a.r, 16 * MT, job, reinterpret_cast<int*>(part), e, row0, rows)) return;
+        if (!f8_job<NW * 64>(a.off, a.experts, a.r, 16 * MT, 0, 1, job, reinterpret_cast<int*>(part), e, row0, rows)) return;
         __syncthreads();
     }
     const int n0 = wt * NT;  // first tile of 16 weight rows
@@ -102,8 +102,11 @@ void dec_t(const F8Mat& a, hipStream_t st) {
 }
 }  // namespace
 
+// us for 5120 x 17408 with one row: two tiles a block 17.1 (one: 18.3, four: 26.7), loads a step ahead 17.7; 34816 x 5120 with one
+// row 31 to 32 by any of these, with 16 rows 35.8 (four waves; eight: 38.9); 160 rows of 512 matrices of 1024 x 2048 43.5 (eight waves; four:
+// 44.6, four tiles: 45).
 void f8_dec(const F8Mat& a, hipStream_t st) {
-    if (a.off) dec_t<1, 2, 8, 2, true>(a, st);
-    else if (a.r <= 16) dec_t<1, 1, 8, 2, false>(a, st);
-    else dec_t<2, 2, 8, 2, false>(a, st);
+    if (a.off) dec_t<1, 2, 8, 1, true>(a, st);
+    else if (a.n >= 16384) dec_t<1, 2, 4, 1, false>(a, st);
+    else dec_t<1, 2, 8, 1, false>(a, st);
 }

@@ -10,7 +10,7 @@
 #include <type_traits>
 
 namespace {
-template <int BT, int BW, int WVT, int WVW, int OUT, bool GROUPED>
+template <int BT, int BW, int WVT, int WVW, int OUT>
 __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Split sp, int ntt, int ntw, bool vec) {
     constexpr int NW = WVT * WVW, NTH = NW * 64, TT = BT / WVT / 16, WT = BW / WVW / 16;
     constexpr int kX = BT * 128, kW = BW * 128, kFirst = WVT * 2048, kS = BT * 4 + 256;  // bytes of a stage
@@ -24,56 +24,34 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Spli
     const int wt = wave / WVW, ww = wave % WVW, r = lane & 15, g = lane >> 4;
     const int blocks = (a.k + 127) >> 7, n16 = (a.n + 15) >> 4;  // of 128 k
 
-    int item, tt, tw, e = 0, row0, rows, z = 0;
+    int item, tt, tw;
     if (!xcd_item(ntt * ntw * sp.parts, item)) return;
-    const int tile = GROUPED ? item : item % (ntt * ntw);
-    if constexpr (GROUPED) {
-        tt = tile / ntw;
-        tw = tile % ntw;
-        if (!f8_job<NTH>(a.off, a.experts, a.r, BT, tt, reinterpret_cast<int*>(lds), e, row0, rows)) return;
-        __syncthreads();
-    } else {
-        z = item / (ntt * ntw);
-        tile_place(tile, ntt, ntw, tt, tw);
-        row0 = tt * BT;
-        rows = min(BT, a.r - row0);
-    }
-    const int from = GROUPED ? 0 : (int)((int64_t)blocks * z / sp.parts), kb = GROUPED ? blocks : (int)((int64_t)blocks * (z + 1) / sp.parts) - from;  // this range
-    // row i of the tile (the last one again behind it) in x; an index outside x: row 0, and zeros in y
-    auto x_row = [&](int i) -> int64_t {
-        const int64_t row = row0 + min(i, rows - 1);
-        if (!GROUPED || !a.rows) return row;
-        const int at = a.rows[row];
-        return (unsigned)at < (unsigned)a.t ? at : 0;
-    };
+    const int z = item / (ntt * ntw);
+    tile_place(item % (ntt * ntw), ntt, ntw, tt, tw);
+    const int row0 = tt * BT, rows = min(BT, a.r - row0);
+    const int from = (int)((int64_t)blocks * z / sp.parts), kb = (int)((int64_t)blocks * (z + 1) / sp.parts) - from;  // this range
     // chunks behind k take the block's first: a row's own finite values times the weights' zeros there
     const int chunk = (lane & 7) ^ (lane >> 3), back = chunk * 16 < a.k - (blocks - 1) * 128 ? 0 : -chunk * 16;
-    // one matrix: offsets from the tile's first row (rows are less than 2^24 bytes apart); grouped: addresses
-    const char* x0 = static_cast<const char*>(a.x) + (GROUPED ? 0 : (int64_t)row0 * a.ldx) + (int64_t)from * 128;
-    const char* xp[XD];
+    // offsets from the tile's first row (rows are less than 2^24 bytes apart); behind the last row that one again
+    const char* const x0 = static_cast<const char*>(a.x) + (int64_t)row0 * a.ldx + (int64_t)from * 128;
     uint32_t xi[XD];
 #pragma unroll
-    for (int i = 0; i < XD; i++) {
-        const int row = (wave * XD + i) * 8 + (lane >> 3);
-        if constexpr (GROUPED) xp[i] = x0 + x_row(row) * a.ldx + chunk * 16;
-        else xi[i] = (uint32_t)min(row, rows - 1) * (uint32_t)a.ldx + chunk * 16;
-    }
+    for (int i = 0; i < XD; i++) xi[i] = (uint32_t)min((wave * XD + i) * 8 + (lane >> 3), rows - 1) * (uint32_t)a.ldx + chunk * 16;
     // scales of the rows, 64 a wave, and of the tile's blocks of 128 weight rows, by the wave after them
-    const float* sc_at = a.xs + (wave < BT / 64 ? x_row(wave * 64 + lane) * a.xs_row : 0);
+    const float* sc_at = a.xs + (wave < BT / 64 ? (row0 + min(wave * 64 + lane, rows - 1)) * a.xs_row : 0);
     int64_t sc_next = a.xs_group;
     if (wave == BT / 64) {
-        sc_at = a.s + ((size_t)e * ((a.n + 127) >> 7) + min(tw * (BW / 128) + (lane & (BW / 128 - 1)), (a.n - 1) >> 7)) * blocks;
+        sc_at = a.s + (size_t)min(tw * (BW / 128) + (lane & (BW / 128 - 1)), (a.n - 1) >> 7) * blocks;
         sc_next = 1;
     }
     const int t16 = tw * (BW / 16) + ww * WT;  // the wave's first 16 weight rows
-    const char* const w0 = static_cast<const char*>(a.q) + ((size_t)e * n16 * blocks + from) * 2048;
+    const char* const w0 = static_cast<const char*>(a.q) + (size_t)from * 2048;
     // DMAs of this wave, past the last block that block again (nobody reads it): 8 rows of x, block b, to LDS byte `to`
     const int tail = blocks - 1 - from;  // the matrix's last block
     auto dma_x = [&](int i, int b, unsigned to) {
         b = min(b, kb - 1);
         const int at = b == tail ? back : 0;
-        if constexpr (GROUPED) dma16(xp[i] + b * 128 + at, to);
-        else dma16_at(scalar(x0 + b * 128), xi[i] + at, to);
+        dma16_at(scalar(x0 + b * 128), xi[i] + at, to);
     };
     auto dma_w = [&](int i, int b, unsigned to) {
         const int d = wave * WD + i;
@@ -179,8 +157,8 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Spli
 #pragma unroll
     for (int p = NP - LAG; p < NP; p++) flush(p);
     const int first = wt * TT * 16;  // row of the tile
-    if (!GROUPED && sp.parts > 1) {
-        f32x4_v* const to = sp.sums + (((size_t)tile * sp.parts + z) * NW + wave) * NP * 64 + lane;
+    if (sp.parts > 1) {
+        f32x4_v* const to = sp.sums + ((((size_t)tt * ntw + tw) * sp.parts + z) * NW + wave) * NP * 64 + lane;
 #pragma unroll
         for (int p = 0; p < NP; p++) to[p * 64] = acc[p % WT][p / WT];
         return;
@@ -190,69 +168,33 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Spli
     if (first < rows && t16 * 16 < a.n)
         store_wave<TT, WT, OUT>(acc, lds + wave * TT * 16 * WT * 32, lane, static_cast<uint16_t*>(a.y) + (int64_t)(row0 + first) * a.ldy + t16 * 16,
                                 a.ldy, rows - first, a.n - t16 * 16, vec,
-                                [&](int i) { return GROUPED && a.rows && (unsigned)a.rows[row0 + first + i] >= (unsigned)a.t; });
+                                [](int) { return false; });
 }
 
-template <int BT, int BW, int WVT, int WVW, bool GROUPED>
+template <int BT, int BW, int WVT, int WVW>
 void gemm_t(const F8Mat& a, int parts, hipStream_t st) {
     constexpr int kLds = 2 * 128 * (BT + BW) + 3 * (WVT * 2048 + BT * 4 + 256);
-    const int64_t ntt = GROUPED ? f8_most_jobs(a.r, a.experts, BT) : (a.r + BT - 1) / BT, ntw = (a.n + BW - 1) / BW;
+    const int64_t ntt = (a.r + BT - 1) / BT, ntw = (a.n + BW - 1) / BW;
     CHECK(ntt * ntw <= kF8MaxBlocks, "matmul_f8: %lld row tiles by %lld column tiles are too many for a call", (long long)ntt, (long long)ntw);
     const bool vec = a.ldy % 8 == 0 && ((uintptr_t)a.y & 15) == 0;
     auto run = [&](const F8Split& sp) {
         const dim3 grid(xcd_blocks(ntt * ntw * sp.parts)), block(WVT * WVW * 64);
-        if (a.out == kF8BF16) gemm_kernel<BT, BW, WVT, WVW, kF8BF16, GROUPED><<<grid, block, kLds, st>>>(a, sp, (int)ntt, (int)ntw, vec);
-        else gemm_kernel<BT, BW, WVT, WVW, kF8F16, GROUPED><<<grid, block, kLds, st>>>(a, sp, (int)ntt, (int)ntw, vec);
+        if (a.out == kF8BF16) gemm_kernel<BT, BW, WVT, WVW, kF8BF16><<<grid, block, kLds, st>>>(a, sp, (int)ntt, (int)ntw, vec);
+        else gemm_kernel<BT, BW, WVT, WVW, kF8F16><<<grid, block, kLds, st>>>(a, sp, (int)ntt, (int)ntw, vec);
         HIP_CHECK(hipGetLastError());
     };
-    if (GROUPED || parts < 2) return run({});
+    if (parts < 2) return run({});
     WsHold hold(st);
     const F8Split sp = f8_split(hold, ntt * ntw, parts, BT, BW);
     run(sp);
     if (sp.parts < 2) return;
     constexpr int QT = BT / WVT / 16 < 4 ? 1 : 2;
     const dim3 grid((unsigned)(ntt * ntw * WVT * WVW * (BT / WVT / 16 / QT)));
-    if (a.out == kF8BF16) sum_kernel<BT, BW, WVT, WVW, QT, kF8BF16><<<grid, dim3(64), 0, st>>>(a, sp, (int)ntt, (int)ntw, vec);
-    else sum_kernel<BT, BW, WVT, WVW, QT, kF8F16><<<grid, dim3(64), 0, st>>>(a, sp, (int)ntt, (int)ntw, vec);
+    if (a.out == kF8BF16) sum_kernel<BT, BW, WVT, WVW, QT, kF8BF16><<<grid, dim3(64), 0, st>>>(a, sp, (int)ntw, vec);
+    else sum_kernel<BT, BW, WVT, WVW, QT, kF8F16><<<grid, dim3(64), 0, st>>>(a, sp, (int)ntw, vec);
     HIP_CHECK(hipGetLastError());
 }
 
-// K ranges of tiles that do not fill the CUs: rounds of steps of 1.6 us, 6 us to start and end a tile, and the sums written and
-// read again
-int parts_of(const F8Mat& a, int bt, int bw) {
-    const int64_t tiles = (int64_t)((a.r + bt - 1) / bt) * ((a.n + bw - 1) / bw);
-    const int blocks = (a.k + 127) / 128, cus = qe_num_cus();
-    int best = 1;
-    double best_us = 1e30;
-    for (int p = 1; p <= 16 && p <= blocks && (p == 1 || tiles * p <= cus); p++) {
-        const double us = (double)((tiles * p + cus - 1) / cus) * (((blocks + p - 1) / p) * 1.6 + 6) + (p > 1 ? 4 + tiles * p * bt * bw * 8 / 4.0e6 : 0);
-        if (us < best_us) best_us = us, best = p;
-    }
-    return best;
-}
 }  // namespace
 
-void f8_gemm(const F8Mat& a, hipStream_t st) {
-    if (a.off) gemm_t<64, 128, 1, 4, true>(a, 1, st);
-    else if (a.r <= 64) gemm_t<64, 128, 1, 4, false>(a, 1, st);
-    else if (a.r <= 128) gemm_t<128, 128, 2, 2, false>(a, 1, st);
-    else gemm_t<256, 256, 2, 4, false>(a, parts_of(a, 256, 256), st);
-}
-
-void f8_matmul(const F8Mat& a, hipStream_t st) {
-    CHECK(a.n > 0 && a.n <= kF8MaxDim && a.k > 0 && a.k <= kF8MaxDim && a.k % 16 == 0, "matmul_f8: n = %d, k = %d", a.n, a.k);
-    CHECK(a.r > 0 && a.r <= kF8MaxRows && a.t >= 0 && a.t <= kF8MaxRows && (a.off || a.t == a.r), "matmul_f8: %d rows of x, %d of y", a.t, a.r);
-    CHECK(a.experts > 0 && a.experts <= kF8MaxExperts && (a.off || (a.experts == 1 && !a.rows)), "matmul_f8: %d matrices", a.experts);
-    CHECK(a.q && a.s && a.y && (a.t == 0 || (a.x && a.xs)), "matmul_f8: a tensor is missing");
-    CHECK(((uintptr_t)a.q & 15) == 0 && ((uintptr_t)a.x & 15) == 0 && a.ldx % 16 == 0, "matmul_f8: x and its rows are 16-byte aligned");
-    F8Mat m = a;
-    if (a.t == 0) {  // every index is outside x: rows that are read and not used
-        m.x = a.q;
-        m.xs = a.s;
-        m.ldx = m.xs_row = 0;
-        m.xs_group = 1;
-    }
-    const bool few = a.off ? a.r <= (int64_t)a.experts * 8 : a.r <= 32;
-    if (few) f8_dec(m, st);
-    else f8_gemm(m, st);
-}
+void f8_gemm(const F8Mat& a, int parts, hipStream_t st) { gemm_t<256, 256, 2, 4>(a, parts, st); }

@@ -1,0 +1,76 @@
+// The 8-bit products' checks and the choice of their kernel (f8.hpp).
+#include "f8.hpp"
+
+#include <algorithm>
+
+namespace {
+struct Choice {
+    int bt = 0, bw = 0, parts = 1;  // bt 256: f8_gemm, else f8_ring
+    double us = 1e30;
+};
+
+// us of a product by rounds of blocks, one a CU (MI355X). A block of the ring takes its stages' bytes at 40 bytes/ns and 4 us to start
+// and end, one of the 256 x 256 tiles 1.6 us a step and 6 us; the weights come at 5.4 TB/s at most. K ranges cost a launch (4 us)
+// and the sums written and read again at 5 TB/s. Measured / modelled: 48 rows of 34816 x 5120: 192 columns a block 36 / 37, 128 48 / 53,
+// 64 44 / 53; of 5120 x 17408: 64 columns in 3 ranges 23 / 27, 128 in 6 23 / 26; 128 rows of 34816 x 5120: 41 / 45; 1000 rows of 5120 x
+// 17408, 256 x 256 in 3 ranges: 100 / 108.
+Choice choose(const F8Mat& a) {
+    const int cus = qe_num_cus(), blocks = (a.k + 127) / 128;
+    Choice best;
+    auto offer = [&](int bt, int bw) {
+        const int64_t tiles = (int64_t)((a.r + bt - 1) / bt) * ((a.n + bw - 1) / bw);
+        for (int p = 1; p <= 16 && p <= blocks && (p == 1 || tiles * p <= cus); p++) {
+            const double rounds = (double)((tiles * p + cus - 1) / cus), steps = (blocks + p - 1) / p;
+            double us = bt == 256 ? rounds * (steps * 1.6 + 6) : std::max(rounds * steps * (bt + bw) * 128 / 40e3, (double)a.n * a.k / 5.4e6) + 4;
+            if (p > 1) us += 4 + 2.0 * tiles * p * bt * bw * 4 / 5e6;
+            if (us < best.us) best = {bt, bw, p, us};
+        }
+    };
+    const int bt = a.r <= 32 ? 32 : a.r <= 64 ? 64 : 128;
+    for (int bw : {64, 128, 192}) offer(bt, bw);
+    if (a.r > 64) offer(256, 256);
+    return best;
+}
+}  // namespace
+
+static void check(const F8Mat& a) {
+    CHECK(a.n > 0 && a.n <= kF8MaxDim && a.k > 0 && a.k <= kF8MaxDim && a.k % 16 == 0, "matmul_f8: n = %d, k = %d", a.n, a.k);
+    CHECK(a.r > 0 && a.r <= kF8MaxRows && a.t >= 0 && a.t <= kF8MaxRows && (a.off || a.t == a.r), "matmul_f8: %d rows of x, %d of y", a.t, a.r);
+    CHECK(a.experts > 0 && a.experts <= kF8MaxExperts && (a.off || (a.experts == 1 && !a.rows)), "matmul_f8: %d matrices", a.experts);
+    CHECK((int64_t)a.r * a.n <= (int64_t)1 << 34, "matmul_f8: %d rows of %d are too many for a call", a.r, a.n);
+    CHECK(a.q && a.s && a.y && (a.t == 0 || (a.x && a.xs)), "matmul_f8: a tensor is missing");
+    CHECK(((uintptr_t)a.q & 15) == 0 && ((uintptr_t)a.x & 15) == 0 && a.ldx % 16 == 0 && a.ldx >= 0 && a.ldx < kF8MaxRowBytes,
+          "matmul_f8: x and its rows are 16-byte aligned, rows less than %d bytes apart", kF8MaxRowBytes);
+}
+
+void f8_matmul(const F8Mat& call, hipStream_t st) {
+    check(call);
+    F8Mat a = call;
+    if (a.t == 0) {  // every index is outside x: rows that are read and not used
+        a.x = a.q;
+        a.xs = a.s;
+        a.ldx = a.xs_row = 0;
+        a.xs_group = 1;
+    }
+    // Grouped: by the rows that a segment has on average. 512 matrices of 1024 x 2048: 160 rows 44 us by f8_dec; 40960 rows
+    // 263 (blocks of 128 rows), 269 (64), 333 (64 x 64).
+    if (a.off) {
+        const int64_t rows = a.r / a.experts;
+        if (rows < 8) return f8_dec(a, st);
+        return f8_ring(a, rows < 24 ? 32 : rows < 64 ? 64 : 128, 128, 1, st);
+    }
+    // 16 rows of 34816 x 5120 36 us by f8_dec, of 5120 x 17408 22
+    if (a.r <= 16) return f8_dec(a, st);
+    const Choice c = choose(a);
+    if (c.bt == 256) f8_gemm(a, c.parts, st);
+    else f8_ring(a, c.bt, c.bw, c.parts, st);
+}
+
+void f8_matmul_choice(const F8Mat& a, int bt, int bw, int parts, hipStream_t st) {
+    check(a);
+    CHECK(!a.off && parts >= 1 && parts <= 16 && parts <= (a.k + 127) / 128, "matmul_f8: %d K ranges of %d", parts, a.k);
+    if (bt == 16) return f8_dec(a, st);
+    if (bt == 256) return f8_gemm(a, parts, st);
+    CHECK((bt == 32 || bt == 64 || bt == 128) && (bw == 64 || bw == 128 || bw == 192), "matmul_f8: blocks of %d x %d", bt, bw);
+    f8_ring(a, bt, bw, parts, st);
+}

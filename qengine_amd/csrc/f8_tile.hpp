@@ -18,12 +18,14 @@ __device__ __forceinline__ const char* scalar(const char* p) {
 // K split (one matrix): a tile's 128-k blocks in `parts` ranges, whose sums go to memory as the lanes hold them and are added in
 // the order of the ranges by sum_kernel
 struct F8Split {
-    f32x4_v* sums = nullptr;  // [tile][range][wave][product][lane]
+    f32x4_v* sums = nullptr;  // [row tile][column tile][range][wave][product][lane]
     int parts = 1;
 };
 
 // Block b runs on XCD b % 8; an XCD takes a run of the items (tiles, or ranges outermost), so that those on it at a time share
-// rows and weights in its L2: tiles in groups of 8 row tiles, inside a group row tiles innermost.
+// rows and weights in its L2: tiles in groups of 8 row tiles, inside a group row tiles innermost. Grouped: a run of the segments' blocks
+// of rows, as many as there are (shared out by the most there can be, two XCDs of eight had nothing to do: 320 us for 40960
+// rows of 512 experts, 1024 x 2048).
 __device__ __forceinline__ bool xcd_item(int items, int& item) {
     const int per = (items + 7) >> 3;
     item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
@@ -41,22 +43,22 @@ inline unsigned xcd_blocks(int64_t items) { return (unsigned)((items + 7) / 8 * 
 // y: the wave's first row and column; rows, cols: how many of them there are; bad(i): row i is zeros
 template <int TT, int WT, int OUT, class Bad>
 __device__ __forceinline__ void store_wave(const f32x4_v (&acc)[WT][TT], char* out, int lane, uint16_t* y, int64_t ldy, int rows, int cols, bool vec, Bad bad) {
-    constexpr int C = WT * 2;  // 16-byte chunks of a row
+    constexpr int C = WT * 2, M = (C & (C - 1)) == 0 ? C - 1 : 0;  // 16-byte chunks of a row (six of them stay in order)
     const int r = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int t = 0; t < TT; t++)
 #pragma unroll
         for (int i = 0; i < WT; i++) {
             const f32x4_v v = acc[i][t];
-            *reinterpret_cast<uint2*>(out + ((t * 16 + r) * C + ((2 * i + (g >> 1)) ^ (r & (C - 1)))) * 16 + (g & 1) * 8) =
+            *reinterpret_cast<uint2*>(out + ((t * 16 + r) * C + ((2 * i + (g >> 1)) ^ (r & M))) * 16 + (g & 1) * 8) =
                 OUT == kF8BF16 ? uint2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])} : uint2{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
         }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll 4
     for (int j = 0; j < (TT * C + 3) / 4; j++) {
         const int at = j * 64 + lane, i = at / C, c = at % C;
-        if (i >= rows || c * 8 >= cols) continue;
-        uint4 v = *reinterpret_cast<const uint4*>(out + (i * C + (c ^ (i & (C - 1)))) * 16);
+        if (at >= TT * 16 * C || i >= rows || c * 8 >= cols) continue;
+        uint4 v = *reinterpret_cast<const uint4*>(out + (i * C + (c ^ (i & M))) * 16);
         if (bad(i)) v = uint4{0, 0, 0, 0};
         uint16_t* const to = y + i * ldy + c * 8;
         if (vec && c * 8 + 8 <= cols) {
@@ -72,12 +74,11 @@ __device__ __forceinline__ void store_wave(const f32x4_v (&acc)[WT][TT], char* o
 
 // the sums of a split tile's ranges: a wave takes QT of the TT x 16 rows of one wave of the tile
 template <int BT, int BW, int WVT, int WVW, int QT, int OUT>
-__global__ void __launch_bounds__(64) sum_kernel(F8Mat a, F8Split sp, int ntt, int ntw, bool vec) {
+__global__ void __launch_bounds__(64) sum_kernel(F8Mat a, F8Split sp, int ntw, bool vec) {
     constexpr int NW = WVT * WVW, TT = BT / WVT / 16, WT = BW / WVW / 16, Q = TT / QT;
     __shared__ __align__(16) char out[QT * 16 * WT * 32];
     const int lane = threadIdx.x, q = blockIdx.x % Q, wave = blockIdx.x / Q % NW, tile = blockIdx.x / Q / NW;
-    int tt, tw;
-    tile_place(tile, ntt, ntw, tt, tw);
+    const int tt = tile / ntw, tw = tile % ntw;
     const int first = tt * BT + wave / WVW * TT * 16 + q * QT * 16, col = tw * BW + wave % WVW * WT * 16;
     if (first >= a.r || col >= a.n) return;
     f32x4_v acc[WT][QT] = {};

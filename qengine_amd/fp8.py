@@ -31,11 +31,13 @@ MAX_DIM = 1 << 20
 MAX_ROWS = 1 << 24
 MAX_PARTS = 1 << 23
 MAX_STRIDE = 1 << 31
+MAX_VALUES = 1 << 34
+MAX_BLOCKS = 1 << 22
 _OUT = {torch.float32: 0, torch.bfloat16: OUT_BF16, torch.float16: F16}
 _IN = {torch.bfloat16: 0, torch.float16: F16}
 
 
-def _matrix(name, t, at, align=1):
+def _matrix(name, t, at, align=1, far=1 << 31):
     """[rows][columns] whose rows the kernels can read: strides and place; -> row stride"""
     if t.dim() != 2:
         raise ValueError(f"{name} has two dimensions, got shape {tuple(t.shape)}")
@@ -47,8 +49,8 @@ def _matrix(name, t, at, align=1):
         raise ValueError(f"{name}: a row's values lie together, got strides {t.stride()}")
     if rows < 2:
         return -(-cols // 16) * 16  # one row: its stride may be anything
-    if row < 0 or row >= MAX_STRIDE or row % align:
-        raise ValueError(f"{name}: rows are {align if align > 1 else 'up to 2^31'} elements apart or a multiple, got {row}")
+    if row >= far or row % align:
+        raise ValueError(f"{name}: rows are less than {far} elements apart, by a multiple of {align}, got {row}")
     return row
 
 
@@ -203,7 +205,7 @@ def _operands(w, q, s, experts):
     at = w.q.get_device()
     if experts != (w.s.dim() == 3):
         raise ValueError("one matrix for matmul_f8, [experts] of them for matmul_f8_grouped")
-    ldx = _matrix("q", q, at, 16)
+    ldx = _matrix("q", q, at, 16, 1 << 24)
     t = q.shape[0]
     if q.shape[1] != w.k or t > MAX_ROWS:
         raise ValueError(f"q is at most {MAX_ROWS} rows of {w.k}, got {tuple(q.shape)}")
@@ -214,12 +216,12 @@ def _operands(w, q, s, experts):
     return at, ldx, t
 
 
-def _product(w, r, dtype, y, at):
+def _product(w, r, dtype, y, at, blocks=0):
     dtype = dtype if y is None else y.dtype
     flags = _IN.get(dtype)
     if flags is None:
         raise TypeError(f"products are bfloat16 or float16, got {dtype}")
-    if r > MAX_ROWS or -(-r // 16) * -(-w.n // 16) > 1 << 28:
+    if r > MAX_ROWS or r * w.n > MAX_VALUES or blocks > MAX_BLOCKS:
         raise ValueError(f"{r} rows of {w.n} are too many for a call")
     if y is None:
         y = torch.empty(r, w.n, dtype=dtype, device=w.q.device)
@@ -238,6 +240,15 @@ def matmul_f8(w: F8, q, s, dtype=torch.bfloat16, y=None):
     return y
 
 
+def matmul_f8_choice(w: F8, q, s, bt, bw, parts, dtype=torch.bfloat16):
+    """matmul_f8 by a given kernel and number of K ranges instead of those that its sizes choose (qe_matmul_f8_choice)"""
+    at, ldx, t = _operands(w, q, s, False)
+    y, ldy, flags = _product(w, t, dtype, None, at)
+    _run(at, "qe_matmul_f8_choice", "ppiiplpllipliiiip", w.q.data_ptr(), w.s.data_ptr(), w.n, w.k, q.data_ptr(), ldx, s.data_ptr(), s.stride(0),
+         s.stride(1), t, y.data_ptr(), ldy, flags, bt, bw, parts)
+    return y
+
+
 def matmul_f8_grouped(w: F8, q, s, off, rows=None, dtype=torch.bfloat16, y=None):
     """Rows off[e] .. off[e + 1] - 1 of y (off int32 [experts + 1], ascending) = matrix e of w times the same rows of (q, s), or
     rows[i] of them for row i (rows int32; a number outside q gives a row of zeros). Rows of y in no segment are left as
@@ -248,7 +259,9 @@ def matmul_f8_grouped(w: F8, q, s, off, rows=None, dtype=torch.bfloat16, y=None)
     if rows is not None:
         _ints("rows", rows, (rows.numel(),), at)
         r = rows.numel()
-    y, ldy, flags = _product(w, r, dtype, y, at)
+    few = r // w.experts  # rows of a segment, as the library picks its blocks by them
+    rows_a_block, cols = (16, 32) if few < 8 else (32 if few < 24 else 64 if few < 64 else 128, 128)
+    y, ldy, flags = _product(w, r, dtype, y, at, (r // rows_a_block + min(r, w.experts)) * -(-w.n // cols))
     if r:
         _run(at, "qe_matmul_f8_grouped", "ppiiiplpllippiplip", w.q.data_ptr(), w.s.data_ptr(), w.n, w.k, w.experts, q.data_ptr(), ldx,
              s.data_ptr(), s.stride(0), s.stride(1), t, off.data_ptr(), None if rows is None else rows.data_ptr(), r, y.data_ptr(), ldy, flags)

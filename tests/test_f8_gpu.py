@@ -45,6 +45,26 @@ def test_whole_numbers(dev, t, n, k):
     assert torch.equal(ops.matmul_f8_grouped(w, x, xs, off, dtype=F16), want.to(F16))
 
 
+BLOCKS = [(16, 0)] + [(bt, bw) for bt in (32, 64, 128) for bw in (64, 128, 192)] + [(256, 256)]
+
+
+@pytest.mark.parametrize("parts", [1, 2, 3, 7])
+@pytest.mark.parametrize("bt,bw", BLOCKS)
+def test_blocks(dev, bt, bw, parts):
+    """every shape of a block and number of K ranges, whole and ragged tiles, K with a short block"""
+    for t, n, k in [(bt, bw or 64, 896), (bt + 1, 2 * bw + 130, 1040), (max(bt // 2 - 3, 1), 97, 912), (2 * bt + 9, 3 * bw + 16, 2000)]:
+        x, xs = ref.activations(dev, t, k, t + 1, 16)
+        q, s = ref.weights(dev, (n, k), n + k)
+        ref.check_product(ops.matmul_f8_choice(ops.tile_f8(q, s), x, xs, bt, bw, parts), x, xs, q, s, f"{t} x {n} x {k}")
+        g = ref.gen(dev, t)
+        x = torch.randint(-8, 9, (t, k), device=dev, generator=g).float().to(ref.F8)
+        q = torch.randint(-8, 9, (n, k), device=dev, generator=g).float().to(ref.F8)
+        xs = torch.exp2(torch.randint(-3, 1, (-(-k // 128), t), device=dev, generator=g).float()).t()
+        s = torch.exp2(torch.randint(-3, 1, (-(-n // 128), -(-k // 128)), device=dev, generator=g).float())
+        want = ref.product(x, xs, q, s)[0]
+        assert torch.equal(ops.matmul_f8_choice(ops.tile_f8(q, s), x, xs, bt, bw, parts, dtype=F16), want.to(F16)), f"{t} x {n} x {k}"
+
+
 # odd ends of both sides, one block, one column, deep sums
 @pytest.mark.parametrize("t", [1, 20, 50, 200, 1100])
 @pytest.mark.parametrize("n,k", [(1, 16), (1, 128), (15, 144), (16, 128), (17, 112), (127, 256), (129, 272), (130, 4096), (384, 2064), (1000, 528)])
@@ -59,7 +79,8 @@ def test_types(dev, t, dtype):
     linear(dev, t, 509, 640, dtype)
 
 
-@pytest.mark.parametrize("t,n,k", [(1, 5120, 17408), (48, 34816, 5120), (1000, 5120, 17408), (2100, 17408, 5120)])
+@pytest.mark.parametrize("t,n,k", [(1, 5120, 17408), (1, 34816, 5120), (24, 5120, 17408), (48, 34816, 5120), (100, 5120, 17408), (128, 34816, 5120),
+                                   (1000, 5120, 17408), (2100, 17408, 5120)])
 def test_large(dev, t, n, k):
     linear(dev, t, n, k, BF)
 
@@ -142,7 +163,7 @@ def test_grouped_types(dev, dtype):
     grouped(dev, [3, 0, 20, 100], 257, 384, dtype)
 
 
-@pytest.mark.parametrize("experts,tokens", [(512, 160), (512, 3000), (1024, 1024), (7, 5000)])
+@pytest.mark.parametrize("experts,tokens", [(512, 160), (512, 3000), (512, 7000), (1024, 1024), (60, 2000), (30, 2500), (7, 5000)])
 def test_grouped_many(dev, experts, tokens):
     g = torch.Generator().manual_seed(experts)
     lens = torch.bincount(torch.randint(experts, (tokens,), generator=g), minlength=experts).tolist()
