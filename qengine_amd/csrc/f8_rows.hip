@@ -112,29 +112,31 @@ __device__ __forceinline__ void quantize8(const float (&v)[8], uint8_t* q, int n
 }
 
 // ---------------------------------------------------------------- the norm
-// A block holds whole rows, one after another, in registers: NV chunks of 8 columns a thread. The mean is of the rounded
+// A block holds whole rows, one after another, in registers: NV chunks of 8 columns a thread, as many threads as that takes. The mean is of the rounded
 // h, what the residual stream holds. Squares of values past 2^63 leave fp32 in the sum: such a row is summed again with a
 // factor of 2^-80 (eps is nothing beside them), so every finite row has finite results.
-template <int T, int WT, int NTH, int NV, bool VEC>
-__global__ void __launch_bounds__(NTH) norm_kernel(F8Norm a) {
-    __shared__ float part[2][NTH / 64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+template <int T, int WT, int NV, bool VEC>
+__global__ void __launch_bounds__(1024) norm_kernel(F8Norm a) {
+    __shared__ float part[2][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, NTH = blockDim.x, waves = NTH >> 6;
     const int chunks = (a.d + 7) >> 3;
-    float w[NV][8];
+    constexpr bool KEEP = NV <= 2;  // the weights for all rows; of long rows they are read again
+    float w[KEEP ? NV : 1][8];
+    if constexpr (KEEP) {
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int c = tid + i * NTH;
-        if (c < chunks) get8<WT, VEC>(a.w, c * 8, a.d - c * 8, w[i]);
+        for (int i = 0; i < NV; i++) {
+            const int c = tid + i * NTH;
+            if (c < chunks) get8<WT, VEC>(a.w, c * 8, a.d - c * 8, w[i]);
+        }
     }
     auto block_sum = [&](float v, int slot) {
 #pragma unroll
         for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-        if constexpr (NTH > 64) {
+        if (waves > 1) {
             if (lane == 0) part[slot][wave] = v;
             __syncthreads();
             v = 0.f;
-#pragma unroll
-            for (int i = 0; i < NTH / 64; i++) v += part[slot][i];
+            for (int i = 0; i < waves; i++) v += part[slot][i];
         }
         return v;
     };
@@ -173,27 +175,26 @@ __global__ void __launch_bounds__(NTH) norm_kernel(F8Norm a) {
         for (int i = 0; i < NV; i++) {
             const int c = tid + i * NTH, n = a.d - c * 8;
             float y[8];
+            if (!KEEP && c < chunks) get8<WT, VEC>(a.w, c * 8, n, w[0]);
 #pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = c < chunks ? v[i][j] * f * rs * w[i][j] : 0.f;
+            for (int j = 0; j < 8; j++) y[j] = c < chunks ? v[i][j] * f * rs * w[KEEP ? i : 0][j] : 0.f;
             if (a.y && c < chunks) put8<T, VEC>(a.y, row * a.ldy + c * 8, n, y);
             if (a.q)
                 quantize8<VEC>(y, reinterpret_cast<uint8_t*>(a.q) + row * a.ldq + c * 8, n, a.s + row * a.s_row + (c >> 4) * a.s_group, lane);
         }
-        if constexpr (NTH > 64) __syncthreads();  // before `part` is written again
+        if (waves > 1) __syncthreads();  // before `part` is written again
     }
 }
 
 template <int T, int WT, bool VEC>
 void norm_t(const F8Norm& a, hipStream_t st) {
     const unsigned blocks = (unsigned)(a.t < (1 << 20) ? a.t : 1 << 20);
-#define QE_NORM(NTH_, NV_) norm_kernel<T, WT, NTH_, NV_, VEC><<<dim3(blocks), dim3(NTH_), 0, st>>>(a)
-    if (a.d <= 512) QE_NORM(64, 1);
-    else if (a.d <= 2048) QE_NORM(256, 1);
-    else if (a.d <= 4096) QE_NORM(256, 2);
-    else if (a.d <= 8192) QE_NORM(512, 2);
-    else if (a.d <= 16384) QE_NORM(1024, 2);
-    else if (a.d <= 32768) QE_NORM(1024, 4);
-    else QE_NORM(1024, 8);
+    const int chunks = (a.d + 7) / 8;
+#define QE_NORM(NV_) norm_kernel<T, WT, NV_, VEC><<<dim3(blocks), dim3((chunks + NV_ * 64 - 1) / (NV_ * 64) * 64), 0, st>>>(a)
+    if (chunks <= 1024) QE_NORM(1);
+    else if (chunks <= 2048) QE_NORM(2);
+    else if (chunks <= 4096) QE_NORM(4);
+    else QE_NORM(8);
 #undef QE_NORM
     HIP_CHECK(hipGetLastError());
 }
@@ -207,6 +208,15 @@ void norm_v(const F8Norm& a, hipStream_t st) {
 }
 
 // ---------------------------------------------------------------- quantized rows, silu(gate) * up
+// g / (1 + exp(-g)). exp(-g) = 2^t, t = -g log2 e, whose rounding (up to half a step of t, 60 steps of the result) is put back by its
+// remainder; from 2^126 on without it, so that infinity stays. exp2 and the reciprocal are the hardware's, one step off at most: with
+// the library's exp and an IEEE division 4096 x 17408 took 84 us, bound by the vector ALU.
+__device__ __forceinline__ float silu(float g) {
+    constexpr float L = 1.44269504088896340736f, Lo = 1.92596299112661746887e-08f, ln2 = 0.693147180559945309417f;
+    const float t = -g * L, rest = fmaf(-g, Lo, fmaf(-g, L, -t)) * ln2, e = __builtin_amdgcn_exp2f(t);
+    return g * __builtin_amdgcn_rcpf(1.f + (t < 126.f ? fmaf(e, rest, e) : e));
+}
+
 // LANES threads a row (a multiple of 16, a power of two), 8 columns each at a time
 template <int T, bool GLU, bool VEC>
 __global__ void __launch_bounds__(256) act_kernel(F8Act a, int shift, int blocks_a_row) {
@@ -221,7 +231,7 @@ __global__ void __launch_bounds__(256) act_kernel(F8Act a, int shift, int blocks
             float u[8];
             get8<T, VEC>(a.x, row * a.ldx + a.d + c * 8, n, u);
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = v[j] / (1.f + expf(-v[j])) * u[j];
+            for (int j = 0; j < 8; j++) v[j] = silu(v[j]) * u[j];
         }
     }
     quantize8<VEC>(v, reinterpret_cast<uint8_t*>(a.q) + row * a.ldq + c * 8, n, a.s + row * a.s_row + (c >> 4) * a.s_group, lane);
@@ -250,14 +260,24 @@ __global__ void __launch_bounds__(256) combine_kernel(F8Combine a, int shift, in
     if (n <= 0) return;
     float sum[8] = {};
     if (a.add) get8<OT, VEC>(a.add, row * a.ldadd + c * 8, n, sum);
-    for (int j = 0; j < a.topk; j++) {
-        const int from = a.inv[row * a.topk + j];
-        const float w = a.w[row * a.topk + j];
-        if ((unsigned)from >= (unsigned)a.rows) continue;
-        float v[8];
-        get8<T, VEC>(a.y, from * a.ldy + c * 8, n, v);
+    constexpr int AHEAD = 4;  // rows on their way
+    for (int j0 = 0; j0 < a.topk; j0 += AHEAD) {
+        float v[AHEAD][8], w[AHEAD];
+        bool has[AHEAD];
 #pragma unroll
-        for (int i = 0; i < 8; i++) sum[i] = fmaf(w, v[i], sum[i]);
+        for (int j = 0; j < AHEAD; j++) {
+            has[j] = j0 + j < a.topk;
+            const int from = has[j] ? a.inv[row * a.topk + j0 + j] : 0;
+            w[j] = has[j] ? a.w[row * a.topk + j0 + j] : 0.f;
+            has[j] = has[j] && (unsigned)from < (unsigned)a.rows;
+            if (has[j]) get8<T, VEC>(a.y, from * a.ldy + c * 8, n, v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; j++)
+            if (has[j]) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) sum[i] = fmaf(w[j], v[j][i], sum[i]);
+            }
     }
     put8<OT, VEC>(a.out, row * a.ldout + c * 8, n, sum);
 }

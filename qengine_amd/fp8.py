@@ -37,8 +37,12 @@ _OUT = {torch.float32: 0, torch.bfloat16: OUT_BF16, torch.float16: F16}
 _IN = {torch.bfloat16: 0, torch.float16: F16}
 
 
+# Decode loops call these wrappers for every layer and token: what is as it should be takes few reads of attributes.
 def _matrix(name, t, at, align=1, far=1 << 31):
     """[rows][columns] whose rows the kernels can read: strides and place; -> row stride"""
+    s = t.stride()
+    if len(s) == 2 and s[1] == 1 and 0 < s[0] < far and s[0] % align == 0 and t.get_device() == at:
+        return s[0]
     if t.dim() != 2:
         raise ValueError(f"{name} has two dimensions, got shape {tuple(t.shape)}")
     if t.get_device() != at:
@@ -55,6 +59,9 @@ def _matrix(name, t, at, align=1, far=1 << 31):
 
 
 def _written(name, t, shape, dtype, at):
+    s = t.stride()
+    if t.dtype is dtype and t.shape == shape and len(s) == 2 and s[1] == 1 and shape[1] <= s[0] < 1 << 31 and t.get_device() == at:
+        return s[0]
     if t.dtype is not dtype:
         raise TypeError(f"{name} is {dtype}, got {t.dtype}")
     if t.shape != shape:
@@ -87,8 +94,7 @@ def _rows_fit(t, d, what):
 def _quantized(t, d, device):
     """room for [t][d] in 8 bits, rows that the products can read, and its scales, group after group"""
     q = torch.empty(t, -(-d // 16) * 16, dtype=E4M3, device=device)
-    s = torch.empty(-(-d // 128), t, dtype=torch.float32, device=device)
-    return q if d % 16 == 0 else q[:, :d], s.t()
+    return q if d % 16 == 0 else q[:, :d], torch.empty_strided((t, -(-d // 128)), (1, t), dtype=torch.float32, device=device)
 
 
 @dataclass
