@@ -452,8 +452,8 @@ size_t qe_f8_bytes(int n, int k);
 
 /* y[t][n] = x[t][k] . W^T, bf16 or (QE_F16) fp16: sums of a block of 128 k by the matrix cores, then over the blocks in fp32 with
  * the product of the two scales, an fp32 number. (The matrix cores add products of 8 consecutive k to 13 bits below the largest
- * exponent among them, 1e-5 of a usual result, and the rest as fp32.) x: 16-byte aligned rows, ldx a multiple of 16 below 2^24.
- * t * n <= 2^34. Which kernel and K ranges a call takes goes by its sizes, so a row's last bits may depend on t. The ranges' sums
+ * exponent among them, 1e-5 of a usual result, and the rest as fp32.) x: 16-byte aligned rows, ldx a multiple of 16 below 2^24; xs_row
+ * below 2^22. t * n <= 2^34. Which kernel and K ranges a call takes goes by its sizes, so a row's last bits may depend on t. The ranges' sums
  * use the library's workspace of the stream (at most 64 MB, allocated by the first call that splits; a captured call's is its graph's). */
 void qe_matmul_f8(const void* q, const float* s, int n, int k, const void* x, int64_t ldx, const float* xs, int64_t xs_row,
                   int64_t xs_group, int t, void* y, int64_t ldy, int flags, void* stream);

@@ -57,6 +57,7 @@ constexpr int kF8MaxCols = 65536;       // of a norm's row
 constexpr int kF8MaxDim = 1 << 20;      // n and k
 constexpr int kF8MaxRows = 1 << 24;     // of a call
 constexpr int kF8MaxRowBytes = 1 << 24;  // from a row of x to the next
+constexpr int kF8MaxScaleStride = 1 << 22;  // elements from a row's scale to the next
 constexpr int64_t kF8MaxBlocks = 1 << 22;  // blocks of 512 threads: a launch takes less than 2^32 threads
 
 void f8_norm(const F8Norm& a, hipStream_t st);

@@ -37,29 +37,34 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Spli
     uint32_t xi[XD];
 #pragma unroll
     for (int i = 0; i < XD; i++) xi[i] = (uint32_t)min((wave * XD + i) * 8 + (lane >> 3), rows - 1) * (uint32_t)a.ldx + chunk * 16;
-    // scales of the rows, 64 a wave, and of the tile's blocks of 128 weight rows, by the wave after them
-    const float* sc_at = a.xs + (wave < BT / 64 ? (row0 + min(wave * 64 + lane, rows - 1)) * a.xs_row : 0);
-    int64_t sc_next = a.xs_group;
+    // scales of the rows, 64 a wave (less than 2^22 elements apart), and of the tile's blocks of 128 weight rows, by the wave after them
+    const char* s0p = reinterpret_cast<const char*>(a.xs + row0 * a.xs_row + from * a.xs_group);
+    int64_t s_next = a.xs_group * 4;
+    uint32_t si = (uint32_t)min(wave * 64 + lane, rows - 1) * (uint32_t)(a.xs_row * 4);
     if (wave == BT / 64) {
-        sc_at = a.s + (size_t)min(tw * (BW / 128) + (lane & (BW / 128 - 1)), (a.n - 1) >> 7) * blocks;
-        sc_next = 1;
+        s0p = reinterpret_cast<const char*>(a.s + from);
+        s_next = 4;
+        si = (uint32_t)min(tw * (BW / 128) + (lane & (BW / 128 - 1)), (a.n - 1) >> 7) * (uint32_t)(blocks * 4);
     }
     const int t16 = tw * (BW / 16) + ww * WT;  // the wave's first 16 weight rows
-    const char* const w0 = static_cast<const char*>(a.q) + (size_t)from * 2048;
+    const char* const w0 = static_cast<const char*>(a.q) + ((size_t)tw * (BW / 16) * blocks + from) * 2048;
     // DMAs of this wave, past the last block that block again (nobody reads it): 8 rows of x, block b, to LDS byte `to`
     const int tail = blocks - 1 - from;  // the matrix's last block
+    uint32_t wi[WD];                     // (uniform) bytes from the first tile's first block: n and k below 2^20 + 1, 16 tiles: below 2^32
+#pragma unroll
+    for (int i = 0; i < WD; i++) {
+        const int d = wave * WD + i;
+        wi[i] = (uint32_t)min(d >> 1, n16 - 1 - tw * (BW / 16)) * (uint32_t)(blocks * 2048) + (d & 1) * 1024;
+    }
     auto dma_x = [&](int i, int b, unsigned to) {
         b = min(b, kb - 1);
-        const int at = b == tail ? back : 0;
-        dma16_at(scalar(x0 + b * 128), xi[i] + at, to);
+        dma16_at(scalar(x0 + b * 128), xi[i] + (b == tail ? back : 0), to);
     };
     auto dma_w = [&](int i, int b, unsigned to) {
-        const int d = wave * WD + i;
-        dma16_at(scalar(w0 + ((size_t)min(tw * (BW / 16) + (d >> 1), n16 - 1) * blocks + min(b, kb - 1)) * 2048 + (d & 1) * 1024), lane * 16, to + d * 1024);
+        dma16_at(scalar(w0 + (size_t)min(b, kb - 1) * 2048 + wi[i]), lane * 16, to + (wave * WD + i) * 1024);
     };
-    sc_at += from * sc_next;
     auto dma_s = [&](int b, unsigned to) {
-        if (wave <= BT / 64) dma4(sc_at + min(b, kb - 1) * sc_next, to + wave * 256);
+        if (wave <= BT / 64) dma4_at(scalar(s0p + min(b, kb - 1) * s_next), si, to + wave * 256);
     };
     // the same for DMA number i of a wave's rows: their first 16 go to the ring for block `early`, the others to a stage
     auto dma_rows = [&](int i, int b, unsigned to, int early, unsigned ring) {
@@ -67,9 +72,10 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Spli
         dma_x(i, f < 2 ? early : b, f < 2 ? ring + (d / (2 * TT) * 2 + f) * 1024 : to + d * 1024);
     };
 
-    // The sums of product number p = t WT + i wait in a ring while the next three products are under way
-    constexpr int RING = 2, LAG = RING - 1, NP = TT * WT, EV = 2 * (WD + XD) < NP ? 2 : 1, RW = NP / (2 * WT);
-    static_assert(NP % RING == 0 && TT > 2 && (TT - 2) * WT >= LAG, "a step begins at the ring's begin; scales outlast their sums");
+    // The sums of product number p = t WT + i wait in a ring while the next two products are under way; the step before's last two
+    // are added before the first two of a step take their places
+    constexpr int RING = 3, LAG = RING - 1, NP = TT * WT, EV = 2 * (WD + XD) < NP ? 2 : 1, RW = NP / (2 * WT);
+    static_assert((NP - LAG) % RING == 0 && WT > LAG, "the last sums lie where the first ones go; scales outlast their sums");
     static_assert(WD + XD < NP && RW * 2 * WT == NP, "a step's DMAs and reads find a product");
     f32x4_v acc[WT][TT] = {}, part[RING] = {};
     i32x8_f8 w[2][WT];
@@ -133,8 +139,9 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Spli
 #pragma unroll
             for (int i = 0; i < WT; i++) {
                 const int p = t * WT + i;
+                if (p < LAG) flush(NP - LAG + p);
                 part[p % RING] = f8_mfma(w[cur][i], x[t & 1]);
-                flush((p + NP - LAG) % NP);
+                if (p >= LAG) flush(p - LAG);
                 const int j = p / EV;  // a DMA behind every product, or every second
                 if (p % EV == 0) {
                     if (j < WD) dma_w(j, b + 2, lds32 + oW + cur * kW);

@@ -41,6 +41,7 @@ static void check(const F8Mat& a) {
     CHECK(a.q && a.s && a.y && (a.t == 0 || (a.x && a.xs)), "matmul_f8: a tensor is missing");
     CHECK(((uintptr_t)a.q & 15) == 0 && ((uintptr_t)a.x & 15) == 0 && a.ldx % 16 == 0 && a.ldx >= 0 && a.ldx < kF8MaxRowBytes,
           "matmul_f8: x and its rows are 16-byte aligned, rows less than %d bytes apart", kF8MaxRowBytes);
+    CHECK(a.t < 2 || (a.xs_row >= 0 && a.xs_row < kF8MaxScaleStride), "matmul_f8: scales of rows are less than %d elements apart", kF8MaxScaleStride);
 }
 
 void f8_matmul(const F8Mat& call, hipStream_t st) {

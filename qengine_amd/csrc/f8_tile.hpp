@@ -7,6 +7,7 @@ namespace {
 using qe_tile::dma16;
 using qe_tile::dma16_at;
 using qe_tile::dma4;
+using qe_tile::dma4_at;
 
 // the same address in scalar registers, where a DMA takes its base from
 __device__ __forceinline__ const char* scalar(const char* p) {

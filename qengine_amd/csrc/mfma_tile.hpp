@@ -76,6 +76,10 @@ __device__ __forceinline__ void dma4(const void* src, unsigned lds_dst) {  // 4 
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_dst), "v"(src) : "memory", "m0");
 }
 
+__device__ __forceinline__ void dma4_at(const void* base, uint32_t offset, unsigned lds_dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_dst), "v"(offset), "s"(base) : "memory", "m0");
+}
+
 // Output of a wave's MFMA tiles held as C^T (lane l: token l % 32 of a 32-token tile, registers of 4 consecutive output
 // columns) through a wave-private LDS buffer: one 32-token tile at a time is written as it lies and read back as whole
 // rows, so that a store instruction writes NC ESZ contiguous bytes a token (64 to 256 B) instead of 8 to 32 B of each

@@ -102,6 +102,8 @@ PRODUCT = [
     (dict(q=z(4 * 272 + 1, dtype=F8)[1:].view(4, 272)), ValueError),
     (dict(s=z(4, 2, dtype=F32)), ValueError),
     (dict(s=z(3, 3, dtype=F32)), ValueError),
+    (dict(s=z((3 << 22) + 3, dtype=F32).as_strided((4, 3), (1 << 22, 1))), ValueError),
+    (dict(q=z(4 << 24, dtype=F8).as_strided((4, 272), (1 << 24, 1))), ValueError),
     (dict(dtype=F32), TypeError),
     (dict(y=z(4, 160, dtype=F32)), TypeError),
     (dict(y=z(4, 161)), ValueError),
