@@ -69,6 +69,7 @@ void f8_matmul_choice(const F8Mat& a, int bt, int bw, int parts, hipStream_t st)
 void f8_dec(const F8Mat& a, hipStream_t st);  // up to 16 rows, or segments of few
 void f8_ring(const F8Mat& a, int bt, int bw, int parts, hipStream_t st);  // blocks of bt rows x bw weight rows, K in ranges
 void f8_gemm(const F8Mat& a, int parts, hipStream_t st);                  // tiles of 256 x 256
+bool f8_gemm_takes(const F8Mat& a);
 
 #ifdef __HIPCC__
 typedef int i32x4_f8 __attribute__((ext_vector_type(4)));

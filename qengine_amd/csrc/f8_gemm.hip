@@ -10,7 +10,7 @@
 #include <type_traits>
 
 namespace {
-template <int BT, int BW, int WVT, int WVW, int OUT>
+template <int BT, int BW, int WVT, int WVW, int OUT, bool GROUPED>
 __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Split sp, int ntt, int ntw, bool vec) {
     constexpr int NW = WVT * WVW, NTH = NW * 64, TT = BT / WVT / 16, WT = BW / WVW / 16;
     constexpr int kX = BT * 128, kW = BW * 128, kFirst = WVT * 2048, kS = BT * 4 + 256;  // bytes of a stage
@@ -24,30 +24,47 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Spli
     const int wt = wave / WVW, ww = wave % WVW, r = lane & 15, g = lane >> 4;
     const int blocks = (a.k + 127) >> 7, n16 = (a.n + 15) >> 4;  // of 128 k
 
-    int item, tt, tw;
-    if (!xcd_item(ntt * ntw * sp.parts, item)) return;
-    const int z = item / (ntt * ntw);
-    tile_place(item % (ntt * ntw), ntt, ntw, tt, tw);
-    const int row0 = tt * BT, rows = min(BT, a.r - row0);
+    int item, tt = 0, tw, e = 0, row0, rows, z = 0;
+    if constexpr (GROUPED) {
+        const int idx = blockIdx.x >> 3;
+        tw = idx % ntw;
+        if (!f8_job<NTH>(a.off, a.experts, a.r, BT, blockIdx.x & 7, 8, idx / ntw, reinterpret_cast<int*>(lds), e, row0, rows)) return;
+        __syncthreads();
+    } else {
+        if (!xcd_item(ntt * ntw * sp.parts, item)) return;
+        z = item / (ntt * ntw);
+        tile_place(item % (ntt * ntw), ntt, ntw, tt, tw);
+        row0 = tt * BT;
+        rows = min(BT, a.r - row0);
+    }
     const int from = (int)((int64_t)blocks * z / sp.parts), kb = (int)((int64_t)blocks * (z + 1) / sp.parts) - from;  // this range
     // chunks behind k take the block's first: a row's own finite values times the weights' zeros there
     const int chunk = (lane & 7) ^ (lane >> 3), back = chunk * 16 < a.k - (blocks - 1) * 128 ? 0 : -chunk * 16;
-    // offsets from the tile's first row (rows are less than 2^24 bytes apart); behind the last row that one again
-    const char* const x0 = static_cast<const char*>(a.x) + (int64_t)row0 * a.ldx + (int64_t)from * 128;
+    // Rows of x by 32-bit offsets, from the tile's first (rows are less than 2^24 bytes apart, their scales less than 2^22 elements), or by
+    // index from the first of all (x and its scales are then less than 2^32 bytes). Behind the last row that one again.
+    const bool by_index = GROUPED && a.rows;
+    auto x_row = [&](int i) -> uint32_t {
+        i = min(i, rows - 1);
+        if (!by_index) return i;
+        const uint32_t at = a.rows[row0 + i];
+        return at < (uint32_t)a.t ? at : 0;  // an index outside x: row 0, and zeros in y
+    };
+    const int64_t x_first = by_index ? 0 : row0;
+    const char* const x0 = static_cast<const char*>(a.x) + x_first * a.ldx + (int64_t)from * 128;
     uint32_t xi[XD];
 #pragma unroll
-    for (int i = 0; i < XD; i++) xi[i] = (uint32_t)min((wave * XD + i) * 8 + (lane >> 3), rows - 1) * (uint32_t)a.ldx + chunk * 16;
-    // scales of the rows, 64 a wave (less than 2^22 elements apart), and of the tile's blocks of 128 weight rows, by the wave after them
-    const char* s0p = reinterpret_cast<const char*>(a.xs + row0 * a.xs_row + from * a.xs_group);
+    for (int i = 0; i < XD; i++) xi[i] = x_row((wave * XD + i) * 8 + (lane >> 3)) * (uint32_t)a.ldx + chunk * 16;
+    // scales of the rows, 64 a wave, and of the tile's blocks of 128 weight rows, by the wave after them
+    const char* s0p = reinterpret_cast<const char*>(a.xs + x_first * a.xs_row + from * a.xs_group);
     int64_t s_next = a.xs_group * 4;
-    uint32_t si = (uint32_t)min(wave * 64 + lane, rows - 1) * (uint32_t)(a.xs_row * 4);
+    uint32_t si = wave < BT / 64 ? x_row(wave * 64 + lane) * (uint32_t)(a.xs_row * 4) : 0;
     if (wave == BT / 64) {
-        s0p = reinterpret_cast<const char*>(a.s + from);
+        s0p = reinterpret_cast<const char*>(a.s + (size_t)e * ((a.n + 127) >> 7) * blocks + from);
         s_next = 4;
         si = (uint32_t)min(tw * (BW / 128) + (lane & (BW / 128 - 1)), (a.n - 1) >> 7) * (uint32_t)(blocks * 4);
     }
     const int t16 = tw * (BW / 16) + ww * WT;  // the wave's first 16 weight rows
-    const char* const w0 = static_cast<const char*>(a.q) + ((size_t)tw * (BW / 16) * blocks + from) * 2048;
+    const char* const w0 = static_cast<const char*>(a.q) + (((size_t)e * n16 + tw * (BW / 16)) * blocks + from) * 2048;
     // DMAs of this wave, past the last block that block again (nobody reads it): 8 rows of x, block b, to LDS byte `to`
     const int tail = blocks - 1 - from;  // the matrix's last block
     uint32_t wi[WD];                     // (uniform) bytes from the first tile's first block: n and k below 2^20 + 1, 16 tiles: below 2^32
@@ -164,7 +181,7 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Spli
 #pragma unroll
     for (int p = NP - LAG; p < NP; p++) flush(p);
     const int first = wt * TT * 16;  // row of the tile
-    if (sp.parts > 1) {
+    if (!GROUPED && sp.parts > 1) {
         f32x4_v* const to = sp.sums + ((((size_t)tt * ntw + tw) * sp.parts + z) * NW + wave) * NP * 64 + lane;
 #pragma unroll
         for (int p = 0; p < NP; p++) to[p * 64] = acc[p % WT][p / WT];
@@ -175,33 +192,42 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Spli
     if (first < rows && t16 * 16 < a.n)
         store_wave<TT, WT, OUT>(acc, lds + wave * TT * 16 * WT * 32, lane, static_cast<uint16_t*>(a.y) + (int64_t)(row0 + first) * a.ldy + t16 * 16,
                                 a.ldy, rows - first, a.n - t16 * 16, vec,
-                                [](int) { return false; });
+                                [&](int i) { return by_index && (unsigned)a.rows[row0 + first + i] >= (unsigned)a.t; });
 }
 
-template <int BT, int BW, int WVT, int WVW>
+template <int BT, int BW, int WVT, int WVW, bool GROUPED>
 void gemm_t(const F8Mat& a, int parts, hipStream_t st) {
     constexpr int kLds = 2 * 128 * (BT + BW) + 3 * (WVT * 2048 + BT * 4 + 256);
-    const int64_t ntt = (a.r + BT - 1) / BT, ntw = (a.n + BW - 1) / BW;
+    const int64_t ntt = GROUPED ? f8_most_jobs(a.r, a.experts, BT) : (a.r + BT - 1) / BT, ntw = (a.n + BW - 1) / BW;
     CHECK(ntt * ntw <= kF8MaxBlocks, "matmul_f8: %lld row tiles by %lld column tiles are too many for a call", (long long)ntt, (long long)ntw);
     const bool vec = a.ldy % 8 == 0 && ((uintptr_t)a.y & 15) == 0;
     auto run = [&](const F8Split& sp) {
-        const dim3 grid(xcd_blocks(ntt * ntw * sp.parts)), block(WVT * WVW * 64);
-        if (a.out == kF8BF16) gemm_kernel<BT, BW, WVT, WVW, kF8BF16><<<grid, block, kLds, st>>>(a, sp, (int)ntt, (int)ntw, vec);
-        else gemm_kernel<BT, BW, WVT, WVW, kF8F16><<<grid, block, kLds, st>>>(a, sp, (int)ntt, (int)ntw, vec);
+        const dim3 grid(GROUPED ? xcd_blocks(ntt) * (unsigned)ntw : xcd_blocks(ntt * ntw * sp.parts)), block(WVT * WVW * 64);
+        if (a.out == kF8BF16) gemm_kernel<BT, BW, WVT, WVW, kF8BF16, GROUPED><<<grid, block, kLds, st>>>(a, sp, (int)ntt, (int)ntw, vec);
+        else gemm_kernel<BT, BW, WVT, WVW, kF8F16, GROUPED><<<grid, block, kLds, st>>>(a, sp, (int)ntt, (int)ntw, vec);
         HIP_CHECK(hipGetLastError());
     };
-    if (parts < 2) return run({});
-    WsHold hold(st);
-    const F8Split sp = f8_split(hold, ntt * ntw, parts, BT, BW);
-    run(sp);
-    if (sp.parts < 2) return;
-    constexpr int QT = BT / WVT / 16 < 4 ? 1 : 2;
-    const dim3 grid((unsigned)(ntt * ntw * WVT * WVW * (BT / WVT / 16 / QT)));
-    if (a.out == kF8BF16) sum_kernel<BT, BW, WVT, WVW, QT, kF8BF16><<<grid, dim3(64), 0, st>>>(a, sp, (int)ntw, vec);
-    else sum_kernel<BT, BW, WVT, WVW, QT, kF8F16><<<grid, dim3(64), 0, st>>>(a, sp, (int)ntw, vec);
-    HIP_CHECK(hipGetLastError());
+    if constexpr (GROUPED) {
+        run({});
+    } else {
+        if (parts < 2) return run({});
+        WsHold hold(st);
+        const F8Split sp = f8_split(hold, ntt * ntw, parts, BT, BW);
+        run(sp);
+        if (sp.parts < 2) return;
+        constexpr int QT = 2;  // of a wave's eight 16-row tiles a block of the sum takes two: 12 us for 80 tiles in 3 ranges
+        const dim3 grid((unsigned)(ntt * ntw * WVT * WVW * (BT / WVT / 16 / QT)));
+        if (a.out == kF8BF16) sum_kernel<BT, BW, WVT, WVW, QT, kF8BF16><<<grid, dim3(64), 0, st>>>(a, sp, (int)ntw, vec);
+        else sum_kernel<BT, BW, WVT, WVW, QT, kF8F16><<<grid, dim3(64), 0, st>>>(a, sp, (int)ntw, vec);
+        HIP_CHECK(hipGetLastError());
+    }
 }
-
 }  // namespace
 
-void f8_gemm(const F8Mat& a, int parts, hipStream_t st) { gemm_t<256, 256, 2, 4>(a, parts, st); }
+bool f8_gemm_takes(const F8Mat& a) {  // rows by index: 32-bit offsets
+    return !a.rows || ((int64_t)a.t * a.ldx < (int64_t)1 << 32 && (int64_t)a.t * a.xs_row * 4 < (int64_t)1 << 32);
+}
+void f8_gemm(const F8Mat& a, int parts, hipStream_t st) {
+    if (a.off) gemm_t<256, 256, 2, 4, true>(a, 1, st);
+    else gemm_t<256, 256, 2, 4, false>(a, parts, st);
+}

@@ -31,6 +31,18 @@ Choice choose(const F8Mat& a) {
     if (a.r > 64) offer(256, 256);
     return best;
 }
+
+// Grouped: segments of ragged lengths end in a block that is half empty on average, and have one at least. A block's step of 128 k takes 0.46 us a CU (64 x
+// 128), 0.8 (128 x 128) or 1.6 (256 x 256, and 14 us to start and end). Measured, 512 matrices of 1024 x 2048, us with blocks of 64 / 128 rows
+// (they read the weights in 200): 4096 rows 181 / 226, 20480 211 / 240, 40960 258 / 262, 81920 386 / 375, 163840 644 / 613.
+int choose_grouped(const F8Mat& a) {
+    if (a.r / a.experts < 8) return 16;
+    const double steps = (a.k + 127) / 128, cus = qe_num_cus();
+    auto us = [&](int bt, int bw, double step) { return std::max(a.r / (double)bt + a.experts * 0.5, (double)a.experts) * ((a.n + bw - 1) / bw) * steps / cus * step; };
+    const double u64 = us(64, 128, 0.46), u128 = us(128, 128, 0.8), u256 = us(256, 256, 1.6 + 14 / steps);
+    if (f8_gemm_takes(a) && u256 < u64 && u256 < u128) return 256;
+    return u64 <= u128 ? 64 : 128;
+}
 }  // namespace
 
 static void check(const F8Mat& a) {
@@ -53,12 +65,12 @@ void f8_matmul(const F8Mat& call, hipStream_t st) {
         a.ldx = a.xs_row = 0;
         a.xs_group = 1;
     }
-    // Grouped: by the rows that a segment has on average. 512 matrices of 1024 x 2048: 160 rows 44 us by f8_dec; 40960 rows
-    // 263 (blocks of 128 rows), 269 (64), 333 (64 x 64).
     if (a.off) {
-        const int64_t rows = a.r / a.experts;
-        if (rows < 8) return f8_dec(a, st);
-        return f8_ring(a, rows < 24 ? 32 : rows < 64 ? 64 : 128, 128, 1, st);
+        const int bt = choose_grouped(a);
+        if (bt == 16) f8_dec(a, st);
+        else if (bt == 256) f8_gemm(a, 1, st);
+        else f8_ring(a, bt, 128, 1, st);
+        return;
     }
     // 16 rows of 34816 x 5120 36 us by f8_dec, of 5120 x 17408 22
     if (a.r <= 16) return f8_dec(a, st);

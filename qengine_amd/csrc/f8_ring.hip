@@ -185,8 +185,7 @@ void ring_t(const F8Mat& a, int parts, hipStream_t st) {
 // Stages: three keep a block fed (four or six took the same time or longer); two where a third would leave one block a CU.
 void f8_ring(const F8Mat& a, int bt, int bw, int parts, hipStream_t st) {
     if (a.off) {
-        if (bt == 32) ring_t<32, 128, 3, true>(a, 1, st);
-        else if (bt == 64) ring_t<64, 128, 3, true>(a, 1, st);
+        if (bt == 64) ring_t<64, 128, 3, true>(a, 1, st);
         else ring_t<128, 128, 2, true>(a, 1, st);
     } else if (bt == 32) {
         if (bw == 64) ring_t<32, 64, 4, false>(a, parts, st);

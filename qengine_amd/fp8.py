@@ -266,8 +266,7 @@ def matmul_f8_grouped(w: F8, q, s, off, rows=None, dtype=torch.bfloat16, y=None)
     if rows is not None:
         _ints("rows", rows, (rows.numel(),), at)
         r = rows.numel()
-    few = r // w.experts  # rows of a segment, as the library picks its blocks by them
-    rows_a_block, cols = (16, 32) if few < 8 else (32 if few < 24 else 64 if few < 64 else 128, 128)
+    rows_a_block, cols = (16, 32) if r // w.experts < 8 else (64, 128)  # the smallest blocks that the library may take
     y, ldy, flags = _product(w, r, dtype, y, at, (r // rows_a_block + min(r, w.experts)) * -(-w.n // cols))
     if r:
         _run(at, "qe_matmul_f8_grouped", "ppiiiplpllippiplip", w.q.data_ptr(), w.s.data_ptr(), w.n, w.k, w.experts, q.data_ptr(), ldx,

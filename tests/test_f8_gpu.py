@@ -148,7 +148,7 @@ def grouped(dev, lens, n, k, dtype=F16, gather=None, first=0, tail=0, seed=0):
             ref.check_product(y[c[i]:c[i + 1]], x.view(torch.uint8)[at].view(ref.F8), xs[at], q[i], s[i], f"segment {i} of {lens[i]}")
 
 
-LENS = [[1], [0, 3, 0], [16, 17, 1, 15, 0, 33], [64, 65, 128, 129, 0, 200], [0] * 30 + [5] + [0] * 33, [300], [40] * 20, [0, 0]]
+LENS = [[1], [0, 3, 0], [700, 0, 513, 256], [16, 17, 1, 15, 0, 33], [64, 65, 128, 129, 0, 200], [0] * 30 + [5] + [0] * 33, [300], [40] * 20, [0, 0]]
 
 
 @pytest.mark.parametrize("lens", LENS, ids=lambda v: str(v)[:24])
