@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Spli
 #pragma unroll
     for (int i = 0; i < XD; i++) {
         dma_rows(i, 0, lds32, 0, lds32 + oFirst);
-        dma_rows(i, 0, lds32, 1, lds32 + oFirst + kFirst);
+        if ((wave * XD + i) % (2 * TT) < 2) dma_rows(i, 0, 0, 1, lds32 + oFirst + kFirst);
     }
 #pragma unroll
     for (int i = 0; i < WD; i++) {

@@ -1,9 +1,11 @@
 """Products of 8-bit weights and activations against their formula in 64 bits (bounds: f8_ref.py)."""
+import threading
+
 import pytest
 import torch
 
 import f8_ref as ref
-from qengine_amd import ops
+from qengine_amd import call, ops
 
 pytestmark = pytest.mark.gpu
 BF, F16 = torch.bfloat16, torch.float16
@@ -295,6 +297,61 @@ def test_captured(dev, t):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(hs, h2)
+
+
+def test_graphs_have_their_own_sums(dev):
+    """products whose K is split use sums that their graph holds: two graphs of one stream replay beside each other and eager calls"""
+    t, n, k = 300, 512, 8192
+    q, s = ref.weights(dev, (n, k), 1)
+    w = ops.tile_f8(q, s)
+    ins = [ref.activations(dev, t, k, i) for i in range(3)]
+    want = [ops.matmul_f8(w, *i) for i in ins]
+    assert call("qe_workspace_count", 6) >= 1
+    side = torch.cuda.Stream()
+    before = call("qe_workspace_count", 6)
+    graphs, outs = [], []
+    for i in ins[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(ops.matmul_f8(w, *i))
+        graphs.append(graph)
+    assert call("qe_workspace_count", 6) == before + 2
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(8):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for st, graph in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                graph.replay()
+        eager = ops.matmul_f8(w, *ins[2])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(eager, want[2])
+    del graphs, graph
+    torch.cuda.synchronize()
+    assert call("qe_workspace_count", 6) == before
+
+
+def test_threads_on_one_stream(dev):
+    """split products of several host threads on the default stream do not mix their sums"""
+    q, s = ref.weights(dev, (512, 8192), 1)
+    w = ops.tile_f8(q, s)
+    ins = [ref.activations(dev, 300, 8192, i) for i in range(4)]
+    want = [ops.matmul_f8(w, *i) for i in ins]
+    got = [[] for _ in ins]
+
+    def work(i):
+        for _ in range(25):
+            got[i].append(ops.matmul_f8(w, *ins[i]))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    for o, y in zip(got, want):
+        assert len(o) == 25 and all(torch.equal(v, y) for v in o)
 
 
 @pytest.mark.parametrize("t", [1, 60, 300, 1200])
