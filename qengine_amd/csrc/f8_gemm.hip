@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Spli
     const char* s0p = reinterpret_cast<const char*>(a.xs + x_first * a.xs_row + from * a.xs_group);
     int64_t s_next = a.xs_group * 4;
     uint32_t si = wave < BT / 64 ? x_row(wave * 64 + lane) * (uint32_t)(a.xs_row * 4) : 0;
-    if (wave == BT / 64) {
+    if (wave >= BT / 64) {  // (the waves after it fetch the same again, so that all count the same DMAs)
         s0p = reinterpret_cast<const char*>(a.s + (size_t)e * ((a.n + 127) >> 7) * blocks + from);
         s_next = 4;
         si = (uint32_t)min(tw * (BW / 128) + (lane & (BW / 128 - 1)), (a.n - 1) >> 7) * (uint32_t)(blocks * 4);
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Spli
         dma16_at(scalar(w0 + (size_t)min(b, kb - 1) * 2048 + wi[i]), lane * 16, to + (wave * WD + i) * 1024);
     };
     auto dma_s = [&](int b, unsigned to) {
-        if (wave <= BT / 64) dma4_at(scalar(s0p + min(b, kb - 1) * s_next), si, to + wave * 256);
+        dma4_at(scalar(s0p + min(b, kb - 1) * s_next), si, to + min(wave, BT / 64) * 256);
     };
     // the same for DMA number i of a wave's rows: their first 16 go to the ring for block `early`, the others to a stage
     auto dma_rows = [&](int i, int b, unsigned to, int early, unsigned ring) {
@@ -91,9 +91,9 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Spli
 
     // The sums of product number p = t WT + i wait in a ring while the next two products are under way; the step before's last two
     // are added before the first two of a step take their places
-    constexpr int RING = 3, LAG = RING - 1, NP = TT * WT, EV = 2 * (WD + XD) < NP ? 2 : 1, RW = NP / (2 * WT);
+    constexpr int RING = 3, LAG = RING - 1, NP = TT * WT, H = NP / 2, EV = H / (XD + 1), RW = H / (2 * WT);
     static_assert((NP - LAG) % RING == 0 && WT > LAG, "the last sums lie where the first ones go; scales outlast their sums");
-    static_assert(WD + XD < NP && RW * 2 * WT == NP, "a step's DMAs and reads find a product");
+    static_assert(EV > 0 && WD <= XD + 1 && RW > 0, "a step's DMAs and reads find a product");
     f32x4_v acc[WT][TT] = {}, part[RING] = {};
     i32x8_f8 w[2][WT];
     i32x8_f8 x[2];
@@ -145,32 +145,43 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Spli
 #pragma unroll
         for (int t = 0; t < TT; t++) {
             sc[t] = s * swb;
-            if (t + 1 < TT) {
-                load_x((t + 1) & 1, lds + cur * kX + (wt * TT + t + 1) * 2048);
-                s = load_s(lds + oS + ring * kS, t + 1);
-            } else {
-                load_x(0, lds + oFirst + next * kFirst + wt * 2048);
-                s0 = load_s(lds + oS + next * kS, 0);
-                sw0 = load_sw(lds + oS + next * kS);
-            }
 #pragma unroll
             for (int i = 0; i < WT; i++) {
                 const int p = t * WT + i;
                 if (p < LAG) flush(NP - LAG + p);
                 part[p % RING] = f8_mfma(w[cur][i], x[t & 1]);
-                if (p >= LAG) flush(p - LAG);
-                const int j = p / EV;  // a DMA behind every product, or every second
-                if (p % EV == 0) {
-                    if (j < WD) dma_w(j, b + 2, lds32 + oW + cur * kW);
-                    else if (j < WD + XD) dma_rows(j - WD, b + 1, lds32 + (cur ^ 1) * kX, b + 2, lds32 + oFirst + after * kFirst);
-                    else if (j == WD + XD) dma_s(b + 2, lds32 + oS + after * kS);
+                if (i == 0) {  // behind the product that needs what was read before: ahead of it the compiler waits for both
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (t + 1 < TT) {
+                        load_x((t + 1) & 1, lds + cur * kX + (wt * TT + t + 1) * 2048);
+                        s = load_s(lds + oS + ring * kS, t + 1);
+                    } else {
+                        load_x(0, lds + oFirst + next * kFirst + wt * 2048);
+                        s0 = load_s(lds + oS + next * kS, 0);
+                        sw0 = load_sw(lds + oS + next * kS);
+                    }
                 }
-                if (p % RW == RW / 2) load_w(cur ^ 1, p / RW / 2, p / RW % 2, lds + oW + (cur ^ 1) * kW);
+                if (p >= LAG) flush(p - LAG);
+                if (p < H && p % EV == 0) {
+                    const int j = p / EV;
+                    if (j < XD) dma_rows(j, b + 1, lds32 + (cur ^ 1) * kX, b + 2, lds32 + oFirst + after * kFirst);
+                    else if (j == XD) dma_s(b + 2, lds32 + oS + after * kS);
+                } else if (p >= H && (p - H) % EV == 0) {
+                    if ((p - H) / EV < WD) dma_w((p - H) / EV, b + 2, lds32 + oW + cur * kW);
+                }
+                if (p >= H && (p - H) % RW == RW - 1) load_w(cur ^ 1, (p - H) / RW / 2, (p - H) / RW % 2, lds + oW + (cur ^ 1) * kW);
+                // the weights fetched in the step before are there, of all waves
+                if (p == H - 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(XD + 1) : "memory");
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
         ring = next;
-        arrive();
+        // what the next step begins with is read (the compiler learns it here: it would wait again behind the barrier)
+        asm volatile("" : "+v"(x[0]), "+v"(s0), "+v"(sw0));
+#pragma unroll
+        for (int i = 0; i < WT; i++) asm volatile("" : "+v"(w[cur ^ 1][i]));
+        // the rows and scales fetched in this step are there (the weights have until the middle of the next), and all have read their stages
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(WD) : "memory");
     };
     int b = 0;
     for (; b + 2 <= kb; b += 2) {
@@ -180,6 +191,7 @@ __global__ void __launch_bounds__(WVT * WVW * 64, 2) gemm_kernel(F8Mat a, F8Spli
     if (b < kb) step(b, std::integral_constant<int, 0>{});
 #pragma unroll
     for (int p = NP - LAG; p < NP; p++) flush(p);
+    arrive();  // nothing is on its way to LDS any more
     const int first = wt * TT * 16;  // row of the tile
     if (!GROUPED && sp.parts > 1) {
         f32x4_v* const to = sp.sums + ((((size_t)tt * ntw + tw) * sp.parts + z) * NW + wave) * NP * 64 + lane;
