@@ -209,12 +209,12 @@ void norm_v(const F8Norm& a, hipStream_t st) {
 
 // ---------------------------------------------------------------- quantized rows, silu(gate) * up
 // g / (1 + exp(-g)). exp(-g) = 2^t, t = -g log2 e, whose rounding (up to half a step of t, 60 steps of the result) is put back by its
-// remainder; from 2^126 on without it, so that infinity stays. exp2 and the reciprocal are the hardware's, one step off at most: with
+// remainder; where |t| is 126 or more, t or e may be infinite, or e next to nothing: without it. exp2 and the reciprocal are the hardware's, one step off at most: with
 // the library's exp and an IEEE division 4096 x 17408 took 84 us, bound by the vector ALU.
 __device__ __forceinline__ float silu(float g) {
     constexpr float L = 1.44269504088896340736f, Lo = 1.92596299112661746887e-08f, ln2 = 0.693147180559945309417f;
     const float t = -g * L, rest = fmaf(-g, Lo, fmaf(-g, L, -t)) * ln2, e = __builtin_amdgcn_exp2f(t);
-    return g * __builtin_amdgcn_rcpf(1.f + (t < 126.f ? fmaf(e, rest, e) : e));
+    return g * __builtin_amdgcn_rcpf(1.f + (fabsf(t) < 126.f ? fmaf(e, rest, e) : e));
 }
 
 // LANES threads a row (a multiple of 16, a power of two), 8 columns each at a time

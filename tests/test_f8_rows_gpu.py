@@ -120,6 +120,22 @@ def test_quantized_far_values(dev):
     ref.check_quantized(q, s, ref.silu_mul(x), ref.SILU)
 
 
+@pytest.mark.parametrize("gate", [3.3e38, 2.4e38, 1e38, 200.0, 88.0, 87.0, -87.0, -88.0, -200.0, -1e38, -3.3e38])
+def test_silu_of_far_values(dev, gate):
+    x = torch.full((2, 256), gate, device=dev, dtype=BF)
+    x[:, 128:] = torch.linspace(-0.9, 0.9, 128, device=dev)
+    q, s = ops.silu_mul_f8(x)
+    ref.check_quantized(q, s, ref.silu_mul(x), ref.SILU)
+
+
+def test_silu_of_infinity(dev):
+    x = torch.ones(1, 512, device=dev, dtype=BF)
+    x[0, 3] = float("inf")
+    q, s = ops.silu_mul_f8(x)
+    assert s[0, 0].isinf() and q[0, 3].float().isnan() and q[0].float().isnan().sum() == 1
+    ref.check_quantized(q[:, 128:], s[:, 1:], ref.silu_mul(torch.ones(1, 256, device=dev)), ref.SILU)
+
+
 @pytest.mark.parametrize("dtype,otype", [(BF, BF), (F16, F16), (F32, F32), (BF, F32), (F16, F32)])
 @pytest.mark.parametrize("t,topk,d", [(1, 1, 1), (1, 10, 2048), (7, 3, 129), (64, 8, 640), (5, 1, 4100), (3, 0, 16), (300, 2, 72)])
 def test_combine(dev, t, topk, d, dtype, otype):
