@@ -114,7 +114,7 @@ __device__ __forceinline__ void quantize8(const float (&v)[8], uint8_t* q, int n
 // ---------------------------------------------------------------- the norm
 // A block holds whole rows, one after another, in registers: NV chunks of 8 columns a thread, as many threads as that takes. The mean is of the rounded
 // h, what the residual stream holds. Squares of values past 2^63 leave fp32 in the sum: such a row is summed again with a
-// factor of 2^-80 (eps is nothing beside them), so every finite row has finite results.
+// factor of 2^-80, and eps with 2^-160, so every finite row has finite results.
 template <int T, int WT, int NV, bool VEC>
 __global__ void __launch_bounds__(1024) norm_kernel(F8Norm a) {
     __shared__ float part[2][16];
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(F8Norm a) {
 #pragma unroll
                     for (int j = 0; j < 8; j++) far = fmaf(v[i][j] * f, v[i][j] * f, far);
                 }
-            rs = rsqrtf(block_sum(far, 1) / a.d);
+            rs = rsqrtf(block_sum(far, 1) / a.d + a.eps * f * f);
         }
 #pragma unroll
         for (int i = 0; i < NV; i++) {

@@ -73,6 +73,14 @@ def test_norm_far_values(dev, dtype):
     assert (q[2].float() == 0).all() and (s[2] > 0).all() and q[6].float().isnan().all()
 
 
+def test_norm_far_values_and_eps(dev):
+    x = torch.zeros(2, 65536, device=dev, dtype=BF)
+    x[:, 5] = 2.0 ** 64  # the mean of the squares: 2^112
+    w = torch.ones(65536, device=dev)
+    q, s = ops.rms_norm(x, w, 2.0 ** 100, f8=True)
+    ref.check_quantized(q, s, ref.norm(x, w, 2.0 ** 100), ref.NORM)
+
+
 @pytest.mark.parametrize("dtype", [BF, F16])
 @pytest.mark.parametrize("t,d", [(1, 1), (1, 5120), (3, 127), (5, 128), (17, 129), (33, 640), (9, 1000), (2, 2048), (3, 2056), (2, 17408), (300, 72), (1, 65537)])
 def test_quantized(dev, t, d, dtype):
