@@ -211,7 +211,7 @@ template <int BT, int BW, int WVT, int WVW, bool GROUPED>
 void gemm_t(const F8Mat& a, int parts, hipStream_t st) {
     constexpr int kLds = 2 * 128 * (BT + BW) + 3 * (WVT * 2048 + BT * 4 + 256);
     const int64_t ntt = GROUPED ? f8_most_jobs(a.r, a.experts, BT) : (a.r + BT - 1) / BT, ntw = (a.n + BW - 1) / BW;
-    CHECK(ntt * ntw <= kF8MaxBlocks, "matmul_f8: %lld row tiles by %lld column tiles are too many for a call", (long long)ntt, (long long)ntw);
+    CHECK(ntt * ntw * parts <= kF8MaxBlocks, "matmul_f8: %lld row tiles by %lld column tiles are too many for a call", (long long)ntt, (long long)ntw);
     const bool vec = a.ldy % 8 == 0 && ((uintptr_t)a.y & 15) == 0;
     auto run = [&](const F8Split& sp) {
         const dim3 grid(GROUPED ? xcd_blocks(ntt) * (unsigned)ntw : xcd_blocks(ntt * ntw * sp.parts)), block(WVT * WVW * 64);

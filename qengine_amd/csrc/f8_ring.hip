@@ -158,7 +158,7 @@ void ring_t(const F8Mat& a, int parts, hipStream_t st) {
     constexpr int kLds = S * ring_stage<BT, BW, S>() + BW * 32;
     static_assert(kLds <= 160 * 1024, "LDS of a CU");
     const int64_t ntt = GROUPED ? f8_most_jobs(a.r, a.experts, BT) : (a.r + BT - 1) / BT, ntw = (a.n + BW - 1) / BW;
-    CHECK(ntt * ntw <= kF8MaxBlocks, "matmul_f8: %lld row tiles by %lld column tiles are too many for a call", (long long)ntt, (long long)ntw);
+    CHECK(ntt * ntw * parts <= kF8MaxBlocks, "matmul_f8: %lld row tiles by %lld column tiles are too many for a call", (long long)ntt, (long long)ntw);
     const bool vec = a.ldy % 8 == 0 && ((uintptr_t)a.y & 15) == 0;
     auto run = [&](const F8Split& sp) {
         const dim3 grid(GROUPED ? xcd_blocks(ntt) * (unsigned)ntw : xcd_blocks(ntt * ntw * sp.parts)), block(kThreads);

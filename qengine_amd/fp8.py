@@ -71,6 +71,31 @@ def _written(name, t, shape, dtype, at):
     return row
 
 
+def _bytes(t):
+    """bytes from a tensor's first value to the end of its last (strides are not negative)"""
+    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _apart(name, out, **others):
+    """a given output shares no memory with what the call reads or writes besides (columns of one matrix are apart)"""
+    a = out.data_ptr()
+    for other, t in others.items():
+        if t is None or not t.numel() or not out.numel():
+            continue
+        b = t.data_ptr()
+        if b >= a + _bytes(out) or a >= b + _bytes(t):
+            continue
+        if out.dim() == 2 and t.dim() == 2 and out.shape[0] > 1 and t.shape[0] > 1:
+            row, size, there = out.stride(0) * out.element_size(), out.shape[1] * out.element_size(), t.shape[1] * t.element_size()
+            if row == t.stride(0) * t.element_size() and t.stride(1) == 1 and size <= (b - a) % row <= row - there:
+                continue
+        raise ValueError(f"{name} overlaps {other}")
+
+
+def _same(a, b):
+    return b is not None and (a is b or (a.data_ptr() == b.data_ptr() and a.stride() == b.stride()))
+
+
 def _ints(name, t, shape, at):
     if t.dtype is not torch.int32:
         raise TypeError(f"{name} is int32, got {t.dtype}")
@@ -98,12 +123,21 @@ def _quantized(t, d, device):
 
 @dataclass
 class F8:
-    """Weights in 8 bits (tile_f8): q uint8 in the products' layout, s fp32 [experts][blocks of n][blocks of k]."""
+    """Weights in 8 bits (tile_f8): q uint8 in the products' layout, s fp32 [blocks of n][blocks of k], or [experts] of these."""
     q: torch.Tensor
     s: torch.Tensor
     n: int
     k: int
     experts: int = 1
+
+    def __post_init__(self):
+        blocks = (-(-self.n // 128), -(-self.k // 128))
+        if self.q.dtype is not torch.uint8 or self.s.dtype is not torch.float32:
+            raise TypeError(f"an F8 is uint8 with float32 scales, got {self.q.dtype} and {self.s.dtype}")
+        if (self.s.shape not in (blocks, (self.experts, *blocks)) or (self.s.dim() == 2 and self.experts != 1)
+                or self.q.numel() != self.experts * -(-self.n // 16) * blocks[1] * 2048 or self.q.get_device() != self.s.get_device()
+                or not self.q.is_contiguous() or not self.s.is_contiguous() or self.q.data_ptr() % 16):
+            raise ValueError(f"not {self.experts} matrices of {self.n} x {self.k} on one device: {tuple(self.q.shape)}, {tuple(self.s.shape)}")
 
 
 def tile_f8(q, s):
@@ -133,8 +167,8 @@ def tile_f8(q, s):
 
 def rms_norm(x, w, eps=1e-6, res=None, res_out=None, out=None, f8=False):
     """Root-mean-square norm of rows x [t][d] (bfloat16 or float16) with weights w [d] (their type or float32). res [t][d]: the
-    residual stream; x + res, rounded to their type, goes to res_out (default: res itself) and is what the norm takes.
-    -> [t][d] of x's type (out, if given); f8=True: (q, s), e4m3 with scales, and the 16-bit values go to `out` if given."""
+    residual stream; x + res, rounded to their type, goes to res_out (default: res itself; or x) and is what the norm takes.
+    -> [t][d] of x's type (out, if given; x, where res_out is not); f8=True: (q, s), e4m3 with scales, and the 16-bit values go to `out` if given."""
     flags, at = _in_type("x", x), x.get_device()
     ldx = _matrix("x", x, at)
     t, d = x.shape
@@ -158,11 +192,16 @@ def rms_norm(x, w, eps=1e-6, res=None, res_out=None, out=None, f8=False):
         if res.shape != x.shape:
             raise ValueError(f"res has x's shape {tuple(x.shape)}, got {tuple(res.shape)}")
         ldr = _matrix("res", res, at)
+        to, px, pw = res_out.data_ptr(), x.data_ptr(), w.data_ptr()
+        end = to + 2 * ((t - 1) * ldro + d)
+        if res_out is not res or (px < end and to < px + 2 * ((t - 1) * ldx + d)) or (pw < end and to < pw + 4 * d):
+            _apart("res_out", res_out, w=w, x=None if _same(res_out, x) else x, res=None if _same(res_out, res) else res)
     elif res_out is not None:
         raise ValueError("res_out without res")
     y, ldy, q, s = out, 0, None, None
     if out is not None:
         ldy = _written("out", out, x.shape, x.dtype, at)
+        _apart("out", out, w=w, x=None if _same(out, x) else x, res=res, res_out=res_out)
     elif not f8:
         y = torch.empty(t, d, dtype=x.dtype, device=x.device)
         ldy = d
@@ -240,7 +279,10 @@ def matmul_f8(w: F8, q, s, dtype=torch.bfloat16, y=None):
     """y [t][n] = rows (q e4m3 [t][k], s fp32 [t][ceil(k / 128)]) times the matrix w; into y, or a new tensor of
     type dtype (bfloat16 or float16)"""
     at, ldx, t = _operands(w, q, s, False)
+    given = y is not None
     y, ldy, flags = _product(w, t, dtype, y, at)
+    if given:
+        _apart("y", y, q=q, s=s, weights=w.q, scales=w.s)
     if t:
         _run(at, "qe_matmul_f8", "ppiiplplliplip", w.q.data_ptr(), w.s.data_ptr(), w.n, w.k, q.data_ptr(), ldx, s.data_ptr(), s.stride(0),
              s.stride(1), t, y.data_ptr(), ldy, flags)
@@ -250,6 +292,10 @@ def matmul_f8(w: F8, q, s, dtype=torch.bfloat16, y=None):
 def matmul_f8_choice(w: F8, q, s, bt, bw, parts, dtype=torch.bfloat16):
     """matmul_f8 by a given kernel and number of K ranges instead of those that its sizes choose (qe_matmul_f8_choice)"""
     at, ldx, t = _operands(w, q, s, False)
+    if not (bt == 16 or (bt == bw == 256) or (bt in (32, 64, 128) and bw in (64, 128, 192))) or not 1 <= parts <= min(16, -(-w.k // 128)):
+        raise ValueError(f"no blocks of {bt} x {bw} with {parts} K ranges")
+    if -(-t // bt) * -(-w.n // max(bw, 32)) * parts > MAX_BLOCKS or not t:
+        raise ValueError(f"{t} rows of {w.n} in {parts} ranges")
     y, ldy, flags = _product(w, t, dtype, None, at)
     _run(at, "qe_matmul_f8_choice", "ppiiplpllipliiiip", w.q.data_ptr(), w.s.data_ptr(), w.n, w.k, q.data_ptr(), ldx, s.data_ptr(), s.stride(0),
          s.stride(1), t, y.data_ptr(), ldy, flags, bt, bw, parts)
@@ -266,8 +312,11 @@ def matmul_f8_grouped(w: F8, q, s, off, rows=None, dtype=torch.bfloat16, y=None)
     if rows is not None:
         _ints("rows", rows, (rows.numel(),), at)
         r = rows.numel()
+    given = y is not None
     rows_a_block, cols = (16, 32) if r // w.experts < 8 else (64, 128)  # the smallest blocks that the library may take
     y, ldy, flags = _product(w, r, dtype, y, at, (r // rows_a_block + min(r, w.experts)) * -(-w.n // cols))
+    if given:
+        _apart("y", y, q=q, s=s, weights=w.q, scales=w.s, off=off, rows=rows)
     if r:
         _run(at, "qe_matmul_f8_grouped", "ppiiiplpllippiplip", w.q.data_ptr(), w.s.data_ptr(), w.n, w.k, w.experts, q.data_ptr(), ldx,
              s.data_ptr(), s.stride(0), s.stride(1), t, off.data_ptr(), None if rows is None else rows.data_ptr(), r, y.data_ptr(), ldy, flags)
@@ -301,6 +350,7 @@ def moe_combine(y, inv, w, add=None, out=None):
         ldout = d
     else:
         ldout = _written("out", out, (t, d), dtype, at)
+        _apart("out", out, y=y, inv=inv, w=w, add=None if _same(out, add) else add)
     if t:
         _run(at, "qe_moe_combine", "plippplpliiiiip", y.data_ptr(), ldy, slots, inv.data_ptr(), w.data_ptr(),
              None if add is None else add.data_ptr(), ldadd, out.data_ptr(), ldout, t, topk, d, yflags, _OUT[dtype])

@@ -153,6 +153,80 @@ def test_combine_refusals(change, error):
     refused(ops.moe_combine, dict(y=z(6, 64), inv=z(6, dtype=I32), w=z(3, 2, dtype=F32)), change, error)
 
 
+BUF = z(64, 512)  # columns of one matrix are apart, shifted by less than a row they are not
+LEFT, RIGHT, MID = BUF[:4, :256], BUF[:4, 256:], BUF[:4, 128:384]
+
+
+@pytest.mark.parametrize("change,name", [
+    (dict(x=LEFT, out=MID), "out overlaps x"),
+    (dict(x=LEFT, out=BUF[1:5, :256]), "out overlaps x"),
+    (dict(res=LEFT, out=LEFT), "out overlaps res"),
+    (dict(res=z(4, 256), res_out=LEFT, out=LEFT), "out overlaps res_out"),
+    (dict(res=MID, x=LEFT), "res_out overlaps x"),
+    (dict(res=MID, res_out=LEFT), "res_out overlaps res"),
+    (dict(x=LEFT, res=z(4, 256), res_out=LEFT, out=LEFT), "out overlaps res_out"),
+    (dict(w=BUF[2, :256], out=LEFT), "out overlaps w"),
+    (dict(w=BUF[2, 256:], out=LEFT), "out overlaps w"),  # between rows: refused too
+    (dict(x=LEFT, out=RIGHT), "on a GPU"),
+    (dict(x=LEFT, out=LEFT), "on a GPU"),
+    (dict(x=LEFT, out=BUF[4:8, :256]), "on a GPU"),
+    (dict(x=LEFT, res=RIGHT), "on a GPU"),
+    (dict(x=LEFT, res=RIGHT, res_out=LEFT), "on a GPU"),
+    (dict(x=LEFT, res=LEFT), "on a GPU"),
+    (dict(x=LEFT, res=RIGHT, out=LEFT), "on a GPU"),
+])
+def test_norm_overlaps(change, name):
+    a = dict(x=z(4, 256), w=z(256))
+    a.update(change)
+    with pytest.raises(ValueError, match=name):
+        ops.rms_norm(**a)
+
+
+def test_product_and_combine_overlaps():
+    q, s, off = z(4, 272, dtype=F8), z(4, 3, dtype=F32), z(4, dtype=I32)
+    y = BUF[:4, :160]
+    with pytest.raises(ValueError, match="y overlaps q"):
+        ops.matmul_f8(mat(), BUF[:4, :136].view(F8), s, y=y)
+    with pytest.raises(ValueError, match="y overlaps q"):
+        ops.matmul_f8_grouped(mat(3), BUF[:4, 80:216].view(F8), s, off, y=y)
+    with pytest.raises(ValueError, match="y overlaps s"):
+        ops.matmul_f8(mat(), q, BUF[:4, 150:156].view(F32), y=y)
+    with pytest.raises(ValueError, match="y overlaps off"):
+        ops.matmul_f8_grouped(mat(3), q, s, BUF[0, :8].view(I32), y=y)
+    with pytest.raises(ValueError, match="on a GPU"):
+        ops.matmul_f8(mat(), BUF[:4, 160:296].view(F8), s, y=y)
+    inv, w = z(6, dtype=I32), z(3, 2, dtype=F32)
+    for add, out, name in [(None, BUF[:3, :64], "overlaps y"), (BUF[8:11, :64], BUF[9:12, :64], "overlaps add"),
+                           (BUF[8:11, :64], BUF[8:11, :64], "on a GPU"), (None, BUF[:3, 64:128], "on a GPU")]:
+        with pytest.raises(ValueError, match=name):
+            ops.moe_combine(BUF[:6, :64], inv, w, add=add, out=out)
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(q=z(10 * 3 * 2048 - 16, dtype=torch.uint8)), ValueError),
+    (dict(q=z(10 * 3 * 2048, dtype=F8)), TypeError),
+    (dict(q=z(10 * 3 * 2048 + 1, dtype=torch.uint8)[1:]), ValueError),
+    (dict(q=z(10 * 3 * 4096, dtype=torch.uint8)[::2]), ValueError),
+    (dict(s=z(2, 3)), TypeError),
+    (dict(s=z(3, 2, dtype=F32)), ValueError),
+    (dict(s=z(3, 2, dtype=F32).t()), ValueError),
+    (dict(s=z(2, 2, 3, dtype=F32)), ValueError),
+    (dict(n=177), ValueError),
+    (dict(k=400), ValueError),
+    (dict(experts=2), ValueError),
+])
+def test_weights_by_hand(change, error):
+    a = dict(q=z(10 * 3 * 2048, dtype=torch.uint8), s=z(2, 3, dtype=F32), n=160, k=272)
+    ops.F8(**a)
+    refused(ops.F8, a, change, error)
+
+
+@pytest.mark.parametrize("bt,bw,parts", [(16, 0, 4), (48, 64, 1), (64, 256, 1), (256, 128, 1), (64, 128, 0), (256, 256, 17)])
+def test_choices(bt, bw, parts):
+    with pytest.raises(ValueError, match="no blocks"):
+        ops.matmul_f8_choice(mat(), z(4, 272, dtype=F8), z(4, 3, dtype=F32), bt, bw, parts)
+
+
 @pytest.mark.parametrize("call,msg", [
     ("qe_rms_norm(P, L(8), None, L(0), None, L(0), P, F(1e-6), P, L(8), None, L(0), None, L(0), L(0), 0, 8, 0, None)", "rms_norm: 0 rows of 8"),
     ("qe_rms_norm(P, L(8), None, L(0), None, L(0), P, F(1e-6), P, L(8), None, L(0), None, L(0), L(0), 1, 65537, 0, None)", "1 rows of 65537"),
