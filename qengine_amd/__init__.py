@@ -1,4 +1,5 @@
-"""qengine_amd - MI355X-native (gfx950) weight-only quantized matmul path of QEngine, with attention and a paged cache.
+"""qengine_amd - MI355X-native (gfx950) weight-only quantized matmul path of QEngine, with attention, a paged cache and
+layers in 8-bit floating point.
 
 The product is libqe_kernels.so (C-ABI in include/qe_kernels.h, HIP kernels in qengine_amd/csrc). This package
 is the host-side mirror of the reference's ctypes test binding (reference tests/qe.py) plus typed torch

@@ -1,5 +1,6 @@
 // Operators in 8-bit floating point (e4m3 as OCP defines it: largest value 448, no infinities) and what stands between them
-// in a layer: host interface and the parts that the kernels share (f8_rows.hip, f8_dec.hip, f8_gemm.hip).
+// in a layer: host interface and the parts that the kernels share (f8_rows.hip, f8_dec.hip,
+// f8_ring.hip, f8_gemm.hip; f8_matmul.cpp chooses).
 //
 // Weights [n][k] have one fp32 scale for each block of 128 x 128, activations one for each row's 128 columns; the last block or
 // group may be shorter. y[t][n] = sum over blocks b of k: sx[t][b] sw[n / 128][b] (sum over k in b: x[t][k] W[n][k]). The inner
@@ -58,7 +59,7 @@ constexpr int kF8MaxDim = 1 << 20;      // n and k
 constexpr int kF8MaxRows = 1 << 24;     // of a call
 constexpr int kF8MaxRowBytes = 1 << 24;  // from a row of x to the next
 constexpr int kF8MaxScaleStride = 1 << 22;  // elements from a row's scale to the next
-constexpr int64_t kF8MaxBlocks = 1 << 22;  // blocks of 512 threads: a launch takes less than 2^32 threads
+constexpr int64_t kF8MaxBlocks = 1 << 22;  // of 512 threads: a launch takes less than 2^32 threads
 
 void f8_norm(const F8Norm& a, hipStream_t st);
 void f8_act(const F8Act& a, hipStream_t st);

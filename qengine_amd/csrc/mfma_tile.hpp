@@ -75,7 +75,7 @@ __device__ __forceinline__ void dma16_at(const void* base, uint32_t offset, unsi
 __device__ __forceinline__ void dma4(const void* src, unsigned lds_dst) {  // 4 bytes per lane
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds_dst), "v"(src) : "memory", "m0");
 }
-
+// 4 bytes per lane from a wave-uniform base and 32-bit offsets
 __device__ __forceinline__ void dma4_at(const void* base, uint32_t offset, unsigned lds_dst) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2" ::"s"(lds_dst), "v"(offset), "s"(base) : "memory", "m0");
 }
