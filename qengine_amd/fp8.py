@@ -71,11 +71,6 @@ def _written(name, t, shape, dtype, at):
     return row
 
 
-def _near(a, lda, b, ldb, rows, cols):
-    """whether the spans of two 16-bit matrices may meet (the quick look before _apart)"""
-    return b < a + 2 * ((rows - 1) * lda + cols) and a < b + 2 * ((rows - 1) * ldb + cols)
-
-
 def _bytes(t):
     """bytes from a tensor's first value to the end of its last (strides are not negative)"""
     return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
@@ -98,7 +93,7 @@ def _apart(name, out, **others):
 
 
 def _same(a, b):
-    return b is not None and (a is b or (a.data_ptr() == b.data_ptr() and a.stride() == b.stride()))
+    return b is not None and (a is b or (a.data_ptr() == b.data_ptr() and (a.shape[0] < 2 or a.stride() == b.stride())))
 
 
 def _ints(name, t, shape, at):
@@ -198,8 +193,11 @@ def rms_norm(x, w, eps=1e-6, res=None, res_out=None, out=None, f8=False):
             raise ValueError(f"res has x's shape {tuple(x.shape)}, got {tuple(res.shape)}")
         ldr = _matrix("res", res, at)
         to, px, pw = res_out.data_ptr(), x.data_ptr(), w.data_ptr()
-        pr = to if res is res_out else res.data_ptr()
-        if _near(to, ldro, px, ldx, t, d) or _near(to, ldro, pw, 0, t, 2 * d) or (pr != to and _near(to, ldro, pr, ldr, t, d)) or ldr != ldro:
+        pr, rows = to if res is res_out else res.data_ptr(), 2 * (t - 1)
+        end = to + rows * ldro + 2 * d
+        # spans that meet are looked at closely
+        if (px < end and to < px + rows * ldx + 2 * d) or (pw < end and to < pw + 4 * d) or (
+                pr < end and to < pr + rows * ldr + 2 * d and (pr != to or ldr != ldro)):
             _apart("res_out", res_out, w=w, x=None if _same(res_out, x) else x, res=None if _same(res_out, res) else res)
     elif res_out is not None:
         raise ValueError("res_out without res")

@@ -169,6 +169,8 @@ LEFT, RIGHT, MID = BUF[:4, :256], BUF[:4, 256:], BUF[:4, 128:384]
     (dict(w=BUF[2, 256:], out=LEFT), "out overlaps w"),  # between rows: refused too
     (dict(x=z(1, 256), res=BUF[2:3, :256], w=BUF[1:3].view(-1)[:512].view(F32)), "on a GPU"),
     (dict(x=z(1, 256), res=BUF[2:3, :256], w=BUF[1:3].view(-1)[2:514].view(F32)), "res_out overlaps w"),
+    (dict(res=LEFT, res_out=BUF.view(128, 256)[:4]), "res_out overlaps res"),
+    (dict(x=z(1, 256), res=BUF[2:3, :256], res_out=BUF.view(128, 256)[4:5]), "on a GPU"),
     (dict(x=LEFT, out=RIGHT), "on a GPU"),
     (dict(x=LEFT, out=LEFT), "on a GPU"),
     (dict(x=LEFT, out=BUF[4:8, :256]), "on a GPU"),
