@@ -188,6 +188,71 @@ def test_grouped_bad_indexes(dev):
         assert (room[:7] == 7).all() and (room[13:] == 7).all()
 
 
+@pytest.mark.parametrize("lens,n,k", [([5, 0, 9], 97, 272), ([30, 100, 1], 640, 512), ([300, 0, 260], 640, 512), ([2100, 900], 1024, 400)])
+def test_grouped_bad_indexes_by_every_kernel(dev, lens, n, k):
+    """as row 0, but zeros"""
+    e, r, t = len(lens), sum(lens), 50
+    q, s = ref.weights(dev, (e, n, k), 1)
+    x, xs = ref.activations(dev, t, k, 2)
+    w = ops.tile_f8(q, s)
+    off = torch.tensor([sum(lens[:i]) for i in range(e + 1)], dtype=torch.int32, device=dev)
+    g = ref.gen(dev, r)
+    rows = torch.randint(t, (r,), device=dev, generator=g).int()
+    bad = torch.rand(r, device=dev, generator=g) < 0.3
+    bad[0] = bad[-1] = True
+    far = torch.tensor([-1, t, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32, device=dev)[torch.arange(r, device=dev) % 4]
+    want = ops.matmul_f8_grouped(w, x, xs, off, rows=torch.where(bad, 0, rows))
+    y = ops.matmul_f8_grouped(w, x, xs, off, rows=torch.where(bad, far, rows))
+    assert torch.equal(y, torch.where(bad[:, None], 0, want))
+
+
+@pytest.mark.parametrize("t", [3, 40, 300])
+def test_far_rows(dev, t):
+    """rows and scales as far apart as a call takes, so that offsets pass 32 bits"""
+    n, k = 530, 400
+    q, s = ref.weights(dev, (n, k), 3)
+    w, one = ops.tile_f8(q, s), ops.tile_f8(q[None], s[None])
+    x, xs = ref.activations(dev, t, k, 4)
+    want = ops.matmul_f8(w, x, xs)
+    far = torch.empty(t << 24, dtype=torch.uint8, device=dev).view(ref.F8).as_strided((t, k), ((1 << 24) - 16, 1))
+    far.view(torch.uint8).copy_(x.view(torch.uint8))
+    xs_far = torch.empty(t << 22, device=dev).as_strided(xs.shape, ((1 << 22) - 1, 1))
+    xs_far.copy_(xs)
+    assert torch.equal(ops.matmul_f8(w, far, xs_far), want)
+    off = torch.tensor([0, t], dtype=torch.int32, device=dev)
+    rows = torch.arange(t - 1, -1, -1, dtype=torch.int32, device=dev)
+    back = rows.long()
+    ref.check_product(ops.matmul_f8_grouped(one, far, xs_far, off, dtype=F16), x, xs, q, s)
+    ref.check_product(ops.matmul_f8_grouped(one, far, xs_far, off, rows=rows, dtype=F16), x.view(torch.uint8)[back].view(ref.F8), xs[back], q, s)
+
+
+def test_large_outputs_and_weights(dev):
+    """y and the experts' weights beyond 2^32 bytes: what lies last"""
+    t, n, k = 17000, 131072, 128
+    q, s = ref.weights(dev, (n, k), 5)
+    x, xs = ref.activations(dev, t, k, 6)
+    y = ops.matmul_f8(ops.tile_f8(q, s), x, xs)
+    last, cols = slice(t - 300, t), slice(n - 512, n)
+    ref.check_product(y[last, cols], x.view(torch.uint8)[last].view(ref.F8), xs[last], q.view(torch.uint8)[cols].view(ref.F8), s[-4:], "last")
+    del y
+    e, n, k = 1024, 2048, 2560
+    q, s = ref.weights(dev, (2, n, k), 7)
+    many = torch.zeros(e, n, k, dtype=torch.uint8, device=dev)
+    many[0], many[-1] = q.view(torch.uint8)[0], q.view(torch.uint8)[1]
+    scales = torch.ones(e, *s.shape[1:], device=dev)
+    scales[0], scales[-1] = s[0], s[1]
+    w = ops.tile_f8(many.view(ref.F8), scales)
+    del many
+    for lens in ([3, 2], [5000, 4000]):
+        off = torch.full((e + 1,), lens[0], dtype=torch.int32, device=dev)
+        off[0], off[-1] = 0, sum(lens)
+        x, xs = ref.activations(dev, sum(lens), k, 8)
+        y = ops.matmul_f8_grouped(w, x, xs, off, dtype=F16)
+        tail = slice(sum(lens) - lens[1], sum(lens))
+        for rows, i in ((slice(0, lens[0]), 0), (tail, 1)):
+            ref.check_product(y[rows], x.view(torch.uint8)[rows].view(ref.F8), xs[rows], q[i], s[i], f"{lens} {i}")
+
+
 def test_no_rows(dev):
     q, s = ref.weights(dev, (2, 32, 128), 1)
     x, xs = ref.activations(dev, 0, 128, 2)

@@ -182,3 +182,26 @@ def test_no_rows(dev):
     q, s = ops.quant_f8(x)
     assert q.shape == (0, 256) and s.shape == (0, 2)
     assert ops.moe_combine(torch.ones(1, 8, device=dev), torch.empty(0, dtype=torch.int32, device=dev), torch.empty(0, 2, device=dev)).shape == (0, 8)
+
+
+def test_large(dev):
+    """values beyond 2^32 bytes: the last rows"""
+    t, d = 40000, 65536
+    x = torch.zeros(t, d, dtype=BF, device=dev)
+    x[-3:] = rows(dev, 3, d, BF, 1)
+    w = torch.ones(d, device=dev)
+    y = ops.rms_norm(x, w)
+    ref.check_16(y[-3:], ref.norm(x[-3:], w, 1e-6), ref.NORM)
+    assert (y[-4] == 0).all()
+    del y
+    q, s = ops.rms_norm(x, w, f8=True)
+    ref.check_quantized(q[-3:], s[-3:], ref.norm(x[-3:], w, 1e-6), ref.NORM)
+    q, s = ops.silu_mul_f8(x)
+    ref.check_quantized(q[-3:], s[-3:], ref.silu_mul(x[-3:]), ref.SILU)
+    inv = torch.tensor([t - 1, t - 2, t - 3, 5], dtype=torch.int32, device=dev)
+    weight = torch.tensor([[0.5, 2.0], [1.0, 1.0]], device=dev)
+    out = ops.moe_combine(x, inv, weight)
+    v = x[-3:].double()
+    want = torch.stack([0.5 * v[2] + 2 * v[1], v[0]])
+    size = torch.stack([0.5 * v[2].abs() + 2 * v[1].abs(), v[0].abs()])
+    ref.within(out, want, 3 * ref.U * size + ref.half(BF, want.abs() + 3 * ref.U * size))
