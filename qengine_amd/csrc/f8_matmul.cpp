@@ -9,26 +9,51 @@ struct Choice {
     double us = 1e30;
 };
 
-// us of a product by rounds of blocks, one a CU (MI355X). A block of the ring takes its stages' bytes at 40 bytes/ns and 4 us to start
-// and end, one of the 256 x 256 tiles 1.6 us a step and 6 us; the weights come at 5.4 TB/s at most. K ranges cost a launch (4 us)
-// and the sums written and read again at 5 TB/s. Measured / modelled: 48 rows of 34816 x 5120: 192 columns a block 36 / 37, 128 48 / 53,
-// 64 44 / 53; of 5120 x 17408: 64 columns in 3 ranges 23 / 27, 128 in 6 23 / 26; 128 rows of 34816 x 5120: 41 / 45; 1000 rows of 5120 x
-// 17408, 256 x 256 in 3 ranges: 100 / 108.
-Choice choose(const F8Mat& a) {
-    const int cus = qe_num_cus(), blocks = (a.k + 127) / 128;
+// us of a product of up to 64 rows by rounds of blocks, one a CU (MI355X): a block takes its stages' bytes at 40 bytes/ns and 4 us to start
+// and end; the weights come at 5.4 TB/s at most. K ranges cost a launch (4 us) and the sums written and read again at 5 TB/s. Measured /
+// modelled: 48 rows of 34816 x 5120: 192 columns a block 36 / 37, 128 48 / 53, 64 44 / 53; of 5120 x 17408: 64 columns in 3 ranges
+// 23 / 27, 128 in 6 23 / 26.
+Choice choose_few(const F8Mat& a) {
+    const int cus = qe_num_cus(), blocks = (a.k + 127) / 128, bt = a.r <= 32 ? 32 : 64;
     Choice best;
-    auto offer = [&](int bt, int bw) {
-        const int64_t tiles = (int64_t)((a.r + bt - 1) / bt) * ((a.n + bw - 1) / bw);
+    for (int bw : {64, 128, 192}) {
+        const int64_t tiles = (a.n + bw - 1) / bw;
         for (int p = 1; p <= 16 && p <= blocks && (p == 1 || tiles * p <= cus); p++) {
             const double rounds = (double)((tiles * p + cus - 1) / cus), steps = (blocks + p - 1) / p;
-            double us = bt == 256 ? rounds * (steps * 1.6 + 6) : std::max(rounds * steps * (bt + bw) * 128 / 40e3, (double)a.n * a.k / 5.4e6) + 4;
+            double us = std::max(rounds * steps * (bt + bw) * 128 / 40e3, (double)a.n * a.k / 5.4e6) + 4;
             if (p > 1) us += 4 + 2.0 * tiles * p * bt * bw * 4 / 5e6;
             if (us < best.us) best = {bt, bw, p, us};
         }
+    }
+    return best;
+}
+
+// More rows: blocks of every shape but 32 x 192, `fit` of them a CU at once, whose step of 128 k takes `alone` us or `each` for each of
+// several; fitted to 2500 measured products of 12 matrices (512 to 34816 rows of 1024 to 17408) with 100 to 2500 rows, blocks and
+// ranges of all shapes. Measured, the choice is 1 % slower than the fastest of them on average and 19 % at most (14336 x 4096, 512 rows:
+// 51 us, by 128 x 128 43); with blocks of 128 or 256 rows only, by the model above, it was 12 %, 74 % at most. 400 rows of 2048 x 6144: 24.1 ->
+// 15.3 us (blocks of 64 x 64, none of them split); 160 of 10240 x 5120: 38.7 -> 22.3; 1000 of 5120 x 17408: 256 x 256 in 3 ranges, 100.
+Choice choose(const F8Mat& a) {
+    if (a.r <= 64) return choose_few(a);
+    struct Shape {
+        int bt, bw, fit;
+        double alone, each;
     };
-    const int bt = a.r <= 32 ? 32 : a.r <= 64 ? 64 : 128;
-    for (int bw : {64, 128, 192}) offer(bt, bw);
-    if (a.r > 64) offer(256, 256);
+    static constexpr Shape kShapes[] = {{32, 64, 3, .10, .156}, {32, 128, 2, .21, .25}, {64, 64, 2, .10, .223}, {64, 128, 2, .33, .33}, {64, 192, 1, .50, .364},
+                                        {128, 64, 2, .34, .36}, {128, 128, 2, .40, .75}, {128, 192, 1, .40, 1.0}, {256, 256, 1, 1.05, 1.32}};
+    const int cus = qe_num_cus(), blocks = (a.k + 127) / 128;
+    Choice best;
+    for (const Shape& s : kShapes) {
+        const int64_t tiles = (int64_t)((a.r + s.bt - 1) / s.bt) * ((a.n + s.bw - 1) / s.bw);
+        for (int p = 1; p <= 16 && p <= blocks && (p == 1 || tiles * p <= cus); p++) {
+            const int64_t most = (tiles * p + cus - 1) / cus, rest = most % s.fit;  // blocks of a CU
+            const double steps = (blocks + p - 1) / p;
+            double us = steps * ((most / s.fit) * std::max(s.alone, s.fit * s.each) + (rest ? std::max(s.alone, rest * s.each) : 0)) + 1.1 * most / s.fit;
+            us = std::max(us, (double)a.n * a.k / 6.3e6) + 4.2;
+            if (p > 1) us += 3.5 + 2.0 * tiles * p * s.bt * s.bw * 4 / 5.2e6;
+            if (us < best.us) best = {s.bt, s.bw, p, us};
+        }
+    }
     return best;
 }
 
