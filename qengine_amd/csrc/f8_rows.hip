@@ -209,12 +209,22 @@ void norm_v(const F8Norm& a, hipStream_t st) {
 
 // ---------------------------------------------------------------- quantized rows, silu(gate) * up
 // g / (1 + exp(-g)). exp(-g) = 2^t, t = -g log2 e, whose rounding (up to half a step of t, 60 steps of the result) is put back by its
-// remainder; where |t| is 126 or more, t or e may be infinite, or e next to nothing: without it. exp2 and the reciprocal are the hardware's, one step off at most: with
+// remainder; where |t| is 126 or more, t may be infinite and e is next to nothing: without it. exp2 and the reciprocal are the hardware's, one step off at most: with
 // the library's exp and an IEEE division 4096 x 17408 took 84 us, bound by the vector ALU.
 __device__ __forceinline__ float silu(float g) {
     constexpr float L = 1.44269504088896340736f, Lo = 1.92596299112661746887e-08f, ln2 = 0.693147180559945309417f;
     const float t = -g * L, rest = fmaf(-g, Lo, fmaf(-g, L, -t)) * ln2, e = __builtin_amdgcn_exp2f(t);
     return g * __builtin_amdgcn_rcpf(1.f + (fabsf(t) < 126.f ? fmaf(e, rest, e) : e));
+}
+
+// silu(g) * u below kFarGate, where 1 + exp(-g) is exp(-g) in fp32, and it or its reciprocal leaves fp32 from -87.3 on: g exp(g) u, the
+// exponential as two equal factors, u between them: both are numbers of full precision, and no product leaves fp32, as far as the result is above what a
+// group's scale makes zero. The factors' two steps each, the remainder's and three products' roundings: 8 half steps, as above.
+constexpr float kFarGate = -40.f;
+__device__ __forceinline__ float silu_far(float g, float u) {
+    constexpr float L = 1.44269504088896340736f, Lo = 1.92596299112661746887e-08f, ln2 = 0.693147180559945309417f;
+    const float t = -g * L, rest = fmaf(-g, Lo, fmaf(-g, L, -t)) * ln2, h = __builtin_amdgcn_exp2f(-0.5f * t);
+    return (t < 256.f ? fmaf(g, -rest, g) : g) * h * u * h;
 }
 
 // LANES threads a row (a multiple of 16, a power of two), 8 columns each at a time
@@ -230,8 +240,16 @@ __global__ void __launch_bounds__(256) act_kernel(F8Act a, int shift, int blocks
         if constexpr (GLU) {
             float u[8];
             get8<T, VEC>(a.x, row * a.ldx + a.d + c * 8, n, u);
+            float least = v[0];
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = silu(v[j]) * u[j];
+            for (int j = 1; j < 8; j++) least = fminf(least, v[j]);
+            if (least < kFarGate) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = v[j] < kFarGate ? silu_far(v[j], u[j]) : silu(v[j]) * u[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = silu(v[j]) * u[j];
+            }
         }
     }
     quantize8<VEC>(v, reinterpret_cast<uint8_t*>(a.q) + row * a.ldq + c * 8, n, a.s + row * a.s_row + (c >> 4) * a.s_group, lane);

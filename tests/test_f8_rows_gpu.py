@@ -205,3 +205,17 @@ def test_large(dev):
     want = torch.stack([0.5 * v[2] + 2 * v[1], v[0]])
     size = torch.stack([0.5 * v[2].abs() + 2 * v[1].abs(), v[0].abs()])
     ref.within(out, want, 3 * ref.U * size + ref.half(BF, want.abs() + 3 * ref.U * size))
+
+
+@pytest.mark.parametrize("gate", [-43.0, -44.25, -45.0, -60.0, -80.0, -87.0, -87.5, -88.0, -88.5, -89.0, -95.0, -120.0, -150.0, -170.0])
+def test_silu_of_far_gates_and_large_values(dev, gate):
+    """exp(-gate) at the end of fp32 and beyond, silu(gate) * up not: alone, and among usual values"""
+    g = ref.gen(dev, int(-4 * gate))
+    x = rows(dev, 4, 1024, BF, 3)
+    up = torch.exp2(torch.rand(4, 512, device=dev, generator=g) * 27 + 100) * torch.where(torch.rand(4, 512, device=dev, generator=g) < 0.5, -1, 1)
+    x[:2, :512], x[:2, 512:] = gate, up[:2]
+    few = torch.rand(4, 512, device=dev, generator=g) < 0.1
+    few[:2] = False
+    x[:, :512][few], x[:, 512:][few] = gate, up.to(BF)[few]
+    q, s = ops.silu_mul_f8(x)
+    ref.check_quantized(q, s, ref.silu_mul(x), ref.SILU)
