@@ -159,9 +159,9 @@ __global__ void __launch_bounds__(1024) norm_kernel(F8Norm a) {
             }
         }
         sum = block_sum(sum, 0);
-        float rs = rsqrtf(sum / a.d + a.eps), f = 1.f;
+        float rs = rsqrtf(sum / a.d + a.eps), half = 1.f;
         if (!(sum <= 3.0e38f)) {  // the same for the whole block
-            f = 8.271806125530277e-25f;  // 2^-80
+            constexpr float f = 8.271806125530277e-25f;  // 2^-80
             float far = 0.f;
 #pragma unroll
             for (int i = 0; i < NV; i++)
@@ -169,7 +169,8 @@ __global__ void __launch_bounds__(1024) norm_kernel(F8Norm a) {
 #pragma unroll
                     for (int j = 0; j < 8; j++) far = fmaf(v[i][j] * f, v[i][j] * f, far);
                 }
-            rs = rsqrtf(block_sum(far, 1) / a.d + a.eps * f * f);
+            half = 9.094947017729282e-13f;  // 2^-40, for the value and for the root: by all of f small values would lose bits
+            rs = rsqrtf(block_sum(far, 1) / a.d + a.eps * f * f) * half;
         }
 #pragma unroll
         for (int i = 0; i < NV; i++) {
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(F8Norm a) {
             float y[8];
             if (!KEEP && c < chunks) get8<WT, VEC>(a.w, c * 8, n, w[0]);
 #pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = c < chunks ? v[i][j] * f * rs * w[KEEP ? i : 0][j] : 0.f;
+            for (int j = 0; j < 8; j++) y[j] = c < chunks ? v[i][j] * half * rs * w[KEEP ? i : 0][j] : 0.f;
             if (a.y && c < chunks) put8<T, VEC>(a.y, row * a.ldy + c * 8, n, y);
             if (a.q)
                 quantize8<VEC>(y, reinterpret_cast<uint8_t*>(a.q) + row * a.ldq + c * 8, n, a.s + row * a.s_row + (c >> 4) * a.s_group, lane);

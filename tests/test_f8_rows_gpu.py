@@ -219,3 +219,17 @@ def test_silu_of_far_gates_and_large_values(dev, gate):
     x[:, :512][few], x[:, 512:][few] = gate, up.to(BF)[few]
     q, s = ops.silu_mul_f8(x)
     ref.check_quantized(q, s, ref.silu_mul(x), ref.SILU)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -66, 2.0 ** -50, 2.0 ** -20, 1.0])
+def test_norm_of_small_values_in_a_far_row(dev, size):
+    """a row whose squares leave fp32 keeps what its small values are"""
+    g = ref.gen(dev, 5)
+    x = (size * (1 + torch.rand(3, 640, device=dev, generator=g))).to(BF)
+    x[:, 5] = 2.0 ** 64
+    for scale in (1.0, 2.0 ** 60):
+        w = torch.full((640,), scale, device=dev)
+        y = torch.empty_like(x)
+        q, s = ops.rms_norm(x, w, 1e-6, out=y, f8=True)
+        ref.check_16(y, ref.norm(x, w, 1e-6), ref.NORM)
+        ref.check_quantized(q, s, ref.norm(x, w, 1e-6), ref.NORM)
