@@ -121,6 +121,11 @@ def _quantized(t, d, device):
     return q if d % 16 == 0 else q[:, :d], torch.empty_strided((t, -(-d // 128)), (1, t), dtype=torch.float32, device=device)
 
 
+def _sizes(n, k, experts):
+    if not 0 < experts <= MAX_EXPERTS or not 0 < n <= MAX_DIM or not 0 < k <= MAX_DIM or k % 16:
+        raise ValueError(f"at most {MAX_EXPERTS} matrices, n and k at most {MAX_DIM}, k a multiple of 16, got {experts} of {n} x {k}")
+
+
 @dataclass
 class F8:
     """Weights in 8 bits (tile_f8): q uint8 in the products' layout, s fp32 [blocks of n][blocks of k], or [experts] of these."""
@@ -131,6 +136,7 @@ class F8:
     experts: int = 1
 
     def __post_init__(self):
+        _sizes(self.n, self.k, self.experts)
         blocks = (-(-self.n // 128), -(-self.k // 128))
         if self.q.dtype is not torch.uint8 or self.s.dtype is not torch.float32:
             raise TypeError(f"an F8 is uint8 with float32 scales, got {self.q.dtype} and {self.s.dtype}")
@@ -149,8 +155,7 @@ def tile_f8(q, s):
         raise ValueError(f"weights are [n][k] or [experts][n][k], got shape {tuple(q.shape)}")
     lead, (n, k) = q.shape[:-2], q.shape[-2:]
     experts = lead[0] if lead else 1
-    if not 0 < experts <= MAX_EXPERTS or not 0 < n <= MAX_DIM or not 0 < k <= MAX_DIM or k % 16:
-        raise ValueError(f"at most {MAX_EXPERTS} matrices, n and k at most {MAX_DIM}, k a multiple of 16, got {tuple(q.shape)}")
+    _sizes(n, k, experts)
     if s.shape != (*lead, -(-n // 128), -(-k // 128)):
         raise ValueError(f"scales have shape {(*lead, -(-n // 128), -(-k // 128))}, got {tuple(s.shape)}")
     at = q.get_device()

@@ -225,6 +225,16 @@ def test_weights_by_hand(change, error):
     refused(ops.F8, a, change, error)
 
 
+@pytest.mark.parametrize("n,k,experts", [(160, 264, 1), (0, 272, 1), (160, 0, 1), (-5, 272, 1), ((1 << 20) + 1, 16, 1), (16, (1 << 20) + 16, 1),
+                                         (16, 16, 1025), (16, 16, 0), (16, 16, -1)])
+def test_weights_by_hand_of_sizes_that_no_product_takes(n, k, experts):
+    """the sizes that the library would end the process for"""
+    bn, bk = max(-(-n // 128), 0), max(-(-k // 128), 0)
+    q, s = z(max(experts, 0) * max(-(-n // 16), 0) * bk * 2048, dtype=torch.uint8), z(max(experts, 0), bn, bk, dtype=F32)
+    with pytest.raises(ValueError, match="at most"):
+        ops.F8(q, s, n, k, experts)
+
+
 @pytest.mark.parametrize("bt,bw,parts", [(16, 0, 4), (48, 64, 1), (64, 256, 1), (256, 128, 1), (64, 128, 0), (256, 256, 17)])
 def test_choices(bt, bw, parts):
     with pytest.raises(ValueError, match="no blocks"):
