@@ -302,7 +302,7 @@ def matmul_f8_choice(w: F8, q, s, bt, bw, parts, dtype=torch.bfloat16):
     at, ldx, t = _operands(w, q, s, False)
     if not (bt == 16 or (bt == bw == 256) or (bt in (32, 64, 128) and bw in (64, 128, 192))) or not 1 <= parts <= min(16, -(-w.k // 128)):
         raise ValueError(f"no blocks of {bt} x {bw} with {parts} K ranges")
-    if -(-t // bt) * -(-w.n // max(bw, 32)) * parts > MAX_BLOCKS or not t:
+    if -(-t // bt) * -(-w.n // (32 if bt == 16 else bw)) * parts > MAX_BLOCKS or not t:
         raise ValueError(f"{t} rows of {w.n} in {parts} ranges")
     y, ldy, flags = _product(w, t, dtype, None, at)
     _run(at, "qe_matmul_f8_choice", "ppiiplpllipliiiip", w.q.data_ptr(), w.s.data_ptr(), w.n, w.k, q.data_ptr(), ldx, s.data_ptr(), s.stride(0),

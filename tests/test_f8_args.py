@@ -241,6 +241,15 @@ def test_choices(bt, bw, parts):
         ops.matmul_f8_choice(mat(), z(4, 272, dtype=F8), z(4, 3, dtype=F32), bt, bw, parts)
 
 
+@pytest.mark.parametrize("bw", [0, 32, 1 << 20])
+def test_choices_of_few_rows_whatever_the_columns(bw):
+    """blocks of 16 rows have 32 columns: too many of them end the process in the library"""
+    t, n = 1 << 17, 1 << 17
+    w = ops.F8(z(n // 16 * 2048, dtype=torch.uint8), z(n // 128, 1, dtype=F32), n, 16)
+    with pytest.raises(ValueError, match="rows of 131072 in"):
+        ops.matmul_f8_choice(w, z(t, 16, dtype=F8), z(t, 1, dtype=F32), 16, bw, 1)
+
+
 @pytest.mark.parametrize("call,msg", [
     ("qe_rms_norm(P, L(8), None, L(0), None, L(0), P, F(1e-6), P, L(8), None, L(0), None, L(0), L(0), 0, 8, 0, None)", "rms_norm: 0 rows of 8"),
     ("qe_rms_norm(P, L(8), None, L(0), None, L(0), P, F(1e-6), P, L(8), None, L(0), None, L(0), L(0), 1, 65537, 0, None)", "1 rows of 65537"),
