@@ -470,6 +470,11 @@ void qe_matmul_f8_choice(const void* q, const float* s, int n, int k, const void
 void qe_matmul_f8_grouped(const void* q, const float* s, int n, int k, int experts, const void* x, int64_t ldx, const float* xs,
                           int64_t xs_row, int64_t xs_group, int t, const int32_t* off, const int32_t* rows, int r, void* y,
                           int64_t ldy, int flags, void* stream);
+/* test hook: qe_matmul_f8_grouped by a given kernel: blocks of bt rows, 16 x 32 columns, 64 or 128 x 128, 256 x 256 (this one with rows
+ * only where t * ldx and t * xs_row * 4 are below 2^32). No counterpart in the reference. */
+void qe_matmul_f8_grouped_choice(const void* q, const float* s, int n, int k, int experts, const void* x, int64_t ldx, const float* xs,
+                                 int64_t xs_row, int64_t xs_group, int t, const int32_t* off, const int32_t* rows, int r, void* y,
+                                 int64_t ldy, int flags, int bt, void* stream);
 
 /* out[i] = add[i] + sum over j of w[i][j] * y[inv[i * topk + j]], in the order of j in fp32, rounded once: the rows of a
  * grouped product back into tokens (inv and w as qe_moe_segment and qe_moe_route give them; add NULL: none). An index outside

@@ -474,6 +474,15 @@ void qe_matmul_f8_grouped(const void* q, const float* s, int n, int k, int exper
               as_stream(st));
 }
 
+void qe_matmul_f8_grouped_choice(const void* q, const float* s, int n, int k, int experts, const void* x, int64_t ldx, const float* xs,
+                                 int64_t xs_row, int64_t xs_group, int t, const int32_t* off, const int32_t* rows, int r, void* y,
+                                 int64_t ldy, int flags, int bt, void* st) {
+    CHECK(off != nullptr, "qe_matmul_f8_grouped_choice: off is missing");
+    CHECK(rows || r <= t, "qe_matmul_f8_grouped_choice: %d rows of y, %d of x", r, t);
+    f8_grouped_choice({q, s, x, xs, off, rows, y, ldx, xs_row, xs_group, ldy, n, k, t, r, experts, f8_type(flags, 0, "qe_matmul_f8_grouped_choice")},
+                      bt, as_stream(st));
+}
+
 void qe_moe_combine(const void* y, int64_t ldy, int rows, const int32_t* inv, const float* w, const void* add, int64_t ldadd, void* out,
                     int64_t ldout, int t, int topk, int d, int yflags, int flags, void* st) {
     const int type = f8_any(yflags, "qe_moe_combine"), otype = f8_any(flags, "qe_moe_combine");

@@ -67,6 +67,7 @@ void f8_combine(const F8Combine& a, hipStream_t st);
 void f8_tile(const void* src, int64_t ld, int64_t mat, int n, int k, int experts, void* dst, hipStream_t st);
 void f8_matmul(const F8Mat& a, hipStream_t st);
 void f8_matmul_choice(const F8Mat& a, int bt, int bw, int parts, hipStream_t st);  // bt 16: f8_dec, 256: f8_gemm
+void f8_grouped_choice(const F8Mat& a, int bt, hipStream_t st);  // the same, 64 and 128: f8_ring
 void f8_dec(const F8Mat& a, hipStream_t st);  // up to 16 rows, or segments of few
 void f8_ring(const F8Mat& a, int bt, int bw, int parts, hipStream_t st);  // blocks of bt rows x bw weight rows, K in ranges
 void f8_gemm(const F8Mat& a, int parts, hipStream_t st);                  // tiles of 256 x 256

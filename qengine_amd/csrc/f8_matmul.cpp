@@ -81,8 +81,7 @@ static void check(const F8Mat& a) {
     CHECK(a.t < 2 || (a.xs_row >= 0 && a.xs_row < kF8MaxScaleStride), "matmul_f8: scales of rows are less than %d elements apart", kF8MaxScaleStride);
 }
 
-void f8_matmul(const F8Mat& call, hipStream_t st) {
-    check(call);
+static void grouped(const F8Mat& call, int bt, hipStream_t st) {
     F8Mat a = call;
     if (a.t == 0) {  // every index is outside x: rows that are read and not used
         a.x = a.q;
@@ -90,13 +89,14 @@ void f8_matmul(const F8Mat& call, hipStream_t st) {
         a.ldx = a.xs_row = 0;
         a.xs_group = 1;
     }
-    if (a.off) {
-        const int bt = choose_grouped(a);
-        if (bt == 16) f8_dec(a, st);
-        else if (bt == 256) f8_gemm(a, 1, st);
-        else f8_ring(a, bt, 128, 1, st);
-        return;
-    }
+    if (bt == 16) f8_dec(a, st);
+    else if (bt == 256) f8_gemm(a, 1, st);
+    else f8_ring(a, bt, 128, 1, st);
+}
+
+void f8_matmul(const F8Mat& a, hipStream_t st) {
+    check(a);
+    if (a.off) return grouped(a, choose_grouped(a), st);
     // 16 rows of 34816 x 5120 36 us by f8_dec, of 5120 x 17408 22
     if (a.r <= 16) return f8_dec(a, st);
     const Choice c = choose(a);
@@ -111,4 +111,10 @@ void f8_matmul_choice(const F8Mat& a, int bt, int bw, int parts, hipStream_t st)
     if (bt == 256) return f8_gemm(a, parts, st);
     CHECK((bt == 32 || bt == 64 || bt == 128) && (bw == 64 || bw == 128 || bw == 192), "matmul_f8: blocks of %d x %d", bt, bw);
     f8_ring(a, bt, bw, parts, st);
+}
+
+void f8_grouped_choice(const F8Mat& a, int bt, hipStream_t st) {
+    check(a);
+    CHECK(a.off && (bt == 16 || bt == 64 || bt == 128 || (bt == 256 && f8_gemm_takes(a))), "matmul_f8_grouped: blocks of %d rows", bt);
+    grouped(a, bt, st);
 }

@@ -331,6 +331,24 @@ def matmul_f8_grouped(w: F8, q, s, off, rows=None, dtype=torch.bfloat16, y=None)
     return y
 
 
+def matmul_f8_grouped_choice(w: F8, q, s, off, bt, rows=None, dtype=torch.bfloat16, y=None):
+    """matmul_f8_grouped by a given kernel instead of the one that its sizes choose (qe_matmul_f8_grouped_choice)"""
+    at, ldx, t = _operands(w, q, s, True)
+    _ints("off", off, (w.experts + 1,), at)
+    if rows is not None:
+        _ints("rows", rows, (rows.numel(),), at)
+    r = t if rows is None else rows.numel()
+    if bt not in (16, 64, 128, 256) or (bt == 256 and rows is not None and t * max(ldx, s.stride(0) * 4) >= 1 << 32) or not r:
+        raise ValueError(f"no blocks of {bt} for {r} of {t} rows")
+    given = y is not None
+    y, ldy, flags = _product(w, r, dtype, y, at, (r // bt + min(r, w.experts)) * -(-w.n // {16: 32, 256: 256}.get(bt, 128)))
+    if given:
+        _apart("y", y, q=q, s=s, weights=w.q, scales=w.s, off=off, rows=rows)
+    _run(at, "qe_matmul_f8_grouped_choice", "ppiiiplpllippipliip", w.q.data_ptr(), w.s.data_ptr(), w.n, w.k, w.experts, q.data_ptr(), ldx,
+         s.data_ptr(), s.stride(0), s.stride(1), t, off.data_ptr(), None if rows is None else rows.data_ptr(), r, y.data_ptr(), ldy, flags, bt)
+    return y
+
+
 def moe_combine(y, inv, w, add=None, out=None):
     """out [t][d] = add + sum over j of w[i][j] * y[inv[i * topk + j]]: the rows y [slots][d] of a grouped product back into
     tokens, inv int32 [t * topk] and w fp32 [t][topk] as moe_segment and moe_route give them (an index outside y adds nothing).

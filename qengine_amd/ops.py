@@ -477,4 +477,4 @@ class SafeTensorsFile:
 from .attention import KVCache, attn_prompt  # noqa: E402,F401
 
 # ---------------------------------------------------------------- layers in 8-bit floating point
-from .fp8 import F8, matmul_f8, matmul_f8_choice, matmul_f8_grouped, moe_combine, quant_f8, rms_norm, silu_mul_f8, tile_f8  # noqa: E402,F401
+from .fp8 import F8, matmul_f8, matmul_f8_choice, matmul_f8_grouped, matmul_f8_grouped_choice, moe_combine, quant_f8, rms_norm, silu_mul_f8, tile_f8  # noqa: E402,F401

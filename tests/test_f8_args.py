@@ -250,6 +250,24 @@ def test_choices_of_few_rows_whatever_the_columns(bw):
         ops.matmul_f8_choice(w, z(t, 16, dtype=F8), z(t, 1, dtype=F32), 16, bw, 1)
 
 
+@pytest.mark.parametrize("change,error,match", [
+    (dict(bt=32), ValueError, "no blocks of 32"),
+    (dict(bt=0), ValueError, "no blocks of 0"),
+    (dict(q=z(0, 272, dtype=F8), s=z(0, 3, dtype=F32)), ValueError, "for 0 of 0 rows"),
+    (dict(w=mat()), ValueError, "of them for matmul_f8_grouped"),
+    (dict(off=z(4, dtype=I64)), TypeError, "off"),
+    (dict(rows=z(2, 2, dtype=I32)), ValueError, "rows"),
+    (dict(y=z(4, 161)), ValueError, "y has shape"),
+    (dict(q=z(1, 272, dtype=F8).expand(1 << 24, 272), s=z(1, 3, dtype=F32).expand(1 << 24, 3), rows=z(4, dtype=I32)), ValueError, "on a GPU"),
+    (dict(), ValueError, "on a GPU"),
+])
+def test_grouped_choice_refusals(change, error, match):
+    a = dict(w=mat(3), q=z(4, 272, dtype=F8), s=z(4, 3, dtype=F32), off=z(4, dtype=I32), bt=256)
+    a.update(change)
+    with pytest.raises(error, match=match):
+        ops.matmul_f8_grouped_choice(**a)
+
+
 @pytest.mark.parametrize("call,msg", [
     ("qe_rms_norm(P, L(8), None, L(0), None, L(0), P, F(1e-6), P, L(8), None, L(0), None, L(0), L(0), 0, 8, 0, None)", "rms_norm: 0 rows of 8"),
     ("qe_rms_norm(P, L(8), None, L(0), None, L(0), P, F(1e-6), P, L(8), None, L(0), None, L(0), L(0), 1, 65537, 0, None)", "1 rows of 65537"),
@@ -271,6 +289,10 @@ def test_choices_of_few_rows_whatever_the_columns(bw):
     ("qe_matmul_f8_grouped(P, P, 16, 32, 2, P, L(32), P, L(1), L(1), 4, None, None, 4, P, L(16), 0, None)", "off is missing"),
     ("qe_matmul_f8_grouped(P, P, 16, 32, 2, P, L(32), P, L(1), L(1), 4, P, None, 5, P, L(16), 0, None)", "5 rows of y, 4 of x"),
     ("qe_matmul_f8_grouped(P, P, 16, 32, 0, P, L(32), P, L(1), L(1), 4, P, None, 4, P, L(16), 0, None)", "0 matrices"),
+    ("qe_matmul_f8_grouped_choice(P, P, 16, 32, 2, P, L(32), P, L(1), L(1), 4, P, None, 4, P, L(16), 0, 32, None)", "blocks of 32 rows"),
+    ("qe_matmul_f8_grouped_choice(P, P, 16, 32, 2, P, L(32), P, L(1), L(1), 4, None, None, 4, P, L(16), 0, 64, None)", "off is missing"),
+    ("qe_matmul_f8_grouped_choice(P, P, 16, 32, 2, P, L(1 << 20), P, L(1), L(1), 4096, P, P, 4, P, L(16), 0, 256, None)", "blocks of 256 rows"),
+    ("qe_matmul_f8_grouped_choice(P, P, 16, 32, 2, P, L(32), P, L(1), L(1), 4, P, None, 5, P, L(16), 0, 64, None)", "5 rows of y, 4 of x"),
     ("qe_moe_combine(P, L(8), 4, P, P, None, L(0), P, L(8), 2, 2000, 8, 0, 0, None)", "2000 rows each"),
     ("qe_moe_combine(P, L(8), 4, P, P, None, L(0), P, L(8), 2, 2, 8, 0, 2, None)", "y's type or fp32"),
     ("qe_moe_combine(P, L(8), 4, P, P, None, L(0), P, L(8), 2, 2, 8, 18, 2, None)", "flags 18"),
