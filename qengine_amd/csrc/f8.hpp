@@ -1,6 +1,6 @@
 // Operators in 8-bit floating point (e4m3 as OCP defines it: largest value 448, no infinities) and what stands between them
 // in a layer: host interface and the parts that the kernels share (f8_rows.hip, f8_dec.hip,
-// f8_ring.hip, f8_gemm.hip; f8_matmul.cpp chooses).
+// f8_ring.hip, f8_gemm.hip; f8_matmul.cpp and f8_choice.hpp choose).
 //
 // Weights [n][k] have one fp32 scale for each block of 128 x 128, activations one for each row's 128 columns; the last block or
 // group may be shorter. y[t][n] = sum over blocks b of k: sx[t][b] sw[n / 128][b] (sum over k in b: x[t][k] W[n][k]). The inner

@@ -1,5 +1,6 @@
 // The 8-bit products' checks and the choice of their kernel (f8.hpp).
 #include "f8.hpp"
+#include "f8_choice.hpp"
 
 #include <algorithm>
 
@@ -56,18 +57,6 @@ Choice choose(const F8Mat& a) {
     }
     return best;
 }
-
-// Grouped: segments of ragged lengths end in a block that is half empty on average, and have one at least. A block's step of 128 k takes 0.46 us a CU (64 x
-// 128), 0.8 (128 x 128) or 1.6 (256 x 256, and 14 us to start and end). Measured, 512 matrices of 1024 x 2048, us with blocks of 64 / 128 rows
-// (they read the weights in 200): 4096 rows 181 / 226, 20480 211 / 240, 40960 258 / 262, 81920 386 / 375, 163840 644 / 613.
-int choose_grouped(const F8Mat& a) {
-    if (a.r / a.experts < 8) return 16;
-    const double steps = (a.k + 127) / 128, cus = qe_num_cus();
-    auto us = [&](int bt, int bw, double step) { return std::max(a.r / (double)bt + a.experts * 0.5, (double)a.experts) * ((a.n + bw - 1) / bw) * steps / cus * step; };
-    const double u64 = us(64, 128, 0.46), u128 = us(128, 128, 0.8), u256 = us(256, 256, 1.6 + 14 / steps);
-    if (f8_gemm_takes(a) && u256 < u64 && u256 < u128) return 256;
-    return u64 <= u128 ? 64 : 128;
-}
 }  // namespace
 
 static void check(const F8Mat& a) {
@@ -96,7 +85,7 @@ static void grouped(const F8Mat& call, int bt, hipStream_t st) {
 
 void f8_matmul(const F8Mat& a, hipStream_t st) {
     check(a);
-    if (a.off) return grouped(a, choose_grouped(a), st);
+    if (a.off) return grouped(a, f8_grouped_rows(a.r, a.n, a.k, a.experts, qe_num_cus(), f8_gemm_takes(a)), st);
     // 16 rows of 34816 x 5120 36 us by f8_dec, of 5120 x 17408 22
     if (a.r <= 16) return f8_dec(a, st);
     const Choice c = choose(a);

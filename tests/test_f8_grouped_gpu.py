@@ -133,7 +133,7 @@ def test_many_segments_and_long_sums(dev, bt):
 
 def test_far_rows_by_index(dev):
     """rows by index more than 2^32 bytes from the first: not by the kernel with 32-bit offsets, whatever the sizes; in order by any"""
-    t, n, k, lens = 260, 1024, 2048, [2560, 2560]
+    t, n, k, lens = 260, 2048, 2048, [2560, 2560]
     q, s = ref.weights(dev, (2, n, k), 3)
     w = ops.tile_f8(q, s)
     x, xs = ref.activations(dev, t, k, 4)
