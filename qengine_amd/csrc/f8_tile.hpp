@@ -98,11 +98,14 @@ __global__ void __launch_bounds__(64) sum_kernel(F8Mat a, F8Split sp, int ntw, b
                             [](int) { return false; });
 }
 
-// room for the sums of tiles * parts blocks of BT x BW, at most 64 MB, else no split; parts is what the caller's model likes best
+// room for the sums of tiles * parts blocks of BT x BW: a stream's buffer holds a block of 256 x 256 for each CU (64 MB) from its first split
+// on, so that it never grows (f8_matmul.cpp splits where the blocks are no more than the CUs); a graph's what its calls need. No split where
+// they need more, or without memory.
 inline F8Split f8_split(WsHold& hold, int64_t tiles, int parts, int bt, int bw) {
     F8Split sp;
-    if (parts < 2) return sp;
-    sp.sums = static_cast<f32x4_v*>(hold.get(kWsF8, (size_t)tiles * parts * bt * bw * 4));
+    const size_t whole = (size_t)qe_num_cus() * 256 * 256 * 4, bytes = (size_t)tiles * parts * bt * bw * 4;
+    if (parts < 2 || bytes > whole) return sp;
+    sp.sums = static_cast<f32x4_v*>(hold.get(kWsF8, bytes, false, whole));
     if (sp.sums) sp.parts = parts;
     return sp;
 }

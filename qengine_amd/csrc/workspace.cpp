@@ -164,13 +164,14 @@ bool needs_sizing(int kind) { return kind == kWsSplit || kind == kWsI8 || kind =
 WsHold::WsHold(hipStream_t st) : st_(st), s_(stream_of(st)) { s_->mu.lock(); }
 WsHold::~WsHold() { s_->mu.unlock(); }
 
-void* WsHold::get(int kind, size_t bytes, bool retry) {
+void* WsHold::get(int kind, size_t bytes, bool retry, size_t whole) {
     CHECK(kind >= 0 && kind < kNumWs, "workspace kind %d", kind);
     Ws& w = s_->ws[kind];
     unsigned long long id = 0;
     hipGraph_t graph = nullptr;
     if (capturing(st_, &id, &graph)) return needs_sizing(kind) && w.bytes < bytes ? nullptr : capture_buf(s_, kind, bytes, id, graph);
     if (w.bytes >= bytes) return w.p;
+    if (bytes < whole) bytes = whole;
     const bool optional = kind != kWsI8 && kind != kWsH;  // the caller runs without it
     if (optional && !retry && w.wait > 0 && bytes >= w.refused) {
         w.wait--;

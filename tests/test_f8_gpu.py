@@ -436,3 +436,33 @@ def test_streams(dev, t):
     torch.cuda.synchronize()
     for o, y in zip(got, want):
         assert all(torch.equal(v, y) for v in o)
+
+
+def test_a_stream_allocates_its_sums_once(dev):
+    """the first split product of a stream allocates what the largest may need: later ones of any size allocate nothing, and one
+    whose sums need more runs unsplit"""
+    k = 2048
+    q, s = ref.weights(dev, (4096, k), 1)
+    w = ops.tile_f8(q, s)
+    x, xs = ref.activations(dev, 4096, k, 2)
+
+    def product(t, n, bt, bw, parts):
+        one = ops.F8(w.q[:n // 16 * (k // 128) * 2048], w.s[:n // 128], n, k)
+        return ops.matmul_f8_choice(one, x[:t], xs[:t].t().contiguous().t(), bt, bw, parts)
+
+    calls = [(40, 256, 64, 64, 2), (300, 512, 128, 128, 4), (1000, 1024, 256, 256, 4), (4096, 1024, 256, 256, 4), (1024, 4096, 256, 256, 4), (2048, 4096, 256, 256, 2)]
+    too_large = [(4096, 4096, 256, 256, 2), (4096, 4096, 256, 256, 16), (4096, 4096, 128, 192, 2)]
+    with torch.cuda.stream(torch.cuda.Stream()):
+        whole = [product(*c[:4], 1) for c in calls + too_large]  # (torch's own blocks are there afterwards)
+        got = [product(*c[:4], 1) for c in calls + too_large]
+        del got
+        got = [product(*calls[0])]
+        torch.cuda.synchronize()
+        count, free = call("qe_workspace_count", 6), torch.cuda.mem_get_info()[0]
+        got += [product(*c) for c in calls[1:] + too_large]
+        torch.cuda.synchronize()
+        assert torch.cuda.mem_get_info()[0] == free and call("qe_workspace_count", 6) == count
+    for c, a, b in zip(calls + too_large, got, whole):
+        t, n = c[:2]
+        ref.check_product(a, x[:t], xs[:t], q[:n], s[:n // 128], str(c))
+        assert c not in too_large or torch.equal(a, b), c

@@ -26,6 +26,11 @@ def test_workspace(model, scenario):
     assert r.returncode == 0 and r.stdout.endswith("OK\n"), r.stdout + r.stderr
 
 
+def test_whole_at_once(model):
+    r = subprocess.run([model, "whole_at_once"], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and r.stdout.endswith("OK\n"), r.stdout + r.stderr
+
+
 @pytest.mark.parametrize("scenario,msg", [("reserve_in_capture", "called during graph capture"),
                                           ("reserve_without_memory", "no memory for 1048576 bytes")])
 def test_reserve_that_cannot_be_met(model, scenario, msg):

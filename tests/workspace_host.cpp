@@ -264,6 +264,26 @@ static void growth_frees() {
     unref(g);
 }
 
+// a buffer made whole at once does not grow after; a capture's is what its calls need
+static void whole_at_once() {
+    hipStream_t st = stream(1);
+    const size_t whole = 64 << 20;
+    auto get = [&](size_t bytes) { return WsHold(st).get(kWsF8, bytes, false, whole); };
+    void* p = get(1 << 20);
+    const size_t allocs = g_allocs;
+    EXPECT(p && sized(st, kWsF8) == whole);
+    for (size_t mb = 1; mb <= 64; mb++) EXPECT(get(mb << 20) == p);
+    EXPECT(g_allocs == allocs && g_synced[st] == 0);
+    const size_t held = g_held;
+    Graph* g = begin_capture(st);
+    EXPECT(get(1 << 20) != p && g_held == held + (1 << 20));
+    end_capture(st);
+    unref(g);
+    g_oom = true;  // a stream without memory for the whole
+    EXPECT(WsHold(stream(2)).get(kWsF8, 1 << 20, false, whole) == nullptr);
+    g_oom = false;
+}
+
 // no memory: the calls that can run without a buffer are told so and do not ask the device each time; they get one later
 static void without_memory() {
     for (int kind : {kWsSplit, kWsDec, kWsSkinny}) {
@@ -308,6 +328,7 @@ int main(int argc, char** argv) {
                                                    {"allocate_beside_a_capture", allocate_beside_a_capture},
                                                    {"capture_without_memory", capture_without_memory},
                                                    {"growth_frees", growth_frees},
+                                                   {"whole_at_once", whole_at_once},
                                                    {"without_memory", without_memory},
                                                    {"reserve_in_capture", reserve_in_capture},
                                                    {"reserve_without_memory", reserve_without_memory}};
