@@ -233,3 +233,67 @@ def test_norm_of_small_values_in_a_far_row(dev, size):
         q, s = ops.rms_norm(x, w, 1e-6, out=y, f8=True)
         ref.check_16(y, ref.norm(x, w, 1e-6), ref.NORM)
         ref.check_quantized(q, s, ref.norm(x, w, 1e-6), ref.NORM)
+
+
+def padded(dev, t, d, dtype, seed, pad):
+    """rows with `pad` columns of sevens behind each -> the rows, and what holds them"""
+    room = torch.full((t, d + pad), 7.0, dtype=dtype, device=dev)
+    room[:, :d] = rows(dev, t, d, dtype, seed)
+    return room[:, :d], room
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("t", [1, 2, 63, 500])
+@pytest.mark.parametrize("d,pads", [(256, (8, 16, 24, 40)), (256, (3, 5, 1, 7)), (1536, (16, 0, 8, 64)), (770, (1, 2, 3, 4))])
+def test_norm_rows_apart(dev, t, d, pads, dtype):
+    """x, the stream, its next buffer and the output each with rows of their own distance"""
+    (x, xr), (r, rr), (h, hr), (y, yr) = (padded(dev, t, d, dtype, i, p) for i, p in enumerate(pads))
+    kept, room = r.clone(), rr.clone()
+    w = 1 + 0.3 * torch.randn(d, device=dev, generator=ref.gen(dev, 9))
+    want = (x.float() + kept.float()).to(dtype)
+    q, s = ops.rms_norm(x, w, res=r, res_out=h, out=y, f8=True)
+    assert torch.equal(h, want) and torch.equal(rr, room)
+    ref.check_16(y, ref.norm(want, w, 1e-6), ref.NORM)
+    ref.check_quantized(q, s, ref.norm(want, w, 1e-6), ref.NORM)
+    for v in (xr, rr, hr, yr):
+        assert (v[:, d:] == 7).all()
+    ops.rms_norm(x, w, res=r, out=y)  # the stream in place
+    assert torch.equal(r, want) and (rr[:, d:] == 7).all() and (yr[:, d:] == 7).all()
+    ref.check_16(y, ref.norm(want, w, 1e-6), ref.NORM)
+    r.copy_(kept)
+    x2 = x.clone()
+    q2, s2 = ops.rms_norm(x, w, res=r, res_out=x, f8=True)  # into x
+    assert torch.equal(x, want) and torch.equal(r, kept) and (xr[:, d:] == 7).all()
+    assert torch.equal(q2.view(torch.uint8), q.view(torch.uint8)) and torch.equal(s2, s)
+    x.copy_(x2)
+    ref.check_16(ops.rms_norm(x, w), ref.norm(x, w, 1e-6), ref.NORM)
+
+
+@pytest.mark.parametrize("dtype,otype", [(BF, BF), (F16, F32), (F32, F32)])
+@pytest.mark.parametrize("t,topk,d", [(1, 10, 256), (7, 3, 129), (64, 8, 640), (300, 2, 72)])
+@pytest.mark.parametrize("pads", [(8, 16, 24), (3, 5, 1), (0, 8, 5)])
+def test_combine_rows_apart(dev, t, topk, d, pads, dtype, otype):
+    """the experts' rows, what they are added to and the output each with rows of their own distance"""
+    g = ref.gen(dev, t + d)
+    (y, yr), (add, ar), (out, outr) = padded(dev, t * topk, d, dtype, 1, pads[0]), padded(dev, t, d, otype, 2, pads[1]), padded(dev, t, d, otype, 3, pads[2])
+    inv = torch.randperm(t * topk, device=dev, generator=g).int()
+    w = torch.rand(t, topk, device=dev, generator=g) - 0.2
+    terms = w[..., None].double() * y[inv.long()].double().view(t, topk, d)
+    for more in (add, None):
+        kept = ar.clone()
+        assert ops.moe_combine(y, inv, w, add=more, out=out) is out
+        assert torch.equal(ar, kept) and (outr[:, d:] == 7).all() and (yr[:, d:] == 7).all()
+        want, size = terms.sum(1), terms.abs().sum(1)
+        if more is not None:
+            want, size = want + more.double(), size + more.double().abs()
+        off = (topk + 1) * ref.U * size
+        ref.within(out, want, off + ref.half(otype, want.abs() + off))
+
+
+@pytest.mark.parametrize("pads", [(8, 16), (3, 5)])
+def test_activation_rows_apart(dev, pads):
+    for pad in pads:
+        x, room = padded(dev, 90, 816, BF, 4, pad)
+        ref.check_quantized(*ops.silu_mul_f8(x), ref.silu_mul(x.contiguous()), ref.SILU)
+        ref.check_quantized(*ops.quant_f8(x), x.double(), 0)
+        assert (room[:, 816:] == 7).all()
