@@ -76,9 +76,9 @@ void dec_t(const F8Mat& a, hipStream_t st) {
 }
 }  // namespace
 
-// us for 5120 x 17408 with one row: two tiles a block 17.1 (one: 18.3, four: 26.7), loads a step ahead 17.7; 34816 x 5120 with one
-// row 31 to 32 by any of these, with 16 rows 35.8 (four waves; eight: 38.9); 160 rows of 512 matrices of 1024 x 2048 43.5 (eight waves; four:
-// 44.6, four tiles: 45).
+// us by two tiles and eight waves a block / one tile / four tiles / two tiles and four waves, weights rotating over three sets: one row of
+// 5120 x 17408 15.9 / 16.5 / 24.4 / 23.8, 16 rows 19.0 / 27.0 / 28.6 / 25.0; one row of 34816 x 5120 32.5 / 31.0 / 35.0 / 32.9, 16 rows 36.1 / 41.8 /
+// 38.2 / 36.0; 160 rows of 512 matrices of 1024 x 2048 47.8 / 61.6 / 48.9 / 48.3.
 void f8_dec(const F8Mat& a, hipStream_t st) {
     if (a.off) dec_t<2, 8, true>(a, st);
     else if (a.n >= 16384) dec_t<2, 4, false>(a, st);

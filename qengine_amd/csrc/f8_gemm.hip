@@ -7,9 +7,9 @@
 // Bound by the matrix cores and what keeps them waiting: a step of 256 x 256 has 2048 cycles of products a SIMD. Issued at once its
 // DMAs kept the waves at the address unit (64 bytes a cycle, 1000 to 1500 cycles) ahead of the products: 4490 cycles a step; the rows' and
 // scales' in its first half, the weights', which have until the middle of the next step, in its second: about 3200. 8192 rows of 17408 x
-// 5120: 652 us, 2.24 PFLOP/s, 1.6 us a step and round; with no DMA in the loop 1.15, with zeros for data (no power limit) 13 % less in all. Two
-// barriers a step: in its middle (the weights of the step before have come) and at its end. Not faster: DMAs closer together or
-// further apart (651 to 672), a third stage of rows (664), weights straight into registers (765: two waves fetch the same ones).
+// 5120: 633 to 654 us, 2.23 to 2.31 PFLOP/s, 1.6 us a step and round; with no DMA in the loop 1.15, with zeros for data (no power limit) 13 % less in all. Two
+// barriers a step: in its middle (the weights of the step before have come) and at its end. Not faster (against
+// 652): DMAs closer together or further apart (651 to 672), a third stage of rows (664), weights straight into registers (765: two waves fetch the same ones).
 #include "f8_tile.hpp"
 #include <type_traits>
 

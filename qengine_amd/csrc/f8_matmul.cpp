@@ -13,7 +13,7 @@ struct Choice {
 // us of a product of up to 64 rows by rounds of blocks, one a CU (MI355X): a block takes its stages' bytes at 40 bytes/ns and 4 us to start
 // and end; the weights come at 5.4 TB/s at most. K ranges cost a launch (4 us) and the sums written and read again at 5 TB/s. Measured /
 // modelled: 48 rows of 34816 x 5120: 192 columns a block 36 / 37, 128 48 / 53, 64 44 / 53; of 5120 x 17408: 64 columns in 3 ranges
-// 23 / 27, 128 in 6 23 / 26.
+// 20 / 27, 128 in 6 21 / 26. Small matrices it splits for nothing: 1024 x 2048 10.8, by blocks of 32 x 64 unsplit 7.9.
 Choice choose_few(const F8Mat& a) {
     const int cus = qe_num_cus(), blocks = (a.k + 127) / 128, bt = a.r <= 32 ? 32 : 64;
     Choice best;
@@ -86,7 +86,7 @@ static void grouped(const F8Mat& call, int bt, hipStream_t st) {
 void f8_matmul(const F8Mat& a, hipStream_t st) {
     check(a);
     if (a.off) return grouped(a, f8_grouped_rows(a.r, a.n, a.k, a.experts, qe_num_cus(), f8_gemm_takes(a)), st);
-    // 16 rows of 34816 x 5120 36 us by f8_dec, of 5120 x 17408 22
+    // 16 rows of 34816 x 5120 36 us by f8_dec, of 5120 x 17408 19
     if (a.r <= 16) return f8_dec(a, st);
     const Choice c = choose(a);
     if (c.bt == 256) f8_gemm(a, c.parts, st);
