@@ -461,7 +461,8 @@ size_t qe_f8_bytes(int n, int k);
 void qe_matmul_f8(const void* q, const float* s, int n, int k, const void* x, int64_t ldx, const float* xs, int64_t xs_row,
                   int64_t xs_group, int t, void* y, int64_t ldy, int flags, void* stream);
 /* test hook: qe_matmul_f8 by a given kernel: blocks of bt rows x bw columns (16: few rows; 32, 64 or 128 x 64, 128 or 192; 256: 256 x
- * 256), K in `parts` ranges (1..16, at most one for each 128; for 16 they are the waves'). No counterpart in the reference. */
+ * 256), K in `parts` ranges (1..16, at most one for each 128; for 16 they are the waves'; one where their sums need more than the
+ * workspace). No counterpart in the reference. */
 void qe_matmul_f8_choice(const void* q, const float* s, int n, int k, const void* x, int64_t ldx, const float* xs, int64_t xs_row,
                          int64_t xs_group, int t, void* y, int64_t ldy, int flags, int bt, int bw, int parts, void* stream);
 
