@@ -88,6 +88,12 @@ def test_within_ten_per_cent_of_the_fastest(choose):
     assert not slow, slow
 
 
+def test_rounds_of_an_xcd(choose):
+    """blocks go to the XCDs in whole rows: tiles of 256 x 256 that are one round of the card may be two of an XCD (us measured by 64,
+    128 and 256 rows: 20.1 / 23.8 / 29.1 and 45.6 / 43.6 / 60.2)"""
+    assert choose([(1662, 5376, 288, 8, CUS, 1), (1171, 5984, 1904, 8, CUS, 1)]) in ([64, 64], [64, 128])
+
+
 def test_few_rows_an_expert(choose):
     assert choose([(7, 1024, 2048, 1, CUS, 1), (4095, 1024, 2048, 512, CUS, 1), (1, 16, 16, 1024, CUS, 1)]) == [16] * 3
 
